@@ -208,7 +208,7 @@ def _plain_attention(s):
     do = s["do"].float().view(B, T, Hkv, H // Hkv, D).permute(0, 2, 3, 1, 4)
     dv = torch.matmul(p.transpose(-1, -2), do).sum(2, keepdim=True)
     ds = torch.matmul(do, v32.transpose(-1, -2))
-    ds = ds.sub_((do * o).sum(-1, keepdim=True)).mul_(p).mul_(scale)
+    ds = ds.sub_((ds * p).sum(-1, keepdim=True)).mul_(p).mul_(scale)  # so a row that sees one key has exactly none
     del p
     return back(o), back(torch.matmul(ds, k32)), back(torch.matmul(ds.transpose(-1, -2), q32).sum(2, keepdim=True)), back(dv)
 
