@@ -1,0 +1,43 @@
+"""Causal attention with a sliding window and sinks: training, prefill and
+single tokens against a cache."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import ext
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                     lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v over the keys that a row sees; [B, T, H, D].
+
+    q is [B, T, H, D], k and v are [B, T, Hkv, D]; H / Hkv query heads share a
+    key head.  Row i of sequence b sees key j iff ``i < lengths[b]``,
+    ``j <= i`` and (``i - j < window`` or ``j < sinks``): the last ``window``
+    tokens, itself among them, and the first ``sinks``.  A window of T or more
+    is full causal attention.  ``lengths`` (int32 [B], on the device, clamped to
+    [0, T]) are the sequences' lengths; rows at or behind them give zeros and
+    get zero gradients, and what they hold is not used.  ``scale`` is
+    D ** -0.5 unless given.
+
+    float32, bfloat16 or float16, D from 1 to 128, any strides (elements of a
+    head that do not lie side by side are copied first).  Scores, softmax
+    statistics and sums are 32-bit.  Gradients flow to q, k and v, each summed
+    in a fixed order: the same inputs give the same bits.
+    """
+    return ext.get_ops().window_attention(q, k, v, window, sinks, lengths, scale)
+
+
+def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, window: int,
+                            sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:
+    """One token per sequence against a cache; [B, H, D].
+
+    q is [B, H, D], the caches are [B, T, Hkv, D] and already hold the token's
+    own key and value: the query is token ``lengths[b] - 1`` of its sequence and
+    sees what that row of ``window_attention`` sees.  ``lengths`` (int32 [B], on
+    the device) are clamped to [0, T]; a length of 0 gives zeros.  Only the keys
+    and values that are seen are read.  No backward pass.
+    """
+    return ext.get_ops().window_attention_decode(q, k_cache, v_cache, lengths, window, sinks, scale)

@@ -1,0 +1,74 @@
+// attn.cuh — what the window-attention kernels share: the mask and the list
+// of key tiles of a query tile (and of query tiles of a key tile).
+#pragma once
+#include "ops_common.cuh"
+
+namespace cailops {
+
+struct AttnArgs {
+    int B, T, H, Hkv, D, group;
+    int window, sinks;
+    float scale, scale_log2;  // scale, scale * log2(e)
+    const int32_t *lengths;
+    const char *q, *k, *v, *dout;
+    char *o, *dq, *dk, *dv;
+    // strides in bytes
+    int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
+    int64_t gb, gt, gh;  // dout
+    int64_t dqb, dqt, dqh, dkb, dkt, dkh, dvb, dvt, dvh;
+    float *lse, *delta;  // [B, H, T]; lse in log2 units of the scaled scores
+    int *error;          // the device's error word (kernels with bounded waits)
+};
+
+// fills everything but D-dependent launch choices; 0 or an error code
+int attn_check(const cail_ops_attention_args *a, bool backward, const char *who);
+AttnArgs attn_args(const cail_ops_attention_args *a, bool backward);
+
+// the tensor-core path (attn_tc_*.cu): whether it takes the call, and the call
+bool tc_takes(const cail_ops_attention_args *a, bool backward);
+int tc_forward(const cail_ops_attention_args *a, cudaStream_t st);
+int tc_backward(const cail_ops_attention_args *a, cudaStream_t st);
+size_t tc_workspace(const cail_ops_attention_args *a);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ bool seen(int i, int j, int n, int window, int sinks) {
+    return i < n && j <= i && (i - j < window || j < sinks);
+}
+
+// A row that sees one key: its probability is 1 whatever the scores, so no
+// gradient reaches q and k through it.  (p (dp - delta) would leave the
+// difference of two roundings where the result is zero.)
+__device__ __forceinline__ bool one_key(int i, int window, int sinks) { return i == 0 || (window == 1 && sinks == 0); }
+
+// The key tiles (of TK keys) that the query rows [i0, i1) of a sequence of n
+// tokens need, in order: [0, sink_end) and [win_begin, win_end).
+struct KeyTiles {
+    int sink_end, win_begin, count;
+    __device__ __forceinline__ KeyTiles(int i0, int i1, int n, int window, int sinks, int tile) {
+        i1 = min(i1, n);
+        if (i0 >= i1) {
+            sink_end = win_begin = count = 0;
+            return;
+        }
+        const int win_end = (i1 - 1) / tile + 1;
+        win_begin = window > i0 ? 0 : (i0 - window + 1) / tile;
+        sink_end = sinks > 0 ? min((min(sinks, n) - 1) / tile + 1, win_begin) : 0;
+        count = sink_end + win_end - win_begin;
+    }
+    __device__ __forceinline__ int at(int x) const { return x < sink_end ? x : x - sink_end + win_begin; }
+};
+
+// The query rows that see some key of [j0, j1): [begin, end)
+__device__ __forceinline__ void query_range(int j0, int j1, int n, int window, int sinks, int &begin, int &end) {
+    begin = j0;
+    const int64_t last = (int64_t)min(j1, n) - 1 + window;  // the last row the window reaches, plus one
+    end = j0 < sinks ? n : (int)min((int64_t)n, last);
+    if (j0 >= n) begin = end = 0;
+}
+
+__device__ __forceinline__ int length_of(const AttnArgs &a, int b) {
+    return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+}
+#endif
+
+}  // namespace cailops

@@ -1,0 +1,405 @@
+// attn_simt.cu — window attention on the FP32 pipes: 32-bit inputs, and head
+// sizes or strides that the tensor-core kernels do not take.
+//
+// Forward: a block owns 64 query rows of one head and goes once over the key
+// tiles that some of them see, with the running maximum and sum of each row
+// (16 threads share a row; each thread holds 4 rows x 4 columns of the scores
+// and 4 rows x D/16 of the output).  Backward: p is recomputed from the kept
+// log-sum; one kernel owns query tiles and writes dq (and delta = do.o), the
+// other owns key tiles, goes over the group's heads and the query tiles that
+// see them, and writes dk and dv.  No atomics: results do not change from run
+// to run.  Rows and keys at or beyond a sequence's length are never read, so
+// what lies there may be anything.  Bound by the FP32 pipe.
+#include "attn.cuh"
+
+namespace cailops {
+namespace {
+
+constexpr int kTile = 64, kThreads = 256;
+constexpr float kNone = -INFINITY;
+
+// rows of shared tiles are DP + 4 floats apart: 16-byte reads of 8 rows in a phase hit different banks
+template <int DP> constexpr int ld() { return DP + 4; }
+constexpr int kLdP = kTile + 4;
+
+// 64 rows of x from row r0 (rows >= n as zeros, columns >= D as zeros), as floats
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(float *s, const char *base, int64_t st, int r0, int n, int D, bool vec, float by) {
+    if (vec) {
+        constexpr int N = 16 / (int)sizeof(T), C = DP / N;
+        for (int i = threadIdx.x; i < kTile * C; i += kThreads) {
+            const int r = i / C, c = (i % C) * N;
+            Vec<T, N> x;
+            const bool in = r0 + r < n && c < D;
+            if (in) x = *reinterpret_cast<const Vec<T, N> *>(base + (int64_t)(r0 + r) * st + c * sizeof(T));
+#pragma unroll
+            for (int k = 0; k < N; ++k) s[r * ld<DP>() + c + k] = in ? to_f(x.v[k]) * by : 0.f;
+        }
+    } else {
+        for (int i = threadIdx.x; i < kTile * DP; i += kThreads) {
+            const int r = i / DP, c = i % DP;
+            const bool in = r0 + r < n && c < D;
+            s[r * ld<DP>() + c] = in ? to_f(*reinterpret_cast<const T *>(base + (int64_t)(r0 + r) * st + c * sizeof(T))) * by : 0.f;
+        }
+    }
+}
+
+// acc[r][c] += sum_d x[ty*4+r][d] * y[tx+16c][d]
+template <int DP> __device__ __forceinline__ void dot_tile(const float *x, const float *y, float acc[4][4], int ty, int tx) {
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+        float4 a[4], b[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4 *>(x + (ty * 4 + r) * ld<DP>() + d);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const float4 *>(y + (tx + 16 * c) * ld<DP>() + d);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                acc[r][c] = fmaf(a[r].x, b[c].x, acc[r][c]);
+                acc[r][c] = fmaf(a[r].y, b[c].y, acc[r][c]);
+                acc[r][c] = fmaf(a[r].z, b[c].z, acc[r][c]);
+                acc[r][c] = fmaf(a[r].w, b[c].w, acc[r][c]);
+            }
+    }
+}
+
+// column c of a thread's DP/16 output columns
+template <int DP> __device__ __forceinline__ int column(int tx, int c) {
+    constexpr int NC = DP / 16;
+    if constexpr (NC <= 4) return tx * NC + c;
+    return (c / 4) * 64 + tx * 4 + c % 4;
+}
+template <int DP> __device__ __forceinline__ void row_of(const float *y, float *w, int tx) {
+    constexpr int NC = DP / 16;
+    if constexpr (NC == 2) {
+        const float2 f = *reinterpret_cast<const float2 *>(y + tx * 2);
+        w[0] = f.x, w[1] = f.y;
+    } else {
+#pragma unroll
+        for (int g = 0; g < NC / 4; ++g) {
+            const float4 f = *reinterpret_cast<const float4 *>(y + g * 64 + tx * 4);
+            w[g * 4] = f.x, w[g * 4 + 1] = f.y, w[g * 4 + 2] = f.z, w[g * 4 + 3] = f.w;
+        }
+    }
+}
+// acc[r][:] += sum_j p[ty*4+r][j] * y[j][:]
+template <int DP> __device__ __forceinline__ void out_tile(const float *p, const float *y, float acc[4][DP / 16], int ty, int tx) {
+    constexpr int NC = DP / 16;
+#pragma unroll 4
+    for (int j = 0; j < kTile; j += 4) {
+        float4 a[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4 *>(p + (ty * 4 + r) * kLdP + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float w[NC];
+            row_of<DP>(y + (j + e) * ld<DP>(), w, tx);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float f = e == 0 ? a[r].x : e == 1 ? a[r].y : e == 2 ? a[r].z : a[r].w;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) acc[r][c] = fmaf(f, w[c], acc[r][c]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float half_max(float x) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+__device__ __forceinline__ float half_sum(float x) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) simt_forward(const AttnArgs a, bool vec) {
+    constexpr int NC = DP / 16;
+    extern __shared__ float4 smem4[];
+    float *sq = reinterpret_cast<float *>(smem4), *sk = sq + kTile * ld<DP>(), *sv = sk + kTile * ld<DP>(), *sp = sv + kTile * ld<DP>();
+    const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
+    const int i0 = (gridDim.x - 1 - blockIdx.x) * kTile;  // the longest rows first
+    const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+    const int n = length_of(a, b);
+    const KeyTiles tiles(i0, i0 + kTile, n, a.window, a.sinks, kTile);
+    const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
+
+    load_tile<T, DP>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec, a.scale_log2);
+    float o[4][NC] = {}, m[4], l[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m[r] = kNone, l[r] = 0.f;
+
+    for (int x = 0; x < tiles.count; ++x) {
+        const int j0 = tiles.at(x) * kTile;
+        __syncthreads();
+        load_tile<T, DP>(sk, kp, a.kt, j0, n, a.D, vec, 1.f);
+        load_tile<T, DP>(sv, vp, a.vt, j0, n, a.D, vec, 1.f);
+        __syncthreads();
+        float s[4][4] = {};
+        dot_tile<DP>(sq, sk, s, ty, tx);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = i0 + ty * 4 + r;
+            float top = kNone;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (!seen(i, j0 + tx + 16 * c, n, a.window, a.sinks)) s[r][c] = kNone;
+                top = fmaxf(top, s[r][c]);
+            }
+            top = fmaxf(m[r], half_max(top));
+            const float base = top == kNone ? 0.f : top, turn = exp2_fast(m[r] - base);
+            m[r] = top;
+            float sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float p = exp2_fast(s[r][c] - base);
+                sum += p;
+                sp[(ty * 4 + r) * kLdP + tx + 16 * c] = p;
+            }
+            l[r] = l[r] * turn + half_sum(sum);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[r][c] *= turn;
+        }
+        __syncwarp();  // a row of p is written and read by one warp
+        out_tile<DP>(sp, sv, o, ty, tx);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int i = i0 + ty * 4 + r;
+        if (i >= a.T) continue;
+        const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+        T *out = reinterpret_cast<T *>(a.o + b * a.ob + (int64_t)i * a.ot + h * a.oh);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = column<DP>(tx, c);
+            if (d < a.D) out[d] = from_f<T>(l[r] == 0.f ? 0.f : o[r][c] * inv);
+        }
+        if (a.lse && tx == 0) a.lse[((int64_t)b * a.H + h) * a.T + i] = l[r] == 0.f ? 0.f : m[r] + log2f(l[r]);
+    }
+}
+
+// dq and delta of 64 query rows
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) simt_dq(const AttnArgs a, bool vec) {
+    constexpr int NC = DP / 16;
+    extern __shared__ float4 smem4[];
+    float *sq = reinterpret_cast<float *>(smem4), *sg = sq + kTile * ld<DP>(), *sk = sg + kTile * ld<DP>(), *sv = sk + kTile * ld<DP>(),
+          *sp = sv + kTile * ld<DP>();
+    const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
+    const int i0 = (gridDim.x - 1 - blockIdx.x) * kTile;
+    const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+    const int n = length_of(a, b);
+    const KeyTiles tiles(i0, i0 + kTile, n, a.window, a.sinks, kTile);
+    const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
+
+    // o passes through the key tile's place
+    load_tile<T, DP>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec, a.scale_log2);
+    load_tile<T, DP>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec, 1.f);
+    load_tile<T, DP>(sk, a.o + b * a.ob + h * a.oh, a.ot, i0, n, a.D, vec, 1.f);
+    __syncthreads();
+    float delta[4], lse[4], dq[4][NC] = {};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int row = ty * 4 + r, i = i0 + row;
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s = fmaf(sg[row * ld<DP>() + tx + 16 * c], sk[row * ld<DP>() + tx + 16 * c], s);
+        delta[r] = half_sum(s);
+        const int64_t at = ((int64_t)b * a.H + h) * a.T + i;
+        lse[r] = i < n ? a.lse[at] : 0.f;
+        if (i < a.T && tx == 0) a.delta[at] = delta[r];
+    }
+    for (int x = 0; x < tiles.count; ++x) {
+        const int j0 = tiles.at(x) * kTile;
+        __syncthreads();
+        load_tile<T, DP>(sk, kp, a.kt, j0, n, a.D, vec, 1.f);
+        load_tile<T, DP>(sv, vp, a.vt, j0, n, a.D, vec, 1.f);
+        __syncthreads();
+        float s[4][4] = {}, dp[4][4] = {};
+        dot_tile<DP>(sq, sk, s, ty, tx);
+        dot_tile<DP>(sg, sv, dp, ty, tx);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int i = i0 + ty * 4 + r;
+                const bool on = seen(i, j0 + tx + 16 * c, n, a.window, a.sinks) && !one_key(i, a.window, a.sinks);
+                sp[(ty * 4 + r) * kLdP + tx + 16 * c] = on ? exp2_fast(s[r][c] - lse[r]) * (dp[r][c] - delta[r]) : 0.f;
+            }
+        __syncwarp();
+        out_tile<DP>(sp, sk, dq, ty, tx);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int i = i0 + ty * 4 + r;
+        if (i >= a.T) continue;
+        T *out = reinterpret_cast<T *>(a.dq + b * a.dqb + (int64_t)i * a.dqt + h * a.dqh);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = column<DP>(tx, c);
+            if (d < a.D) out[d] = from_f<T>(dq[r][c] * a.scale);
+        }
+    }
+}
+
+// dk and dv of 64 keys, over the group's heads and the query rows that see them
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) simt_dkv(const AttnArgs a, bool vec) {
+    constexpr int NC = DP / 16;
+    extern __shared__ float4 smem4[];
+    float *sk = reinterpret_cast<float *>(smem4), *sv = sk + kTile * ld<DP>(), *sq = sv + kTile * ld<DP>(), *sg = sq + kTile * ld<DP>(),
+          *sp = sg + kTile * ld<DP>(), *sd = sp + kTile * kLdP;
+    __shared__ float row_lse[kTile], row_delta[kTile];
+    const int hk = blockIdx.y, b = blockIdx.z;
+    const int j0 = blockIdx.x * kTile;
+    const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+    const int n = length_of(a, b);
+    int begin, end;
+    query_range(j0, j0 + kTile, n, a.window, a.sinks, begin, end);
+    load_tile<T, DP>(sk, a.k + b * a.kb + hk * a.kh, a.kt, j0, n, a.D, vec, a.scale_log2);
+    load_tile<T, DP>(sv, a.v + b * a.vb + hk * a.vh, a.vt, j0, n, a.D, vec, 1.f);
+    float dk[4][NC] = {}, dv[4][NC] = {};
+    for (int h = hk * a.group; h < (hk + 1) * a.group; ++h)
+        for (int i0 = begin / kTile * kTile; i0 < end; i0 += kTile) {
+            __syncthreads();
+            load_tile<T, DP>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec, 1.f);
+            load_tile<T, DP>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec, 1.f);
+            if (tid < kTile) {
+                const int64_t at = ((int64_t)b * a.H + h) * a.T + i0 + tid;
+                row_lse[tid] = i0 + tid < n ? a.lse[at] : 0.f;
+                row_delta[tid] = i0 + tid < n ? a.delta[at] : 0.f;
+            }
+            __syncthreads();
+            float s[4][4] = {}, dp[4][4] = {};
+            dot_tile<DP>(sk, sq, s, ty, tx);
+            dot_tile<DP>(sv, sg, dp, ty, tx);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int i = tx + 16 * c;
+                    const bool on = seen(i0 + i, j0 + ty * 4 + r, n, a.window, a.sinks);
+                    const float p = on ? exp2_fast(s[r][c] - row_lse[i]) : 0.f;
+                    sp[(ty * 4 + r) * kLdP + i] = p;
+                    sd[(ty * 4 + r) * kLdP + i] = on && !one_key(i0 + i, a.window, a.sinks) ? p * (dp[r][c] - row_delta[i]) : 0.f;
+                }
+            __syncwarp();
+            out_tile<DP>(sp, sg, dv, ty, tx);
+            out_tile<DP>(sd, sq, dk, ty, tx);
+        }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int j = j0 + ty * 4 + r;
+        if (j >= a.T) continue;
+        T *ok = reinterpret_cast<T *>(a.dk + b * a.dkb + (int64_t)j * a.dkt + hk * a.dkh);
+        T *ov = reinterpret_cast<T *>(a.dv + b * a.dvb + (int64_t)j * a.dvt + hk * a.dvh);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = column<DP>(tx, c);
+            if (d < a.D) ok[d] = from_f<T>(dk[r][c] * a.scale), ov[d] = from_f<T>(dv[r][c]);
+        }
+    }
+}
+
+template <typename K> int prepare(K kernel, size_t smem) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    return e == cudaSuccess ? CAIL_OPS_OK : fail(CAIL_OPS_ECUDA, "window attention: %s", cudaGetErrorString(e));
+}
+
+template <typename T, int DP> int forward(const AttnArgs &a, bool vec, cudaStream_t st) {
+    const size_t smem = (3 * kTile * ld<DP>() + kTile * kLdP) * sizeof(float);
+    if (int rc = prepare(simt_forward<T, DP>, smem)) return rc;
+    simt_forward<T, DP><<<dim3((a.T + kTile - 1) / kTile, a.H, a.B), kThreads, smem, st>>>(a, vec);
+    return launched("window attention");
+}
+template <typename T, int DP> int backward(const AttnArgs &a, bool vec, cudaStream_t st) {
+    const unsigned tiles = (a.T + kTile - 1) / kTile;
+    size_t smem = (4 * kTile * ld<DP>() + kTile * kLdP) * sizeof(float);
+    if (int rc = prepare(simt_dq<T, DP>, smem)) return rc;
+    simt_dq<T, DP><<<dim3(tiles, a.H, a.B), kThreads, smem, st>>>(a, vec);
+    if (int rc = launched("window attention backward")) return rc;
+    smem += kTile * kLdP * sizeof(float);
+    if (int rc = prepare(simt_dkv<T, DP>, smem)) return rc;
+    simt_dkv<T, DP><<<dim3(tiles, a.Hkv, a.B), kThreads, smem, st>>>(a, vec);
+    return launched("window attention backward");
+}
+template <typename T> int run(const AttnArgs &a, bool vec, bool back, cudaStream_t st) {
+    if (a.D <= 32) return back ? backward<T, 32>(a, vec, st) : forward<T, 32>(a, vec, st);
+    if (a.D <= 64) return back ? backward<T, 64>(a, vec, st) : forward<T, 64>(a, vec, st);
+    return back ? backward<T, 128>(a, vec, st) : forward<T, 128>(a, vec, st);
+}
+
+}  // namespace
+
+int attn_check(const cail_ops_attention_args *a, bool backward, const char *who) {
+    if (a->type < CAIL_OPS_F32 || a->type > CAIL_OPS_F16) return fail(CAIL_OPS_EINVAL, "%s: unknown element type %d", who, a->type);
+    if (a->B < 0 || a->T < 0 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv || a->D < 1 || a->D > 128)
+        return fail(CAIL_OPS_EINVAL, "%s: bad sizes (B %d T %d H %d Hkv %d D %d)", who, a->B, a->T, a->H, a->Hkv, a->D);
+    if (a->B > 65535 || a->H > 65535) return fail(CAIL_OPS_EINVAL, "%s: at most 65535 sequences and heads", who);
+    if (a->T > (1 << 30)) return fail(CAIL_OPS_EINVAL, "%s: at most 2^30 tokens", who);
+    if (a->window < 1 || a->sinks < 0) return fail(CAIL_OPS_EINVAL, "%s: window %d and sinks %d", who, a->window, a->sinks);
+    if (backward && (!a->lse || !a->delta)) return fail(CAIL_OPS_EINVAL, "%s: lse and delta are needed", who);
+    return CAIL_OPS_OK;
+}
+
+AttnArgs attn_args(const cail_ops_attention_args *a, bool backward) {
+    const int64_t s = (int64_t)type_size(a->type);
+    AttnArgs x = {};
+    x.B = a->B, x.T = a->T, x.H = a->H, x.Hkv = a->Hkv, x.D = a->D, x.group = a->H / a->Hkv;
+    x.window = a->window, x.sinks = a->sinks;
+    x.scale = a->scale, x.scale_log2 = a->scale * kLog2e;
+    x.lengths = a->lengths;
+    x.q = static_cast<const char *>(a->q.ptr), x.qb = a->q.sb * s, x.qt = a->q.st * s, x.qh = a->q.sh * s;
+    x.k = static_cast<const char *>(a->k.ptr), x.kb = a->k.sb * s, x.kt = a->k.st * s, x.kh = a->k.sh * s;
+    x.v = static_cast<const char *>(a->v.ptr), x.vb = a->v.sb * s, x.vt = a->v.st * s, x.vh = a->v.sh * s;
+    x.o = static_cast<char *>(a->o.ptr), x.ob = a->o.sb * s, x.ot = a->o.st * s, x.oh = a->o.sh * s;
+    x.lse = a->lse;
+    if (backward) {
+        x.dout = static_cast<const char *>(a->dout.ptr), x.gb = a->dout.sb * s, x.gt = a->dout.st * s, x.gh = a->dout.sh * s;
+        x.dq = static_cast<char *>(a->dq.ptr), x.dqb = a->dq.sb * s, x.dqt = a->dq.st * s, x.dqh = a->dq.sh * s;
+        x.dk = static_cast<char *>(a->dk.ptr), x.dkb = a->dk.sb * s, x.dkt = a->dk.st * s, x.dkh = a->dk.sh * s;
+        x.dv = static_cast<char *>(a->dv.ptr), x.dvb = a->dv.sb * s, x.dvt = a->dv.st * s, x.dvh = a->dv.sh * s;
+        x.delta = a->delta;
+    }
+    return x;
+}
+
+}  // namespace cailops
+
+using namespace cailops;
+
+static bool attn_vectors(const cail_ops_attention_args *a, bool backward) {
+    const size_t s = type_size(a->type);
+    return a->D % (16 / s) == 0 && rows_aligned(a->q, a->B, a->T, a->H, s, 16) && rows_aligned(a->k, a->B, a->T, a->Hkv, s, 16) &&
+           rows_aligned(a->v, a->B, a->T, a->Hkv, s, 16) &&
+           (!backward || (rows_aligned(a->o, a->B, a->T, a->H, s, 16) && rows_aligned(a->dout, a->B, a->T, a->H, s, 16)));
+}
+
+extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_ops_stream stream) {
+    if (int rc = attn_check(a, false, "window attention")) return rc;
+    if (a->B == 0 || a->T == 0) return CAIL_OPS_OK;
+    auto st = static_cast<cudaStream_t>(stream);
+    const AttnArgs x = attn_args(a, false);
+    const bool vec = attn_vectors(a, false);
+    if (a->type == CAIL_OPS_F32) return run<float>(x, vec, false, st);
+    if (a->type == CAIL_OPS_BF16) return run<__nv_bfloat16>(x, vec, false, st);
+    return run<__half>(x, vec, false, st);
+}
+
+extern "C" size_t cail_ops_window_attention_workspace(const cail_ops_attention_args *a) { return 0; }
+
+extern "C" int cail_ops_window_attention_backward(const cail_ops_attention_args *a, cail_ops_stream stream) {
+    if (int rc = attn_check(a, true, "window attention backward")) return rc;
+    if (a->B == 0 || a->T == 0) return CAIL_OPS_OK;
+    auto st = static_cast<cudaStream_t>(stream);
+    const AttnArgs x = attn_args(a, true);
+    const bool vec = attn_vectors(a, true);
+    if (a->type == CAIL_OPS_F32) return run<float>(x, vec, true, st);
+    if (a->type == CAIL_OPS_BF16) return run<__nv_bfloat16>(x, vec, true, st);
+    return run<__half>(x, vec, true, st);
+}

@@ -1,0 +1,76 @@
+// ops_common.cuh — what the language-model kernels share: element types,
+// 16-byte vectors, warp reductions, error text and launch accounting.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cail_ops.h"
+
+namespace cailops {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// ------------------------------------------------------------------- host
+int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+int launched(const char *what);  // after a launch: counts it, reports a launch error
+int sm_count();                  // of the current device (0: no device)
+int *device_error_flag();        // device address of the current device's error word (nullptr: none could be made)
+
+inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+inline size_t type_size(int type) { return type == CAIL_OPS_F32 ? 4 : 2; }
+
+// whether rows of a [B, T, H, D] array start on multiples of `bytes`
+inline bool rows_aligned(const cail_ops_bthd &x, int B, int T, int H, size_t size, size_t bytes) {
+    return aligned(x.ptr, bytes) && (B == 1 || (x.sb * (int64_t)size) % (int64_t)bytes == 0) &&
+           (T == 1 || (x.st * (int64_t)size) % (int64_t)bytes == 0) &&
+           (H == 1 || (x.sh * (int64_t)size) % (int64_t)bytes == 0);
+}
+
+#ifdef __CUDACC__
+// ----------------------------------------------------------------- device
+template <typename T> __device__ __forceinline__ float to_f(T x);
+template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+
+// N elements of T as one aligned load or store
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+
+// two floats packed as T2 (first in the low half)
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+#endif
+
+}  // namespace cailops

@@ -1,0 +1,819 @@
+"""Window attention, rotary positions and distillation against plain 64-bit
+forms (tests/lm_reference.py), and their refusals.
+
+Tolerances, as 2-norms relative to the wanted result.  u is half a step of
+the type (bf16 2^-8 ... as torch.finfo(t).eps / 2), e = 2^-24 that of float32.
+
+* Rotary: one rounding of each output (u) after two products and a sum in 32
+  bits of a sine and cosine good to 4 e: at most u + 8 e.
+* Attention forward: the output's rounding (u), and the probabilities'
+  rounding to the type before the second product (at most u relative to each
+  term).  Terms of either sign: the error's 2-norm is at most u times the norm
+  of p |v|, which for values of independent sign is of the order of the
+  output's own norm; 32-bit sums add e times the number of terms' root.  Bound
+  used: 3 u + 64 e (64 e: scores of up to |s| = 32 carry s e each in the
+  exponent, and sums of up to a few hundred terms).
+* Attention gradients: the same two roundings, and ds = p (dp - delta) is
+  rounded where it enters a product, where dp - delta cancels partly (the
+  norm of ds is kept by its terms, so u stays relative to them): 5 u + 256 e.
+* Distillation: loss in 32 bits, of at most 16 e |z| / tau for the exponents
+  and 8 e for sums and logarithms: 2e-6 on losses of the order of 1 to 10.
+  Gradient: one rounding u, and 64 e from exponents of up to 32.
+"""
+import random
+
+import pytest
+import torch
+
+import lm_reference as ref
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+E = 2.0 ** -24
+
+
+def ids_of(t):
+    return str(t).replace("torch.", "")
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32, by=1.0):
+    return (torch.randn(*shape, generator=g, dtype=torch.float64) * by).to(dtype).cuda()
+
+
+def ops():
+    from cail_b200 import ops as o
+
+    return o
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built(build):
+    from cail_b200.ops import ext
+
+    ext.build_ops()
+
+
+# ------------------------------------------------------------ refusals (CPU)
+
+
+def test_rotary_plan_refuses():
+    R = ops().Rotary
+    for kw in (dict(dim=3), dict(dim=0), dict(dim=64, base=0.0), dict(dim=64, factor=0.0), dict(dim=64, scaling="other"),
+               dict(dim=2, scaling="ntk", factor=2.0), dict(dim=64, scaling="parts", factor=2.0),
+               dict(dim=64, scaling="parts", factor=2.0, original=8, fast=1.0, slow=1.0)):
+        with pytest.raises(ValueError):
+            R(device="cpu", **kw)
+
+
+def test_rotary_refuses():
+    o = ops()
+    plan = o.Rotary(8, device="cpu")
+    q = torch.zeros(2, 3, 4, 8)
+    bad = [
+        (ValueError, (q[0], None)), (ValueError, (torch.zeros(2, 3, 4, 6), None)), (ValueError, (q, torch.zeros(2, 2, 4, 8))),
+        (TypeError, (q, q.half())), (TypeError, (q.double(), None)), (ValueError, (q, None, torch.zeros(2, dtype=torch.int64))),
+        (TypeError, (q, None, torch.zeros(3))), (ValueError, (q, None, torch.zeros(2, 4, dtype=torch.int32))),
+        (ValueError, (torch.zeros(1, 1, 1, 1026), None)),
+    ]
+    for kind, args in bad:
+        with pytest.raises(kind):
+            o.rotary(args[0], args[1], plan, *args[2:])
+        with pytest.raises(kind):
+            o.rotary_(args[0], args[1], plan, *args[2:])
+    with pytest.raises(ValueError, match="CUDA"):
+        o.rotary(q, None, plan)
+    with pytest.raises(ValueError, match="gradient"):
+        o.rotary_(q.clone().requires_grad_(), None, plan)
+    with pytest.raises(ValueError, match="share memory"):
+        o.rotary_(q, q, plan)
+    with pytest.raises(ValueError, match="share memory"):
+        o.rotary_(torch.zeros(1, 3, 4, 8).expand(2, 3, 4, 8), None, plan)
+    with pytest.raises(ValueError, match="side by side"):
+        o.rotary_(torch.zeros(2, 3, 8, 4).transpose(2, 3), None, plan)
+
+
+def test_window_attention_refuses():
+    o = ops()
+    q, k = torch.zeros(2, 5, 4, 8), torch.zeros(2, 5, 2, 8)
+    n = torch.zeros(2, dtype=torch.int32)
+    bad = [
+        (ValueError, (q[0], k, k, 4)), (ValueError, (q, k[:, :4], k[:, :4], 4)), (ValueError, (q, k, k[:, :, :1], 4)),
+        (ValueError, (q, torch.zeros(2, 5, 3, 8), torch.zeros(2, 5, 3, 8), 4)), (ValueError, (q, k[:, :, :0], k[:, :, :0], 4)),
+        (ValueError, (torch.zeros(2, 5, 4, 136), torch.zeros(2, 5, 2, 136), torch.zeros(2, 5, 2, 136), 4)),
+        (ValueError, (q, k, k, 0)), (ValueError, (q, k, k, -1)), (ValueError, (q, k, k, 4, -1)),
+        (TypeError, (q, k.half(), k, 4)), (TypeError, (q.double(), k.double(), k.double(), 4)),
+        (TypeError, (q, k, k, 4, 0, n.long())), (ValueError, (q, k, k, 4, 0, n[:1])),
+        (ValueError, (q, k, k, 4, 0, None, float("nan"))), (ValueError, (q, k, k, 4)),
+    ]
+    for kind, args in bad:
+        with pytest.raises(kind):
+            o.window_attention(*args)
+    with pytest.raises(ValueError, match="CUDA"):
+        o.window_attention(q, k, k, 4)
+    one = torch.zeros(2, 4, 8)
+    for kind, args in [
+        (ValueError, (q, k, k, n, 4)), (ValueError, (one, k, k[:1], n, 4)), (TypeError, (one, k, k, n.long(), 4)),
+        (ValueError, (one, k, k, n, 0)), (ValueError, (one.clone().requires_grad_(), k, k, n, 4)), (ValueError, (one, k, k, n, 4)),
+    ]:
+        with pytest.raises(kind):
+            o.window_attention_decode(*args)
+
+
+def test_distill_loss_refuses():
+    o = ops()
+    z, ids, t, y = torch.zeros(3, 11), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2), torch.zeros(3, dtype=torch.int64)
+    bad = [
+        (ValueError, dict(logits=z[0])), (ValueError, dict(teacher_ids=ids[:2])), (ValueError, dict(teacher_logits=t[:, :1])),
+        (TypeError, dict(teacher_ids=t)), (TypeError, dict(logits=z.double())), (TypeError, dict(teacher_logits=t.double())),
+        (ValueError, dict(targets=y[:2])), (TypeError, dict(targets=y.float())), (ValueError, dict(temperature=0.0)),
+        (ValueError, dict(temperature=float("inf"))), (ValueError, dict(temperature=1e-45)), (ValueError, dict(hard_weight=1.5)),
+        (ValueError, dict(hard_weight=0.5)), (ValueError, dict(reduction="median")),
+        (ValueError, dict(teacher_logits=t.clone().requires_grad_())),
+        (ValueError, dict(teacher_ids=torch.zeros(3, 1025, dtype=torch.int64), teacher_logits=torch.zeros(3, 1025))),
+        (ValueError, dict(logits=torch.zeros(3, 0))),
+    ]
+    for kind, kw in bad:
+        with pytest.raises(kind):
+            o.distill_loss(**{**dict(logits=z, teacher_ids=ids, teacher_logits=t), **kw})
+    with pytest.raises(ValueError, match="CUDA"):
+        o.distill_loss(z, ids, t)
+
+
+def test_c_entries_refuse_without_touching_a_device():
+    """Bad sizes come back as CAIL_OPS_EINVAL with a text, before any CUDA call."""
+    import ctypes
+    import os
+
+    from conftest import LIB
+
+    lib = ctypes.CDLL(os.path.join(LIB, "libcail_ops.so"))
+    lib.cail_ops_last_error.restype = ctypes.c_char_p
+    zero = (ctypes.c_char * 1024)()
+    for name in ("cail_ops_window_attention", "cail_ops_window_attention_backward", "cail_ops_window_attention_decode",
+                 "cail_ops_distill", "cail_ops_distill_backward", "cail_ops_rotary"):
+        assert getattr(lib, name)(ctypes.byref(zero), None) == 1, name
+        assert lib.cail_ops_last_error() != b""
+
+
+# -------------------------------------------------------------------- rotary
+
+SCALINGS = [dict(), dict(scaling="linear", factor=8.0), dict(scaling="ntk", factor=4.0), dict(scaling="parts", factor=16.0, original=2048)]
+
+
+def freqs(dim, base=10000.0, scaling=None, factor=1.0, original=0, fast=32.0, slow=1.0):
+    import math
+
+    if scaling == "ntk":
+        base *= factor ** (dim / (dim - 2))
+    f = [base ** (-2 * i / dim) for i in range(dim // 2)]
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    if scaling == "parts":
+        out = []
+        for x in f:
+            turns = original * x / (2 * math.pi)
+            w = min(1.0, max(0.0, (turns - slow) / (fast - slow)))
+            out.append(x * w + x / factor * (1 - w))
+        f = out
+    return f, (0.1 * math.log(factor) + 1 if scaling == "parts" else 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("inter", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("B,T,H,Hk,D,part", [(1, 1, 1, 1, 2, 2), (2, 7, 3, 1, 64, 64), (3, 130, 4, 2, 80, 20), (1, 33, 2, 2, 128, 64),
+                                             (2, 5, 5, 3, 17, 6), (1, 3, 40, 8, 1024, 1024), (2, 1, 7, 7, 40, 38)])
+def test_rotary_matches_64_bit(dtype, inter, B, T, H, Hk, D, part):
+    o = ops()
+    g = gen(B * 100 + D)
+    for n, how in enumerate(SCALINGS):
+        if how.get("scaling") == "ntk" and part < 4:
+            continue
+        plan = o.Rotary(part, interleaved=inter, **how)
+        f, amp = freqs(part, **how)
+        q, k = randn(g, B, T, H, D, dtype=dtype), randn(g, B, T, Hk, D, dtype=dtype)
+        pos = [None, torch.randint(0, 10 ** 6, (T,), generator=g).cuda(), torch.randint(-50, 300000, (B, T), generator=g).int().cuda(),
+               torch.arange(T).cuda() + 2 ** 31][n]
+        at = torch.arange(T).cuda() if pos is None else pos
+        at = at.expand(B, T) if at.dim() == 1 else at
+        q.requires_grad_(), k.requires_grad_()
+        qo, ko = o.rotary(q, k, plan, pos)
+        gq, gk = randn(g, B, T, H, D, dtype=dtype), randn(g, B, T, Hk, D, dtype=dtype)
+        dq, dk = torch.autograd.grad((qo, ko), (q, k), (gq, gk))
+        tol = ref.half_step(dtype) + 8 * E
+        for got, x, inv in ((qo, q, False), (ko, k, False), (dq, gq, True), (dk, gk, True)):
+            want = ref.rotate(x.detach(), at, f, amp, inter, inv)
+            assert got.dtype == dtype and got.is_contiguous()
+            assert ref.rel(got, want) <= tol, (how, inv)
+        with torch.no_grad():
+            q2, k2 = q.detach().clone(), k.detach().clone()
+            a, b = o.rotary_(q2, k2, plan, pos)
+            assert a is q2 and torch.equal(q2, qo) and torch.equal(k2, ko)
+            assert torch.equal(o.rotary(q2, None, plan, pos), o.rotary(q2, k2, plan, pos)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inter", [False, True], ids=["half", "interleaved"])
+def test_rotary_strides(inter):
+    """q and k as parts of one projection, heads before tokens, elements apart,
+    rows on odd addresses, expanded gradients."""
+    o = ops()
+    g = gen(5)
+    plan = o.Rotary(16, interleaved=inter)
+    f, amp = freqs(16)
+    at = torch.arange(6).cuda().expand(2, 6)
+    tol = ref.half_step(torch.bfloat16) + 8 * E
+    fused = randn(g, 2, 6, 3 * 4 * 20, dtype=torch.bfloat16)
+    q, k = (x.view(2, 6, 4, 20) for x in fused.split(80, 2)[:2])
+    flat = randn(g, 2 * 6 * 4 * 20 + 1, dtype=torch.bfloat16)
+    odd = flat[1:].view(2, 6, 4, 20)
+    for x in (q, k, q.transpose(1, 2).contiguous().transpose(1, 2), odd, randn(g, 2, 6, 20, 4, dtype=torch.bfloat16).transpose(2, 3),
+              randn(g, 2, 6, 1, 20, dtype=torch.bfloat16).expand(2, 6, 4, 20)):
+        assert ref.rel(o.rotary(x, None, plan), ref.rotate(x, at, f, amp, inter)) <= tol
+    want = ref.rotate(q, at, f, amp, inter), ref.rotate(k, at, f, amp, inter)
+    rest = fused[:, :, 160:].clone()
+    o.rotary_(q, k, plan)  # in place on parts of one tensor; the rest of it stays
+    assert ref.rel(q, want[0]) <= tol and ref.rel(k, want[1]) <= tol and torch.equal(fused[:, :, 160:], rest)
+    x = randn(g, 2, 6, 4, 20).requires_grad_()
+    o.rotary(x, None, plan).sum().backward()
+    assert ref.rel(x.grad, ref.rotate(torch.ones_like(x), at, f, amp, inter, True)) <= 16 * E
+
+
+@pytest.mark.gpu
+def test_rotary_empty_and_second_derivative():
+    o = ops()
+    plan = o.Rotary(4)
+    assert o.rotary(torch.zeros(0, 3, 2, 4).cuda(), torch.zeros(0, 3, 1, 4).cuda(), plan)[0].shape == (0, 3, 2, 4)
+    assert o.rotary(torch.zeros(2, 0, 2, 4).cuda(), None, plan).shape == (2, 0, 2, 4)
+    x = randn(gen(1), 1, 3, 2, 6).requires_grad_()
+    y = o.rotary(x, None, plan)
+    (d,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)  # 2 x on the rotation: turned there and back
+    (dd,) = torch.autograd.grad(d.sum(), x)
+    assert ref.rel(dd, torch.full_like(x, 2.0)) <= 32 * E
+
+
+# ----------------------------------------------------------------- attention
+
+# B, T, H, Hkv, D, window, sinks, lengths
+ATTENTION = [
+    (1, 1, 1, 1, 64, 1, 0, None),
+    (2, 5, 2, 1, 16, 2, 1, [5, 0]),
+    (1, 63, 2, 2, 33, 7, 3, None),
+    (2, 64, 2, 1, 64, 64, 0, [64, 1]),
+    (1, 65, 3, 3, 80, 1, 0, None),
+    (1, 128, 2, 2, 128, 200, 5, None),
+    (2, 129, 4, 2, 64, 33, 70, [129, 65]),
+    (1, 200, 4, 1, 128, 64, 0, None),
+    (3, 257, 2, 2, 72, 100, 130, [257, 128, 129]),
+    (1, 511, 8, 2, 64, 128, 4, [500]),
+    (1, 700, 2, 1, 128, 1000, 0, [699]),
+    (2, 640, 2, 2, 8, 250, 1000, [640, 3]),
+    (1, 1100, 1, 1, 64, 300, 260, None),
+]
+
+
+def attention_inputs(case, dtype, seed=0, by=1.0):
+    B, T, H, Hkv, D, window, sinks, lengths = case
+    g = gen(seed + T)
+    q, k, v, do = (randn(g, B, T, h, D, dtype=dtype, by=by) for h in (H, Hkv, Hkv, H))
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32).cuda()
+    return q, k, v, do, n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("case", ATTENTION, ids=str)
+def test_window_attention_matches_64_bit(dtype, case):
+    o = ops()
+    window, sinks = case[5:7]
+    q, k, v, do, n = attention_inputs(case, dtype)
+    with torch.no_grad():
+        plain = o.window_attention(q, k, v, window, sinks, lengths=n)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    out = o.window_attention(*leaves, window, sinks, lengths=n)
+    assert torch.equal(out, plain)
+    grads = torch.autograd.grad(out, leaves, do)
+    r = [x.double().requires_grad_() for x in (q, k, v)]
+    want = ref.attention(*r, window, sinks, n)
+    dwant = torch.autograd.grad(want, r, do.double())
+    u = ref.half_step(dtype)
+    assert out.dtype == dtype and out.is_contiguous()
+    assert ref.rel(out, want) <= 3 * u + 64 * E
+    for name, got, w in zip("qkv", grads, dwant):
+        assert got.dtype == dtype
+        assert ref.rel(got, w) <= 5 * u + 256 * E, "d" + name
+    if n is not None:  # rows behind a sequence: exact zeros
+        for b, m in enumerate(n.tolist()):
+            for x in (out, *grads):
+                assert not x[b, m:].any()
+    again = torch.autograd.grad(o.window_attention(*leaves, window, sinks, lengths=n), leaves, do)
+    assert all(torch.equal(x, y) for x, y in zip(grads, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+def test_window_attention_ignores_what_lies_behind(dtype):
+    """NaN and infinity behind a sequence's length reach no output."""
+    o = ops()
+    for D in (64, 128, 33):
+        case = (2, 200, 4, 2, D, 70, 5, [131, 64])
+        q, k, v, do, n = attention_inputs(case, dtype)
+        clean = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = o.window_attention(*clean, 70, 5, lengths=n)
+        want = torch.autograd.grad(out, clean, do)
+        dirty = [x.clone() for x in (q, k, v, do)]
+        for x in dirty:
+            for b, m in enumerate(n.tolist()):
+                x[b, m:] = float("nan")
+                x[b, m + 3:m + 9] = float("inf")
+                x[b, m + 11:] = torch.finfo(dtype).min
+        leaves = [x.requires_grad_() for x in dirty[:3]]
+        got_out = o.window_attention(*leaves, 70, 5, lengths=n)
+        got = torch.autograd.grad(got_out, leaves, dirty[3])
+        assert torch.equal(got_out, out)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+def test_window_attention_strides(dtype):
+    """Parts of one projection, heads before tokens, elements apart, rows off
+    16-byte addresses, broadcast keys and gradients."""
+    o = ops()
+    B, T, H, D = 2, 150, 4, 64
+    g = gen(9)
+    u = ref.half_step(dtype)
+    fused = randn(g, B, T, 3 * H * D, dtype=dtype)
+    q, k, v = (x.view(B, T, H, D) for x in fused.split(H * D, 2))
+    off = randn(g, B * T * H * D + 1, dtype=dtype)[1:].view(B, T, H, D)
+    bhtd = randn(g, B, H, T, D, dtype=dtype).transpose(1, 2)
+    apart = randn(g, B, T, D, H, dtype=dtype).transpose(2, 3)
+    wide = randn(g, B, T, H, D + 4, dtype=dtype)[..., :D]
+    shared = randn(g, 1, T, H, D, dtype=dtype).expand(B, T, H, D)
+    one_head = randn(g, B, T, 1, D, dtype=dtype).expand(B, T, H, D)
+    back = randn(g, B, T, H, D, dtype=dtype)
+    for x, y, z in ((q, k, v), (off, bhtd, apart), (bhtd, off, wide), (wide, shared, one_head), (one_head, apart, shared)):
+        leaves = [t.detach().requires_grad_() for t in (x, y, z)]
+        for do in (back, back[:, :, :1].expand(B, T, H, D), back.transpose(1, 2).contiguous().transpose(1, 2)):
+            out = o.window_attention(*leaves, 40, 3)
+            grads = torch.autograd.grad(out, leaves, do)
+            r = [t.detach().double().requires_grad_() for t in (x, y, z)]
+            want = ref.attention(*r, 40, 3)
+            dwant = torch.autograd.grad(want, r, do.double())
+            assert ref.rel(out, want) <= 3 * u + 64 * E
+            for got, w in zip(grads, dwant):
+                assert ref.rel(got, w) <= 5 * u + 256 * E
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("by", [1e-4, 30.0])
+def test_window_attention_small_and_large_gradients(dtype, by):
+    """Output gradients far from 1 keep their relative accuracy (in 16 bits the
+    products' operands are scaled where the type's range is short).  float16
+    gradients of 1e-4 are themselves held to 2^-25 / 1e-4 of their size, inputs
+    here, and dq, dk and dv of that size to the same: 2^-24 absolute on values
+    whose root mean square is rms adds 2^-25 / rms."""
+    o = ops()
+    case = (1, 300, 2, 1, 64, 120, 4, None)
+    q, k, v, do, _ = attention_inputs(case, dtype)
+    do = (do.float() * by).to(dtype)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(o.window_attention(*leaves, 120, 4), leaves, do)
+    r = [x.detach().double().requires_grad_() for x in leaves]
+    dwant = torch.autograd.grad(ref.attention(*r, 120, 4), r, do.double())
+    for got, w in zip(grads, dwant):
+        floor = 2.0 ** -25 / float(w.square().mean().sqrt()) if dtype == torch.float16 else 0.0
+        assert ref.rel(got, w) <= 5 * ref.half_step(dtype) + 256 * E + floor
+
+
+@pytest.mark.gpu
+def test_window_attention_against_differences():
+    """The float32 gradients against central differences of the 64-bit form
+    along random directions: a step of 1e-5 leaves 1e-9 of the differences'
+    own error, far below the 256 e of the gradients (relative to the norm of
+    gradient times direction)."""
+    o = ops()
+    case = (2, 37, 4, 2, 16, 9, 2, [37, 20])
+    q, k, v, do, n = attention_inputs(case, torch.float32)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(o.window_attention(*leaves, 9, 2, lengths=n), leaves, do)
+    g = gen(3)
+    for at in range(3):
+        base = [x.detach().double() for x in leaves]
+        d = randn(g, *base[at].shape).double()
+        f = []
+        for h in (1e-5, -1e-5):
+            moved = list(base)
+            moved[at] = base[at] + h * d
+            f.append(float((ref.attention(*moved, 9, 2, n) * do.double()).sum()))
+        slope = (f[0] - f[1]) / 2e-5
+        got = float((grads[at].double() * d).sum())
+        assert abs(got - slope) <= 256 * E * float(grads[at].norm() * d.norm())
+
+
+@pytest.mark.gpu
+def test_window_attention_extreme_scores():
+    """Scores of several hundred: one key takes all, no overflow; scores of
+    -inf from finite inputs' overflow do not occur in 32 bits."""
+    o = ops()
+    for dtype in TYPES:
+        case = (1, 200, 2, 2, 64, 90, 2, None)
+        q, k, v, do, _ = attention_inputs(case, dtype, by=8.0)
+        v, do = v / 8, do / 8
+        out = o.window_attention(q, k, v, 90, 2)
+        # scores of up to |s| = 64 * 8 * 8 * 4 / 8 = 1024 carry s * 2e in the exponent
+        assert ref.rel(out, ref.attention(q, k, v, 90, 2)) <= 3 * ref.half_step(dtype) + 2048 * 2 * E
+
+
+@pytest.mark.gpu
+def test_window_attention_empty():
+    o = ops()
+    for shape in ((0, 4, 2, 8), (2, 0, 2, 8)):
+        x = torch.zeros(*shape).cuda().requires_grad_()
+        out = o.window_attention(x, x, x, 3)
+        assert out.shape == shape
+        assert torch.autograd.grad(out, x, torch.zeros_like(out))[0].shape == shape
+    x = torch.zeros(2, 5, 2, 8).cuda().requires_grad_()
+    out = o.window_attention(x, x, x, 3, lengths=torch.tensor([-4, 99], dtype=torch.int32).cuda())
+    assert not out.any()
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+DECODE = [
+    # B, T, H, Hkv, D, window, sinks, lengths
+    (1, 1, 1, 1, 16, 1, 0, [1]),
+    (3, 9, 2, 2, 64, 4, 2, [9, 0, 1]),
+    (2, 300, 6, 2, 64, 100, 5, [300, 99]),
+    (2, 300, 4, 1, 128, 1000, 0, [300, 257]),
+    (1, 2000, 16, 2, 128, 1500, 130, [1999]),
+    (4, 70, 5, 1, 33, 16, 3, [70, 17, 16, 2]),
+    (2, 130, 9, 1, 80, 64, 300, [130, 128]),
+    (1, 5000, 1, 1, 64, 5000, 0, [5000]),
+    (2, 40, 3, 3, 8, 7, 1, [-3, 99]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("case", DECODE, ids=str)
+def test_decode_matches_64_bit(dtype, case):
+    o = ops()
+    B, T, H, Hkv, D, window, sinks, lengths = case
+    g = gen(T)
+    q, k, v = randn(g, B, H, D, dtype=dtype), randn(g, B, T, Hkv, D, dtype=dtype), randn(g, B, T, Hkv, D, dtype=dtype)
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    want = ref.decode(q, k, v, n, window, sinks)
+    u = ref.half_step(dtype)
+    got = o.window_attention_decode(q, k, v, n, window, sinks)
+    assert ref.rel(got, want) <= 3 * u + 64 * E
+    # what it does not see may hold anything: other rows, and caches in other layouts
+    for c in (k, v):
+        for b, m in enumerate(lengths):
+            m = min(max(m, 0), T)
+            c[b, m:] = float("nan")
+            c[b, sinks:max(sinks, m - window)] = float("inf")
+    assert torch.equal(o.window_attention_decode(q, k, v, n, window, sinks), got)
+    kt, vt = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (k, v))
+    assert torch.equal(o.window_attention_decode(q, kt, vt, n, window, sinks), got)
+    off = torch.empty(k.numel() + 1, dtype=dtype, device="cuda")[1:].view(k.shape).copy_(k)
+    assert ref.rel(o.window_attention_decode(q, off, v, n, window, sinks), want) <= 3 * u + 64 * E
+
+
+@pytest.mark.gpu
+def test_decode_past_32_bit_offsets():
+    """A cache of more than 2^32 bytes and 2^31 elements: the last token of the
+    last sequence."""
+    o = ops()
+    B, T, H, D = 3, 1 << 20, 8, 128
+    k = torch.zeros(B, T, H, D, dtype=torch.bfloat16, device="cuda")
+    assert k.numel() > 2 ** 31
+    g = gen(2)
+    tail = randn(g, 40, H, D, dtype=torch.bfloat16)
+    k[2, -40:] = tail
+    q = randn(g, B, H, D, dtype=torch.bfloat16)
+    n = torch.tensor([0, 3, T], dtype=torch.int32).cuda()
+    got = o.window_attention_decode(q, k, k, n, 40)
+    want = ref.decode(q[2:], tail[None], tail[None], [40], 40, 0)
+    assert ref.rel(got[2:], want) <= 3 * ref.half_step(torch.bfloat16) + 64 * E
+    assert not got[:2].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+def test_decode_is_the_last_row_of_attention(dtype):
+    o = ops()
+    case = (3, 190, 4, 2, 64, 50, 6, [190, 51, 7])
+    q, k, v, _, n = attention_inputs(case, dtype)
+    full = o.window_attention(q, k, v, 50, 6, lengths=n)
+    last = torch.stack([q[b, m - 1] for b, m in enumerate(case[7])])
+    got = o.window_attention_decode(last, k, v, n, 50, 6)
+    for b, m in enumerate(case[7]):
+        assert ref.rel(got[b], full[b, m - 1]) <= 4 * ref.half_step(dtype) + 128 * E
+
+
+# -------------------------------------------------------------- distillation
+
+# N, V, K, tau, hard, targets, gone entries
+DISTILL = [
+    (1, 1, 1, 1.0, 0.0, False, 0.0),
+    (2, 7, 3, 2.0, 0.5, True, 0.0),
+    (5, 257, 257, 1.0, 1.0, True, 0.3),
+    (3, 513, 1, 3.7, 0.25, True, 0.0),
+    (7, 1001, 20, 2.0, 0.0, True, 0.5),
+    (4, 50257, 33, 1.0, 0.5, True, 0.1),
+    (2, 50257, 64, 2.0, 0.3, True, 0.0),
+    (3, 32768, 1024, 0.7, 0.9, True, 0.2),
+    (2, 65537, 16, 1.5, 0.0, False, 1.0),
+    (6, 100, 0, 1.0, 0.5, True, 0.0),
+]
+
+
+def distill_inputs(case, dtype, seed=0):
+    N, V, K, tau, hard, has_y, gone = case
+    g = gen(seed + V)
+    z = randn(g, N, V, dtype=dtype, by=2.0)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(N)])
+    ids[torch.rand(N, K, generator=g) < gone] = -1
+    t = randn(g, N, K, by=1.5)
+    y = torch.randint(0, V, (N,), generator=g).cuda() if has_y else None
+    if has_y and N > 2:
+        y[1], y[2] = -100, V
+    if K > 3:
+        ids[0, 2] = ids[0, 0]  # the same id twice
+        if has_y:
+            ids[0, 3] = y[0]
+        ids[-1, 1] = V + 5
+    return z, ids.cuda(), t, y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("case", DISTILL, ids=str)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_distill_matches_64_bit(dtype, case, reduction):
+    o = ops()
+    N, V, K, tau, hard = case[:5]
+    z, ids, t, y = distill_inputs(case, dtype)
+    kw = dict(temperature=tau, hard_weight=hard, reduction=reduction)
+    with torch.no_grad():
+        plain = o.distill_loss(z, ids, t, y, **kw)
+    z.requires_grad_()
+    loss = o.distill_loss(z, ids, t, y, **kw)
+    assert torch.equal(loss, plain) and loss.dtype == torch.float32
+    g = randn(gen(1), *loss.shape) if reduction == "none" else torch.tensor(256.0).cuda()
+    (dz,) = torch.autograd.grad(loss, z, g)
+    r = z.detach().double().requires_grad_()
+    want = ref.distill(r, ids, t, y, tau, hard, reduction)
+    assert float((loss.double() - want).abs().max()) <= 2e-6 * (1 + float(want.abs().max())) * (N if reduction == "sum" else 1)
+    if want.requires_grad:
+        (dwant,) = torch.autograd.grad(want, r, g.double())
+    else:
+        dwant = torch.zeros_like(r)
+    # float16: values below its smallest normal carry 2^-25 each, absolute
+    floor = 2.0 ** -25 * dz.numel() ** 0.5 / max(float(dwant.norm()), 1e-30) if dtype == torch.float16 else 0.0
+    assert dz.dtype == dtype and ref.rel(dz, dwant) <= ref.half_step(dtype) + 64 * E + floor
+    if y is not None and N > 2:
+        assert not dz[1:3].any()
+    (again,) = torch.autograd.grad(o.distill_loss(z, ids, t, y, **kw), z, g)
+    assert torch.equal(again, dz)
+
+
+@pytest.mark.gpu
+def test_distill_strides_types_and_padding():
+    """Rows of a wider projection (padded vocabulary), rows off 16 bytes,
+    transposed logits, 32-bit ids and targets, 16-bit teachers, logits of -inf
+    in a padded vocabulary, rows that are left out and hold NaN."""
+    o = ops()
+    case = (6, 333, 9, 2.0, 0.5, True, 0.2)
+    for dtype in TYPES:
+        z, ids, t, y = distill_inputs(case, dtype)
+        tol = ref.half_step(dtype) + 64 * E
+        wide = torch.full((6, 350), 7.0, dtype=dtype, device="cuda")
+        wide[:, 3:336] = z
+        off = torch.zeros(6 * 333 + 1, dtype=dtype, device="cuda")[1:].view(6, 333).copy_(z)
+        far = torch.zeros(6, 2000, dtype=dtype, device="cuda")
+        far[:, 1:334] = z
+        for x in (wide[:, 3:336], z.T.contiguous().T, off, far[:, 1:334], wide[:, 3:336][:1].expand(6, 333)):
+            x = x.detach().requires_grad_()
+            loss = o.distill_loss(x, ids.int(), t, y.int(), temperature=2.0, hard_weight=0.5)
+            (dz,) = torch.autograd.grad(loss, x)
+            r = x.detach().double().requires_grad_()
+            want = ref.distill(r, ids, t, y, 2.0, 0.5)
+            (dwant,) = torch.autograd.grad(want, r)
+            floor = 2.0 ** -25 * dz.numel() ** 0.5 / float(dwant.norm()) if dtype == torch.float16 else 0.0
+            assert abs(float(loss) - float(want)) <= 2e-5 and ref.rel(dz, dwant) <= tol + floor
+        for tt in (t.bfloat16(), t.half()):
+            a = o.distill_loss(z, ids, tt, y, temperature=2.0, hard_weight=0.5)
+            assert abs(float(a) - float(ref.distill(z, ids, tt, y, 2.0, 0.5))) <= 2e-5
+        padded = torch.full((6, 400), float("-inf"), dtype=dtype, device="cuda")
+        padded[:, :333] = z
+        padded[1] = float("nan")  # a row that is left out
+        padded.requires_grad_()
+        loss = o.distill_loss(padded, ids.where(ids < 333, -1), t, y.where(y < 333, -1), temperature=2.0, hard_weight=0.5)
+        (dz,) = torch.autograd.grad(loss, padded)
+        x = z.clone().requires_grad_()
+        same = o.distill_loss(x, ids, t, y, temperature=2.0, hard_weight=0.5)
+        (dx,) = torch.autograd.grad(same, x)
+        assert abs(float(loss) - float(same)) <= 4e-6
+        assert not dz[:, 333:].any() and not dz[1].any() and ref.rel(dz[:, :333], dx) <= 2 * tol
+
+
+@pytest.mark.gpu
+def test_distill_against_differences():
+    """The float32 gradient against central differences of the 64-bit form."""
+    o = ops()
+    for case in ((4, 57, 6, 2.0, 0.5, True, 0.2), (3, 40, 5, 1.3, 0.0, False, 0.0)):
+        z, ids, t, y = distill_inputs(case, torch.float32)
+        z.requires_grad_()
+        (dz,) = torch.autograd.grad(o.distill_loss(z, ids, t, y, temperature=case[3], hard_weight=case[4]), z)
+        d = randn(gen(4), *z.shape).double()
+        f = [float(ref.distill(z.detach().double() + h * d, ids, t, y, case[3], case[4])) for h in (1e-5, -1e-5)]
+        assert abs((f[0] - f[1]) / 2e-5 - float((dz.double() * d).sum())) <= 64 * E * float(dz.norm() * d.norm()) + 1e-8
+
+
+@pytest.mark.gpu
+def test_distill_empty_and_nothing_counts():
+    o = ops()
+    z = torch.zeros(0, 9).cuda().requires_grad_()
+    e, t = torch.zeros(0, 2, dtype=torch.int64).cuda(), torch.zeros(0, 2).cuda()
+    loss = o.distill_loss(z, e, t)
+    assert float(loss) == 0.0 and torch.autograd.grad(loss, z)[0].shape == (0, 9)
+    z = randn(gen(1), 3, 9).requires_grad_()
+    loss = o.distill_loss(z, torch.zeros(3, 2, dtype=torch.int64).cuda(), torch.zeros(3, 2).cuda(), torch.full((3,), -100).cuda(), hard_weight=0.5)
+    assert float(loss) == 0.0 and not torch.autograd.grad(loss, z)[0].any()
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(o.distill_loss(z, torch.zeros(3, 2, dtype=torch.int64).cuda(), torch.zeros(3, 2).cuda()), z, create_graph=True)
+
+
+# ------------------------------------------------- streams, graphs, together
+
+
+def step(o, x, plan, window, sinks, n, ids, t, y):
+    """rotary, attention, a projection and the loss: a model's tail in small."""
+    q, k, v, w = x
+    qr, kr = o.rotary(q, k, plan)
+    a = o.window_attention(qr, kr, v, window, sinks, lengths=n)
+    logits = a.flatten(2).flatten(0, 1) @ w
+    return o.distill_loss(logits, ids, t, y, temperature=2.0, hard_weight=0.5)
+
+
+def step_inputs(seed, dtype=torch.bfloat16):
+    g = gen(seed)
+    B, T, H, D, V, K = 2, 140, 4, 64, 301, 7
+    x = [randn(g, B, T, H, D, dtype=dtype), randn(g, B, T, 2, D, dtype=dtype), randn(g, B, T, 2, D, dtype=dtype),
+         randn(g, H * D, V, dtype=dtype, by=0.2)]
+    n = torch.tensor([140, 77], dtype=torch.int32).cuda()
+    ids = torch.randint(0, V, (B * T, K), generator=g).cuda()
+    y = torch.randint(0, V, (B * T,), generator=g).cuda()
+    y[140 + 77:] = -100
+    return x, n, ids, randn(g, B * T, K), y
+
+
+@pytest.mark.gpu
+def test_operators_together_match_64_bit():
+    o = ops()
+    plan = o.Rotary(32)
+    f, amp = freqs(32)
+    x, n, ids, t, y = step_inputs(1)
+    leaves = [p.requires_grad_() for p in x]
+    loss = step(o, leaves, plan, 50, 4, n, ids, t, y)
+    grads = torch.autograd.grad(loss, leaves)
+    r = [p.detach().double().requires_grad_() for p in x]
+    at = torch.arange(140).cuda().expand(2, 140)
+    a = ref.attention(ref.rotate(r[0], at, f, amp, False), ref.rotate(r[1], at, f, amp, False), r[2], 50, 4, n)
+    want = ref.distill(a.flatten(2).flatten(0, 1) @ r[3], ids, t, y, 2.0, 0.5)
+    dwant = torch.autograd.grad(want, r)
+    u = ref.half_step(torch.bfloat16)
+    # the loss sees logits of the order of 3 that carry a few roundings each, averaged over 217 rows
+    assert abs(float(loss) - float(want)) <= 4 * u * 3
+    for got, w in zip(grads, dwant):  # eight roundings to 16 bits lie between the inputs and their gradients
+        assert ref.rel(got, w) <= 8 * u
+
+
+@pytest.mark.gpu
+def test_operators_on_another_stream_and_captured():
+    """A whole step on a side stream, and captured into two graphs that are
+    replayed in turn with new inputs, gives the bits of the eager step."""
+    o = ops()
+    plan = o.Rotary(32)
+    want, data = [], [step_inputs(s) for s in (1, 2, 3)]
+    for x, n, ids, t, y in data:
+        leaves = [p.clone().requires_grad_() for p in x]
+        loss = step(o, leaves, plan, 50, 4, n, ids, t, y)
+        grads = torch.autograd.grad(loss, leaves)
+        want.append((loss.detach().clone(), *grads))
+        del loss, leaves
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        x, n, ids, t, y = data[1]
+        leaves = [p.clone().requires_grad_() for p in x]
+        loss = step(o, leaves, plan, 50, 4, n, ids, t, y)
+        got = (loss.detach(), *torch.autograd.grad(loss, leaves))
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1]))
+    del loss, leaves
+
+    runs = []
+    for first in (0, 1):
+        x, n, ids, t, y = data[first]
+        static = [p.clone().requires_grad_() for p in x] + [n.clone(), ids.clone(), t.clone(), y.clone()]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = step(o, static[:4], plan, 50, 4, *static[4:])
+            out = (loss.detach(), *torch.autograd.grad(loss, static[:4]))
+            del loss
+        runs.append((graph, static, out))
+    for order in (0, 2, 1):
+        for graph, static, out in runs:
+            x, *rest = data[order]
+            with torch.no_grad():
+                for dst, src in zip(static, [*x, *rest]):
+                    dst.copy_(src)
+        for graph, _, _ in runs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, _, out in runs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[order]))
+
+
+@pytest.mark.gpu
+def test_decode_captured_follows_the_lengths():
+    o = ops()
+    g = gen(8)
+    q, k, v = randn(g, 2, 4, 64, dtype=torch.bfloat16), *(randn(g, 2, 500, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    n = torch.tensor([1, 0], dtype=torch.int32).cuda()
+    o.window_attention_decode(q, k, v, n, 100, 4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = o.window_attention_decode(q, k, v, n, 100, 4)
+    for lengths in ([500, 37], [3, 0], [101, 104]):
+        n.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(out, o.window_attention_decode(q, k, v, n, 100, 4))
+        assert ref.rel(out, ref.decode(q, k, v, lengths, 100, 4)) <= 3 * ref.half_step(torch.bfloat16) + 64 * E
+
+
+@pytest.mark.gpu
+def test_operators_from_two_threads():
+    """Two threads on streams of their own, the same bits as one after the other."""
+    import threading
+
+    o = ops()
+    plan = o.Rotary(32)
+    data = [step_inputs(s) for s in (4, 5)]
+
+    def run(d):
+        x, n, ids, t, y = d
+        leaves = [p.clone().requires_grad_() for p in x]
+        loss = step(o, leaves, plan, 50, 4, n, ids, t, y)
+        return (loss.detach(), *torch.autograd.grad(loss, leaves))
+
+    want = [run(d) for d in data]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = run(data[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(6))
+def test_window_attention_drawn(seed):
+    """Sizes drawn over the range."""
+    o = ops()
+    r = random.Random(seed)
+    for _ in range(4):
+        dtype = r.choice(TYPES)
+        Hkv = r.randint(1, 3)
+        T = r.choice([1, r.randint(2, 60), r.randint(61, 600)])
+        case = (r.randint(1, 3), T, Hkv * r.randint(1, 4), Hkv, r.choice([4, 24, 40, 64, 100, 104, 128]), r.randint(1, T + 20),
+                r.choice([0, r.randint(0, T)]), None)
+        q, k, v, do, _ = attention_inputs(case, dtype, seed)
+        n = torch.tensor([r.randint(0, T) for _ in range(case[0])], dtype=torch.int32).cuda() if r.random() < 0.5 else None
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        out = o.window_attention(*leaves, *case[5:7], lengths=n)
+        grads = torch.autograd.grad(out, leaves, do)
+        rr = [x.detach().double().requires_grad_() for x in leaves]
+        want = ref.attention(*rr, *case[5:7], n)
+        dwant = torch.autograd.grad(want, rr, do.double())
+        u = ref.half_step(dtype)
+        assert ref.rel(out, want) <= 3 * u + 64 * E, case
+        for got, w in zip(grads, dwant):
+            assert ref.rel(got, w) <= 5 * u + 256 * E, case
