@@ -384,6 +384,7 @@ extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_
     if (int rc = attn_check(a, false, "window attention")) return rc;
     if (a->B == 0 || a->T == 0) return CAIL_OPS_OK;
     auto st = static_cast<cudaStream_t>(stream);
+    if (tc_takes(a, false)) return tc_forward(a, st);
     const AttnArgs x = attn_args(a, false);
     const bool vec = attn_vectors(a, false);
     if (a->type == CAIL_OPS_F32) return run<float>(x, vec, false, st);

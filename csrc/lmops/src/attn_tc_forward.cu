@@ -1,0 +1,304 @@
+// attn_tc_forward.cu — window attention on the tensor cores (bf16, fp16).
+//
+// A block owns 128 query rows of one head and goes once over the key tiles
+// (64 keys) that some of them see.  One thread loads tiles by TMA, one issues
+// the matrix products, 128 threads hold one row each: S = Q K^T arrives in
+// tensor memory (two buffers, so the next product runs under this softmax),
+// the row's thread keeps the running maximum and sum in registers without any
+// exchange, writes p back over S as 16-bit, and O += P V takes it from there.
+// O stays in tensor memory; it is rescaled only when a row's maximum has grown
+// by more than 2^8 since the scale in use, so p stays below 256 and most tiles
+// touch O in no other way than the product.  p is rounded to the input type
+// for that product (its sum is not); everything else is 32-bit.
+//
+// 64 keys per tile and two blocks per SM (256 columns of tensor memory each):
+// the exponentials (16 a clock and SM) bound it at D = 64, 512 clocks per tile
+// against 320 for the products, so two blocks whose softmax and products
+// alternate beat one block with larger tiles.
+#include "attn.cuh"
+#include "tc.cuh"
+
+namespace cailops {
+namespace {
+
+constexpr int kRows = 128, kKeys = 64, kThreads = 192;
+
+template <int DP> struct Shape {
+    static constexpr int panels = DP / 64;
+    static constexpr int stages = DP == 64 ? 4 : 2;
+    static constexpr int q_bytes = kRows * DP * 2, kv_bytes = kKeys * DP * 2;
+    static constexpr int barriers = 1 + 4 * stages + 2 + 2 + 2;
+    static constexpr int smem = 1024 + q_bytes + 2 * stages * kv_bytes;
+    static constexpr int o_col = 2 * kKeys;  // S0, S1, O
+};
+
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs a, const __grid_constant__ Maps maps) {
+    using S = Shape<DP>;
+    constexpr bool bf = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ char raw[];
+    __shared__ __align__(8) uint64_t bars[S::barriers];
+    __shared__ uint32_t tmem_at;
+    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+    const uint32_t sq = base, sk = sq + S::q_bytes, sv = sk + S::stages * S::kv_bytes;
+    const uint32_t bar0 = smem_u32(bars);
+    auto bar = [&](int i) { return bar0 + 8u * i; };
+    const uint32_t q_full = bar(0), k_full = bar(1), k_free = bar(1 + S::stages), v_full = bar(1 + 2 * S::stages),
+                   v_free = bar(1 + 3 * S::stages), s_full = bar(1 + 4 * S::stages), p_full = s_full + 16, o_done = p_full + 16, o_last = o_done + 8;
+
+    const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
+    const int i0 = (gridDim.x - 1 - blockIdx.x) * kRows;  // the longest rows first
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n = length_of(a, b);
+    const KeyTiles tiles(i0, i0 + kRows, n, a.window, a.sinks, kKeys);
+
+    if (tiles.count == 0) {  // rows behind the sequence: zeros
+        constexpr int C = DP / 8;
+        for (int i = tid; i < kRows * C; i += kThreads) {
+            const int r = i0 + i / C, d = (i % C) * 8;
+            if (r < a.T && d < a.D) *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh + d * 2) = make_uint4(0, 0, 0, 0);
+        }
+        if (a.lse && tid < kRows && i0 + tid < a.T) a.lse[((int64_t)b * a.H + h) * a.T + i0 + tid] = 0.f;
+        return;
+    }
+    if (warp == 4) {
+        tmem_alloc<256>(smem_u32(&tmem_at));
+        if (lane == 0) {
+            tma_prefetch(&maps.q), tma_prefetch(&maps.k), tma_prefetch(&maps.v);
+        }
+    }
+    if (tid == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < S::stages; ++s) {
+            mbar_init(k_full + 8 * s, 1), mbar_init(k_free + 8 * s, 1);
+            mbar_init(v_full + 8 * s, 1), mbar_init(v_free + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 128);
+        mbar_init(o_done, 1), mbar_init(o_last, 1);
+        fence_barrier_init();
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tm = tmem_at;
+    bool ok = true;
+
+    if (warp == 4) {
+        if (lane == 0) {  // loads
+            mbar_expect(q_full, S::q_bytes);
+            for (int p = 0; p < S::panels; ++p) tma_load(sq + p * kRows * 128, &maps.q, q_full, p * 64, i0, h, b);
+            for (int x = 0; x < tiles.count && ok; ++x) {
+                const int s = x % S::stages;
+                const uint32_t round = (x / S::stages) & 1;
+                const int j0 = tiles.at(x) * kKeys;
+                if (x >= S::stages) ok = mbar_wait(k_free + 8 * s, round ^ 1);
+                if (!ok) break;
+                mbar_expect(k_full + 8 * s, S::kv_bytes);
+                for (int p = 0; p < S::panels; ++p) tma_load(sk + s * S::kv_bytes + p * kKeys * 128, &maps.k, k_full + 8 * s, p * 64, j0, hk, b);
+                if (x >= S::stages) ok = mbar_wait(v_free + 8 * s, round ^ 1);
+                if (!ok) break;
+                mbar_expect(v_full + 8 * s, S::kv_bytes);
+                for (int p = 0; p < S::panels; ++p) tma_load(sv + s * S::kv_bytes + p * kKeys * 128, &maps.v, v_full + 8 * s, p * 64, j0, hk, b);
+            }
+            if (!ok) {  // gave up: the copies in flight still land before the block ends
+                report(a.error);
+                mbar_wait(q_full, 0);
+                for (int s = 0; s < S::stages; ++s)
+                    for (uint32_t par = 0; par < 2; ++par) mbar_try(k_full + 8 * s, par), mbar_try(v_full + 8 * s, par);
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {  // products
+            constexpr uint32_t kind_s = mma_kind<bf, kRows, kKeys, false>(), kind_o = mma_kind<bf, kRows, DP, true>();
+            auto scores = [&](int x) {
+                const int s = x % S::stages;
+                if (!mbar_wait(k_full + 8 * s, (x / S::stages) & 1)) return false;
+                tc_after();
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_ss(tm + (x & 1) * kKeys, operand(sq + (kk / 4) * kRows * 128 + (kk % 4) * 32, 0),
+                           operand(sk + s * S::kv_bytes + (kk / 4) * kKeys * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
+                mma_commit(k_free + 8 * s);
+                mma_commit(s_full + 8 * (x & 1));
+                return true;
+            };
+            ok = mbar_wait(q_full, 0) && scores(0) && (tiles.count < 2 || scores(1));
+            for (int x = 0; x < tiles.count && ok; ++x) {
+                const int s = x % S::stages;
+                ok = mbar_wait(p_full + 8 * (x & 1), (x >> 1) & 1) && mbar_wait(v_full + 8 * s, (x / S::stages) & 1);
+                if (!ok) break;
+                tc_after();
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                    mma_ts(tm + S::o_col, tm + (x & 1) * kKeys + kk * 8, operand(sv + s * S::kv_bytes + kk * 2048, kKeys * 128), kind_o,
+                           x > 0 || kk > 0);
+                mma_commit(v_free + 8 * s);
+                mma_commit(o_done);
+                if (x + 2 < tiles.count) ok = scores(x + 2);
+            }
+            mma_commit(o_last);
+            if (!ok) report(a.error);
+        }
+    } else {  // one row each
+        const int i = i0 + tid;
+        const uint32_t mine = tm + ((uint32_t)(warp * 32) << 16);
+        float m = -INFINITY, l = 0.f;  // m: the maximum in use, in scores
+        for (int x = 0; x < tiles.count; ++x) {
+            const int j0 = tiles.at(x) * kKeys;
+            ok = mbar_wait(s_full + 8 * (x & 1), (x >> 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_after();
+            const uint32_t at = mine + (x & 1) * kKeys;
+            uint32_t u[kKeys];
+            float *f = reinterpret_cast<float *>(u);
+            tc_ld32(at, u);
+            tc_ld32(at + 32, u + 32);
+            tc_wait_ld(u);
+            tc_touch(u + 32);
+            // every row of the tile sees every key, unless the tile crosses the diagonal or the window's edge
+            const bool whole = j0 + kKeys - 1 <= i0 && (i0 + kRows - 1 - j0 < a.window || j0 + kKeys <= a.sinks);
+            if (!whole) {
+#pragma unroll
+                for (int c = 0; c < kKeys; ++c) {
+                    const int j = j0 + c;
+                    if (!(j <= i && (i - j < a.window || j < a.sinks))) f[c] = -INFINITY;
+                }
+            }
+            float top = f[0];
+#pragma unroll
+            for (int c = 1; c < kKeys; ++c) top = fmaxf(top, f[c]);
+            float turn = 1.f;
+            if (m == -INFINITY) {
+                m = top;  // nothing of this row is in O yet
+            } else if ((top - m) * a.scale_log2 > 8.f) {
+                turn = exp2_fast((m - top) * a.scale_log2);
+                l *= turn;
+                m = top;
+            }
+            if (__any_sync(0xffffffffu, turn != 1.f)) {
+                // until the previous product is in O (the scores of this tile were queued behind the one before it)
+                ok = mbar_wait(o_done, (x - 1) & 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                tc_after();
+#pragma unroll
+                for (int c = 0; c < DP; c += 32) {
+                    uint32_t w[32];
+                    tc_ld32(mine + S::o_col + c, w);
+                    tc_wait_ld(w);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * turn);
+                    tc_st32(mine + S::o_col + c, w);
+                }
+            }
+            const float off = m == -INFINITY ? 0.f : m * a.scale_log2;
+            float sum[4] = {};
+            uint32_t p[kKeys / 2];
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 2) {
+                const float p0 = exp2_fast(fmaf(f[c], a.scale_log2, -off)), p1 = exp2_fast(fmaf(f[c + 1], a.scale_log2, -off));
+                sum[(c / 2) % 4] += p0 + p1;
+                p[c / 2] = pack2(p0, p1, T());
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_st32(at, p);
+            // keys behind the sequence meet p = 0, but what they hold may be infinite: their values are zeroed
+            if (n < a.T && j0 + kKeys > n) {
+                const int s = x % S::stages;
+                ok = mbar_wait(v_full + 8 * s, (x / S::stages) & 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                constexpr int C = DP / 8;
+                const int first = n - j0;
+                for (int e = tid; e < (kKeys - first) * C; e += kRows) {
+                    const int r = first + e / C, c = e % C;
+                    const uint32_t dst = sv + s * S::kv_bytes + (c / 8) * kKeys * 128 + r * 128 + (c % 8) * 16;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+                }
+                fence_async();
+                __syncwarp();
+            }
+            tc_wait_st();
+            tc_before();
+            mbar_arrive(p_full + 8 * (x & 1));
+        }
+        if (ok) ok = mbar_wait(o_last, 0);
+        if (__all_sync(0xffffffffu, ok)) {
+            tc_after();
+            const bool live = i < n;
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            // rows go through shared memory (the queries' place) so that stores are whole rows
+            const uint32_t row = sq + tid * 128;
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t w[32];
+                tc_ld32(mine + S::o_col + c, w);
+                tc_wait_ld(w);
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        y[k] = live && l != 0.f
+                                   ? pack2(__uint_as_float(w[e + 2 * k]) * inv, __uint_as_float(w[e + 2 * k + 1]) * inv, T())
+                                   : 0u;
+                    const int chunk = (c % 64 + e) / 8;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (c / 64) * kRows * 128 + ((chunk ^ (tid & 7)) * 16)),
+                                 "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
+                                 : "memory");
+                }
+            }
+            __syncwarp();
+            constexpr int C = DP / 8;
+            for (int e = lane; e < 32 * C; e += 32) {
+                const int r = warp * 32 + e / C, c = e % C;
+                uint4 y;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                             : "r"(sq + (c / 8) * kRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16)));
+                if (i0 + r < a.T && c * 8 < a.D) *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)(i0 + r) * a.ot + h * a.oh + c * 16) = y;
+            }
+            if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.T + i] = live && l > 0.f ? fmaf(m, a.scale_log2, log2f(l)) : 0.f;
+        } else if (lane == 0) {
+            report(a.error);
+        }
+        tc_before();
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == 4) tmem_free<256>(tm);
+}
+
+template <typename T, int DP> int launch(const cail_ops_attention_args *c, const AttnArgs &a, cudaStream_t st) {
+    using S = Shape<DP>;
+    Maps maps;
+    if (int rc = tensor_map(&maps.q, c->q, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
+    if (int rc = tensor_map(&maps.k, c->k, c->type, a.B, a.T, a.Hkv, a.D, kKeys)) return rc;
+    if (int rc = tensor_map(&maps.v, c->v, c->type, a.B, a.T, a.Hkv, a.D, kKeys)) return rc;
+    cudaError_t e = cudaFuncSetAttribute(tc_forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+    if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention: %s", cudaGetErrorString(e));
+    tc_forward_kernel<T, DP><<<dim3((a.T + kRows - 1) / kRows, a.H, a.B), kThreads, S::smem, st>>>(a, maps);
+    return launched("window attention");
+}
+
+}  // namespace
+
+// 16-bit elements in rows that TMA can load (16-byte multiples), a positive
+// scale (the row maximum is taken before scaling)
+bool tc_takes(const cail_ops_attention_args *a, bool backward) {
+    if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f)) return false;
+    if (!tma_takes(a->q, a->B, a->T, a->H) || !tma_takes(a->k, a->B, a->T, a->Hkv) || !tma_takes(a->v, a->B, a->T, a->Hkv)) return false;
+    return rows_aligned(a->o, a->B, a->T, a->H, 2, 16);
+}
+
+int tc_forward(const cail_ops_attention_args *c, cudaStream_t st) {
+    AttnArgs a = attn_args(c, false);
+    a.error = device_error_flag();
+    if (!a.error) return fail(CAIL_OPS_ECUDA, "window attention: no error word for this device");
+    if (c->type == CAIL_OPS_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(c, a, st) : launch<__nv_bfloat16, 128>(c, a, st);
+    return a.D <= 64 ? launch<__half, 64>(c, a, st) : launch<__half, 128>(c, a, st);
+}
+
+}  // namespace cailops
