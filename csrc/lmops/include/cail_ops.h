@@ -55,6 +55,9 @@ typedef struct {
 } cail_ops_rotary_args;
 int cail_ops_rotary(const cail_ops_rotary_args *a, cail_ops_stream stream);
 
+/* values of lse and of delta: rows of T rounded up to 4, and 64 behind the last (tiles are read whole) */
+#define CAIL_OPS_LSE_FLOATS(B, H, T) ((size_t)(B) * (size_t)(H) * (((size_t)(T) + 3) / 4 * 4) + 64)
+
 /* Causal attention with a sliding window and sinks.  Row i sees key j iff
  * i < n, j <= i and (i - j < window or j < sinks), n = lengths[b] (T when
  * lengths is NULL; clamped to [0, T]).  Rows that see nothing give zeros. */
@@ -64,10 +67,11 @@ typedef struct {
     float scale;
     const int32_t *lengths;
     cail_ops_bthd q, k, v, o;
-    float *lse;             /* [B, H, T] written by forward, read by backward (log2 units); NULL: not kept */
+    float *lse;             /* CAIL_OPS_LSE_FLOATS(B, H, T) values, 16-byte aligned, kept by forward for
+                               backward (B * H rows, T rounded up to 4 apart); NULL: not kept */
     /* backward only */
     cail_ops_bthd dout, dq, dk, dv;
-    float *delta;           /* [B, H, T] scratch */
+    float *delta;           /* scratch of the same size and alignment */
     void *workspace;        /* cail_ops_window_attention_workspace() bytes, 16-byte aligned */
     size_t workspace_bytes;
 } cail_ops_attention_args;

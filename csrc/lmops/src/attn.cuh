@@ -16,7 +16,8 @@ struct AttnArgs {
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
     int64_t gb, gt, gh;  // dout
     int64_t dqb, dqt, dqh, dkb, dkt, dkh, dvb, dvt, dvh;
-    float *lse, *delta;  // [B, H, T]; lse in log2 units of the scaled scores
+    float *lse, *delta;  // [B, H] rows of `lse_row` values; lse in log2 units of the scaled scores
+    int64_t lse_row;     // T rounded up to 4
     int *error;          // the device's error word (kernels with bounded waits)
 };
 
@@ -25,7 +26,8 @@ int attn_check(const cail_ops_attention_args *a, bool backward, const char *who)
 AttnArgs attn_args(const cail_ops_attention_args *a, bool backward);
 
 // the tensor-core path (attn_tc_*.cu): whether it takes the call, and the call
-bool tc_takes(const cail_ops_attention_args *a, bool backward);
+bool tc_takes(const cail_ops_attention_args *a);
+bool tc_takes_backward(const cail_ops_attention_args *a);
 int tc_forward(const cail_ops_attention_args *a, cudaStream_t st);
 int tc_backward(const cail_ops_attention_args *a, cudaStream_t st);
 size_t tc_workspace(const cail_ops_attention_args *a);

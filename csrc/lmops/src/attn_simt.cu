@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) simt_forward(const AttnArgs a, bool 
             const int d = column<DP>(tx, c);
             if (d < a.D) out[d] = from_f<T>(l[r] == 0.f ? 0.f : o[r][c] * inv);
         }
-        if (a.lse && tx == 0) a.lse[((int64_t)b * a.H + h) * a.T + i] = l[r] == 0.f ? 0.f : m[r] + log2f(l[r]);
+        if (a.lse && tx == 0) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = l[r] == 0.f ? 0.f : m[r] + log2f(l[r]);
     }
 }
 
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) simt_dq(const AttnArgs a, bool vec) 
 #pragma unroll
         for (int c = 0; c < NC; ++c) s = fmaf(sg[row * ld<DP>() + tx + 16 * c], sk[row * ld<DP>() + tx + 16 * c], s);
         delta[r] = half_sum(s);
-        const int64_t at = ((int64_t)b * a.H + h) * a.T + i;
+        const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + i;
         lse[r] = i < n ? a.lse[at] : 0.f;
         if (i < a.T && tx == 0) a.delta[at] = delta[r];
     }
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) simt_dkv(const AttnArgs a, bool vec)
             load_tile<T, DP>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec, 1.f);
             load_tile<T, DP>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec, 1.f);
             if (tid < kTile) {
-                const int64_t at = ((int64_t)b * a.H + h) * a.T + i0 + tid;
+                const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + i0 + tid;
                 row_lse[tid] = i0 + tid < n ? a.lse[at] : 0.f;
                 row_delta[tid] = i0 + tid < n ? a.delta[at] : 0.f;
             }
@@ -358,7 +358,7 @@ AttnArgs attn_args(const cail_ops_attention_args *a, bool backward) {
     x.k = static_cast<const char *>(a->k.ptr), x.kb = a->k.sb * s, x.kt = a->k.st * s, x.kh = a->k.sh * s;
     x.v = static_cast<const char *>(a->v.ptr), x.vb = a->v.sb * s, x.vt = a->v.st * s, x.vh = a->v.sh * s;
     x.o = static_cast<char *>(a->o.ptr), x.ob = a->o.sb * s, x.ot = a->o.st * s, x.oh = a->o.sh * s;
-    x.lse = a->lse;
+    x.lse = a->lse, x.lse_row = (a->T + 3) / 4 * 4;
     if (backward) {
         x.dout = static_cast<const char *>(a->dout.ptr), x.gb = a->dout.sb * s, x.gt = a->dout.st * s, x.gh = a->dout.sh * s;
         x.dq = static_cast<char *>(a->dq.ptr), x.dqb = a->dq.sb * s, x.dqt = a->dq.st * s, x.dqh = a->dq.sh * s;
@@ -384,7 +384,7 @@ extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_
     if (int rc = attn_check(a, false, "window attention")) return rc;
     if (a->B == 0 || a->T == 0) return CAIL_OPS_OK;
     auto st = static_cast<cudaStream_t>(stream);
-    if (tc_takes(a, false)) return tc_forward(a, st);
+    if (tc_takes(a)) return tc_forward(a, st);
     const AttnArgs x = attn_args(a, false);
     const bool vec = attn_vectors(a, false);
     if (a->type == CAIL_OPS_F32) return run<float>(x, vec, false, st);
@@ -392,12 +392,16 @@ extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_
     return run<__half>(x, vec, false, st);
 }
 
-extern "C" size_t cail_ops_window_attention_workspace(const cail_ops_attention_args *a) { return 0; }
+extern "C" size_t cail_ops_window_attention_workspace(const cail_ops_attention_args *a) {
+    if (attn_check(a, true, "window attention backward") || a->B == 0 || a->T == 0) return 0;
+    return tc_takes_backward(a) ? tc_workspace(a) : 0;
+}
 
 extern "C" int cail_ops_window_attention_backward(const cail_ops_attention_args *a, cail_ops_stream stream) {
     if (int rc = attn_check(a, true, "window attention backward")) return rc;
     if (a->B == 0 || a->T == 0) return CAIL_OPS_OK;
     auto st = static_cast<cudaStream_t>(stream);
+    if (tc_takes_backward(a)) return tc_backward(a, st);
     const AttnArgs x = attn_args(a, true);
     const bool vec = attn_vectors(a, true);
     if (a->type == CAIL_OPS_F32) return run<float>(x, vec, true, st);

@@ -1,0 +1,493 @@
+// attn_tc_backward.cu — gradients of window attention on the tensor cores
+// (bf16, fp16).
+//
+// Two kernels of one shape.  A block keeps 128 rows of X and Y in shared
+// memory, streams tiles of 64 rows of U and W past them, and for every tile
+//   S = X U^T,  dP = Y W^T          (into tensor memory)
+//   p = exp2(S - lse), ds = p (dP - delta)   (256 threads, 32 columns each)
+//   acc0 += ds U  [, acc1 += p W]   (p and ds from tensor memory)
+// where, with i a query and j a key,
+//   dq:     X = Q, Y = dO (rows i), U = K, W = V: acc0 = dq; delta = do.o on the way
+//   dk, dv: X = K, Y = V (rows j), U = Q, W = dO over the group's heads: acc0 = dk, acc1 = dv
+// Seven products instead of the five of a kernel that adds dq with atomics:
+// every output is summed by one block in one order, so results do not change
+// from run to run.  The sinks' key tiles are seen by all queries; where that
+// would make them the last blocks running, their queries are split and the
+// parts joined in order by a third kernel.
+//
+// p and ds are rounded to the input type for their products, all else is
+// 32-bit.  fp16 has no range for small gradients: ds is scaled by a power of
+// two taken from max |do| (of the row for dq; of the key head for dk), taken
+// back out of the sums.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn.cuh"
+#include "tc.cuh"
+
+namespace cailops {
+namespace {
+
+constexpr int kRows = 128, kStream = 64, kMath = 256, kThreads = kMath + 64;
+
+template <int DP, bool DKV> struct Shape {
+    static constexpr int panels = DP / 64;
+    static constexpr int stages = 3;
+    static constexpr int buffers = DP == 64 ? 1 : 2;  // of S and dP
+    static constexpr int per_sm = DP == 64 ? 2 : 1;
+    static constexpr int x_bytes = kRows * DP * 2, u_bytes = kStream * DP * 2;
+    static constexpr int vec_bytes = DKV ? 2 * kStream * 4 : 0;  // lse and delta of a tile's queries
+    static constexpr int barriers = 1 + 2 * stages + 2 * buffers + 1;
+    static constexpr int smem = 1024 + 2 * x_bytes + stages * (2 * u_bytes + vec_bytes);
+    static constexpr int acc = buffers * 2 * kStream;  // column of acc0; acc1 follows
+    static constexpr int columns = DP == 64 ? 256 : 512;
+};
+
+struct Maps {
+    CUtensorMap x, y, u, w;
+};
+
+struct Extra {
+    unsigned *amax;       // [B, Hkv] bits of max |do| (fp16)
+    float *parts;         // [B, Hkv, sink tiles, splits, 2, 128, DP] partial dk and dv
+    int splits, sink_tiles;
+};
+
+// the power of two that brings a value whose largest is `bits` to [1/4, 1/2)
+__device__ __forceinline__ float amp_of(unsigned bits) {
+    const int e = min(max((int)(bits >> 23) - 127, -30), 30);
+    return bits == 0 ? 1.f : __uint_as_float((unsigned)(125 - e) << 23);
+}
+
+template <typename T, int DP, bool DKV>
+__global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
+    tc_backward_kernel(const AttnArgs a, const Extra ex, const __grid_constant__ Maps maps) {
+    using S = Shape<DP, DKV>;
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int NB = S::buffers, ST = S::stages;
+    extern __shared__ char raw[];
+    __shared__ __align__(8) uint64_t bars[S::barriers];
+    __shared__ uint32_t tmem_at;
+    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+    const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + ST * S::u_bytes, svec = sw + ST * S::u_bytes;
+    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int b = blockIdx.z, n = length_of(a, b);
+    // rows of this block, and the tiles that pass: x = 0 .. count - 1
+    int r0, count, h, hk, split = 0, q_begin = 0, q_tiles = 0, first = 0;
+    bool parted = false;
+    KeyTiles keys(0, 0, 0, 1, 0, kStream);
+    if constexpr (DKV) {
+        hk = blockIdx.y, h = hk * a.group;
+        int tile = blockIdx.x;
+        parted = ex.splits > 1 && tile < ex.sink_tiles * ex.splits;
+        if (parted) split = tile % ex.splits, tile /= ex.splits;
+        else if (ex.splits > 1) tile -= ex.sink_tiles * (ex.splits - 1);
+        r0 = tile * kRows;
+        int begin, end;
+        query_range(r0, r0 + kRows, n, a.window, a.sinks, begin, end);
+        q_begin = begin / kStream;
+        q_tiles = end > begin ? (end - 1) / kStream + 1 - q_begin : 0;
+        count = a.group * q_tiles;
+        if (parted) {  // this part of the tiles
+            const int per = (count + ex.splits - 1) / ex.splits;
+            first = min(count, split * per);
+            count = min(count, first + per) - first;
+        }
+    } else {
+        h = blockIdx.y, hk = h / a.group;
+        r0 = (gridDim.x - 1 - blockIdx.x) * kRows;  // the longest rows first
+        keys = KeyTiles(r0, r0 + kRows, n, a.window, a.sinks, kStream);
+        count = keys.count;
+    }
+    // tile x: its first row, and its query head (dk, dv)
+    auto tile_row = [&](int x) { return DKV ? (q_begin + (first + x) % q_tiles) * kStream : keys.at(x) * kStream; };
+    auto tile_head = [&](int x) { return DKV ? h + (first + x) / q_tiles : h; };
+
+    if (count == 0) {  // nothing sees or is seen: zeros
+        constexpr int C = DP / 8;
+        if (DKV && parted) {
+            float4 *p = reinterpret_cast<float4 *>(ex.parts) +
+                        ((((int64_t)b * a.Hkv + hk) * ex.sink_tiles + r0 / kRows) * ex.splits + split) * (2 * kRows * DP / 4);
+            for (int i = tid; i < 2 * kRows * DP / 4; i += kThreads) p[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            return;
+        }
+        for (int i = tid; i < kRows * C; i += kThreads) {
+            const int r = r0 + i / C, d = (i % C) * 8;
+            if (r >= a.T || d >= a.D) continue;
+            if (DKV) {
+                *reinterpret_cast<uint4 *>(a.dk + b * a.dkb + (int64_t)r * a.dkt + hk * a.dkh + d * 2) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(a.dv + b * a.dvb + (int64_t)r * a.dvt + hk * a.dvh + d * 2) = make_uint4(0, 0, 0, 0);
+            } else {
+                *reinterpret_cast<uint4 *>(a.dq + b * a.dqb + (int64_t)r * a.dqt + h * a.dqh + d * 2) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        return;
+    }
+
+    if (warp == 8) {
+        tmem_alloc<S::columns>(smem_u32(&tmem_at));
+        if (lane == 0) tma_prefetch(&maps.x), tma_prefetch(&maps.y), tma_prefetch(&maps.u), tma_prefetch(&maps.w);
+    }
+    if (tid == 0) {
+        mbar_init(x_full, 1);
+        for (int s = 0; s < ST; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
+        for (int s = 0; s < NB; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(ds_full + 8 * s, kMath);
+        mbar_init(last, 1);
+        fence_barrier_init();
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tm = tmem_at;
+    bool ok = true;
+
+    if (warp == 8) {
+        if (lane == 0) {  // loads
+            mbar_expect(x_full, 2 * S::x_bytes);
+            for (int p = 0; p < S::panels; ++p) {
+                tma_load(sx + p * kRows * 128, &maps.x, x_full, p * 64, r0, DKV ? hk : h, b);
+                tma_load(sy + p * kRows * 128, &maps.y, x_full, p * 64, r0, DKV ? hk : h, b);
+            }
+            int x = 0;
+            for (; x < count; ++x) {
+                const int s = x % ST, t0 = tile_row(x), th = DKV ? tile_head(x) : hk;
+                if (x >= ST) ok = mbar_wait(free_ + 8 * s, ((x / ST) & 1) ^ 1);
+                if (!ok) break;
+                const uint32_t bar = full + 8 * s;
+                mbar_expect(bar, 2 * S::u_bytes + S::vec_bytes);
+                for (int p = 0; p < S::panels; ++p) {
+                    tma_load(su + s * S::u_bytes + p * kStream * 128, &maps.u, bar, p * 64, t0, th, b);
+                    tma_load(sw + s * S::u_bytes + p * kStream * 128, &maps.w, bar, p * 64, t0, th, b);
+                }
+                if constexpr (DKV) {
+                    // 64 values each, which may reach into the next row or the padding behind the last one: those are masked
+                    const int64_t at = ((int64_t)b * a.H + th) * a.lse_row + t0;
+                    bulk_load(svec + s * S::vec_bytes, a.lse + at, kStream * 4, bar);
+                    bulk_load(svec + s * S::vec_bytes + kStream * 4, a.delta + at, kStream * 4, bar);
+                }
+            }
+            if (!ok) {  // gave up: the copies in flight land before the block ends
+                report(a.error);
+                mbar_wait(x_full, 0);
+                for (int y = max(0, x - ST); y < x; ++y) mbar_wait(full + 8 * (y % ST), (y / ST) & 1);
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {  // products
+            constexpr uint32_t kind_s = mma_kind<bf, kRows, kStream, false>(), kind_acc = mma_kind<bf, kRows, DP, true>();
+            const int steps = (a.D + 15) / 16;
+            auto scores = [&](int x) {
+                const int s = x % ST;
+                if (!mbar_wait(full + 8 * s, (x / ST) & 1)) return false;
+                tc_after();
+                const uint32_t d = tm + (x % NB) * 2 * kStream;
+                for (int kk = 0; kk < steps; ++kk)
+                    mma_ss(d, operand(sx + (kk / 4) * kRows * 128 + (kk % 4) * 32, 0),
+                           operand(su + s * S::u_bytes + (kk / 4) * kStream * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
+                for (int kk = 0; kk < steps; ++kk)
+                    mma_ss(d + kStream, operand(sy + (kk / 4) * kRows * 128 + (kk % 4) * 32, 0),
+                           operand(sw + s * S::u_bytes + (kk / 4) * kStream * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
+                mma_commit(s_full + 8 * (x % NB));
+                return true;
+            };
+            ok = mbar_wait(x_full, 0);
+            for (int x = 0; x < NB && x < count && ok; ++x) ok = scores(x);
+            for (int x = 0; x < count && ok; ++x) {
+                const int s = x % ST;
+                ok = mbar_wait(ds_full + 8 * (x % NB), (x / NB) & 1);
+                if (!ok) break;
+                tc_after();
+                const uint32_t d = tm + (x % NB) * 2 * kStream;
+                // 32 columns of each half lie packed in the first 16 of their place
+                if constexpr (DKV) {
+#pragma unroll
+                    for (int kk = 0; kk < kStream / 16; ++kk)
+                        mma_ts(tm + S::acc + DP, d + (kk / 2) * 32 + (kk % 2) * 8, operand(sw + s * S::u_bytes + kk * 2048, kStream * 128), kind_acc,
+                               x > 0 || kk > 0);
+                }
+#pragma unroll
+                for (int kk = 0; kk < kStream / 16; ++kk)
+                    mma_ts(tm + S::acc, d + kStream + (kk / 2) * 32 + (kk % 2) * 8, operand(su + s * S::u_bytes + kk * 2048, kStream * 128), kind_acc,
+                           x > 0 || kk > 0);
+                mma_commit(free_ + 8 * s);
+                if (x + NB < count) ok = scores(x + NB);
+            }
+            mma_commit(last);
+            if (!ok) report(a.error);
+        }
+    } else {  // a row and 32 columns each
+        const int half = warp >> 2, row = tid & 127, r = r0 + row;
+        const uint32_t mine = tm + ((uint32_t)((warp & 3) * 32) << 16);
+        float lse = 0.f, delta = 0.f, amp = 1.f;
+        if constexpr (!DKV) {
+            ok = mbar_wait(x_full, 0);
+            if (ok) {
+                float top = 0.f;
+                if (r < n) {
+                    const char *o = a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh;
+                    for (int c = 0; c * 8 < a.D; ++c) {
+                        Vec<T, 8> x = *reinterpret_cast<const Vec<T, 8> *>(o + c * 16), g;
+                        uint4 w;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                     : "r"(sy + (c / 8) * kRows * 128 + row * 128 + (((c % 8) ^ (row & 7)) * 16)));
+                        *reinterpret_cast<uint4 *>(&g) = w;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float f = to_f(g.v[e]);
+                            delta = fmaf(to_f(x.v[e]), f, delta);
+                            if (!bf) top = fmaxf(top, fabsf(f));
+                        }
+                    }
+                    const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + r;
+                    lse = a.lse[at];
+                    if (half == 0) a.delta[at] = delta;
+                }
+                if (!bf) {
+                    amp = amp_of(__float_as_uint(top));
+                    top = warp_max(top);
+                    if (half == 0 && lane == 0 && top > 0.f) atomicMax(ex.amax + b * a.Hkv + hk, __float_as_uint(top));
+                }
+            }
+        } else if (!bf) {
+            amp = amp_of(ex.amax[b * a.Hkv + hk]);
+        }
+        for (int x = 0; x < count; ++x) {
+            const int t0 = tile_row(x), s = x % ST;
+            if (ok) ok = mbar_wait(s_full + 8 * (x % NB), (x / NB) & 1);
+            if (DKV && ok) ok = mbar_wait(full + 8 * s, (x / ST) & 1);  // lse and delta of the tile (done by then)
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_after();
+            const uint32_t at = mine + (x % NB) * 2 * kStream + half * 32;
+            uint32_t us[32], ud[32];
+            tc_ld32(at, us);
+            tc_ld32(at + kStream, ud);
+            tc_wait_ld(us);
+            tc_touch(ud);
+            const int c0 = t0 + half * 32;
+            bool whole;
+            if (DKV) whole = r0 + kRows - 1 <= t0 && t0 + kStream <= n && (t0 + kStream - 1 - r0 < a.window || r0 + kRows <= a.sinks);
+            else whole = t0 + kStream - 1 <= r0 && (r0 + kRows - 1 - t0 < a.window || t0 + kStream <= a.sinks);
+            uint32_t pp[16], pd[16];
+            auto math = [&](auto masked) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    float l4[4] = {lse, lse, lse, lse}, d4[4] = {delta, delta, delta, delta};
+                    if constexpr (DKV) {
+                        const uint32_t v = svec + s * S::vec_bytes + (half * 32 + c) * 4;
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(l4[0]), "=f"(l4[1]), "=f"(l4[2]), "=f"(l4[3]) : "r"(v));
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(d4[0]), "=f"(d4[1]), "=f"(d4[2]), "=f"(d4[3])
+                                     : "r"(v + kStream * 4));
+                    }
+                    float p[4], d[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[e] = exp2_fast(fmaf(__uint_as_float(us[c + e]), a.scale_log2, -l4[e]));
+                        d[e] = p[e] * (__uint_as_float(ud[c + e]) - d4[e]);
+                        if (!bf) d[e] *= amp;
+                        if (masked.value) {
+                            const int i = DKV ? c0 + c + e : r, j = DKV ? r : c0 + c + e;
+                            const bool on = j <= i && (i - j < a.window || j < a.sinks) && (!DKV || i < n);
+                            if (!on) p[e] = 0.f;
+                            if (!on || one_key(i, a.window, a.sinks)) d[e] = 0.f;
+                        }
+                    }
+                    if constexpr (DKV) pp[c / 2] = pack2(p[0], p[1], T()), pp[c / 2 + 1] = pack2(p[2], p[3], T());
+                    pd[c / 2] = pack2(d[0], d[1], T()), pd[c / 2 + 1] = pack2(d[2], d[3], T());
+                }
+            };
+            if (whole) math(std::false_type());
+            else math(std::true_type());
+            if constexpr (DKV) tc_st16(at, pp);
+            tc_st16(at + kStream, pd);
+            // rows behind the sequence meet zeros, but what they hold may be infinite: they are zeroed
+            if (n < a.T && t0 + kStream > n) {
+                constexpr int C = DP / 8;
+                const int lo = n - t0;
+                for (int e = tid; e < (kStream - lo) * C; e += kMath) {
+                    const int rr = lo + e / C, c = e % C;
+                    const uint32_t off = s * S::u_bytes + (c / 8) * kStream * 128 + rr * 128 + (c % 8) * 16;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(su + off), "r"(0) : "memory");
+                    if (DKV) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sw + off), "r"(0) : "memory");
+                }
+                fence_async();
+                __syncwarp();
+            }
+            tc_wait_st();
+            tc_before();
+            mbar_arrive(ds_full + 8 * (x % NB));
+        }
+        if (ok) ok = mbar_wait(last, 0);
+        if (__all_sync(0xffffffffu, ok)) {
+            tc_after();
+            // dq: each half takes its half of the columns; dk and dv: one each
+            const uint32_t stage = DKV && half ? sy : sx;
+            const uint32_t from = mine + S::acc + (DKV && half ? DP : 0);
+            const int c_lo = DKV ? 0 : half * (DP / 2), c_hi = DKV ? DP : c_lo + DP / 2;
+            const float by = DKV && half ? 1.f : a.scale / amp;
+            const bool live = r < n;
+            float *part = nullptr;
+            if (DKV && parted)
+                part = ex.parts + (((((int64_t)b * a.Hkv + hk) * ex.sink_tiles + r0 / kRows) * ex.splits + split) * 2 + half) * (kRows * DP) + row * DP;
+#pragma unroll 1
+            for (int c = c_lo; c < c_hi; c += 32) {
+                uint32_t w[32];
+                tc_ld32(from + c, w);
+                tc_wait_ld(w);
+                if (DKV && parted) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(part + c + e) =
+                            live ? make_float4(__uint_as_float(w[e]) * by, __uint_as_float(w[e + 1]) * by, __uint_as_float(w[e + 2]) * by,
+                                               __uint_as_float(w[e + 3]) * by)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        y[k] = live ? pack2(__uint_as_float(w[e + 2 * k]) * by, __uint_as_float(w[e + 2 * k + 1]) * by, T()) : 0u;
+                    const int chunk = (c % 64 + e) / 8;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (c / 64) * kRows * 128 + row * 128 + ((chunk ^ (row & 7)) * 16)),
+                                 "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
+                                 : "memory");
+                }
+            }
+            __syncwarp();
+            if (!(DKV && parted)) {
+                char *out = DKV ? (half ? a.dv + b * a.dvb + hk * a.dvh : a.dk + b * a.dkb + hk * a.dkh) : a.dq + b * a.dqb + h * a.dqh;
+                const int64_t step = DKV ? (half ? a.dvt : a.dkt) : a.dqt;
+                constexpr int C = DKV ? DP / 8 : DP / 16;
+                for (int e = lane; e < 32 * C; e += 32) {
+                    const int rr = (warp & 3) * 32 + e / C, c = e % C + c_lo / 8;
+                    uint4 y;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                                 : "r"(stage + (c / 8) * kRows * 128 + rr * 128 + (((c % 8) ^ (rr & 7)) * 16)));
+                    if (r0 + rr < a.T && c * 8 < a.D) *reinterpret_cast<uint4 *>(out + (int64_t)(r0 + rr) * step + c * 16) = y;
+                }
+            }
+        } else if (lane == 0) {
+            report(a.error);
+        }
+        tc_before();
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == 8) tmem_free<S::columns>(tm);
+}
+
+// dk and dv of the sinks' key tiles from their parts, in order
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, const Extra ex) {
+    const int hk = blockIdx.y, b = blockIdx.z;
+    const int64_t tile0 = ((int64_t)b * a.Hkv + hk) * ex.sink_tiles;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < ex.sink_tiles * 2 * kRows * (DP / 8); i += gridDim.x * 256) {
+        const int d = (i % (DP / 8)) * 8, row = i / (DP / 8) % kRows, which = i / (DP / 8) / kRows % 2, tile = i / (DP / 8) / kRows / 2;
+        const int j = tile * kRows + row;
+        if (j >= a.T || d >= a.D) continue;
+        float s[8] = {};
+        for (int p = 0; p < ex.splits; ++p) {
+            const float4 *f = reinterpret_cast<const float4 *>(ex.parts + ((((tile0 + tile) * ex.splits + p) * 2 + which) * kRows + row) * DP + d);
+            const float4 x = f[0], y = f[1];
+            s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w, s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
+        }
+        char *out = which ? a.dv + b * a.dvb + (int64_t)j * a.dvt + hk * a.dvh : a.dk + b * a.dkb + (int64_t)j * a.dkt + hk * a.dkh;
+        *reinterpret_cast<uint4 *>(out + d * 2) = make_uint4(pack2(s[0], s[1], T()), pack2(s[2], s[3], T()), pack2(s[4], s[5], T()), pack2(s[6], s[7], T()));
+    }
+}
+
+// how many parts the sinks' key tiles are cut into: so that a part is no longer than a key tile without sinks or than an SM's
+// share of all tiles, whichever is more
+int splits_of(const cail_ops_attention_args *c, int sms) {
+    if (c->sinks == 0 || c->window >= c->T) return 1;
+    const int64_t group = c->H / c->Hkv, tiles = (c->T + kRows - 1) / kRows, q_tiles = (c->T + kStream - 1) / kStream;
+    int64_t sink_tiles = (std::min(c->sinks, c->T) + kRows - 1) / kRows;
+    const int64_t plain = group * ((c->window + kRows) / kStream + 1), sunk = group * q_tiles;
+    if (sunk <= plain) return 1;
+    const int64_t all = (int64_t)c->B * c->Hkv * ((tiles - sink_tiles) * plain + sink_tiles * sunk);
+    const int64_t slots = (int64_t)sms * (c->D <= 64 ? 2 : 1), share = std::max(plain, all / slots);
+    return (int)std::min<int64_t>(32, (sunk + share - 1) / share);
+}
+
+struct Layout {
+    size_t amax, parts, total;
+    int splits, sink_tiles;
+};
+Layout layout_of(const cail_ops_attention_args *c) {
+    Layout l = {};
+    l.splits = splits_of(c, sm_count());
+    l.sink_tiles = l.splits > 1 ? (std::min(c->sinks, c->T) + kRows - 1) / kRows : 0;
+    size_t at = 0;
+    l.amax = at;
+    if (c->type == CAIL_OPS_F16) at += ((size_t)c->B * c->Hkv * 4 + 255) / 256 * 256;
+    l.parts = at;
+    const size_t dp = c->D <= 64 ? 64 : 128;
+    if (l.splits > 1) at += (size_t)c->B * c->Hkv * l.sink_tiles * l.splits * 2 * kRows * dp * 4;
+    l.total = at;
+    return l;
+}
+
+template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnArgs a, cudaStream_t st) {
+    const Layout l = layout_of(c);
+    if (c->workspace_bytes < l.total || (l.total && (!c->workspace || !aligned(c->workspace, 16))))
+        return fail(CAIL_OPS_EINVAL, "window attention backward: a workspace of %zu bytes is needed", l.total);
+    Extra ex = {};
+    ex.amax = reinterpret_cast<unsigned *>(static_cast<char *>(c->workspace) + l.amax);
+    ex.parts = reinterpret_cast<float *>(static_cast<char *>(c->workspace) + l.parts);
+    ex.splits = l.splits, ex.sink_tiles = l.sink_tiles;
+    if (c->type == CAIL_OPS_F16) {
+        cudaError_t e = cudaMemsetAsync(ex.amax, 0, (size_t)a.B * a.Hkv * 4, st);
+        if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
+    }
+    // the same arrays with boxes of 128 and of 64 rows
+    Maps q, k;
+    if (int rc = tensor_map(&q.x, c->q, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
+    if (int rc = tensor_map(&q.y, c->dout, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
+    if (int rc = tensor_map(&q.u, c->k, c->type, a.B, a.T, a.Hkv, a.D, kStream)) return rc;
+    if (int rc = tensor_map(&q.w, c->v, c->type, a.B, a.T, a.Hkv, a.D, kStream)) return rc;
+    if (int rc = tensor_map(&k.x, c->k, c->type, a.B, a.T, a.Hkv, a.D, kRows)) return rc;
+    if (int rc = tensor_map(&k.y, c->v, c->type, a.B, a.T, a.Hkv, a.D, kRows)) return rc;
+    if (int rc = tensor_map(&k.u, c->q, c->type, a.B, a.T, a.H, a.D, kStream)) return rc;
+    if (int rc = tensor_map(&k.w, c->dout, c->type, a.B, a.T, a.H, a.D, kStream)) return rc;
+    const unsigned tiles = (a.T + kRows - 1) / kRows;
+    constexpr int sm_q = Shape<DP, false>::smem, sm_k = Shape<DP, true>::smem;
+    cudaError_t e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_q);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_k);
+    if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
+    tc_backward_kernel<T, DP, false><<<dim3(tiles, a.H, a.B), kThreads, sm_q, st>>>(a, ex, q);
+    if (int rc = launched("window attention backward")) return rc;
+    const unsigned blocks = tiles + ex.sink_tiles * (ex.splits - 1);
+    tc_backward_kernel<T, DP, true><<<dim3(blocks, a.Hkv, a.B), kThreads, sm_k, st>>>(a, ex, k);
+    if (int rc = launched("window attention backward")) return rc;
+    if (ex.splits == 1) return CAIL_OPS_OK;
+    const unsigned grid = ((unsigned)ex.sink_tiles * 2 * kRows * (DP / 8) + 255) / 256;
+    join_kernel<T, DP><<<dim3(std::min(grid, 1024u), a.Hkv, a.B), 256, 0, st>>>(a, ex);
+    return launched("window attention backward");
+}
+
+}  // namespace
+
+bool tc_takes_backward(const cail_ops_attention_args *a) {
+    return tc_takes(a) && tma_takes(a->dout, a->B, a->T, a->H) && rows_aligned(a->dq, a->B, a->T, a->H, 2, 16) &&
+           rows_aligned(a->dk, a->B, a->T, a->Hkv, 2, 16) && rows_aligned(a->dv, a->B, a->T, a->Hkv, 2, 16) && aligned(a->lse, 16) &&
+           aligned(a->delta, 16);
+}
+
+size_t tc_workspace(const cail_ops_attention_args *c) { return layout_of(c).total; }
+
+int tc_backward(const cail_ops_attention_args *c, cudaStream_t st) {
+    AttnArgs a = attn_args(c, true);
+    a.error = device_error_flag();
+    if (!a.error) return fail(CAIL_OPS_ECUDA, "window attention backward: no error word for this device");
+    if (c->type == CAIL_OPS_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(c, a, st) : launch<__nv_bfloat16, 128>(c, a, st);
+    return a.D <= 64 ? launch<__half, 64>(c, a, st) : launch<__half, 128>(c, a, st);
+}
+
+}  // namespace cailops

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             const int r = i0 + i / C, d = (i % C) * 8;
             if (r < a.T && d < a.D) *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh + d * 2) = make_uint4(0, 0, 0, 0);
         }
-        if (a.lse && tid < kRows && i0 + tid < a.T) a.lse[((int64_t)b * a.H + h) * a.T + i0 + tid] = 0.f;
+        if (a.lse && tid < kRows && i0 + tid < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i0 + tid] = 0.f;
         return;
     }
     if (warp == 4) {
@@ -114,12 +114,12 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
     } else if (warp == 5) {
         if (lane == 0) {  // products
             constexpr uint32_t kind_s = mma_kind<bf, kRows, kKeys, false>(), kind_o = mma_kind<bf, kRows, DP, true>();
+            const int steps = (a.D + 15) / 16;
             auto scores = [&](int x) {
                 const int s = x % S::stages;
                 if (!mbar_wait(k_full + 8 * s, (x / S::stages) & 1)) return false;
                 tc_after();
-#pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
+                for (int kk = 0; kk < steps; ++kk)
                     mma_ss(tm + (x & 1) * kKeys, operand(sq + (kk / 4) * kRows * 128 + (kk % 4) * 32, 0),
                            operand(sk + s * S::kv_bytes + (kk / 4) * kKeys * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
                 mma_commit(k_free + 8 * s);
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
                              : "r"(sq + (c / 8) * kRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16)));
                 if (i0 + r < a.T && c * 8 < a.D) *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)(i0 + r) * a.ot + h * a.oh + c * 16) = y;
             }
-            if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.T + i] = live && l > 0.f ? fmaf(m, a.scale_log2, log2f(l)) : 0.f;
+            if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = live && l > 0.f ? fmaf(m, a.scale_log2, log2f(l)) : 0.f;
         } else if (lane == 0) {
             report(a.error);
         }
@@ -287,7 +287,7 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, const
 
 // 16-bit elements in rows that TMA can load (16-byte multiples), a positive
 // scale (the row maximum is taken before scaling)
-bool tc_takes(const cail_ops_attention_args *a, bool backward) {
+bool tc_takes(const cail_ops_attention_args *a) {
     if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f)) return false;
     if (!tma_takes(a->q, a->B, a->T, a->H) || !tma_takes(a->k, a->B, a->T, a->Hkv) || !tma_takes(a->v, a->B, a->T, a->Hkv)) return false;
     return rows_aligned(a->o, a->B, a->T, a->H, 2, 16);

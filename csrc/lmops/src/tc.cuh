@@ -70,6 +70,12 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *m, uin
         "l"(m), "r"(x), "r"(t), "r"(h), "r"(b), "r"(bar)
         : "memory");
 }
+// `bytes` (a multiple of 16) from a 16-byte boundary
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap *m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
 
 // ------------------------------------------------------------ tensor memory

@@ -299,7 +299,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
                           int64_t window, int64_t sinks, double scale) {
         const Tensor lengths = or_none(lengths_);
         const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
-        Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+        Tensor lse = at::empty({(int64_t)CAIL_OPS_LSE_FLOATS(q.size(0), q.size(2), q.size(1))}, q.options().dtype(at::kFloat));
         Tensor o = attention_forward(q, k, v, {lengths, window, sinks, scale}, lse.data_ptr<float>());
         ctx->save_for_backward({q, k, v, o, lse, lengths});
         ctx->saved_data["window"] = window;
