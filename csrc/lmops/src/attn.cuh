@@ -28,6 +28,8 @@ AttnArgs attn_args(const cail_ops_attention_args *a, bool backward);
 // the tensor-core path (attn_tc_*.cu): whether it takes the call, and the call
 bool tc_takes(const cail_ops_attention_args *a);
 bool tc_takes_backward(const cail_ops_attention_args *a);
+bool tc_takes_decode(const cail_ops_attention_args *a);
+int tc_decode(const cail_ops_attention_args *a, cudaStream_t st);
 int tc_forward(const cail_ops_attention_args *a, cudaStream_t st);
 int tc_backward(const cail_ops_attention_args *a, cudaStream_t st);
 size_t tc_workspace(const cail_ops_attention_args *a);

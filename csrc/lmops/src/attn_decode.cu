@@ -216,6 +216,7 @@ extern "C" int cail_ops_window_attention_decode(const cail_ops_attention_args *a
     if (int rc = attn_check(a, false, "window attention decode")) return rc;
     if (!a->lengths) return fail(CAIL_OPS_EINVAL, "window attention decode: lengths are needed");
     if (a->B == 0) return CAIL_OPS_OK;
+    if (tc_takes_decode(a)) return tc_decode(a, static_cast<cudaStream_t>(stream));
     const size_t s = type_size(a->type);
     const bool vec = a->D % (16 / s) == 0 && rows_aligned(a->q, a->B, 1, a->H, s, 16) &&
                      rows_aligned(a->k, a->B, a->T, a->Hkv, s, 16) && rows_aligned(a->v, a->B, a->T, a->Hkv, s, 16);

@@ -1,0 +1,344 @@
+// attn_tc_decode.cu — one token per sequence against a long 16-bit cache, on
+// the tensor cores.
+//
+// The cache is the only large operand, so it takes the 128-row side of both
+// products and up to 16 query heads that share a key head take the other:
+//   S^T [128 keys x 16 heads] = K Q^T,   O^T [D x 16] += V^T P
+// K and V tiles stream through shared memory by TMA and are never touched by
+// a thread; 128 threads hold one key each, take 16 scores from tensor memory,
+// agree on the heads' running maxima and put p (in the cache's type) into
+// shared memory for the second product.  O^T stays in tensor memory and is
+// rescaled only when a maximum has grown by more than 2^8.
+//
+// The keys are the sinks (padded to 16) and then the window; they are split
+// over the blocks of a cluster, which join over distributed shared memory.
+// Bound by reading the cache: 2 blocks per SM with 96 KB of tiles in flight
+// each.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn.cuh"
+#include "tc.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace cailops {
+namespace {
+
+constexpr int kKeys = 128, kHeads = 16, kThreads = 192;
+
+template <int DP> struct Shape {
+    static constexpr int panels = DP / 64;
+    static constexpr int slots = DP == 64 ? 6 : 3;  // tiles of K and V in turn
+    static constexpr int tile_bytes = kKeys * DP * 2, q_bytes = kHeads * DP * 2, p_bytes = kHeads * kKeys * 2;
+    static constexpr int smem = 1024 + slots * tile_bytes + q_bytes + 2 * p_bytes;
+    static constexpr int barriers = 2 * slots + 2 + 2 + 3;
+};
+
+struct Maps {
+    CUtensorMap k, v, k16, v16;  // boxes of 128 keys and of 16
+};
+
+__device__ __forceinline__ float warp_max_fast(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a, const __grid_constant__ Maps maps) {
+    using S = Shape<DP>;
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ char raw[];
+    __shared__ __align__(8) uint64_t bars[S::barriers];
+    __shared__ uint32_t tmem_at;
+    __shared__ float wmax[2][4][kHeads];
+    __shared__ float bm[kHeads], bl[kHeads], wl[4][kHeads];
+    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+    const uint32_t st = base, sq = st + S::slots * S::tile_bytes, sp = sq + S::q_bytes;
+    // [kHeads][DP], this block's sums: in the place of the tiles, when all of them are done with
+    float *const bo = reinterpret_cast<float *>(raw + (base - smem_u32(raw)));
+    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t full = bar0, free_ = full + 8 * S::slots, s_full = free_ + 8 * S::slots, p_full = s_full + 16, o_done = p_full + 16,
+                   o_last = o_done + 8, q_full = o_last + 8;
+    cg::cluster_group cl = cg::this_cluster();
+    const int blocks = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    const int chunks = (a.group + kHeads - 1) / kHeads;
+    const int b = blockIdx.z, hk = blockIdx.y / chunks, h0 = hk * a.group + (blockIdx.y % chunks) * kHeads;
+    const int heads = min(kHeads, (hk + 1) * a.group - h0);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n = length_of(a, b);
+    // the keys, numbered: the sinks before the window, up to a multiple of 16, then the window
+    const int win0 = max(0, n - a.window), nsink = min(a.sinks, win0), pad = (nsink + 15) / 16 * 16, total = pad + n - win0;
+    const int tiles = (total + kKeys - 1) / kKeys, per = (tiles + blocks - 1) / blocks;
+    const int from = min(tiles, rank * per), count = min(tiles, from + per) - from;
+
+    if (warp == 4) {
+        tmem_alloc<64>(smem_u32(&tmem_at));
+        if (lane == 0) tma_prefetch(&maps.k), tma_prefetch(&maps.v);
+    }
+    if (tid == 0) {
+        for (int s = 0; s < S::slots; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
+        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 128);
+        mbar_init(o_done, 1), mbar_init(o_last, 1), mbar_init(q_full, 128);
+        fence_barrier_init();
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tm = tmem_at;
+    bool ok = true;
+
+    if (count == 0) {
+        if (tid < kHeads) bm[tid] = -INFINITY, bl[tid] = 0.f;
+        for (int i = tid; i < kHeads * DP; i += kThreads) bo[i] = 0.f;
+    } else if (warp == 4) {
+        if (lane == 0) {  // loads
+            int y = 0;
+            for (; y < 2 * count; ++y) {
+                const int s = y % S::slots, v0 = (from + y / 2) * kKeys;
+                const bool is_v = y & 1;
+                if (y >= S::slots) ok = mbar_wait(free_ + 8 * s, ((y / S::slots) & 1) ^ 1);
+                if (!ok) break;
+                const uint32_t bar = full + 8 * s, dst = st + s * S::tile_bytes;
+                mbar_expect(bar, S::tile_bytes);
+                for (int p = 0; p < S::panels; ++p) {
+                    if (v0 >= pad || v0 + kKeys <= pad) {
+                        tma_load(dst + p * kKeys * 128, is_v ? &maps.v : &maps.k, bar, p * 64, v0 >= pad ? win0 + v0 - pad : v0, hk, b);
+                    } else {  // sinks and window in one tile
+                        for (int g = 0; g < kKeys; g += 16)
+                            tma_load(dst + p * kKeys * 128 + g * 128, is_v ? &maps.v16 : &maps.k16, bar, p * 64,
+                                     v0 + g < pad ? v0 + g : win0 + v0 + g - pad, hk, b);
+                    }
+                }
+            }
+            if (!ok) {  // gave up: the copies in flight land before the block ends
+                report(a.error);
+                for (int z = max(0, y - S::slots); z < y; ++z) mbar_wait(full + 8 * (z % S::slots), (z / S::slots) & 1);
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {  // products
+            constexpr uint32_t kind_s = mma_kind<bf, kKeys, kHeads, false>();
+            // A = V^T: its rows (D) run along the tile's rows: MN-major
+            constexpr uint32_t kind_o = mma_kind<bf, 128, kHeads, false>() | (1u << 15);
+            const int steps = (a.D + 15) / 16;
+            auto scores = [&](int x) {
+                const int y = 2 * x, s = y % S::slots;
+                if (!mbar_wait(full + 8 * s, (y / S::slots) & 1)) return false;
+                tc_after();
+                for (int kk = 0; kk < steps; ++kk)
+                    mma_ss(tm + (x & 1) * kHeads, operand(st + s * S::tile_bytes + (kk / 4) * kKeys * 128 + (kk % 4) * 32, 0),
+                           operand(sq + (kk / 4) * kHeads * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
+                mma_commit(free_ + 8 * s);
+                mma_commit(s_full + 8 * (x & 1));
+                return true;
+            };
+            ok = mbar_wait(q_full, 0) && scores(0) && (count < 2 || scores(1));
+            for (int x = 0; x < count && ok; ++x) {
+                const int y = 2 * x + 1, s = y % S::slots;
+                ok = mbar_wait(full + 8 * s, (y / S::slots) & 1) && mbar_wait(p_full + 8 * (x & 1), (x >> 1) & 1);
+                if (!ok) break;
+                tc_after();
+                // D = 64: rows 64 and up of the product are not used; their operand lies 8 keys on, inside the tiles
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                    mma_ss(tm + 2 * kHeads, operand(st + s * S::tile_bytes + kk * 2048, DP == 64 ? 1024 : kKeys * 128),
+                           operand(sp + (x & 1) * S::p_bytes + (kk / 4) * kHeads * 128 + (kk % 4) * 32, 0), kind_o, x > 0 || kk > 0);
+                mma_commit(free_ + 8 * s);
+                mma_commit(o_done);
+                if (x + 2 < count) ok = scores(x + 2);
+            }
+            mma_commit(o_last);
+            if (!ok) report(a.error);
+        }
+    } else {  // one key each
+        // the queries, zeros beyond the heads and D, and zeros for p beyond the heads
+        for (int i = tid; i < kHeads * DP / 8; i += 128) {
+            const int g = i / (DP / 8), c = i % (DP / 8);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (g < heads && c * 8 < a.D) x = *reinterpret_cast<const uint4 *>(a.q + b * a.qb + (h0 + g) * a.qh + c * 16);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + (c / 8) * kHeads * 128 + g * 128 + (((c % 8) ^ (g & 7)) * 16)), "r"(x.x),
+                         "r"(x.y), "r"(x.z), "r"(x.w)
+                         : "memory");
+        }
+        for (int i = tid; i < 2 * S::p_bytes / 16; i += 128)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sp + i * 16), "r"(0) : "memory");
+        fence_async();
+        mbar_arrive(q_full);
+        const uint32_t mine = tm + ((uint32_t)(warp * 32) << 16);
+        float m[kHeads], l[kHeads];
+#pragma unroll
+        for (int g = 0; g < kHeads; ++g) m[g] = -INFINITY, l[g] = 0.f;
+        for (int x = 0; x < count; ++x) {
+            const int v = (from + x) * kKeys + tid;
+            const bool valid = v < pad ? v < nsink : v < total;
+            ok = ok && mbar_wait(s_full + 8 * (x & 1), (x >> 1) & 1);
+            uint32_t u[16];
+            float *f = reinterpret_cast<float *>(u);
+            __syncwarp();
+            tc_after();
+            tc_ld16(mine + (x & 1) * kHeads, u);
+            tc_wait_ld16(u);
+#pragma unroll
+            for (int g = 0; g < kHeads; ++g) {
+                if (g >= heads) break;
+                f[g] = valid ? f[g] * a.scale_log2 : -INFINITY;
+                const float w = warp_max_fast(f[g]);
+                if (lane == 0) wmax[x & 1][warp][g] = w;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            bool turned = false;
+            float turn[kHeads];
+#pragma unroll
+            for (int g = 0; g < kHeads; ++g) {
+                turn[g] = 1.f;
+                if (g >= heads) break;
+                const float top = fmaxf(fmaxf(wmax[x & 1][0][g], wmax[x & 1][1][g]), fmaxf(wmax[x & 1][2][g], wmax[x & 1][3][g]));
+                if (m[g] == -INFINITY) {
+                    m[g] = top;  // nothing of this head is in O yet
+                } else if (top - m[g] > 8.f) {
+                    turn[g] = exp2_fast(m[g] - top);
+                    l[g] *= turn[g];
+                    m[g] = top;
+                    turned = true;
+                }
+            }
+            if (turned) {  // the same in all 128 threads
+                ok = ok && mbar_wait(o_done, (x - 1) & 1);
+                __syncwarp();
+                tc_after();
+                uint32_t w[16];
+                tc_ld16(mine + 2 * kHeads, w);
+                tc_wait_ld16(w);
+#pragma unroll
+                for (int g = 0; g < kHeads; ++g) w[g] = __float_as_uint(__uint_as_float(w[g]) * turn[g]);
+                tc_st16(mine + 2 * kHeads, w);
+                tc_wait_st();
+            }
+            const uint32_t col = sp + (x & 1) * S::p_bytes + (tid / 64) * kHeads * 128 + (tid % 8) * 2;
+#pragma unroll
+            for (int g = 0; g < kHeads; ++g) {
+                if (g >= heads) break;
+                const float p = exp2_fast(f[g] - (m[g] == -INFINITY ? 0.f : m[g]));
+                l[g] += p;
+                const T t = from_f<T>(p);
+                asm volatile("st.shared.b16 [%0], %1;" ::"r"(col + g * 128 + (((tid % 64) / 8) ^ (g & 7)) * 16), "h"(*reinterpret_cast<const uint16_t *>(&t))
+                             : "memory");
+            }
+            if (!valid) {  // what a key that is not seen holds may be infinite: its values are zeroed
+                const int y = 2 * x + 1, s = y % S::slots;
+                ok = ok && mbar_wait(full + 8 * s, (y / S::slots) & 1);
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(st + s * S::tile_bytes + (c / 8) * kKeys * 128 + tid * 128 + (c % 8) * 16),
+                                 "r"(0)
+                                 : "memory");
+            }
+            __syncwarp();
+            fence_async();
+            tc_before();
+            mbar_arrive(p_full + 8 * (x & 1));
+        }
+        ok = ok && mbar_wait(o_last, 0);
+        __syncwarp();
+        if (!ok && lane == 0) report(a.error);
+        tc_after();
+        uint32_t w[16];
+        tc_ld16(mine + 2 * kHeads, w);
+        tc_wait_ld16(w);
+        if (tid < DP)
+#pragma unroll
+            for (int g = 0; g < kHeads; ++g) bo[g * DP + tid] = __uint_as_float(w[g]);
+#pragma unroll
+        for (int g = 0; g < kHeads; ++g) {
+            if (g >= heads) break;
+            const float sum = warp_sum(l[g]);
+            if (lane == 0) wl[warp][g] = sum;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (tid < heads) bl[tid] = (wl[0][tid] + wl[1][tid]) + (wl[2][tid] + wl[3][tid]);
+#pragma unroll
+        for (int g = 0; g < kHeads; ++g)
+            if (tid == g) bm[g] = m[g];
+        tc_before();
+    }
+    __syncwarp();
+    cl.sync();
+    // blocks of the cluster: each joins a part of the output
+    for (int i = rank * kThreads + tid; i < heads * a.D; i += blocks * kThreads) {
+        const int g = i / a.D, d = i % a.D;
+        float top = -INFINITY;
+        for (int r = 0; r < blocks; ++r) top = fmaxf(top, *cl.map_shared_rank(&bm[g], r));
+        const float off = top == -INFINITY ? 0.f : top;
+        float x = 0.f, sum = 0.f;
+        for (int r = 0; r < blocks; ++r) {
+            const float f = exp2_fast(*cl.map_shared_rank(&bm[g], r) - off);
+            x = fmaf(*cl.map_shared_rank(bo + g * DP + d, r), f, x);
+            sum = fmaf(*cl.map_shared_rank(&bl[g], r), f, sum);
+        }
+        reinterpret_cast<T *>(a.o + b * a.ob + (h0 + g) * a.oh)[d] = from_f<T>(sum == 0.f ? 0.f : x / sum);
+    }
+    cl.sync();  // the others' sums stay until they are read
+    if (warp == 4) tmem_free<64>(tm);
+}
+
+template <typename T, int DP> int launch(const cail_ops_attention_args *c, const AttnArgs &a, cudaStream_t st) {
+    using S = Shape<DP>;
+    Maps maps;
+    if (int rc = tensor_map(&maps.k, c->k, c->type, a.B, a.T, a.Hkv, a.D, kKeys)) return rc;
+    if (int rc = tensor_map(&maps.v, c->v, c->type, a.B, a.T, a.Hkv, a.D, kKeys)) return rc;
+    if (int rc = tensor_map(&maps.k16, c->k, c->type, a.B, a.T, a.Hkv, a.D, 16)) return rc;
+    if (int rc = tensor_map(&maps.v16, c->v, c->type, a.B, a.T, a.Hkv, a.D, 16)) return rc;
+    cudaError_t e = cudaFuncSetAttribute(tc_decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+    if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention decode: %s", cudaGetErrorString(e));
+    e = cudaFuncSetAttribute(tc_decode_kernel<T, DP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention decode: %s", cudaGetErrorString(e));
+    const int chunks = (a.group + kHeads - 1) / kHeads;
+    const int64_t work = (int64_t)a.B * a.Hkv * chunks, keys = std::min((int64_t)a.T, (int64_t)a.window + a.sinks);
+    // Blocks per sequence and group: as many as give every SM up to two, each
+    // with two tiles or more.  More of them only add their starts and joins
+    // (64 sequences x 8 groups of 4096 keys, D 128: 170 us with 1, 185 with 2,
+    // 206 with 4).  Clusters of 16 only while they get an SM each: 8 groups of
+    // 16384 keys, 19.5 us against 29.6 with 8; 16 groups, 44 against 40.
+    const int64_t sms = sm_count();
+    int blocks = 1;
+    while (blocks < 16 && work * blocks * 2 <= (blocks < 8 ? 2 * sms : sms) && keys >= blocks * 2 * 2 * kKeys) blocks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks, a.Hkv * chunks, a.B);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)blocks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, tc_decode_kernel<T, DP>, a, maps);
+    return launched("window attention decode");
+}
+
+}  // namespace
+
+// 16-bit caches in rows that TMA can load, and enough of them: below this the
+// other kernel's shorter start wins (one head of 64: 256 keys 5.0 against
+// 7.3 us, 1024 keys 6.9 against 7.5, 4096 keys 16 against 10; a group of four
+// heads of 128: 64 keys 10.5 against 9.3, 1024 keys 15 against 9.3)
+bool tc_takes_decode(const cail_ops_attention_args *a) {
+    if (a->type == CAIL_OPS_F32 || a->D % 8 || a->T < 1) return false;
+    if (!rows_aligned(a->q, a->B, 1, a->H, 2, 16) || !tma_takes(a->k, a->B, a->T, a->Hkv) || !tma_takes(a->v, a->B, a->T, a->Hkv)) return false;
+    const int64_t keys = std::min((int64_t)a->T, (int64_t)a->window + a->sinks);
+    return keys * (a->H / a->Hkv >= 4 ? 2 : 1) * (a->D > 64 ? 2 : 1) >= 1024;
+}
+
+int tc_decode(const cail_ops_attention_args *c, cudaStream_t st) {
+    AttnArgs a = attn_args(c, false);
+    a.error = device_error_flag();
+    if (!a.error) return fail(CAIL_OPS_ECUDA, "window attention decode: no error word for this device");
+    if (c->type == CAIL_OPS_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(c, a, st) : launch<__nv_bfloat16, 128>(c, a, st);
+    return a.D <= 64 ? launch<__half, 64>(c, a, st) : launch<__half, 128>(c, a, st);
+}
+
+}  // namespace cailops

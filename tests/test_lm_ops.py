@@ -455,6 +455,12 @@ DECODE = [
     (2, 130, 9, 1, 80, 64, 300, [130, 128]),
     (1, 5000, 1, 1, 64, 5000, 0, [5000]),
     (2, 40, 3, 3, 8, 7, 1, [-3, 99]),
+    (3, 1300, 5, 1, 64, 1111, 17, [1300, 1128, 900]),
+    (1, 3000, 20, 1, 128, 2500, 33, [2999]),
+    (2, 2048, 1, 1, 72, 2048, 0, [2048, 0]),
+    (2, 1500, 4, 1, 128, 300, 300, [1500, 512]),
+    (1, 9000, 2, 2, 40, 9000, 5, [8999]),
+    (5, 1100, 2, 2, 64, 1024, 16, [1100, 1024, 1040, 1, 0]),
 ]
 
 
