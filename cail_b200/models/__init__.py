@@ -1,4 +1,4 @@
 """Models used by the benchmarks."""
-from .gpt2 import GPT2, GPT2Config
+from .gpt2 import GPT2, GPT2Config, KVCache
 
-__all__ = ["GPT2", "GPT2Config"]
+__all__ = ["GPT2", "GPT2Config", "KVCache"]
