@@ -102,9 +102,25 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         keys = KeyTiles(r0, r0 + kRows, n, a.window, a.sinks, kStream);
         count = keys.count;
     }
-    // tile x: its first row, and its query head (dk, dv)
-    auto tile_row = [&](int x) { return DKV ? (q_begin + (first + x) % q_tiles) * kStream : keys.at(x) * kStream; };
-    auto tile_head = [&](int x) { return DKV ? h + (first + x) / q_tiles : h; };
+    // a walk over the tiles: the first row of the tile at hand, and its query head (dk, dv)
+    struct Walk {
+        int x, row, head;
+    };
+    auto begin_walk = [&] {
+        Walk w = {0, 0, h};
+        if constexpr (DKV) w.row = (q_begin + first % q_tiles) * kStream, w.head = h + first / q_tiles;
+        else w.row = keys.at(0) * kStream;
+        return w;
+    };
+    auto step = [&](Walk &w) {
+        ++w.x;
+        if constexpr (DKV) {
+            w.row += kStream;
+            if (w.row == (q_begin + q_tiles) * kStream) w.row = q_begin * kStream, ++w.head;
+        } else {
+            w.row = keys.at(w.x) * kStream;
+        }
+    };
 
     if (count == 0) {  // nothing sees or is seen: zeros
         constexpr int C = DP / 8;
@@ -134,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     if (tid == 0) {
         mbar_init(x_full, 1);
         for (int s = 0; s < ST; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
-        for (int s = 0; s < NB; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(ds_full + 8 * s, kMath);
+        for (int s = 0; s < NB; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(ds_full + 8 * s, kMath / 32);
         mbar_init(last, 1);
         fence_barrier_init();
     }
@@ -151,9 +167,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 tma_load(sx + p * kRows * 128, &maps.x, x_full, p * 64, r0, DKV ? hk : h, b);
                 tma_load(sy + p * kRows * 128, &maps.y, x_full, p * 64, r0, DKV ? hk : h, b);
             }
-            int x = 0;
-            for (; x < count; ++x) {
-                const int s = x % ST, t0 = tile_row(x), th = DKV ? tile_head(x) : hk;
+            Walk w = begin_walk();
+            for (; w.x < count; step(w)) {
+                const int x = w.x, s = x % ST, t0 = w.row, th = DKV ? w.head : hk;
                 if (x >= ST) ok = mbar_wait(free_ + 8 * s, ((x / ST) & 1) ^ 1);
                 if (!ok) break;
                 const uint32_t bar = full + 8 * s;
@@ -172,24 +188,32 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             if (!ok) {  // gave up: the copies in flight land before the block ends
                 report(a.error);
                 mbar_wait(x_full, 0);
-                for (int y = max(0, x - ST); y < x; ++y) mbar_wait(full + 8 * (y % ST), (y / ST) & 1);
+                for (int y = max(0, w.x - ST); y < w.x; ++y) mbar_wait(full + 8 * (y % ST), (y / ST) & 1);
             }
         }
     } else if (warp == 9) {
         if (lane == 0) {  // products
             constexpr uint32_t kind_s = mma_kind<bf, kRows, kStream, false>(), kind_acc = mma_kind<bf, kRows, DP, true>();
             const int steps = (a.D + 15) / 16;
+            // U and W as operands along their rows (scores) and down them (sums)
+            const uint64_t dx = operand(sx, 0), dy = operand(sy, 0), du = operand(su, 0), dw = operand(sw, 0), dut = operand(su, kStream * 128),
+                           dwt = operand(sw, kStream * 128);
             auto scores = [&](int x) {
                 const int s = x % ST;
                 if (!mbar_wait(full + 8 * s, (x / ST) & 1)) return false;
                 tc_after();
                 const uint32_t d = tm + (x % NB) * 2 * kStream;
-                for (int kk = 0; kk < steps; ++kk)
-                    mma_ss(d, operand(sx + (kk / 4) * kRows * 128 + (kk % 4) * 32, 0),
-                           operand(su + s * S::u_bytes + (kk / 4) * kStream * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
-                for (int kk = 0; kk < steps; ++kk)
-                    mma_ss(d + kStream, operand(sy + (kk / 4) * kRows * 128 + (kk % 4) * 32, 0),
-                           operand(sw + s * S::u_bytes + (kk / 4) * kStream * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
+                const uint64_t dus = moved(du, s * S::u_bytes), dws = moved(dw, s * S::u_bytes);
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    if (kk < steps)
+                        mma_ss(d, moved(dx, (kk / 4) * kRows * 128 + (kk % 4) * 32), moved(dus, (kk / 4) * kStream * 128 + (kk % 4) * 32), kind_s,
+                               kk > 0);
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    if (kk < steps)
+                        mma_ss(d + kStream, moved(dy, (kk / 4) * kRows * 128 + (kk % 4) * 32),
+                               moved(dws, (kk / 4) * kStream * 128 + (kk % 4) * 32), kind_s, kk > 0);
                 mma_commit(s_full + 8 * (x % NB));
                 return true;
             };
@@ -205,12 +229,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 if constexpr (DKV) {
 #pragma unroll
                     for (int kk = 0; kk < kStream / 16; ++kk)
-                        mma_ts(tm + S::acc + DP, d + (kk / 2) * 32 + (kk % 2) * 8, operand(sw + s * S::u_bytes + kk * 2048, kStream * 128), kind_acc,
+                        mma_ts(tm + S::acc + DP, d + (kk / 2) * 32 + (kk % 2) * 8, moved(dwt, s * S::u_bytes + kk * 2048), kind_acc,
                                x > 0 || kk > 0);
                 }
 #pragma unroll
                 for (int kk = 0; kk < kStream / 16; ++kk)
-                    mma_ts(tm + S::acc, d + kStream + (kk / 2) * 32 + (kk % 2) * 8, operand(su + s * S::u_bytes + kk * 2048, kStream * 128), kind_acc,
+                    mma_ts(tm + S::acc, d + kStream + (kk / 2) * 32 + (kk % 2) * 8, moved(dut, s * S::u_bytes + kk * 2048), kind_acc,
                            x > 0 || kk > 0);
                 mma_commit(free_ + 8 * s);
                 if (x + NB < count) ok = scores(x + NB);
@@ -255,8 +279,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         } else if (!bf) {
             amp = amp_of(ex.amax[b * a.Hkv + hk]);
         }
-        for (int x = 0; x < count; ++x) {
-            const int t0 = tile_row(x), s = x % ST;
+        for (Walk w = begin_walk(); w.x < count; step(w)) {
+            const int x = w.x, t0 = w.row, s = x % ST;
             if (ok) ok = mbar_wait(s_full + 8 * (x % NB), (x / NB) & 1);
             if (DKV && ok) ok = mbar_wait(full + 8 * s, (x / ST) & 1);  // lse and delta of the tile (done by then)
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -272,24 +296,34 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             if (DKV) whole = r0 + kRows - 1 <= t0 && t0 + kStream <= n && (t0 + kStream - 1 - r0 < a.window || r0 + kRows <= a.sinks);
             else whole = t0 + kStream - 1 <= r0 && (r0 + kRows - 1 - t0 < a.window || t0 + kStream <= a.sinks);
             uint32_t pp[16], pd[16];
+            const uint64_t scale2 = two(a.scale_log2, a.scale_log2);
             auto math = [&](auto masked) {
 #pragma unroll
                 for (int c = 0; c < 32; c += 4) {
-                    float l4[4] = {lse, lse, lse, lse}, d4[4] = {delta, delta, delta, delta};
+                    // minus lse and minus delta of the columns
+                    uint64_t l2[2] = {two(-lse, -lse), two(-lse, -lse)}, d2[2] = {two(-delta, -delta), two(-delta, -delta)};
                     if constexpr (DKV) {
                         const uint32_t v = svec + s * S::vec_bytes + (half * 32 + c) * 4;
+                        float l4[4], d4[4];
                         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(l4[0]), "=f"(l4[1]), "=f"(l4[2]), "=f"(l4[3]) : "r"(v));
                         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                                      : "=f"(d4[0]), "=f"(d4[1]), "=f"(d4[2]), "=f"(d4[3])
                                      : "r"(v + kStream * 4));
+                        l2[0] = two(-l4[0], -l4[1]), l2[1] = two(-l4[2], -l4[3]);
+                        d2[0] = two(-d4[0], -d4[1]), d2[1] = two(-d4[2], -d4[3]);
                     }
                     float p[4], d[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        p[e] = exp2_fast(fmaf(__uint_as_float(us[c + e]), a.scale_log2, -l4[e]));
-                        d[e] = p[e] * (__uint_as_float(ud[c + e]) - d4[e]);
-                        if (!bf) d[e] *= amp;
-                        if (masked.value) {
+                    for (int e = 0; e < 4; e += 2) {
+                        apart(fma_two(two(__uint_as_float(us[c + e]), __uint_as_float(us[c + e + 1])), scale2, l2[e / 2]), p[e], p[e + 1]);
+                        p[e] = exp2_fast(p[e]), p[e + 1] = exp2_fast(p[e + 1]);
+                        uint64_t t = add_two(two(__uint_as_float(ud[c + e]), __uint_as_float(ud[c + e + 1])), d2[e / 2]);
+                        if (!bf) t = mul_two(t, two(amp, amp));
+                        apart(mul_two(t, two(p[e], p[e + 1])), d[e], d[e + 1]);
+                    }
+                    if (masked.value) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
                             const int i = DKV ? c0 + c + e : r, j = DKV ? r : c0 + c + e;
                             const bool on = j <= i && (i - j < a.window || j < a.sinks) && (!DKV || i < n);
                             if (!on) p[e] = 0.f;
@@ -319,7 +353,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             }
             tc_wait_st();
             tc_before();
-            mbar_arrive(ds_full + 8 * (x % NB));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_full + 8 * (x % NB));
         }
         if (ok) ok = mbar_wait(last, 0);
         if (__all_sync(0xffffffffu, ok)) {

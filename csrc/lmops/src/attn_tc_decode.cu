@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a
     }
     if (tid == 0) {
         for (int s = 0; s < S::slots; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
-        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 128);
+        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 4);
         mbar_init(o_done, 1), mbar_init(o_last, 1), mbar_init(q_full, 128);
         fence_barrier_init();
     }
@@ -125,13 +125,17 @@ __global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a
             // A = V^T: its rows (D) run along the tile's rows: MN-major
             constexpr uint32_t kind_o = mma_kind<bf, 128, kHeads, false>() | (1u << 15);
             const int steps = (a.D + 15) / 16;
+            // D = 64: rows 64 and up of the second product are not used; their operand lies 8 keys on, inside the tiles
+            const uint64_t dt = operand(st, 0), dq = operand(sq, 0), dvt = operand(st, DP == 64 ? 1024 : kKeys * 128), dp = operand(sp, 0);
             auto scores = [&](int x) {
                 const int y = 2 * x, s = y % S::slots;
                 if (!mbar_wait(full + 8 * s, (y / S::slots) & 1)) return false;
                 tc_after();
-                for (int kk = 0; kk < steps; ++kk)
-                    mma_ss(tm + (x & 1) * kHeads, operand(st + s * S::tile_bytes + (kk / 4) * kKeys * 128 + (kk % 4) * 32, 0),
-                           operand(sq + (kk / 4) * kHeads * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    if (kk < steps)
+                        mma_ss(tm + (x & 1) * kHeads, moved(dt, s * S::tile_bytes + (kk / 4) * kKeys * 128 + (kk % 4) * 32),
+                               moved(dq, (kk / 4) * kHeads * 128 + (kk % 4) * 32), kind_s, kk > 0);
                 mma_commit(free_ + 8 * s);
                 mma_commit(s_full + 8 * (x & 1));
                 return true;
@@ -142,11 +146,10 @@ __global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a
                 ok = mbar_wait(full + 8 * s, (y / S::slots) & 1) && mbar_wait(p_full + 8 * (x & 1), (x >> 1) & 1);
                 if (!ok) break;
                 tc_after();
-                // D = 64: rows 64 and up of the product are not used; their operand lies 8 keys on, inside the tiles
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
-                    mma_ss(tm + 2 * kHeads, operand(st + s * S::tile_bytes + kk * 2048, DP == 64 ? 1024 : kKeys * 128),
-                           operand(sp + (x & 1) * S::p_bytes + (kk / 4) * kHeads * 128 + (kk % 4) * 32, 0), kind_o, x > 0 || kk > 0);
+                    mma_ss(tm + 2 * kHeads, moved(dvt, s * S::tile_bytes + kk * 2048),
+                           moved(dp, (x & 1) * S::p_bytes + (kk / 4) * kHeads * 128 + (kk % 4) * 32), kind_o, x > 0 || kk > 0);
                 mma_commit(free_ + 8 * s);
                 mma_commit(o_done);
                 if (x + 2 < count) ok = scores(x + 2);
@@ -240,7 +243,8 @@ __global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a
             __syncwarp();
             fence_async();
             tc_before();
-            mbar_arrive(p_full + 8 * (x & 1));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 8 * (x & 1));
         }
         ok = ok && mbar_wait(o_last, 0);
         __syncwarp();

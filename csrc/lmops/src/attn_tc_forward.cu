@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             mbar_init(k_full + 8 * s, 1), mbar_init(k_free + 8 * s, 1);
             mbar_init(v_full + 8 * s, 1), mbar_init(v_free + 8 * s, 1);
         }
-        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 128);
+        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 4);
         mbar_init(o_done, 1), mbar_init(o_last, 1);
         fence_barrier_init();
     }
@@ -115,13 +115,18 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
         if (lane == 0) {  // products
             constexpr uint32_t kind_s = mma_kind<bf, kRows, kKeys, false>(), kind_o = mma_kind<bf, kRows, DP, true>();
             const int steps = (a.D + 15) / 16;
+            const uint64_t dq = operand(sq, 0), dk = operand(sk, 0), dv = operand(sv, kKeys * 128);
             auto scores = [&](int x) {
                 const int s = x % S::stages;
                 if (!mbar_wait(k_full + 8 * s, (x / S::stages) & 1)) return false;
                 tc_after();
-                for (int kk = 0; kk < steps; ++kk)
-                    mma_ss(tm + (x & 1) * kKeys, operand(sq + (kk / 4) * kRows * 128 + (kk % 4) * 32, 0),
-                           operand(sk + s * S::kv_bytes + (kk / 4) * kKeys * 128 + (kk % 4) * 32, 0), kind_s, kk > 0);
+                const uint64_t dks = moved(dk, s * S::kv_bytes);
+                const uint32_t d = tm + (x & 1) * kKeys;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    if (kk < steps)
+                        mma_ss(d, moved(dq, (kk / 4) * kRows * 128 + (kk % 4) * 32), moved(dks, (kk / 4) * kKeys * 128 + (kk % 4) * 32), kind_s,
+                               kk > 0);
                 mma_commit(k_free + 8 * s);
                 mma_commit(s_full + 8 * (x & 1));
                 return true;
@@ -132,10 +137,10 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
                 ok = mbar_wait(p_full + 8 * (x & 1), (x >> 1) & 1) && mbar_wait(v_full + 8 * s, (x / S::stages) & 1);
                 if (!ok) break;
                 tc_after();
+                const uint64_t dvs = moved(dv, s * S::kv_bytes);
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
-                    mma_ts(tm + S::o_col, tm + (x & 1) * kKeys + kk * 8, operand(sv + s * S::kv_bytes + kk * 2048, kKeys * 128), kind_o,
-                           x > 0 || kk > 0);
+                    mma_ts(tm + S::o_col, tm + (x & 1) * kKeys + kk * 8, moved(dvs, kk * 2048), kind_o, x > 0 || kk > 0);
                 mma_commit(v_free + 8 * s);
                 mma_commit(o_done);
                 if (x + 2 < tiles.count) ok = scores(x + 2);
@@ -168,9 +173,10 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
                     if (!(j <= i && (i - j < a.window || j < a.sinks))) f[c] = -INFINITY;
                 }
             }
-            float top = f[0];
+            float tops[4] = {f[0], f[1], f[2], f[3]};
 #pragma unroll
-            for (int c = 1; c < kKeys; ++c) top = fmaxf(top, f[c]);
+            for (int c = 4; c < kKeys; ++c) tops[c % 4] = fmaxf(tops[c % 4], f[c]);
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             float turn = 1.f;
             if (m == -INFINITY) {
                 m = top;  // nothing of this row is in O yet
@@ -195,15 +201,20 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
                 }
             }
             const float off = m == -INFINITY ? 0.f : m * a.scale_log2;
-            float sum[4] = {};
+            const uint64_t scale2 = two(a.scale_log2, a.scale_log2), off2 = two(-off, -off);
+            uint64_t sum[4] = {};
             uint32_t p[kKeys / 2];
 #pragma unroll
             for (int c = 0; c < kKeys; c += 2) {
-                const float p0 = exp2_fast(fmaf(f[c], a.scale_log2, -off)), p1 = exp2_fast(fmaf(f[c + 1], a.scale_log2, -off));
-                sum[(c / 2) % 4] += p0 + p1;
+                float p0, p1;
+                apart(fma_two(two(f[c], f[c + 1]), scale2, off2), p0, p1);
+                p0 = exp2_fast(p0), p1 = exp2_fast(p1);
+                sum[(c / 2) % 4] = add_two(sum[(c / 2) % 4], two(p0, p1));
                 p[c / 2] = pack2(p0, p1, T());
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float s0, s1;
+            apart(add_two(add_two(sum[0], sum[1]), add_two(sum[2], sum[3])), s0, s1);
+            l += s0 + s1;
             tc_st32(at, p);
             // keys behind the sequence meet p = 0, but what they hold may be infinite: their values are zeroed
             if (n < a.T && j0 + kKeys > n) {
@@ -222,7 +233,8 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             }
             tc_wait_st();
             tc_before();
-            mbar_arrive(p_full + 8 * (x & 1));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 8 * (x & 1));
         }
         if (ok) ok = mbar_wait(o_last, 0);
         if (__all_sync(0xffffffffu, ok)) {

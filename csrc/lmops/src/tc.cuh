@@ -150,6 +150,10 @@ __device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t lbo) {
     return (uint64_t)((at & 0x3ffff) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
            ((uint64_t)2 << 61);
 }
+// The issuing thread forms an operand's descriptor once and moves it by a
+// constant number of bytes per step (addresses stay below 2^18: no carry out
+// of the address field).
+__device__ __forceinline__ uint64_t moved(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 // kind::f16 with 32-bit sums: M x N, operands bf16 (or fp16), B MN-major or K-major
 template <bool BF16, int M, int N, bool B_MN> __device__ __forceinline__ constexpr uint32_t mma_kind() {
     return (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
