@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
     const int b = blockIdx.z, n = length_of(a, b);
     // rows of this block, and the tiles that pass: x = 0 .. count - 1
     int r0, count, h, hk, split = 0, q_begin = 0, q_tiles = 0, first = 0;
@@ -192,18 +192,20 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             }
         }
     } else if (warp == 9) {
-        if (lane == 0) {  // products
-            constexpr uint32_t kind_s = mma_kind<bf, kRows, kStream, false>(), kind_acc = mma_kind<bf, kRows, DP, true>();
-            const int steps = (a.D + 15) / 16;
-            // U and W as operands along their rows (scores) and down them (sums)
-            const uint64_t dx = operand(sx, 0), dy = operand(sy, 0), du = operand(su, 0), dw = operand(sw, 0), dut = operand(su, kStream * 128),
-                           dwt = operand(sw, kStream * 128);
-            auto scores = [&](int x) {
-                const int s = x % ST;
-                if (!mbar_wait(full + 8 * s, (x / ST) & 1)) return false;
-                tc_after();
-                const uint32_t d = tm + (x % NB) * 2 * kStream;
-                const uint64_t dus = moved(du, s * S::u_bytes), dws = moved(dw, s * S::u_bytes);
+        // products: the whole warp runs the loop, one lane issues
+        const bool leader = elect_one();
+        constexpr uint32_t kind_s = mma_kind<bf, kRows, kStream, false>(), kind_acc = mma_kind<bf, kRows, DP, true>();
+        const int steps = (a.D + 15) / 16;
+        // U and W as operands along their rows (scores) and down them (sums)
+        const uint64_t dx = operand(sx, 0), dy = operand(sy, 0), du = operand(su, 0), dw = operand(sw, 0), dut = operand(su, kStream * 128),
+                       dwt = operand(sw, kStream * 128);
+        auto scores = [&](int x) {
+            const int s = x % ST;
+            if (!warp_wait(full + 8 * s, (x / ST) & 1)) return false;
+            tc_after();
+            const uint32_t d = tm + (x % NB) * 2 * kStream;
+            const uint64_t dus = moved(du, s * S::u_bytes), dws = moved(dw, s * S::u_bytes);
+            if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
                     if (kk < steps)
@@ -215,16 +217,19 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                         mma_ss(d + kStream, moved(dy, (kk / 4) * kRows * 128 + (kk % 4) * 32),
                                moved(dws, (kk / 4) * kStream * 128 + (kk % 4) * 32), kind_s, kk > 0);
                 mma_commit(s_full + 8 * (x % NB));
-                return true;
-            };
-            ok = mbar_wait(x_full, 0);
-            for (int x = 0; x < NB && x < count && ok; ++x) ok = scores(x);
-            for (int x = 0; x < count && ok; ++x) {
-                const int s = x % ST;
-                ok = mbar_wait(ds_full + 8 * (x % NB), (x / NB) & 1);
-                if (!ok) break;
-                tc_after();
-                const uint32_t d = tm + (x % NB) * 2 * kStream;
+            }
+            __syncwarp();
+            return true;
+        };
+        ok = warp_wait(x_full, 0);
+        for (int x = 0; x < NB && x < count && ok; ++x) ok = scores(x);
+        for (int x = 0; x < count && ok; ++x) {
+            const int s = x % ST;
+            ok = warp_wait(ds_full + 8 * (x % NB), (x / NB) & 1);
+            if (!ok) break;
+            tc_after();
+            const uint32_t d = tm + (x % NB) * 2 * kStream;
+            if (leader) {
                 // 32 columns of each half lie packed in the first 16 of their place
                 if constexpr (DKV) {
 #pragma unroll
@@ -237,8 +242,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                     mma_ts(tm + S::acc, d + kStream + (kk / 2) * 32 + (kk % 2) * 8, moved(dut, s * S::u_bytes + kk * 2048), kind_acc,
                            x > 0 || kk > 0);
                 mma_commit(free_ + 8 * s);
-                if (x + NB < count) ok = scores(x + NB);
             }
+            __syncwarp();
+            if (x + NB < count) ok = scores(x + NB);
+        }
+        if (leader) {
             mma_commit(last);
             if (!ok) report(a.error);
         }

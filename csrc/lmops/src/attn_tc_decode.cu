@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a
     const int chunks = (a.group + kHeads - 1) / kHeads;
     const int b = blockIdx.z, hk = blockIdx.y / chunks, h0 = hk * a.group + (blockIdx.y % chunks) * kHeads;
     const int heads = min(kHeads, (hk + 1) * a.group - h0);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
     const int n = length_of(a, b);
     // the keys, numbered: the sinks before the window, up to a multiple of 16, then the window
     const int win0 = max(0, n - a.window), nsink = min(a.sinks, win0), pad = (nsink + 15) / 16 * 16, total = pad + n - win0;
@@ -120,17 +120,19 @@ __global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a
             }
         }
     } else if (warp == 5) {
-        if (lane == 0) {  // products
-            constexpr uint32_t kind_s = mma_kind<bf, kKeys, kHeads, false>();
-            // A = V^T: its rows (D) run along the tile's rows: MN-major
-            constexpr uint32_t kind_o = mma_kind<bf, 128, kHeads, false>() | (1u << 15);
-            const int steps = (a.D + 15) / 16;
-            // D = 64: rows 64 and up of the second product are not used; their operand lies 8 keys on, inside the tiles
-            const uint64_t dt = operand(st, 0), dq = operand(sq, 0), dvt = operand(st, DP == 64 ? 1024 : kKeys * 128), dp = operand(sp, 0);
-            auto scores = [&](int x) {
-                const int y = 2 * x, s = y % S::slots;
-                if (!mbar_wait(full + 8 * s, (y / S::slots) & 1)) return false;
-                tc_after();
+        // products: the whole warp runs the loop, one lane issues
+        const bool leader = elect_one();
+        constexpr uint32_t kind_s = mma_kind<bf, kKeys, kHeads, false>();
+        // A = V^T: its rows (D) run along the tile's rows: MN-major
+        constexpr uint32_t kind_o = mma_kind<bf, 128, kHeads, false>() | (1u << 15);
+        const int steps = (a.D + 15) / 16;
+        // D = 64: rows 64 and up of the second product are not used; their operand lies 8 keys on, inside the tiles
+        const uint64_t dt = operand(st, 0), dq = operand(sq, 0), dvt = operand(st, DP == 64 ? 1024 : kKeys * 128), dp = operand(sp, 0);
+        auto scores = [&](int x) {
+            const int y = 2 * x, s = y % S::slots;
+            if (!warp_wait(full + 8 * s, (y / S::slots) & 1)) return false;
+            tc_after();
+            if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
                     if (kk < steps)
@@ -138,22 +140,28 @@ __global__ void __launch_bounds__(kThreads, 2) tc_decode_kernel(const AttnArgs a
                                moved(dq, (kk / 4) * kHeads * 128 + (kk % 4) * 32), kind_s, kk > 0);
                 mma_commit(free_ + 8 * s);
                 mma_commit(s_full + 8 * (x & 1));
-                return true;
-            };
-            ok = mbar_wait(q_full, 0) && scores(0) && (count < 2 || scores(1));
-            for (int x = 0; x < count && ok; ++x) {
-                const int y = 2 * x + 1, s = y % S::slots;
-                ok = mbar_wait(full + 8 * s, (y / S::slots) & 1) && mbar_wait(p_full + 8 * (x & 1), (x >> 1) & 1);
-                if (!ok) break;
-                tc_after();
+            }
+            __syncwarp();
+            return true;
+        };
+        ok = warp_wait(q_full, 0) && scores(0) && (count < 2 || scores(1));
+        for (int x = 0; x < count && ok; ++x) {
+            const int y = 2 * x + 1, s = y % S::slots;
+            ok = warp_wait(full + 8 * s, (y / S::slots) & 1) && warp_wait(p_full + 8 * (x & 1), (x >> 1) & 1);
+            if (!ok) break;
+            tc_after();
+            if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
                     mma_ss(tm + 2 * kHeads, moved(dvt, s * S::tile_bytes + kk * 2048),
                            moved(dp, (x & 1) * S::p_bytes + (kk / 4) * kHeads * 128 + (kk % 4) * 32), kind_o, x > 0 || kk > 0);
                 mma_commit(free_ + 8 * s);
                 mma_commit(o_done);
-                if (x + 2 < count) ok = scores(x + 2);
             }
+            __syncwarp();
+            if (x + 2 < count) ok = scores(x + 2);
+        }
+        if (leader) {
             mma_commit(o_last);
             if (!ok) report(a.error);
         }

@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
 
     const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
     const int i0 = (gridDim.x - 1 - blockIdx.x) * kRows;  // the longest rows first
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
     const int n = length_of(a, b);
     const KeyTiles tiles(i0, i0 + kRows, n, a.window, a.sinks, kKeys);
 
@@ -112,16 +112,18 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             }
         }
     } else if (warp == 5) {
-        if (lane == 0) {  // products
-            constexpr uint32_t kind_s = mma_kind<bf, kRows, kKeys, false>(), kind_o = mma_kind<bf, kRows, DP, true>();
-            const int steps = (a.D + 15) / 16;
-            const uint64_t dq = operand(sq, 0), dk = operand(sk, 0), dv = operand(sv, kKeys * 128);
-            auto scores = [&](int x) {
-                const int s = x % S::stages;
-                if (!mbar_wait(k_full + 8 * s, (x / S::stages) & 1)) return false;
-                tc_after();
-                const uint64_t dks = moved(dk, s * S::kv_bytes);
-                const uint32_t d = tm + (x & 1) * kKeys;
+        // products: the whole warp runs the loop, one lane issues
+        const bool leader = elect_one();
+        constexpr uint32_t kind_s = mma_kind<bf, kRows, kKeys, false>(), kind_o = mma_kind<bf, kRows, DP, true>();
+        const int steps = (a.D + 15) / 16;
+        const uint64_t dq = operand(sq, 0), dk = operand(sk, 0), dv = operand(sv, kKeys * 128);
+        auto scores = [&](int x) {
+            const int s = x % S::stages;
+            if (!warp_wait(k_full + 8 * s, (x / S::stages) & 1)) return false;
+            tc_after();
+            const uint64_t dks = moved(dk, s * S::kv_bytes);
+            const uint32_t d = tm + (x & 1) * kKeys;
+            if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
                     if (kk < steps)
@@ -129,22 +131,28 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
                                kk > 0);
                 mma_commit(k_free + 8 * s);
                 mma_commit(s_full + 8 * (x & 1));
-                return true;
-            };
-            ok = mbar_wait(q_full, 0) && scores(0) && (tiles.count < 2 || scores(1));
-            for (int x = 0; x < tiles.count && ok; ++x) {
-                const int s = x % S::stages;
-                ok = mbar_wait(p_full + 8 * (x & 1), (x >> 1) & 1) && mbar_wait(v_full + 8 * s, (x / S::stages) & 1);
-                if (!ok) break;
-                tc_after();
-                const uint64_t dvs = moved(dv, s * S::kv_bytes);
+            }
+            __syncwarp();
+            return true;
+        };
+        ok = warp_wait(q_full, 0) && scores(0) && (tiles.count < 2 || scores(1));
+        for (int x = 0; x < tiles.count && ok; ++x) {
+            const int s = x % S::stages;
+            ok = warp_wait(p_full + 8 * (x & 1), (x >> 1) & 1) && warp_wait(v_full + 8 * s, (x / S::stages) & 1);
+            if (!ok) break;
+            tc_after();
+            const uint64_t dvs = moved(dv, s * S::kv_bytes);
+            if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
                     mma_ts(tm + S::o_col, tm + (x & 1) * kKeys + kk * 8, moved(dvs, kk * 2048), kind_o, x > 0 || kk > 0);
                 mma_commit(v_free + 8 * s);
                 mma_commit(o_done);
-                if (x + 2 < tiles.count) ok = scores(x + 2);
             }
+            __syncwarp();
+            if (x + 2 < tiles.count) ok = scores(x + 2);
+        }
+        if (leader) {
             mma_commit(o_last);
             if (!ok) report(a.error);
         }

@@ -22,6 +22,19 @@ bool tma_takes(const cail_ops_bthd &x, int B, int T, int H);
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// the warp's number as a value that the compiler knows to be the same in all its lanes
+__device__ __forceinline__ int warp_number() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
+// true in one lane of a converged warp.  The warp that issues products runs
+// its whole loop converged and only the instructions themselves in one lane,
+// so descriptors and addresses stay in uniform registers (issued from a lane
+// of its own, each product cost 70 to 80 clocks to issue).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // ---------------------------------------------------------------- mbarriers
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -56,6 +69,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
         }
     }
 }
+// the same by all lanes of a converged warp
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 __device__ __forceinline__ void report(int *error) {
     if (error) asm volatile("st.relaxed.sys.global.s32 [%0], %1;" ::"l"(error), "r"(1) : "memory");
 }
