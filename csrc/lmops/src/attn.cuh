@@ -70,6 +70,33 @@ __device__ __forceinline__ void query_range(int j0, int j1, int n, int window, i
     if (j0 >= n) begin = end = 0;
 }
 
+// bits [lo, hi] of 32 (none where lo > hi); lo and hi may lie outside
+__device__ __forceinline__ uint32_t bits(int lo, int hi) {
+    if (lo > hi || lo > 31 || hi < 0) return 0u;
+    return (0xffffffffu << max(lo, 0)) & (0xffffffffu >> (31 - min(hi, 31)));
+}
+// which of the keys j0 .. j0 + 31 row i sees (i < n)
+__device__ __forceinline__ uint32_t keys_of_row(int i, int j0, int window, int sinks) {
+    return bits(i - window + 1 - j0, i - j0) | bits(0, min(sinks - 1, i) - j0);
+}
+// which of the rows i0 .. i0 + 31 see key j
+__device__ __forceinline__ uint32_t rows_of_key(int j, int i0, int n, int window, int sinks) {
+    return bits(j - i0, (j < sinks || window > n - j ? n - 1 : j + window - 1) - i0) & bits(0, n - 1 - i0);
+}
+
+// A launch's blocks in one dimension: tiles in the outer place, heads of all
+// sequences in the inner one, so that blocks start in the tiles' order.
+struct BlockAt {
+    int tile, h, b;
+    __device__ __forceinline__ BlockAt(int heads, int B) {
+        const unsigned hb = (unsigned)heads * (unsigned)B;
+        tile = (int)(blockIdx.x / hb);
+        const unsigned r = blockIdx.x - (unsigned)tile * hb;
+        b = (int)(r / (unsigned)heads);
+        h = (int)(r - (unsigned)b * heads);
+    }
+};
+
 __device__ __forceinline__ int length_of(const AttnArgs &a, int b) {
     return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
 }

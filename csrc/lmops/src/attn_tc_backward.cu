@@ -74,14 +74,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB;
 
     const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
-    const int b = blockIdx.z, n = length_of(a, b);
+    const BlockAt at_(DKV ? a.Hkv : a.H, a.B);
+    const int b = at_.b, n = length_of(a, b);
     // rows of this block, and the tiles that pass: x = 0 .. count - 1
     int r0, count, h, hk, split = 0, q_begin = 0, q_tiles = 0, first = 0;
     bool parted = false;
     KeyTiles keys(0, 0, 0, 1, 0, kStream);
     if constexpr (DKV) {
-        hk = blockIdx.y, h = hk * a.group;
-        int tile = blockIdx.x;
+        hk = at_.h, h = hk * a.group;
+        int tile = at_.tile;
         parted = ex.splits > 1 && tile < ex.sink_tiles * ex.splits;
         if (parted) split = tile % ex.splits, tile /= ex.splits;
         else if (ex.splits > 1) tile -= ex.sink_tiles * (ex.splits - 1);
@@ -97,8 +98,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             count = min(count, first + per) - first;
         }
     } else {
-        h = blockIdx.y, hk = h / a.group;
-        r0 = (gridDim.x - 1 - blockIdx.x) * kRows;  // the longest rows first
+        h = at_.h, hk = h / a.group;
+        r0 = ((a.T - 1) / kRows - at_.tile) * kRows;  // the longest rows first
         keys = KeyTiles(r0, r0 + kRows, n, a.window, a.sinks, kStream);
         count = keys.count;
     }
@@ -255,13 +256,24 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         const uint32_t mine = tm + ((uint32_t)((warp & 3) * 32) << 16);
         float lse = 0.f, delta = 0.f, amp = 1.f;
         if constexpr (!DKV) {
+            // the row's output and lse, on their way while do arrives
+            Vec<T, 8> o[DP / 8];
+            const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + r;
+            if (r < n) {
+                const char *p = a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh;
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c)
+                    if (c * 8 < a.D) o[c] = *reinterpret_cast<const Vec<T, 8> *>(p + c * 16);
+                lse = a.lse[at];
+            }
             ok = mbar_wait(x_full, 0);
             if (ok) {
                 float top = 0.f;
                 if (r < n) {
-                    const char *o = a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh;
-                    for (int c = 0; c * 8 < a.D; ++c) {
-                        Vec<T, 8> x = *reinterpret_cast<const Vec<T, 8> *>(o + c * 16), g;
+#pragma unroll
+                    for (int c = 0; c < DP / 8; ++c) {
+                        if (c * 8 >= a.D) break;
+                        Vec<T, 8> g;
                         uint4 w;
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                      : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
@@ -270,12 +282,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const float f = to_f(g.v[e]);
-                            delta = fmaf(to_f(x.v[e]), f, delta);
+                            delta = fmaf(to_f(o[c].v[e]), f, delta);
                             if (!bf) top = fmaxf(top, fabsf(f));
                         }
                     }
-                    const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + r;
-                    lse = a.lse[at];
                     if (half == 0) a.delta[at] = delta;
                 }
                 if (!bf) {
@@ -306,6 +316,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             uint32_t pp[16], pd[16];
             const uint64_t scale2 = two(a.scale_log2, a.scale_log2);
             auto math = [&](auto masked) {
+                uint32_t on = 0, on_ds = 0;  // which of the 32 are seen; which of them carry ds
+                if (masked.value) {
+                    on = DKV ? rows_of_key(r, c0, n, a.window, a.sinks) : keys_of_row(r, c0, a.window, a.sinks);
+                    on_ds = a.window == 1 && a.sinks == 0 ? 0u : on;
+                    if (DKV ? c0 == 0 : r == 0) on_ds &= DKV ? ~1u : 0u;  // row 0 sees one key
+                }
 #pragma unroll
                 for (int c = 0; c < 32; c += 4) {
                     // minus lse and minus delta of the columns
@@ -332,10 +348,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                     if (masked.value) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int i = DKV ? c0 + c + e : r, j = DKV ? r : c0 + c + e;
-                            const bool on = j <= i && (i - j < a.window || j < a.sinks) && (!DKV || i < n);
-                            if (!on) p[e] = 0.f;
-                            if (!on || one_key(i, a.window, a.sinks)) d[e] = 0.f;
+                            if (!(on & (1u << (c + e)))) p[e] = 0.f;
+                            if (!(on_ds & (1u << (c + e)))) d[e] = 0.f;
                         }
                     }
                     if constexpr (DKV) pp[c / 2] = pack2(p[0], p[1], T()), pp[c / 2 + 1] = pack2(p[2], p[3], T());
@@ -504,10 +518,11 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     cudaError_t e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_q);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_k);
     if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
-    tc_backward_kernel<T, DP, false><<<dim3(tiles, a.H, a.B), kThreads, sm_q, st>>>(a, ex, q);
+    const int64_t blocks_q = (int64_t)tiles * a.H * a.B, blocks_k = ((int64_t)tiles + ex.sink_tiles * (ex.splits - 1)) * a.Hkv * a.B;
+    if (blocks_q > 0x7fffffff || blocks_k > 0x7fffffff) return fail(CAIL_OPS_EINVAL, "window attention backward: too many tokens");
+    tc_backward_kernel<T, DP, false><<<(unsigned)blocks_q, kThreads, sm_q, st>>>(a, ex, q);
     if (int rc = launched("window attention backward")) return rc;
-    const unsigned blocks = tiles + ex.sink_tiles * (ex.splits - 1);
-    tc_backward_kernel<T, DP, true><<<dim3(blocks, a.Hkv, a.B), kThreads, sm_k, st>>>(a, ex, k);
+    tc_backward_kernel<T, DP, true><<<(unsigned)blocks_k, kThreads, sm_k, st>>>(a, ex, k);
     if (int rc = launched("window attention backward")) return rc;
     if (ex.splits == 1) return CAIL_OPS_OK;
     const unsigned grid = ((unsigned)ex.sink_tiles * 2 * kRows * (DP / 8) + 255) / 256;

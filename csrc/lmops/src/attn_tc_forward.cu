@@ -50,8 +50,9 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
     const uint32_t q_full = bar(0), k_full = bar(1), k_free = bar(1 + S::stages), v_full = bar(1 + 2 * S::stages),
                    v_free = bar(1 + 3 * S::stages), s_full = bar(1 + 4 * S::stages), p_full = s_full + 16, o_done = p_full + 16, o_last = o_done + 8;
 
-    const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
-    const int i0 = (gridDim.x - 1 - blockIdx.x) * kRows;  // the longest rows first
+    const BlockAt at_(a.H, a.B);
+    const int h = at_.h, b = at_.b, hk = h / a.group;
+    const int i0 = ((a.T - 1) / kRows - at_.tile) * kRows;  // the longest rows first
     const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
     const int n = length_of(a, b);
     const KeyTiles tiles(i0, i0 + kRows, n, a.window, a.sinks, kKeys);
@@ -175,11 +176,10 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             // every row of the tile sees every key, unless the tile crosses the diagonal or the window's edge
             const bool whole = j0 + kKeys - 1 <= i0 && (i0 + kRows - 1 - j0 < a.window || j0 + kKeys <= a.sinks);
             if (!whole) {
+                const uint32_t on[2] = {keys_of_row(i, j0, a.window, a.sinks), keys_of_row(i, j0 + 32, a.window, a.sinks)};
 #pragma unroll
-                for (int c = 0; c < kKeys; ++c) {
-                    const int j = j0 + c;
-                    if (!(j <= i && (i - j < a.window || j < a.sinks))) f[c] = -INFINITY;
-                }
+                for (int c = 0; c < kKeys; ++c)
+                    if (!(on[c / 32] & (1u << (c % 32)))) f[c] = -INFINITY;
             }
             float tops[4] = {f[0], f[1], f[2], f[3]};
 #pragma unroll
@@ -299,7 +299,9 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, const
     if (int rc = tensor_map(&maps.v, c->v, c->type, a.B, a.T, a.Hkv, a.D, kKeys)) return rc;
     cudaError_t e = cudaFuncSetAttribute(tc_forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
     if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention: %s", cudaGetErrorString(e));
-    tc_forward_kernel<T, DP><<<dim3((a.T + kRows - 1) / kRows, a.H, a.B), kThreads, S::smem, st>>>(a, maps);
+    const int64_t grid = ((int64_t)a.T + kRows - 1) / kRows * a.H * a.B;
+    if (grid > 0x7fffffff) return fail(CAIL_OPS_EINVAL, "window attention: too many tokens");
+    tc_forward_kernel<T, DP><<<(unsigned)grid, kThreads, S::smem, st>>>(a, maps);
     return launched("window attention");
 }
 
