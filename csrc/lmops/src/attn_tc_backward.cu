@@ -35,16 +35,18 @@ template <int DP, bool DKV> struct Shape {
     static constexpr int stages = 3;
     static constexpr int buffers = DP == 64 ? 1 : 2;  // of S and dP
     static constexpr int per_sm = DP == 64 ? 2 : 1;
+    static constexpr int chunk = DKV && DP == 64 ? 16 : 32;  // columns at a time, by the registers that two blocks leave
     static constexpr int x_bytes = kRows * DP * 2, u_bytes = kStream * DP * 2;
     static constexpr int vec_bytes = DKV ? 2 * kStream * 4 : 0;  // lse and delta of a tile's queries
     static constexpr int barriers = 1 + 2 * stages + 2 * buffers + 1;
-    static constexpr int smem = 1024 + 2 * x_bytes + stages * (2 * u_bytes + vec_bytes);
+    static constexpr int o_bytes = DKV ? 0 : x_bytes;  // the output's rows, for delta
+    static constexpr int smem = 1024 + 2 * x_bytes + stages * (2 * u_bytes + vec_bytes) + o_bytes;
     static constexpr int acc = buffers * 2 * kStream;  // column of acc0; acc1 follows
     static constexpr int columns = DP == 64 ? 256 : 512;
 };
 
 struct Maps {
-    CUtensorMap x, y, u, w;
+    CUtensorMap x, y, u, w, o;
 };
 
 struct Extra {
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     __shared__ __align__(8) uint64_t bars[S::barriers];
     __shared__ uint32_t tmem_at;
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + ST * S::u_bytes, svec = sw + ST * S::u_bytes;
+    const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + ST * S::u_bytes, svec = sw + ST * S::u_bytes, so = svec;
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB;
 
@@ -144,17 +146,40 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         return;
     }
 
-    if (warp == 8) {
-        tmem_alloc<S::columns>(smem_u32(&tmem_at));
-        if (lane == 0) tma_prefetch(&maps.x), tma_prefetch(&maps.y), tma_prefetch(&maps.u), tma_prefetch(&maps.w);
-    }
-    if (tid == 0) {
+    auto load = [&](const Walk &w) {
+        const int s = w.x % ST, t0 = w.row, th = DKV ? w.head : hk;
+        const uint32_t bar = full + 8 * s;
+        mbar_expect(bar, 2 * S::u_bytes + S::vec_bytes);
+        for (int p = 0; p < S::panels; ++p) {
+            tma_load(su + s * S::u_bytes + p * kStream * 128, &maps.u, bar, p * 64, t0, th, b);
+            tma_load(sw + s * S::u_bytes + p * kStream * 128, &maps.w, bar, p * 64, t0, th, b);
+        }
+        if constexpr (DKV) {
+            // 64 values each, which may reach into the next row or the padding behind the last one: those are masked
+            const int64_t at = ((int64_t)b * a.H + th) * a.lse_row + t0;
+            bulk_load(svec + s * S::vec_bytes, a.lse + at, kStream * 4, bar);
+            bulk_load(svec + s * S::vec_bytes + kStream * 4, a.delta + at, kStream * 4, bar);
+        }
+    };
+    Walk walk = begin_walk();
+    if (warp == 8 && lane == 0) {
         mbar_init(x_full, 1);
         for (int s = 0; s < ST; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
         for (int s = 0; s < NB; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(ds_full + 8 * s, kMath / 32);
         mbar_init(last, 1);
         fence_barrier_init();
+        // what needs no free slot is on its way before the block has met
+        mbar_expect(x_full, 2 * S::x_bytes + S::o_bytes);
+        for (int p = 0; p < S::panels; ++p) tma_load(sx + p * kRows * 128, &maps.x, x_full, p * 64, r0, DKV ? hk : h, b);
+        load(walk);
+        for (int p = 0; p < S::panels; ++p) {
+            tma_load(sy + p * kRows * 128, &maps.y, x_full, p * 64, r0, DKV ? hk : h, b);
+            if (!DKV) tma_load(so + p * kRows * 128, &maps.o, x_full, p * 64, r0, h, b);
+        }
+        for (step(walk); walk.x < ST && walk.x < count; step(walk)) load(walk);
     }
+    if (warp == 9) tmem_alloc<S::columns>(smem_u32(&tmem_at));
+    __syncwarp();
     tc_before();
     __syncthreads();
     tc_after();
@@ -162,34 +187,16 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     bool ok = true;
 
     if (warp == 8) {
-        if (lane == 0) {  // loads
-            mbar_expect(x_full, 2 * S::x_bytes);
-            for (int p = 0; p < S::panels; ++p) {
-                tma_load(sx + p * kRows * 128, &maps.x, x_full, p * 64, r0, DKV ? hk : h, b);
-                tma_load(sy + p * kRows * 128, &maps.y, x_full, p * 64, r0, DKV ? hk : h, b);
-            }
-            Walk w = begin_walk();
-            for (; w.x < count; step(w)) {
-                const int x = w.x, s = x % ST, t0 = w.row, th = DKV ? w.head : hk;
-                if (x >= ST) ok = mbar_wait(free_ + 8 * s, ((x / ST) & 1) ^ 1);
+        if (lane == 0) {  // the loads that wait for a slot
+            for (; walk.x < count; step(walk)) {
+                ok = mbar_wait(free_ + 8 * (walk.x % ST), ((walk.x / ST) & 1) ^ 1);
                 if (!ok) break;
-                const uint32_t bar = full + 8 * s;
-                mbar_expect(bar, 2 * S::u_bytes + S::vec_bytes);
-                for (int p = 0; p < S::panels; ++p) {
-                    tma_load(su + s * S::u_bytes + p * kStream * 128, &maps.u, bar, p * 64, t0, th, b);
-                    tma_load(sw + s * S::u_bytes + p * kStream * 128, &maps.w, bar, p * 64, t0, th, b);
-                }
-                if constexpr (DKV) {
-                    // 64 values each, which may reach into the next row or the padding behind the last one: those are masked
-                    const int64_t at = ((int64_t)b * a.H + th) * a.lse_row + t0;
-                    bulk_load(svec + s * S::vec_bytes, a.lse + at, kStream * 4, bar);
-                    bulk_load(svec + s * S::vec_bytes + kStream * 4, a.delta + at, kStream * 4, bar);
-                }
+                load(walk);
             }
             if (!ok) {  // gave up: the copies in flight land before the block ends
                 report(a.error);
                 mbar_wait(x_full, 0);
-                for (int y = max(0, w.x - ST); y < w.x; ++y) mbar_wait(full + 8 * (y % ST), (y / ST) & 1);
+                for (int y = max(0, walk.x - ST); y < walk.x; ++y) mbar_wait(full + 8 * (y % ST), (y / ST) & 1);
             }
         }
     } else if (warp == 9) {
@@ -256,16 +263,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         const uint32_t mine = tm + ((uint32_t)((warp & 3) * 32) << 16);
         float lse = 0.f, delta = 0.f, amp = 1.f;
         if constexpr (!DKV) {
-            // the row's output and lse, on their way while do arrives
-            Vec<T, 8> o[DP / 8];
             const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + r;
-            if (r < n) {
-                const char *p = a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh;
-#pragma unroll
-                for (int c = 0; c < DP / 8; ++c)
-                    if (c * 8 < a.D) o[c] = *reinterpret_cast<const Vec<T, 8> *>(p + c * 16);
-                lse = a.lse[at];
-            }
+            if (r < n) lse = a.lse[at];  // on its way while do and o arrive
             ok = mbar_wait(x_full, 0);
             if (ok) {
                 float top = 0.f;
@@ -273,16 +272,17 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
 #pragma unroll
                     for (int c = 0; c < DP / 8; ++c) {
                         if (c * 8 >= a.D) break;
-                        Vec<T, 8> g;
+                        Vec<T, 8> g, o;
+                        const uint32_t at = (c / 8) * kRows * 128 + row * 128 + (((c % 8) ^ (row & 7)) * 16);
                         uint4 w;
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                                     : "r"(sy + (c / 8) * kRows * 128 + row * 128 + (((c % 8) ^ (row & 7)) * 16)));
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(sy + at));
                         *reinterpret_cast<uint4 *>(&g) = w;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(so + at));
+                        *reinterpret_cast<uint4 *>(&o) = w;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const float f = to_f(g.v[e]);
-                            delta = fmaf(to_f(o[c].v[e]), f, delta);
+                            delta = fmaf(to_f(o.v[e]), f, delta);
                             if (!bf) top = fmaxf(top, fabsf(f));
                         }
                     }
@@ -297,24 +297,21 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         } else if (!bf) {
             amp = amp_of(ex.amax[b * a.Hkv + hk]);
         }
-        for (Walk w = begin_walk(); w.x < count; step(w)) {
-            const int x = w.x, t0 = w.row, s = x % ST;
+        const float delta_amp = delta * amp;
+        for (; walk.x < count; step(walk)) {
+            const int x = walk.x, t0 = walk.row, s = x % ST;
             if (ok) ok = mbar_wait(s_full + 8 * (x % NB), (x / NB) & 1);
             if (DKV && ok) ok = mbar_wait(full + 8 * s, (x / ST) & 1);  // lse and delta of the tile (done by then)
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_after();
             const uint32_t at = mine + (x % NB) * 2 * kStream + half * 32;
-            uint32_t us[32], ud[32];
-            tc_ld32(at, us);
-            tc_ld32(at + kStream, ud);
-            tc_wait_ld(us);
-            tc_touch(ud);
             const int c0 = t0 + half * 32;
             bool whole;
             if (DKV) whole = r0 + kRows - 1 <= t0 && t0 + kStream <= n && (t0 + kStream - 1 - r0 < a.window || r0 + kRows <= a.sinks);
             else whole = t0 + kStream - 1 <= r0 && (r0 + kRows - 1 - t0 < a.window || t0 + kStream <= a.sinks);
-            uint32_t pp[16], pd[16];
-            const uint64_t scale2 = two(a.scale_log2, a.scale_log2);
+            // signs turned where that costs nothing: exp2(-(lse - s)), and -ds = p (delta - dp), put right in the sums' scale
+            const uint64_t scale2 = two(-a.scale_log2, -a.scale_log2), minus = two(-amp, -amp);
+            constexpr int CH = S::chunk;
             auto math = [&](auto masked) {
                 uint32_t on = 0, on_ds = 0;  // which of the 32 are seen; which of them carry ds
                 if (masked.value) {
@@ -323,43 +320,50 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                     if (DKV ? c0 == 0 : r == 0) on_ds &= DKV ? ~1u : 0u;  // row 0 sees one key
                 }
 #pragma unroll
-                for (int c = 0; c < 32; c += 4) {
-                    // minus lse and minus delta of the columns
-                    uint64_t l2[2] = {two(-lse, -lse), two(-lse, -lse)}, d2[2] = {two(-delta, -delta), two(-delta, -delta)};
-                    if constexpr (DKV) {
-                        const uint32_t v = svec + s * S::vec_bytes + (half * 32 + c) * 4;
-                        float l4[4], d4[4];
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(l4[0]), "=f"(l4[1]), "=f"(l4[2]), "=f"(l4[3]) : "r"(v));
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(d4[0]), "=f"(d4[1]), "=f"(d4[2]), "=f"(d4[3])
-                                     : "r"(v + kStream * 4));
-                        l2[0] = two(-l4[0], -l4[1]), l2[1] = two(-l4[2], -l4[3]);
-                        d2[0] = two(-d4[0], -d4[1]), d2[1] = two(-d4[2], -d4[3]);
-                    }
-                    float p[4], d[4];
+                for (int c1 = 0; c1 < 32; c1 += CH) {
+                    uint32_t us[CH], ud[CH], pp[CH / 2], pd[CH / 2];
+                    tc_ld<CH>(at + c1, us);
+                    tc_ld<CH>(at + kStream + c1, ud);
+                    tc_wait_both<CH>(us, ud);
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        apart(fma_two(two(__uint_as_float(us[c + e]), __uint_as_float(us[c + e + 1])), scale2, l2[e / 2]), p[e], p[e + 1]);
-                        p[e] = exp2_fast(p[e]), p[e + 1] = exp2_fast(p[e + 1]);
-                        uint64_t t = add_two(two(__uint_as_float(ud[c + e]), __uint_as_float(ud[c + e + 1])), d2[e / 2]);
-                        if (!bf) t = mul_two(t, two(amp, amp));
-                        apart(mul_two(t, two(p[e], p[e + 1])), d[e], d[e + 1]);
-                    }
-                    if (masked.value) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (!(on & (1u << (c + e)))) p[e] = 0.f;
-                            if (!(on_ds & (1u << (c + e)))) d[e] = 0.f;
+                    for (int c = 0; c < CH; c += 4) {
+                        uint64_t l2[2] = {two(lse, lse), two(lse, lse)}, d2[2] = {two(delta_amp, delta_amp), two(delta_amp, delta_amp)};
+                        if constexpr (DKV) {
+                            const uint32_t v = svec + s * S::vec_bytes + (half * 32 + c1 + c) * 4;
+                            float l4[4], d4[4];
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(l4[0]), "=f"(l4[1]), "=f"(l4[2]), "=f"(l4[3]) : "r"(v));
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(d4[0]), "=f"(d4[1]), "=f"(d4[2]), "=f"(d4[3])
+                                         : "r"(v + kStream * 4));
+                            l2[0] = two(l4[0], l4[1]), l2[1] = two(l4[2], l4[3]);
+                            d2[0] = two(d4[0], d4[1]), d2[1] = two(d4[2], d4[3]);
+                            if (!bf) d2[0] = mul_two(d2[0], two(amp, amp)), d2[1] = mul_two(d2[1], two(amp, amp));
                         }
+                        float p[4], d[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            apart(fma_two(two(__uint_as_float(us[c + e]), __uint_as_float(us[c + e + 1])), scale2, l2[e / 2]), p[e], p[e + 1]);
+                            p[e] = exp2_fast(-p[e]), p[e + 1] = exp2_fast(-p[e + 1]);
+                            const uint64_t t = fma_two(two(__uint_as_float(ud[c + e]), __uint_as_float(ud[c + e + 1])), minus, d2[e / 2]);
+                            apart(mul_two(t, two(p[e], p[e + 1])), d[e], d[e + 1]);
+                        }
+                        if (masked.value) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (!(on & (1u << (c1 + c + e)))) p[e] = 0.f;
+                                if (!(on_ds & (1u << (c1 + c + e)))) d[e] = 0.f;
+                            }
+                        }
+                        if constexpr (DKV) pp[c / 2] = pack2(p[0], p[1], T()), pp[c / 2 + 1] = pack2(p[2], p[3], T());
+                        pd[c / 2] = pack2(d[0], d[1], T()), pd[c / 2 + 1] = pack2(d[2], d[3], T());
                     }
-                    if constexpr (DKV) pp[c / 2] = pack2(p[0], p[1], T()), pp[c / 2 + 1] = pack2(p[2], p[3], T());
-                    pd[c / 2] = pack2(d[0], d[1], T()), pd[c / 2 + 1] = pack2(d[2], d[3], T());
+                    // packed behind one another at the beginning of the 32 columns: over values that are in registers by now
+                    if constexpr (DKV) tc_st<CH / 2>(at + c1 / 2, pp);
+                    tc_st<CH / 2>(at + kStream + c1 / 2, pd);
                 }
             };
             if (whole) math(std::false_type());
             else math(std::true_type());
-            if constexpr (DKV) tc_st16(at, pp);
-            tc_st16(at + kStream, pd);
             // rows behind the sequence meet zeros, but what they hold may be infinite: they are zeroed
             if (n < a.T && t0 + kStream > n) {
                 constexpr int C = DP / 8;
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             const uint32_t stage = DKV && half ? sy : sx;
             const uint32_t from = mine + S::acc + (DKV && half ? DP : 0);
             const int c_lo = DKV ? 0 : half * (DP / 2), c_hi = DKV ? DP : c_lo + DP / 2;
-            const float by = DKV && half ? 1.f : a.scale / amp;
+            const float by = DKV && half ? 1.f : -a.scale / amp;
             const bool live = r < n;
             float *part = nullptr;
             if (DKV && parted)
@@ -437,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     }
     __syncwarp();
     __syncthreads();
-    if (warp == 8) tmem_free<S::columns>(tm);
+    if (warp == 9) tmem_free<S::columns>(tm);
 }
 
 // dk and dv of the sinks' key tiles from their parts, in order
@@ -504,7 +508,8 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
         if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
     }
     // the same arrays with boxes of 128 and of 64 rows
-    Maps q, k;
+    Maps q = {}, k = {};
+    if (int rc = tensor_map(&q.o, c->o, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.x, c->q, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.y, c->dout, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.u, c->k, c->type, a.B, a.T, a.Hkv, a.D, kStream)) return rc;
@@ -533,7 +538,7 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
 }  // namespace
 
 bool tc_takes_backward(const cail_ops_attention_args *a) {
-    return tc_takes(a) && tma_takes(a->dout, a->B, a->T, a->H) && rows_aligned(a->dq, a->B, a->T, a->H, 2, 16) &&
+    return tc_takes(a) && tma_takes(a->dout, a->B, a->T, a->H) && tma_takes(a->o, a->B, a->T, a->H) && rows_aligned(a->dq, a->B, a->T, a->H, 2, 16) &&
            rows_aligned(a->dk, a->B, a->T, a->Hkv, 2, 16) && rows_aligned(a->dv, a->B, a->T, a->Hkv, 2, 16) && aligned(a->lse, 16) &&
            aligned(a->delta, 16);
 }

@@ -66,13 +66,17 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
         if (a.lse && tid < kRows && i0 + tid < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i0 + tid] = 0.f;
         return;
     }
-    if (warp == 4) {
-        tmem_alloc<256>(smem_u32(&tmem_at));
-        if (lane == 0) {
-            tma_prefetch(&maps.q), tma_prefetch(&maps.k), tma_prefetch(&maps.v);
-        }
-    }
-    if (tid == 0) {
+    auto load_k = [&](int x) {
+        const int s = x % S::stages, j0 = tiles.at(x) * kKeys;
+        mbar_expect(k_full + 8 * s, S::kv_bytes);
+        for (int p = 0; p < S::panels; ++p) tma_load(sk + s * S::kv_bytes + p * kKeys * 128, &maps.k, k_full + 8 * s, p * 64, j0, hk, b);
+    };
+    auto load_v = [&](int x) {
+        const int s = x % S::stages, j0 = tiles.at(x) * kKeys;
+        mbar_expect(v_full + 8 * s, S::kv_bytes);
+        for (int p = 0; p < S::panels; ++p) tma_load(sv + s * S::kv_bytes + p * kKeys * 128, &maps.v, v_full + 8 * s, p * 64, j0, hk, b);
+    };
+    if (warp == 4 && lane == 0) {
         mbar_init(q_full, 1);
         for (int s = 0; s < S::stages; ++s) {
             mbar_init(k_full + 8 * s, 1), mbar_init(k_free + 8 * s, 1);
@@ -81,7 +85,13 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
         for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 4);
         mbar_init(o_done, 1), mbar_init(o_last, 1);
         fence_barrier_init();
+        // what needs no free slot is on its way before the block has met
+        mbar_expect(q_full, S::q_bytes);
+        for (int p = 0; p < S::panels; ++p) tma_load(sq + p * kRows * 128, &maps.q, q_full, p * 64, i0, h, b);
+        for (int x = 0; x < S::stages && x < tiles.count; ++x) load_k(x), load_v(x);
     }
+    if (warp == 5) tmem_alloc<256>(smem_u32(&tmem_at));
+    __syncwarp();
     tc_before();
     __syncthreads();
     tc_after();
@@ -89,27 +99,23 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
     bool ok = true;
 
     if (warp == 4) {
-        if (lane == 0) {  // loads
-            mbar_expect(q_full, S::q_bytes);
-            for (int p = 0; p < S::panels; ++p) tma_load(sq + p * kRows * 128, &maps.q, q_full, p * 64, i0, h, b);
-            for (int x = 0; x < tiles.count && ok; ++x) {
+        if (lane == 0) {  // the loads that wait for a slot
+            int x = S::stages;
+            for (; x < tiles.count; ++x) {
                 const int s = x % S::stages;
-                const uint32_t round = (x / S::stages) & 1;
-                const int j0 = tiles.at(x) * kKeys;
-                if (x >= S::stages) ok = mbar_wait(k_free + 8 * s, round ^ 1);
+                const uint32_t before = ((x / S::stages) & 1) ^ 1;
+                ok = mbar_wait(k_free + 8 * s, before);
                 if (!ok) break;
-                mbar_expect(k_full + 8 * s, S::kv_bytes);
-                for (int p = 0; p < S::panels; ++p) tma_load(sk + s * S::kv_bytes + p * kKeys * 128, &maps.k, k_full + 8 * s, p * 64, j0, hk, b);
-                if (x >= S::stages) ok = mbar_wait(v_free + 8 * s, round ^ 1);
+                load_k(x);
+                ok = mbar_wait(v_free + 8 * s, before);
                 if (!ok) break;
-                mbar_expect(v_full + 8 * s, S::kv_bytes);
-                for (int p = 0; p < S::panels; ++p) tma_load(sv + s * S::kv_bytes + p * kKeys * 128, &maps.v, v_full + 8 * s, p * 64, j0, hk, b);
+                load_v(x);
             }
-            if (!ok) {  // gave up: the copies in flight still land before the block ends
+            if (!ok) {  // gave up: the copies in flight land before the block ends
                 report(a.error);
                 mbar_wait(q_full, 0);
-                for (int s = 0; s < S::stages; ++s)
-                    for (uint32_t par = 0; par < 2; ++par) mbar_try(k_full + 8 * s, par), mbar_try(v_full + 8 * s, par);
+                for (int y = x - S::stages; y < x; ++y)
+                    mbar_wait(k_full + 8 * (y % S::stages), (y / S::stages) & 1), mbar_wait(v_full + 8 * (y % S::stages), (y / S::stages) & 1);
             }
         }
     } else if (warp == 5) {
@@ -288,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
     }
     __syncwarp();
     __syncthreads();
-    if (warp == 4) tmem_free<256>(tm);
+    if (warp == 5) tmem_free<256>(tm);
 }
 
 template <typename T, int DP> int launch(const cail_ops_attention_args *c, const AttnArgs &a, cudaStream_t st) {
