@@ -16,7 +16,7 @@
 // order: results do not change from run to run.
 #include <cooperative_groups.h>
 
-#include "ops_common.cuh"
+#include "tc.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -51,39 +51,107 @@ __device__ __forceinline__ float teacher_at(const Args &a, int64_t i) {
     return to_f(static_cast<const __half *>(a.teacher)[i]);
 }
 
+// 16 bytes of a row as pairs of floats, and their maximum (NaN aside)
+template <typename T> struct Pairs {
+    static constexpr int count = 8 / (int)sizeof(T);
+    uint64_t x[count];
+    float top;
+    __device__ __forceinline__ explicit Pairs(const uint4 &u);
+};
+template <> __device__ __forceinline__ Pairs<float>::Pairs(const uint4 &u) {
+    const float a = __uint_as_float(u.x), b = __uint_as_float(u.y), c = __uint_as_float(u.z), d = __uint_as_float(u.w);
+    x[0] = two(a, b), x[1] = two(c, d);
+    top = fmaxf(fmaxf(a, b), fmaxf(c, d));
+}
+template <> __device__ __forceinline__ Pairs<__nv_bfloat16>::Pairs(const uint4 &u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    __nv_bfloat162 m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        m[i] = *reinterpret_cast<const __nv_bfloat162 *>(&w[i]);
+    }
+    const __nv_bfloat162 t = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    top = fmaxf(__low2float(t), __high2float(t));
+}
+template <> __device__ __forceinline__ Pairs<__half>::Pairs(const uint4 &u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    __half2 m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m[i] = *reinterpret_cast<const __half2 *>(&w[i]);
+        const float2 f = __half22float2(m[i]);
+        x[i] = two(f.x, f.y);
+    }
+    const __half2 t = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    top = fmaxf(__low2float(t), __high2float(t));
+}
+
 // MODE of the sums: which of exp(z - m) and exp((z - m) / tau) are needed.
 // kSquare: both with tau = 2, where the first is the second squared.
 enum { kOne, kSquare, kBoth };
 
+// exp(c (x - m)) is taken as exp2(c x - c m): one instruction before the
+// exponential.  c m is rounded once for the whole row, the same in forward
+// and backward, so it cancels in the probabilities.
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
 template <int MODE> struct Sums {
     float m = -INFINITY, s1 = 0.f, st = 0.f;
-    // kOne keeps one sum, st, at the scale `c` (1 / tau, or 1 for the label alone)
-    __device__ __forceinline__ static float base(float m) { return m == -INFINITY ? 0.f : m; }
+    // kOne keeps one sum, st, at the scale `c` (log2(e) / tau, or log2(e) for the label alone)
     __device__ __forceinline__ void scale_to(float n, float c) {
         if (n == m) return;
-        const float d = base(m) - base(n);  // m = -inf: sums are 0
-        if (MODE == kOne) st *= exp2_fast(d * c);
-        if (MODE == kSquare) {
-            const float e = exp2_fast(d * c);
-            st *= e, s1 *= e * e;
-        }
-        if (MODE == kBoth) st *= exp2_fast(d * c), s1 *= exp2_fast(d * kLog2e);
+        const float b = base_of(m), d = base_of(n);  // m = -inf: sums are 0
+        const float e = exp2_fast(b * c - d * c);
+        st *= e;
+        if (MODE == kSquare) s1 *= e * e;
+        if (MODE == kBoth) s1 *= exp2_fast(b * kLog2e - d * kLog2e);
         m = n;
     }
-    __device__ __forceinline__ void add(float x, float b, float c) {
-        const float e = exp2_fast((x - b) * c);
+    __device__ __forceinline__ void take(float x, float c) {
+        scale_to(fmaxf(m, x), c);
+        const float b = base_of(m), e = exp2_fast(fmaf(x, c, -(b * c)));
         st += e;
         if (MODE == kSquare) s1 = fmaf(e, e, s1);
-        if (MODE == kBoth) s1 += exp2_fast((x - b) * kLog2e);
+        if (MODE == kBoth) s1 += exp2_fast(fmaf(x, kLog2e, -(b * kLog2e)));
     }
-    template <int N> __device__ __forceinline__ void take(const float *x, float c) {
-        float n = m;
+    // U vectors at once
+    template <typename T, int U> __device__ __forceinline__ void take(const uint4 (&u)[U], float c) {
+        const uint64_t c2 = two(c, c), e2 = two(kLog2e, kLog2e);
+        float top = m;
+        uint64_t x[U][Pairs<T>::count];
 #pragma unroll
-        for (int i = 0; i < N; ++i) n = fmaxf(n, x[i]);
-        scale_to(n, c);
-        const float b = base(m);
+        for (int k = 0; k < U; ++k) {
+            const Pairs<T> p(u[k]);
+            top = fmaxf(top, p.top);
 #pragma unroll
-        for (int i = 0; i < N; ++i) add(x[i], b, c);
+            for (int i = 0; i < Pairs<T>::count; ++i) x[k][i] = p.x[i];
+        }
+        scale_to(top, c);
+        const float b = base_of(m);
+        const uint64_t b2 = two(-(b * c), -(b * c)), b1 = two(-(b * kLog2e), -(b * kLog2e));
+        uint64_t t2[2] = {0, 0}, q2[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int i = 0; i < Pairs<T>::count; ++i) {
+                float e0, e1;
+                apart(fma_two(x[k][i], c2, b2), e0, e1);
+                const uint64_t e = two(exp2_fast(e0), exp2_fast(e1));
+                t2[i & 1] = add_two(t2[i & 1], e);
+                if (MODE == kSquare) q2[i & 1] = fma_two(e, e, q2[i & 1]);
+                if (MODE == kBoth) {
+                    apart(fma_two(x[k][i], e2, b1), e0, e1);
+                    q2[i & 1] = add_two(q2[i & 1], two(exp2_fast(e0), exp2_fast(e1)));
+                }
+            }
+        float a0, a1;
+        apart(add_two(t2[0], t2[1]), a0, a1);
+        st += a0 + a1;
+        if (MODE != kOne) {
+            apart(add_two(q2[0], q2[1]), a0, a1);
+            s1 += a0 + a1;
+        }
     }
     __device__ __forceinline__ void join(float om, float os1, float ost, float c) {
         Sums o;
@@ -103,6 +171,77 @@ __device__ __forceinline__ void part_of(int64_t n, int64_t head, int per16, int 
     lo = r == 0 ? 0 : min(n, head + r * per * per16);
     hi = r == blocks - 1 ? n : min(n, head + (r + 1) * per * per16);
 }
+
+// The teacher's side of a row, in one warp: softmax over its valid entries,
+// and the divergence from the student's log probabilities.  The first entries
+// and the student's logits there are loaded ahead.
+struct Teacher {
+    static constexpr int E = 4;
+    int64_t ids[E];
+    float t[E], x[E];
+    __device__ __forceinline__ static bool valid(const Args &a, int64_t id) { return id >= 0 && id < a.V; }
+    __device__ __forceinline__ void entries(const Args &a, int64_t row, int lane) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const bool on = a.hard != 1.f && lane + 32 * k < a.K;
+            ids[k] = on ? id_at(a, row * a.K + lane + 32 * k) : -1;
+            t[k] = on ? teacher_at(a, row * a.K + lane + 32 * k) * a.inv_tau : 0.f;
+        }
+    }
+    template <typename T> __device__ __forceinline__ void logits(const Args &a, const T *z) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) x[k] = valid(a, ids[k]) ? to_f(z[ids[k]]) : 0.f;
+    }
+    // the row's loss and what backward needs of it, from the sums over the row
+    template <typename T, int MODE>
+    __device__ __forceinline__ void finish(const Args &a, int64_t row, const T *z, int lane, float m, float s1, float st, float zy) {
+        const int64_t base = row * a.K;
+        float tmax = -INFINITY, tsum = 0.f, kl = 0.f;
+        if (a.hard != 1.f) {
+#pragma unroll
+            for (int k = 0; k < E; ++k)
+                if (valid(a, ids[k])) tmax = fmaxf(tmax, t[k]);
+            for (int k = lane + 32 * E; k < a.K; k += 32)
+                if (valid(a, id_at(a, base + k))) tmax = fmaxf(tmax, teacher_at(a, base + k) * a.inv_tau);
+            tmax = warp_max(tmax);
+            if (tmax != -INFINITY) {
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (valid(a, ids[k])) tsum += expf(t[k] - tmax);
+                for (int k = lane + 32 * E; k < a.K; k += 32)
+                    if (valid(a, id_at(a, base + k))) tsum += expf(teacher_at(a, base + k) * a.inv_tau - tmax);
+                tsum = warp_sum(tsum);
+                const float log_tsum = logf(tsum), log_st = logf(st), inv = 1.f / tsum;
+                auto entry = [&](float te, float xe) {
+                    const float lt = te - tmax, p = expf(lt) * inv;
+                    // p = 0 adds nothing, whatever the student says
+                    if (p > 0.f) kl += p * ((lt - log_tsum) - ((xe - m) * a.inv_tau - log_st));
+                };
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (valid(a, ids[k])) entry(t[k], x[k]);
+                for (int k = lane + 32 * E; k < a.K; k += 32) {
+                    const int64_t id = id_at(a, base + k);
+                    if (valid(a, id)) entry(teacher_at(a, base + k) * a.inv_tau, to_f(z[id]));
+                }
+                kl = warp_sum(kl);
+            }
+        }
+        if (lane != 0) return;
+        float loss = 0.f;
+        if (a.hard != 1.f) loss = (1.f - a.hard) * a.tau * a.tau * kl;
+        // exp(z - m) summed: the one sum of kOne (tau = 1 or labels alone), s1 otherwise
+        if (a.hard != 0.f) loss += a.hard * (logf(MODE == kOne ? st : s1) + (m - zy));
+        a.rows[row] = loss;
+        float *q = a.stats + row * kStats;
+        q[0] = m;
+        q[1] = MODE == kOne ? st : s1;
+        q[2] = st;
+        q[3] = tmax;
+        q[4] = tmax == -INFINITY ? 0.f : 1.f / tsum;
+        q[5] = 1.f;
+    }
+};
 
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kThreads) distill_kernel(const Args a) {
@@ -124,41 +263,35 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const Args a) {
     const T *z = static_cast<const T *>(a.z) + row * a.ldz;
     const float c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
 
+    // the first warp of the row's first block will need the teacher's entries and
+    // the student's logits there: the first of them are on their way from here
+    Teacher teacher;
+    if (r == 0 && warp == 0) teacher.entries(a, row, lane), teacher.logits(a, z);
+    const float zy = a.hard != 0.f && r == 0 && tid == 0 ? to_f(z[y]) : 0.f;
+
     Sums<MODE> s;
     const int64_t head = min(a.V, (int64_t)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int64_t)sizeof(T));
     int64_t lo, hi;
     part_of(a.V, head, N, r, blocks, lo, hi);
     if (r == 0) {
-        for (int64_t i = tid; i < head; i += kThreads) {
-            const float x = to_f(z[i]);
-            s.template take<1>(&x, c);
-        }
+        for (int64_t i = tid; i < head; i += kThreads) s.take(to_f(z[i]), c);
         lo = head;
     }
-    const int64_t vecs = hi > lo ? (hi - lo) / N : 0;
-    const V *zv = reinterpret_cast<const V *>(z + lo);
+    const int vecs = hi > lo ? (int)((hi - lo) / N) : 0;
+    const uint4 *zv = reinterpret_cast<const uint4 *>(z + lo);
     constexpr int U = 4;  // vectors in flight per thread
-    int64_t i = tid;
+    int i = tid;
     for (; i + (U - 1) * kThreads < vecs; i += U * kThreads) {
-        V x[U];
+        uint4 x[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) x[k] = zv[i + k * kThreads];
-        float f[U * N];
-#pragma unroll
-        for (int k = 0; k < U * N; ++k) f[k] = to_f(x[k / N].v[k % N]);
-        s.template take<U * N>(f, c);
+        s.template take<T, U>(x, c);
     }
     for (; i < vecs; i += kThreads) {
-        const V x = zv[i];
-        float f[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) f[k] = to_f(x.v[k]);
-        s.template take<N>(f, c);
+        const uint4 x[1] = {zv[i]};
+        s.template take<T, 1>(x, c);
     }
-    for (int64_t e = lo + vecs * N + tid; e < hi; e += kThreads) {
-        const float x = to_f(z[e]);
-        s.template take<1>(&x, c);
-    }
+    for (int64_t e = lo + (int64_t)vecs * N + tid; e < hi; e += kThreads) s.take(to_f(z[e]), c);
 
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -186,51 +319,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const Args a) {
     __syncthreads();
     const float m = part[0], s1 = part[1], st = part[2];
 
-    // the teacher's side, one warp: softmax over its valid entries, then the
-    // divergence from the student's log probabilities
-    if (warp != 0) return;
-    const int64_t base = row * a.K;
-    float tmax = -INFINITY, tsum = 0.f, kl = 0.f;
-    if (a.hard != 1.f) {
-        for (int k = lane; k < a.K; k += 32) {
-            const int64_t id = id_at(a, base + k);
-            if (id >= 0 && id < a.V) tmax = fmaxf(tmax, teacher_at(a, base + k) * a.inv_tau);
-        }
-        tmax = warp_max(tmax);
-        if (tmax != -INFINITY) {
-            for (int k = lane; k < a.K; k += 32) {
-                const int64_t id = id_at(a, base + k);
-                if (id >= 0 && id < a.V) tsum += expf(teacher_at(a, base + k) * a.inv_tau - tmax);
-            }
-            tsum = warp_sum(tsum);
-            const float log_tsum = logf(tsum), log_st = logf(st), inv = 1.f / tsum;
-            for (int k = lane; k < a.K; k += 32) {
-                const int64_t id = id_at(a, base + k);
-                if (id < 0 || id >= a.V) continue;
-                const float lt = teacher_at(a, base + k) * a.inv_tau - tmax;
-                const float p = expf(lt) * inv;
-                // p = 0 adds nothing, whatever the student says
-                if (p > 0.f) kl += p * ((lt - log_tsum) - ((to_f(z[id]) - m) * a.inv_tau - log_st));
-            }
-            kl = warp_sum(kl);
-        }
-    }
-    if (lane == 0) {
-        float loss = 0.f;
-        if (a.hard != 1.f) loss = (1.f - a.hard) * a.tau * a.tau * kl;
-        if (a.hard != 0.f) {
-            // exp(z - m) summed: the one sum of kOne (tau = 1 or labels alone), s1 otherwise
-            loss += a.hard * (logf(MODE == kOne ? st : s1) + (m - to_f(z[y])));
-        }
-        a.rows[row] = loss;
-        float *q = a.stats + row * kStats;
-        q[0] = m;
-        q[1] = MODE == kOne ? st : s1;
-        q[2] = st;
-        q[3] = tmax;
-        q[4] = tmax == -INFINITY ? 0.f : 1.f / tsum;
-        q[5] = 1.f;
-    }
+    if (warp == 0) teacher.finish<T, MODE>(a, row, z, lane, m, s1, st, zy);
 }
 
 // loss = sum of the rows, or their mean over those that count, and the factor
@@ -253,13 +342,43 @@ __global__ void __launch_bounds__(1024)
     }
 }
 
-// one element's gradient without its teacher and label terms
-template <int MODE>
-__device__ __forceinline__ float smooth(float x, float m, float c, float at, float a1) {
-    const float e = exp2_fast((x - m) * c);
-    if (MODE == kOne) return at * e;
-    if (MODE == kSquare) return e * fmaf(a1, e, at);
-    return fmaf(at, e, a1 * exp2_fast((x - m) * kLog2e));
+// gradients without their teacher and label terms: at exp((z - m) / tau) + a1 exp(z - m)
+template <int MODE> struct Smooth {
+    float c, b, b1, at, a1;
+    __device__ __forceinline__ float one(float x) const {
+        const float e = exp2_fast(fmaf(x, c, b));
+        if (MODE == kOne) return at * e;
+        if (MODE == kSquare) return e * fmaf(a1, e, at);
+        return fmaf(at, e, a1 * exp2_fast(fmaf(x, kLog2e, b1)));
+    }
+    __device__ __forceinline__ uint64_t pair(uint64_t x) const {
+        float e0, e1;
+        apart(fma_two(x, two(c, c), two(b, b)), e0, e1);
+        const uint64_t e = two(exp2_fast(e0), exp2_fast(e1)), t = two(at, at), q = two(a1, a1);
+        if (MODE == kOne) return mul_two(t, e);
+        if (MODE == kSquare) return mul_two(e, fma_two(q, e, t));
+        apart(fma_two(x, two(kLog2e, kLog2e), two(b1, b1)), e0, e1);
+        return fma_two(t, e, mul_two(q, two(exp2_fast(e0), exp2_fast(e1))));
+    }
+};
+// 16 bytes of gradients from 16 bytes of logits
+template <int MODE> __device__ __forceinline__ uint4 smooth16(const Smooth<MODE> &f, const uint4 &u, float) {
+    const Pairs<float> p(u);
+    float a, b, c, d;
+    apart(f.pair(p.x[0]), a, b);
+    apart(f.pair(p.x[1]), c, d);
+    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+}
+template <int MODE, typename T> __device__ __forceinline__ uint4 smooth16(const Smooth<MODE> &f, const uint4 &u, T t) {
+    const Pairs<T> p(u);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        apart(f.pair(p.x[i]), a, b);
+        w[i] = pack2(a, b, t);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <typename T, int MODE>
@@ -297,42 +416,35 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Args a
         for (int64_t e = lo + vecs * N + tid; e < hi; e += kThreads) g[e] = zero;
         return;
     }
-    const float m = q[0] == -INFINITY ? 0.f : q[0];
-    const float c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
+    const float m = base_of(q[0]);
     const float soft = (1.f - a.hard) * a.tau * scale;
+    Smooth<MODE> f;
+    f.c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
+    f.b = -(m * f.c), f.b1 = -(m * kLog2e);
     // the factors of exp((z - m) / tau) and of exp(z - m)
-    float at = q[4] != 0.f ? soft / q[2] : 0.f, a1 = a.hard * scale / q[1];
-    if (MODE == kOne) at += a1;
+    f.at = q[4] != 0.f ? soft / q[2] : 0.f, f.a1 = a.hard * scale / q[1];
+    if (MODE == kOne) f.at += f.a1;
 
-    auto one = [&](int64_t i) { g[i] = from_f<T>(smooth<MODE>(to_f(z[i]), m, c, at, a1)); };
+    auto one = [&](int64_t i) { g[i] = from_f<T>(f.one(to_f(z[i]))); };
     if (vec) {
         if (r == 0) {
             for (int64_t i = tid; i < head; i += kThreads) one(i);
             lo = head;
         }
-        const int64_t vecs = hi > lo ? (hi - lo) / N : 0;
-        const V *zv = reinterpret_cast<const V *>(z + lo);
-        V *gv = reinterpret_cast<V *>(g + lo);
+        const int vecs = hi > lo ? (int)((hi - lo) / N) : 0;
+        const uint4 *zv = reinterpret_cast<const uint4 *>(z + lo);
+        uint4 *gv = reinterpret_cast<uint4 *>(g + lo);
         constexpr int U = 2;
-        int64_t i = tid;
+        int i = tid;
         for (; i + (U - 1) * kThreads < vecs; i += U * kThreads) {
-            V x[U];
+            uint4 x[U];
 #pragma unroll
             for (int k = 0; k < U; ++k) x[k] = zv[i + k * kThreads];
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) x[k].v[j] = from_f<T>(smooth<MODE>(to_f(x[k].v[j]), m, c, at, a1));
-                gv[i + k * kThreads] = x[k];
-            }
+            for (int k = 0; k < U; ++k) gv[i + k * kThreads] = smooth16<MODE>(f, x[k], T());
         }
-        for (; i < vecs; i += kThreads) {
-            V x = zv[i];
-#pragma unroll
-            for (int j = 0; j < N; ++j) x.v[j] = from_f<T>(smooth<MODE>(to_f(x.v[j]), m, c, at, a1));
-            gv[i] = x;
-        }
-        for (int64_t e = lo + vecs * N + tid; e < hi; e += kThreads) one(e);
+        for (; i < vecs; i += kThreads) gv[i] = smooth16<MODE>(f, zv[i], T());
+        for (int64_t e = lo + (int64_t)vecs * N + tid; e < hi; e += kThreads) one(e);
     } else {
         for (int64_t e = lo + tid; e < hi; e += kThreads) one(e);
     }
@@ -367,8 +479,261 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Args a
         for (int j = k + 1; j < n; ++j)
             if (ids[j] == id) t += terms[j];
         const int64_t e = from + id;
-        g[e] = from_f<T>(smooth<MODE>(to_f(z[e]), m, c, at, a1) - t);
+        g[e] = from_f<T>(f.one(to_f(z[e])) - t);
     }
+}
+
+// ------------------------------------------------------------ many rows
+//
+// With rows for every SM, blocks stay and take row after row.  One thread
+// streams the rows through a ring of shared memory with bulk copies (16 KB
+// pieces, 64 KB a block, three blocks an SM), across the rows' ends, so the
+// memory never waits for a row's reductions; 256 threads take the pieces from
+// there.  Backward turns a piece into gradients in place, puts the teacher's
+// and the label's terms in, and copies it out the same way.
+
+constexpr int kMath = 256, kRingThreads = kMath + 32, kStages = 4, kPiece = 16384;
+
+struct Ring {
+    uint32_t data, full, free_;
+    __device__ __forceinline__ void init() const {
+        for (int s = 0; s < kStages; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
+        fence_barrier_init();
+    }
+};
+// where the vectors of a row begin, and how many there are
+template <typename T> struct RowShape {
+    int64_t head;
+    int64_t bytes;
+    __device__ __forceinline__ RowShape(const T *z, int64_t V) {
+        head = min(V, (int64_t)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int64_t)sizeof(T));
+        bytes = (V - head) * (int64_t)sizeof(T) / 16 * 16;
+    }
+    __device__ __forceinline__ int pieces() const { return (int)((bytes + kPiece - 1) / kPiece); }
+};
+__device__ __forceinline__ bool row_counts(const Args &a, int64_t row) {
+    if (!a.targets) return true;
+    const int64_t y = a.targets[row];
+    return y >= 0 && y < a.V;
+}
+// the loading thread: every row of this block that counts, piece by piece
+template <typename T> __device__ __forceinline__ void stream_rows(const Args &a, const Ring &ring, int *error) {
+    uint32_t g = 0;
+    for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+        if (!row_counts(a, row)) continue;
+        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+        const RowShape<T> shape(z, a.V);
+        const char *src = reinterpret_cast<const char *>(z + shape.head);
+        for (int64_t at = 0; at < shape.bytes; at += kPiece, ++g) {
+            const uint32_t s = g % kStages;
+            if (g >= kStages && !mbar_wait(ring.free_ + 8 * s, ((g / kStages) & 1) ^ 1)) {
+                report(error);
+                for (uint32_t k = g - kStages; k < g; ++k) mbar_wait(ring.full + 8 * (k % kStages), (k / kStages) & 1);
+                return;
+            }
+            const uint32_t bytes = (uint32_t)min((int64_t)kPiece, shape.bytes - at);
+            mbar_expect(ring.full + 8 * s, bytes);
+            bulk_load(ring.data + s * kPiece, src + at, bytes, ring.full + 8 * s);
+        }
+    }
+}
+__device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 u;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at));
+    return u;
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRingThreads, 3) distill_ring_kernel(const Args a, int *error) {
+    extern __shared__ __align__(128) char ring_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kStages];
+    __shared__ float red[2][3][kMath / 32];
+    const Ring ring = {smem_u32(ring_raw), smem_u32(bars), smem_u32(bars) + 8 * kStages};
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) ring.init();
+    __syncthreads();
+    if (warp == kMath / 32) {
+        if (lane == 0) stream_rows<T>(a, ring, error);
+        return;
+    }
+    const float c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
+    uint32_t g = 0, turn = 0;
+    bool ok = true;
+    for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+        if (!row_counts(a, row)) {
+            if (tid == 0) a.rows[row] = 0.f, a.stats[row * kStats + 5] = 0.f;
+            continue;
+        }
+        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+        const RowShape<T> shape(z, a.V);
+        Teacher teacher;
+        if (warp == 0) teacher.entries(a, row, lane);
+        const float zy = tid == 0 && a.hard != 0.f ? to_f(z[a.targets[row]]) : 0.f;
+        // elements before the first vector and behind the last: one for each of the last warp's threads
+        const int64_t tail = shape.head + shape.bytes / (int64_t)sizeof(T), odd = shape.head + (a.V - tail);
+        const int mine = tid - (kMath - 32);
+        float loose = 0.f;
+        if (mine >= 0 && mine < odd) loose = to_f(z[mine < shape.head ? mine : tail + mine - shape.head]);
+        if (warp == 0) teacher.logits(a, z);
+
+        Sums<MODE> s;
+        for (int64_t at = 0; at < shape.bytes; at += kPiece, ++g) {
+            const uint32_t st = g % kStages;
+            ok = ok && mbar_wait(ring.full + 8 * st, (g / kStages) & 1);
+            const int vecs = (int)(min((int64_t)kPiece, shape.bytes - at) / 16);
+            const uint32_t src = ring.data + st * kPiece;
+            if (vecs == kPiece / 16) {
+#pragma unroll
+                for (int h = 0; h < kPiece / 16 / kMath; h += 2) {
+                    const uint4 u[2] = {lds16(src + (tid + h * kMath) * 16), lds16(src + (tid + (h + 1) * kMath) * 16)};
+                    s.template take<T, 2>(u, c);
+                }
+            } else {
+                for (int i = tid; i < vecs; i += kMath) {
+                    const uint4 u[1] = {lds16(src + i * 16)};
+                    s.template take<T, 1>(u, c);
+                }
+            }
+            math_sync();
+            if (tid == 0) mbar_arrive(ring.free_ + 8 * st);
+        }
+        if (mine >= 0 && mine < odd) s.take(loose, c);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, s.m, o), o1 = __shfl_xor_sync(0xffffffffu, s.s1, o),
+                        ot = __shfl_xor_sync(0xffffffffu, s.st, o);
+            s.join(om, o1, ot, c);
+        }
+        turn ^= 1;  // two sets: the next row's sums do not wait for this one's reader
+        if (lane == 0) red[turn][0][warp] = s.m, red[turn][1][warp] = s.s1, red[turn][2][warp] = s.st;
+        math_sync();
+        if (warp != 0) continue;
+        for (int w = 1; w < kMath / 32; ++w) s.join(red[turn][0][w], red[turn][1][w], red[turn][2][w], c);
+        teacher.finish<T, MODE>(a, row, z, lane, s.m, s.s1, s.st, zy);
+    }
+    if (!ok && lane == 0) report(error);
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRingThreads, 3) distill_backward_ring_kernel(const Args a, int *error) {
+    constexpr int N = 16 / (int)sizeof(T);
+    extern __shared__ __align__(128) char ring_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kStages];
+    __shared__ int32_t ids[CAIL_OPS_DISTILL_MAX_K + 1];
+    __shared__ float terms[CAIL_OPS_DISTILL_MAX_K + 1];
+    const Ring ring = {smem_u32(ring_raw), smem_u32(bars), smem_u32(bars) + 8 * kStages};
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) ring.init();
+    __syncthreads();
+    if (warp == kMath / 32) {
+        if (lane == 0) stream_rows<T>(a, ring, error);
+        return;
+    }
+    Smooth<MODE> f;
+    f.c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
+    const float factor = a.per_row_grad ? 1.f : a.grad_loss[0] * *a.factor;
+    uint32_t g = 0;
+    bool ok = true;
+    for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+        T *out = static_cast<T *>(a.grad) + row * a.ldg;
+        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+        const RowShape<T> shape(z, a.V);
+        const int64_t tail = shape.head + shape.bytes / (int64_t)sizeof(T), odd = shape.head + (a.V - tail);
+        const int64_t loose = tid < odd ? (tid < shape.head ? tid : tail + tid - shape.head) : -1;
+        if (!row_counts(a, row)) {  // zeros
+            const T zero = from_f<T>(0.f);
+            if (loose >= 0) out[loose] = zero;
+            for (int64_t i = tid; i < shape.bytes / 16; i += kMath) reinterpret_cast<uint4 *>(out + shape.head)[i] = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const float *q = a.stats + row * kStats;
+        const float scale = a.per_row_grad ? a.grad_loss[row] : factor;
+        const float m = base_of(q[0]), soft = (1.f - a.hard) * a.tau * scale;
+        f.b = -(m * f.c), f.b1 = -(m * kLog2e);
+        f.at = q[4] != 0.f ? soft / q[2] : 0.f, f.a1 = a.hard * scale / q[1];
+        if (MODE == kOne) f.at += f.a1;
+
+        // the terms of single entries: the same id twice adds up, at its first place
+        const int64_t base = row * a.K;
+        const int K = q[4] != 0.f && soft != 0.f ? a.K : 0, n = K + (a.hard != 0.f ? 1 : 0);
+        math_sync();  // the row before is done with them
+        for (int k = tid; k < K; k += kMath) {
+            const int64_t id = id_at(a, base + k);
+            const bool on = id >= 0 && id < a.V;
+            ids[k] = on ? (int32_t)id : -1;
+            terms[k] = on ? soft * expf(teacher_at(a, base + k) * a.inv_tau - q[3]) * q[4] : 0.f;
+        }
+        if (tid == 0 && n > K) ids[K] = (int32_t)a.targets[row], terms[K] = a.hard * scale;
+        math_sync();
+        int32_t own[4];  // what this thread puts in: up to 4 entries of its own (n <= 1025)
+        float own_term[4];
+        int owned = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int k = tid + x * kMath;
+            own[x] = -1;
+            if (k >= n || ids[k] < 0) continue;
+            bool first = true;
+            for (int j = 0; j < k; ++j) first &= ids[j] != ids[k];
+            if (!first) continue;
+            float t = terms[k];
+            for (int j = k + 1; j < n; ++j)
+                if (ids[j] == ids[k]) t += terms[j];
+            own[x] = ids[k], own_term[x] = t, owned = 1;
+        }
+        float rest = 0.f;  // the 1025th entry (a label beside 1024 teacher entries): thread 0's own
+        int32_t rest_id = -1;
+        if (tid == 0 && n > 4 * kMath) {
+            rest_id = ids[n - 1], rest = terms[n - 1];
+            for (int j = 0; j < n - 1; ++j)
+                if (ids[j] == rest_id) rest_id = -1;  // added where it came first
+        }
+
+        int64_t at = 0;
+        for (; at < shape.bytes; at += kPiece, ++g) {
+            const uint32_t st = g % kStages;
+            ok = ok && mbar_wait(ring.full + 8 * st, (g / kStages) & 1);
+            const int bytes = (int)min((int64_t)kPiece, shape.bytes - at), vecs = bytes / 16;
+            const uint32_t src = ring.data + st * kPiece;
+            // this piece's entries: the logit is kept before the piece is overwritten
+            const int64_t e0 = shape.head + at / (int64_t)sizeof(T), e1 = e0 + vecs * N;
+            float keep[5];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (owned && own[x] >= e0 && own[x] < e1) keep[x] = to_f(*reinterpret_cast<const T *>(ring_raw + st * kPiece + (own[x] - e0) * sizeof(T)));
+            if (rest_id >= e0 && rest_id < e1) keep[4] = to_f(*reinterpret_cast<const T *>(ring_raw + st * kPiece + (rest_id - e0) * sizeof(T)));
+            math_sync();
+            for (int i = tid; i < vecs; i += kMath) {
+                const uint4 y = smooth16<MODE>(f, lds16(src + i * 16), T());
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(src + i * 16), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+            }
+            math_sync();
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (owned && own[x] >= e0 && own[x] < e1)
+                    *reinterpret_cast<T *>(ring_raw + st * kPiece + (own[x] - e0) * sizeof(T)) = from_f<T>(f.one(keep[x]) - own_term[x]);
+            if (rest_id >= e0 && rest_id < e1)
+                *reinterpret_cast<T *>(ring_raw + st * kPiece + (rest_id - e0) * sizeof(T)) = from_f<T>(f.one(keep[4]) - rest);
+            fence_async();
+            math_sync();
+            if (tid == 0) {
+                bulk_store(reinterpret_cast<char *>(out + shape.head) + at, src, bytes);
+                // the piece before has been read out by now, or soon is
+                bulk_wait_read<1>();
+                if (g > 0) mbar_arrive(ring.free_ + 8 * ((g - 1) % kStages));
+            }
+        }
+        // the elements outside the vectors
+        if (loose >= 0) {
+            float t = 0.f;
+            for (int j = 0; j < n; ++j)
+                if (ids[j] == (int32_t)loose) t += terms[j];
+            out[loose] = from_f<T>(f.one(to_f(z[loose])) - t);
+        }
+    }
+    if (tid == 0) bulk_wait_all();
+    if (!ok && lane == 0) report(error);
 }
 
 int check(const cail_ops_distill_args *d) {
@@ -406,6 +771,9 @@ int blocks_per_row(int64_t N, int64_t V, size_t size, int sms) {
     return b;
 }
 
+// rows for every SM, of a piece or more
+bool streams(const Args &a, size_t size) { return a.N >= sm_count() && a.V * (int64_t)size >= kPiece; }
+
 template <typename T, int MODE> int launch(const Args &a, int blocks, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.N * blocks));
@@ -419,12 +787,33 @@ template <typename T, int MODE> int launch(const Args &a, int blocks, cudaStream
     cudaLaunchKernelEx(&cfg, distill_kernel<T, MODE>, a);
     return launched("distill");
 }
+template <typename K> int ring(K kernel, const Args &a, const char *who, cudaStream_t st) {
+    int *error = device_error_flag();
+    if (!error) return fail(CAIL_OPS_ECUDA, "%s: no error word for this device", who);
+    constexpr int smem = kStages * kPiece;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "%s: %s", who, cudaGetErrorString(e));
+    const unsigned grid = (unsigned)min(a.N, 3 * (int64_t)sm_count());
+    kernel<<<grid, kRingThreads, smem, st>>>(a, error);
+    return launched(who);
+}
 template <typename T> int launch(const Args &a, int mode, int blocks, cudaStream_t st) {
+    if (streams(a, sizeof(T))) {
+        if (mode == kOne) return ring(distill_ring_kernel<T, kOne>, a, "distill", st);
+        if (mode == kSquare) return ring(distill_ring_kernel<T, kSquare>, a, "distill", st);
+        return ring(distill_ring_kernel<T, kBoth>, a, "distill", st);
+    }
     if (mode == kOne) return launch<T, kOne>(a, blocks, st);
     if (mode == kSquare) return launch<T, kSquare>(a, blocks, st);
     return launch<T, kBoth>(a, blocks, st);
 }
 template <typename T> int launch_backward(const Args &a, int mode, int blocks, cudaStream_t st) {
+    // in place in the ring: gradients must lie as the logits do, modulo 16 bytes
+    if (streams(a, sizeof(T)) && ((uintptr_t)a.z - (uintptr_t)a.grad) % 16 == 0 && (a.ldz - a.ldg) * (int64_t)sizeof(T) % 16 == 0) {
+        if (mode == kOne) return ring(distill_backward_ring_kernel<T, kOne>, a, "distill backward", st);
+        if (mode == kSquare) return ring(distill_backward_ring_kernel<T, kSquare>, a, "distill backward", st);
+        return ring(distill_backward_ring_kernel<T, kBoth>, a, "distill backward", st);
+    }
     const unsigned grid = (unsigned)(a.N * blocks);
     if (mode == kOne) distill_backward_kernel<T, kOne><<<grid, kThreads, 0, st>>>(a, blocks);
     else if (mode == kSquare) distill_backward_kernel<T, kSquare><<<grid, kThreads, 0, st>>>(a, blocks);

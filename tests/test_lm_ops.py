@@ -538,6 +538,16 @@ DISTILL = [
     (6, 100, 0, 1.0, 0.5, True, 0.0),
 ]
 
+# enough rows for the kernels that stream them: rows of one and several pieces, odd lengths, more rows than blocks, K at its largest
+DISTILL_MANY = [
+    (150, 8193, 5, 2.0, 0.5, True, 0.2),
+    (700, 8200, 33, 1.0, 0.3, True, 0.0),
+    (460, 20011, 129, 3.0, 0.5, True, 0.3),
+    (160, 17001, 1024, 2.0, 0.7, True, 0.1),
+    (300, 9001, 16, 1.7, 0.0, False, 0.5),
+    (200, 16387, 12, 1.0, 1.0, True, 0.0),
+]
+
 
 def distill_inputs(case, dtype, seed=0):
     N, V, K, tau, hard, has_y, gone = case
@@ -587,6 +597,59 @@ def test_distill_matches_64_bit(dtype, case, reduction):
         assert not dz[1:3].any()
     (again,) = torch.autograd.grad(o.distill_loss(z, ids, t, y, **kw), z, g)
     assert torch.equal(again, dz)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("case", DISTILL_MANY, ids=str)
+def test_distill_many_rows(dtype, case):
+    """Loss, gradient and both again on rows further apart; the form of many
+    rows at once, built on torch's log_softmax in 64 bits."""
+    o = ops()
+    N, V, K, tau, hard, has_y, gone = case
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = (torch.randn(N, V, generator=g, device="cuda") * 2).to(dtype)
+    ids = torch.randint(0, V, (N, K), generator=g, device="cuda")
+    ids[torch.rand(N, K, generator=g, device="cuda") < gone] = -1
+    ids[::3, 0] = V - 1  # the last element, and
+    ids[1::3, 0] = 0     # the first, outside the vectors of most rows
+    if K > 3:
+        ids[::2, 1] = ids[::2, 3]
+    t = torch.randn(N, K, generator=g, device="cuda") * 1.5
+    y = torch.randint(0, V, (N,), generator=g, device="cuda") if has_y else None
+    if has_y:
+        y[::7] = -100
+        y[1::7] = 0
+        y[2::7] = V - 1
+        if K > 3:
+            ids[3::7, 2] = y[3::7]
+    r = z.double().requires_grad_()
+    counts = torch.ones(N, dtype=torch.bool, device="cuda") if y is None else (y >= 0) & (y < V)
+    ok = (ids >= 0) & (ids < V)
+    p = torch.where(ok, torch.softmax(torch.where(ok, t.double() / tau, -1e300), 1), 0.0)
+    lq = torch.log_softmax(r / tau, 1).gather(1, ids.clamp(min=0))
+    rows = (1 - hard) * tau * tau * (torch.special.xlogy(p, p) - p * lq).sum(1)
+    if hard:
+        rows = rows - hard * torch.log_softmax(r, 1).gather(1, y.clamp(min=0)[:, None])[:, 0]
+    want = torch.where(counts, rows, 0.0).sum() / counts.sum()
+    (dwant,) = torch.autograd.grad(want, r, torch.tensor(512.0, dtype=torch.float64).cuda())
+    tol = ref.half_step(dtype) + 64 * E
+    floor = 2.0 ** -25 * dwant.numel() ** 0.5 / float(dwant.norm()) if dtype == torch.float16 else 0.0
+    wide = torch.zeros(N, V + 24, dtype=dtype, device="cuda")
+    wide[:, 5:V + 5] = z
+    for x in (z, wide[:, 5:V + 5]):
+        x = x.detach().requires_grad_()
+        loss = o.distill_loss(x, ids, t, y, temperature=tau, hard_weight=hard)
+        (dz,) = torch.autograd.grad(loss, x, torch.tensor(512.0).cuda())
+        assert abs(float(loss.detach()) - float(want.detach())) <= 2e-6 * (1 + float(want.detach()))
+        assert ref.rel(dz, dwant) <= tol + floor
+        assert not dz[~counts].any()
+        # element by element: a misplaced term of one entry does not drown in the norm
+        err = (dz.double() - dwant).abs()
+        assert float((err - (tol * dwant.abs() + 64 * E * 512 / float(counts.sum()) + 2.0 ** -24)).max()) <= 0
+        (again,) = torch.autograd.grad(o.distill_loss(x, ids, t, y, temperature=tau, hard_weight=hard), x, torch.tensor(512.0).cuda())
+        assert torch.equal(again, dz)
+    assert torch.equal(wide[:, :5], torch.zeros_like(wide[:, :5])) and not wide[:, V + 5:].any()
 
 
 @pytest.mark.gpu
