@@ -51,40 +51,50 @@ __device__ __forceinline__ float teacher_at(const Args &a, int64_t i) {
     return to_f(static_cast<const __half *>(a.teacher)[i]);
 }
 
-// 16 bytes of a row as pairs of floats, and their maximum (NaN aside)
+// 16 bytes of a row as pairs of floats, and the running maximum of such
+// vectors (NaN aside), kept packed for the 16-bit types
 template <typename T> struct Pairs {
     static constexpr int count = 8 / (int)sizeof(T);
     uint64_t x[count];
-    float top;
     __device__ __forceinline__ explicit Pairs(const uint4 &u);
 };
 template <> __device__ __forceinline__ Pairs<float>::Pairs(const uint4 &u) {
-    const float a = __uint_as_float(u.x), b = __uint_as_float(u.y), c = __uint_as_float(u.z), d = __uint_as_float(u.w);
-    x[0] = two(a, b), x[1] = two(c, d);
-    top = fmaxf(fmaxf(a, b), fmaxf(c, d));
+    x[0] = two(__uint_as_float(u.x), __uint_as_float(u.y)), x[1] = two(__uint_as_float(u.z), __uint_as_float(u.w));
 }
 template <> __device__ __forceinline__ Pairs<__nv_bfloat16>::Pairs(const uint4 &u) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    __nv_bfloat162 m[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[i] = two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-        m[i] = *reinterpret_cast<const __nv_bfloat162 *>(&w[i]);
-    }
-    const __nv_bfloat162 t = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
-    top = fmaxf(__low2float(t), __high2float(t));
+    for (int i = 0; i < 4; ++i) x[i] = two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
 template <> __device__ __forceinline__ Pairs<__half>::Pairs(const uint4 &u) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    __half2 m[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        m[i] = *reinterpret_cast<const __half2 *>(&w[i]);
-        const float2 f = __half22float2(m[i]);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
         x[i] = two(f.x, f.y);
     }
-    const __half2 t = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
-    top = fmaxf(__low2float(t), __high2float(t));
+}
+template <int U> __device__ __forceinline__ float top_of(const uint4 (&u)[U], float) {
+    float t = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+        t = fmaxf(t, fmaxf(fmaxf(__uint_as_float(u[k].x), __uint_as_float(u[k].y)), fmaxf(__uint_as_float(u[k].z), __uint_as_float(u[k].w))));
+    return t;
+}
+template <typename H2, int U> __device__ __forceinline__ H2 packed_top(const uint4 (&u)[U]) {
+    auto h = [](const uint32_t &w) { return *reinterpret_cast<const H2 *>(&w); };
+    H2 t = __hmax2(__hmax2(h(u[0].x), h(u[0].y)), __hmax2(h(u[0].z), h(u[0].w)));
+#pragma unroll
+    for (int k = 1; k < U; ++k) t = __hmax2(t, __hmax2(__hmax2(h(u[k].x), h(u[k].y)), __hmax2(h(u[k].z), h(u[k].w))));
+    return t;
+}
+template <int U> __device__ __forceinline__ float top_of(const uint4 (&u)[U], __nv_bfloat16) {
+    const __nv_bfloat162 t = packed_top<__nv_bfloat162>(u);
+    return fmaxf(__low2float(t), __high2float(t));
+}
+template <int U> __device__ __forceinline__ float top_of(const uint4 (&u)[U], __half) {
+    const __half2 t = packed_top<__half2>(u);
+    return fmaxf(__low2float(t), __high2float(t));
 }
 
 // MODE of the sums: which of exp(z - m) and exp((z - m) / tau) are needed.
@@ -96,6 +106,9 @@ enum { kOne, kSquare, kBoth };
 // and backward, so it cancels in the probabilities.
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
+// m is a reference, not always the maximum: it moves only when a value lies so
+// far above it (a factor of 2^40 in a sum) that the sums could leave 32 bits'
+// range.
 template <int MODE> struct Sums {
     float m = -INFINITY, s1 = 0.f, st = 0.f;
     // kOne keeps one sum, st, at the scale `c` (log2(e) / tau, or log2(e) for the label alone)
@@ -108,51 +121,6 @@ template <int MODE> struct Sums {
         if (MODE == kBoth) s1 *= exp2_fast(b * kLog2e - d * kLog2e);
         m = n;
     }
-    __device__ __forceinline__ void take(float x, float c) {
-        scale_to(fmaxf(m, x), c);
-        const float b = base_of(m), e = exp2_fast(fmaf(x, c, -(b * c)));
-        st += e;
-        if (MODE == kSquare) s1 = fmaf(e, e, s1);
-        if (MODE == kBoth) s1 += exp2_fast(fmaf(x, kLog2e, -(b * kLog2e)));
-    }
-    // U vectors at once
-    template <typename T, int U> __device__ __forceinline__ void take(const uint4 (&u)[U], float c) {
-        const uint64_t c2 = two(c, c), e2 = two(kLog2e, kLog2e);
-        float top = m;
-        uint64_t x[U][Pairs<T>::count];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const Pairs<T> p(u[k]);
-            top = fmaxf(top, p.top);
-#pragma unroll
-            for (int i = 0; i < Pairs<T>::count; ++i) x[k][i] = p.x[i];
-        }
-        scale_to(top, c);
-        const float b = base_of(m);
-        const uint64_t b2 = two(-(b * c), -(b * c)), b1 = two(-(b * kLog2e), -(b * kLog2e));
-        uint64_t t2[2] = {0, 0}, q2[2] = {0, 0};
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-#pragma unroll
-            for (int i = 0; i < Pairs<T>::count; ++i) {
-                float e0, e1;
-                apart(fma_two(x[k][i], c2, b2), e0, e1);
-                const uint64_t e = two(exp2_fast(e0), exp2_fast(e1));
-                t2[i & 1] = add_two(t2[i & 1], e);
-                if (MODE == kSquare) q2[i & 1] = fma_two(e, e, q2[i & 1]);
-                if (MODE == kBoth) {
-                    apart(fma_two(x[k][i], e2, b1), e0, e1);
-                    q2[i & 1] = add_two(q2[i & 1], two(exp2_fast(e0), exp2_fast(e1)));
-                }
-            }
-        float a0, a1;
-        apart(add_two(t2[0], t2[1]), a0, a1);
-        st += a0 + a1;
-        if (MODE != kOne) {
-            apart(add_two(q2[0], q2[1]), a0, a1);
-            s1 += a0 + a1;
-        }
-    }
     __device__ __forceinline__ void join(float om, float os1, float ost, float c) {
         Sums o;
         o.m = om, o.s1 = os1, o.st = ost;
@@ -160,6 +128,61 @@ template <int MODE> struct Sums {
         scale_to(n, c);
         o.scale_to(n, c);
         s1 += o.s1, st += o.st;
+    }
+};
+// The sums while a thread goes through its part of a row: two packed sums
+// each, and what the exponents need of the reference worked out once.
+template <int MODE> struct Running {
+    float c, reach;          // reach: how far above the reference a value may lie
+    float m = -INFINITY, limit = -INFINITY;
+    uint64_t b2 = 0, b1 = 0;  // minus the reference, in exponents
+    uint64_t t2[2] = {0, 0}, q2[2] = {0, 0};
+    __device__ __forceinline__ explicit Running(float c_) : c(c_) {
+        const float steepest = MODE == kOne ? c : fmaxf(c, kLog2e);
+        reach = (MODE == kSquare ? 20.f / c : 40.f / steepest);
+    }
+    __device__ __forceinline__ Sums<MODE> sums() const {
+        Sums<MODE> s;
+        float a0, a1;
+        s.m = m;
+        apart(add_two(t2[0], t2[1]), a0, a1);
+        s.st = a0 + a1;
+        apart(add_two(q2[0], q2[1]), a0, a1);
+        s.s1 = a0 + a1;
+        return s;
+    }
+    __device__ __forceinline__ void move_to(float top) {
+        Sums<MODE> s = sums();
+        s.scale_to(top, c);
+        m = top, limit = top + reach;
+        const float b = base_of(m);
+        b2 = two(-(b * c), -(b * c)), b1 = two(-(b * kLog2e), -(b * kLog2e));
+        t2[0] = two(s.st, 0.f), t2[1] = 0, q2[0] = two(s.s1, 0.f), q2[1] = 0;
+    }
+    __device__ __forceinline__ void add(uint64_t x, int i) {
+        float e0, e1;
+        apart(fma_two(x, two(c, c), b2), e0, e1);
+        const uint64_t e = two(exp2_fast(e0), exp2_fast(e1));
+        t2[i] = add_two(t2[i], e);
+        if (MODE == kSquare) q2[i] = fma_two(e, e, q2[i]);
+        if (MODE == kBoth) {
+            apart(fma_two(x, two(kLog2e, kLog2e), b1), e0, e1);
+            q2[i] = add_two(q2[i], two(exp2_fast(e0), exp2_fast(e1)));
+        }
+    }
+    __device__ __forceinline__ void take(float x) {
+        if (x > limit) move_to(x);
+        add(two(x, -INFINITY), 0);
+    }
+    template <typename T, int U> __device__ __forceinline__ void take(const uint4 (&u)[U]) {
+        const float top = top_of(u, T());
+        if (top > limit) move_to(top);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const Pairs<T> p(u[k]);
+#pragma unroll
+            for (int i = 0; i < Pairs<T>::count; ++i) add(p.x[i], i & 1);
+        }
     }
 };
 
@@ -269,12 +292,12 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const Args a) {
     if (r == 0 && warp == 0) teacher.entries(a, row, lane), teacher.logits(a, z);
     const float zy = a.hard != 0.f && r == 0 && tid == 0 ? to_f(z[y]) : 0.f;
 
-    Sums<MODE> s;
+    Running<MODE> run(c);
     const int64_t head = min(a.V, (int64_t)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int64_t)sizeof(T));
     int64_t lo, hi;
     part_of(a.V, head, N, r, blocks, lo, hi);
     if (r == 0) {
-        for (int64_t i = tid; i < head; i += kThreads) s.take(to_f(z[i]), c);
+        for (int64_t i = tid; i < head; i += kThreads) run.take(to_f(z[i]));
         lo = head;
     }
     const int vecs = hi > lo ? (int)((hi - lo) / N) : 0;
@@ -285,13 +308,14 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const Args a) {
         uint4 x[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) x[k] = zv[i + k * kThreads];
-        s.template take<T, U>(x, c);
+        run.template take<T, U>(x);
     }
     for (; i < vecs; i += kThreads) {
         const uint4 x[1] = {zv[i]};
-        s.template take<T, 1>(x, c);
+        run.template take<T, 1>(x);
     }
-    for (int64_t e = lo + (int64_t)vecs * N + tid; e < hi; e += kThreads) s.take(to_f(z[e]), c);
+    for (int64_t e = lo + (int64_t)vecs * N + tid; e < hi; e += kThreads) run.take(to_f(z[e]));
+    Sums<MODE> s = run.sums();
 
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -496,8 +520,8 @@ constexpr int kMath = 256, kRingThreads = kMath + 32, kStages = 4, kPiece = 1638
 
 struct Ring {
     uint32_t data, full, free_;
-    __device__ __forceinline__ void init() const {
-        for (int s = 0; s < kStages; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
+    __device__ __forceinline__ void init(int readers) const {
+        for (int s = 0; s < kStages; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, readers);
         fence_barrier_init();
     }
 };
@@ -551,7 +575,7 @@ __global__ void __launch_bounds__(kRingThreads, 3) distill_ring_kernel(const Arg
     __shared__ float red[2][3][kMath / 32];
     const Ring ring = {smem_u32(ring_raw), smem_u32(bars), smem_u32(bars) + 8 * kStages};
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) ring.init();
+    if (tid == 0) ring.init(kMath / 32);
     __syncthreads();
     if (warp == kMath / 32) {
         if (lane == 0) stream_rows<T>(a, ring, error);
@@ -577,28 +601,28 @@ __global__ void __launch_bounds__(kRingThreads, 3) distill_ring_kernel(const Arg
         if (mine >= 0 && mine < odd) loose = to_f(z[mine < shape.head ? mine : tail + mine - shape.head]);
         if (warp == 0) teacher.logits(a, z);
 
-        Sums<MODE> s;
+        Running<MODE> run(c);
         for (int64_t at = 0; at < shape.bytes; at += kPiece, ++g) {
             const uint32_t st = g % kStages;
             ok = ok && mbar_wait(ring.full + 8 * st, (g / kStages) & 1);
             const int vecs = (int)(min((int64_t)kPiece, shape.bytes - at) / 16);
             const uint32_t src = ring.data + st * kPiece;
             if (vecs == kPiece / 16) {
-#pragma unroll
-                for (int h = 0; h < kPiece / 16 / kMath; h += 2) {
-                    const uint4 u[2] = {lds16(src + (tid + h * kMath) * 16), lds16(src + (tid + (h + 1) * kMath) * 16)};
-                    s.template take<T, 2>(u, c);
-                }
+                static_assert(kPiece / 16 == 4 * kMath);
+                const uint4 u[4] = {lds16(src + tid * 16), lds16(src + (tid + kMath) * 16), lds16(src + (tid + 2 * kMath) * 16),
+                                    lds16(src + (tid + 3 * kMath) * 16)};
+                run.template take<T, 4>(u);
             } else {
                 for (int i = tid; i < vecs; i += kMath) {
                     const uint4 u[1] = {lds16(src + i * 16)};
-                    s.template take<T, 1>(u, c);
+                    run.template take<T, 1>(u);
                 }
             }
-            math_sync();
-            if (tid == 0) mbar_arrive(ring.free_ + 8 * st);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ring.free_ + 8 * st);
         }
-        if (mine >= 0 && mine < odd) s.take(loose, c);
+        if (mine >= 0 && mine < odd) run.take(loose);
+        Sums<MODE> s = run.sums();
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             const float om = __shfl_xor_sync(0xffffffffu, s.m, o), o1 = __shfl_xor_sync(0xffffffffu, s.s1, o),
@@ -624,7 +648,7 @@ __global__ void __launch_bounds__(kRingThreads, 3) distill_backward_ring_kernel(
     __shared__ float terms[CAIL_OPS_DISTILL_MAX_K + 1];
     const Ring ring = {smem_u32(ring_raw), smem_u32(bars), smem_u32(bars) + 8 * kStages};
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) ring.init();
+    if (tid == 0) ring.init(1);
     __syncthreads();
     if (warp == kMath / 32) {
         if (lane == 0) stream_rows<T>(a, ring, error);
