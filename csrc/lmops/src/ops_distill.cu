@@ -568,38 +568,60 @@ __device__ __forceinline__ uint4 lds16(uint32_t at) {
     return u;
 }
 
+// Forward: eight warps sum, one loads, and one has the teacher's side, so the
+// chain of its loads and logarithms is not in the summing warps' way.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kRingThreads, 3) distill_ring_kernel(const Args a, int *error) {
+__global__ void __launch_bounds__(kRingThreads + 32, 3) distill_ring_kernel(const Args a, int *error) {
     extern __shared__ __align__(128) char ring_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kStages];
-    __shared__ float red[2][3][kMath / 32];
+    __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
+    __shared__ float red[2][3][kMath / 32];  // the warps' sums of two rows
     const Ring ring = {smem_u32(ring_raw), smem_u32(bars), smem_u32(bars) + 8 * kStages};
+    const uint32_t sums_full = ring.free_ + 8 * kStages, sums_free = sums_full + 16;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) ring.init(kMath / 32);
+    if (tid == 0) {
+        for (int s = 0; s < 2; ++s) mbar_init(sums_full + 8 * s, kMath / 32), mbar_init(sums_free + 8 * s, 1);
+        ring.init(kMath / 32);
+    }
     __syncthreads();
     if (warp == kMath / 32) {
         if (lane == 0) stream_rows<T>(a, ring, error);
         return;
     }
     const float c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
-    uint32_t g = 0, turn = 0;
+    uint32_t g = 0, done = 0;  // pieces and rows so far
     bool ok = true;
+    int64_t y = a.targets ? a.targets[blockIdx.x] : 0;
     for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
-        if (!row_counts(a, row)) {
-            if (tid == 0) a.rows[row] = 0.f, a.stats[row * kStats + 5] = 0.f;
+        const bool counts = y >= 0 && y < a.V;
+        const int64_t label = y;
+        if (a.targets && row + gridDim.x < a.N) y = a.targets[row + gridDim.x];  // the next row's, ahead of its use
+        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+        const uint32_t set = done & 1, phase = (done >> 1) & 1;
+        if (warp > kMath / 32) {  // the teacher's side
+            if (!counts) {
+                if (lane == 0) a.rows[row] = 0.f, a.stats[row * kStats + 5] = 0.f;
+                continue;
+            }
+            Teacher teacher;
+            teacher.entries(a, row, lane);
+            const float zy = a.hard != 0.f ? to_f(z[label]) : 0.f;
+            teacher.logits(a, z);
+            ok = ok && mbar_wait(sums_full + 8 * set, phase);
+            Sums<MODE> s;
+            for (int w = 0; w < kMath / 32; ++w) s.join(red[set][0][w], red[set][1][w], red[set][2][w], c);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sums_free + 8 * set);
+            teacher.finish<T, MODE>(a, row, z, lane, s.m, s.s1, s.st, zy);
+            ++done;
             continue;
         }
-        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+        if (!counts) continue;
         const RowShape<T> shape(z, a.V);
-        Teacher teacher;
-        if (warp == 0) teacher.entries(a, row, lane);
-        const float zy = tid == 0 && a.hard != 0.f ? to_f(z[a.targets[row]]) : 0.f;
         // elements before the first vector and behind the last: one for each of the last warp's threads
         const int64_t tail = shape.head + shape.bytes / (int64_t)sizeof(T), odd = shape.head + (a.V - tail);
         const int mine = tid - (kMath - 32);
         float loose = 0.f;
         if (mine >= 0 && mine < odd) loose = to_f(z[mine < shape.head ? mine : tail + mine - shape.head]);
-        if (warp == 0) teacher.logits(a, z);
 
         Running<MODE> run(c);
         for (int64_t at = 0; at < shape.bytes; at += kPiece, ++g) {
@@ -629,12 +651,12 @@ __global__ void __launch_bounds__(kRingThreads, 3) distill_ring_kernel(const Arg
                         ot = __shfl_xor_sync(0xffffffffu, s.st, o);
             s.join(om, o1, ot, c);
         }
-        turn ^= 1;  // two sets: the next row's sums do not wait for this one's reader
-        if (lane == 0) red[turn][0][warp] = s.m, red[turn][1][warp] = s.s1, red[turn][2][warp] = s.st;
-        math_sync();
-        if (warp != 0) continue;
-        for (int w = 1; w < kMath / 32; ++w) s.join(red[turn][0][w], red[turn][1][w], red[turn][2][w], c);
-        teacher.finish<T, MODE>(a, row, z, lane, s.m, s.s1, s.st, zy);
+        if (done >= 2) ok = ok && mbar_wait(sums_free + 8 * set, phase ^ 1);
+        if (lane == 0) {
+            red[set][0][warp] = s.m, red[set][1][warp] = s.s1, red[set][2][warp] = s.st;
+            mbar_arrive(sums_full + 8 * set);
+        }
+        ++done;
     }
     if (!ok && lane == 0) report(error);
 }
@@ -811,21 +833,21 @@ template <typename T, int MODE> int launch(const Args &a, int blocks, cudaStream
     cudaLaunchKernelEx(&cfg, distill_kernel<T, MODE>, a);
     return launched("distill");
 }
-template <typename K> int ring(K kernel, const Args &a, const char *who, cudaStream_t st) {
+template <typename K> int ring(K kernel, int threads, const Args &a, const char *who, cudaStream_t st) {
     int *error = device_error_flag();
     if (!error) return fail(CAIL_OPS_ECUDA, "%s: no error word for this device", who);
     constexpr int smem = kStages * kPiece;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "%s: %s", who, cudaGetErrorString(e));
     const unsigned grid = (unsigned)min(a.N, 3 * (int64_t)sm_count());
-    kernel<<<grid, kRingThreads, smem, st>>>(a, error);
+    kernel<<<grid, threads, smem, st>>>(a, error);
     return launched(who);
 }
 template <typename T> int launch(const Args &a, int mode, int blocks, cudaStream_t st) {
     if (streams(a, sizeof(T))) {
-        if (mode == kOne) return ring(distill_ring_kernel<T, kOne>, a, "distill", st);
-        if (mode == kSquare) return ring(distill_ring_kernel<T, kSquare>, a, "distill", st);
-        return ring(distill_ring_kernel<T, kBoth>, a, "distill", st);
+        if (mode == kOne) return ring(distill_ring_kernel<T, kOne>, kRingThreads + 32, a, "distill", st);
+        if (mode == kSquare) return ring(distill_ring_kernel<T, kSquare>, kRingThreads + 32, a, "distill", st);
+        return ring(distill_ring_kernel<T, kBoth>, kRingThreads + 32, a, "distill", st);
     }
     if (mode == kOne) return launch<T, kOne>(a, blocks, st);
     if (mode == kSquare) return launch<T, kSquare>(a, blocks, st);
@@ -834,9 +856,9 @@ template <typename T> int launch(const Args &a, int mode, int blocks, cudaStream
 template <typename T> int launch_backward(const Args &a, int mode, int blocks, cudaStream_t st) {
     // in place in the ring: gradients must lie as the logits do, modulo 16 bytes
     if (streams(a, sizeof(T)) && ((uintptr_t)a.z - (uintptr_t)a.grad) % 16 == 0 && (a.ldz - a.ldg) * (int64_t)sizeof(T) % 16 == 0) {
-        if (mode == kOne) return ring(distill_backward_ring_kernel<T, kOne>, a, "distill backward", st);
-        if (mode == kSquare) return ring(distill_backward_ring_kernel<T, kSquare>, a, "distill backward", st);
-        return ring(distill_backward_ring_kernel<T, kBoth>, a, "distill backward", st);
+        if (mode == kOne) return ring(distill_backward_ring_kernel<T, kOne>, kRingThreads, a, "distill backward", st);
+        if (mode == kSquare) return ring(distill_backward_ring_kernel<T, kSquare>, kRingThreads, a, "distill backward", st);
+        return ring(distill_backward_ring_kernel<T, kBoth>, kRingThreads, a, "distill backward", st);
     }
     const unsigned grid = (unsigned)(a.N * blocks);
     if (mode == kOne) distill_backward_kernel<T, kOne><<<grid, kThreads, 0, st>>>(a, blocks);
