@@ -1,7 +1,7 @@
 // attn_simt.cu — window attention on the FP32 pipes: 32-bit inputs, and head
 // sizes or strides that the tensor-core kernels do not take.
 //
-// Forward: a block owns 64 query rows of one head and goes once over the key
+// Forward: a block owns 64 query rows (32 where there are few) of one head and goes once over the key
 // tiles that some of them see, with the running maximum and sum of each row
 // (16 threads share a row; each thread holds 4 rows x 4 columns of the scores
 // and 4 rows x D/16 of the output).  Backward: p is recomputed from the kept
@@ -15,34 +15,56 @@
 namespace cailops {
 namespace {
 
-constexpr int kTile = 64, kThreads = 256;
+constexpr int kTile = 64;  // rows of the tiles that pass; a block owns TR rows, 4 threads' worth each
 constexpr float kNone = -INFINITY;
 
 // rows of shared tiles are DP + 4 floats apart: 16-byte reads of 8 rows in a phase hit different banks
 template <int DP> constexpr int ld() { return DP + 4; }
 constexpr int kLdP = kTile + 4;
 
-// 64 rows of x from row r0 (rows >= n as zeros, columns >= D as zeros), as floats
-template <typename T, int DP>
-__device__ __forceinline__ void load_tile(float *s, const char *base, int64_t st, int r0, int n, int D, bool vec, float by) {
-    if (vec) {
-        constexpr int N = 16 / (int)sizeof(T), C = DP / N;
-        for (int i = threadIdx.x; i < kTile * C; i += kThreads) {
-            const int r = i / C, c = (i % C) * N;
-            Vec<T, N> x;
-            const bool in = r0 + r < n && c < D;
-            if (in) x = *reinterpret_cast<const Vec<T, N> *>(base + (int64_t)(r0 + r) * st + c * sizeof(T));
+// ROWS rows of x from row r0 (rows >= n as zeros, columns >= D as zeros), as
+// floats.  32-bit rows in whole vectors go by asynchronous copies (the caller
+// commits and waits); the others through registers, all loads before the
+// first store.
+template <typename T, int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void load_tile(float *s, const char *base, int64_t st, int r0, int n, int D, bool vec) {
+    constexpr int N = 16 / (int)sizeof(T), C = DP / N, ITER = ROWS * C / THREADS;
+    static_assert(ROWS * C % THREADS == 0);
+    if (vec && sizeof(T) == 4) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) s[r * ld<DP>() + c + k] = in ? to_f(x.v[k]) * by : 0.f;
+        for (int k = 0; k < ITER; ++k) {
+            const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N;
+            const bool in = r0 + r < n && c < D;
+            const char *src = in ? base + (int64_t)(r0 + r) * st + c * sizeof(T) : base;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(s + r * ld<DP>() + c)), "l"(src),
+                         "r"(in ? 16 : 0)
+                         : "memory");
+        }
+    } else if (vec) {
+        Vec<T, N> x[ITER];
+#pragma unroll
+        for (int k = 0; k < ITER; ++k) {
+            const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N;
+            if (r0 + r < n && c < D) x[k] = *reinterpret_cast<const Vec<T, N> *>(base + (int64_t)(r0 + r) * st + c * sizeof(T));
+        }
+#pragma unroll
+        for (int k = 0; k < ITER; ++k) {
+            const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N;
+            const bool in = r0 + r < n && c < D;
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[r * ld<DP>() + c + e] = in ? to_f(x[k].v[e]) : 0.f;
         }
     } else {
-        for (int i = threadIdx.x; i < kTile * DP; i += kThreads) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
             const int r = i / DP, c = i % DP;
             const bool in = r0 + r < n && c < D;
-            s[r * ld<DP>() + c] = in ? to_f(*reinterpret_cast<const T *>(base + (int64_t)(r0 + r) * st + c * sizeof(T))) * by : 0.f;
+            s[r * ld<DP>() + c] = in ? to_f(*reinterpret_cast<const T *>(base + (int64_t)(r0 + r) * st + c * sizeof(T))) : 0.f;
         }
     }
 }
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // acc[r][c] += sum_d x[ty*4+r][d] * y[tx+16c][d]
 template <int DP> __device__ __forceinline__ void dot_tile(const float *x, const float *y, float acc[4][4], int ty, int tx) {
@@ -117,28 +139,35 @@ __device__ __forceinline__ float half_sum(float x) {
     return x;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) simt_forward(const AttnArgs a, bool vec) {
+template <typename T, int DP, int TR>
+__global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool vec) {
     constexpr int NC = DP / 16;
     extern __shared__ float4 smem4[];
-    float *sq = reinterpret_cast<float *>(smem4), *sk = sq + kTile * ld<DP>(), *sv = sk + kTile * ld<DP>(), *sp = sv + kTile * ld<DP>();
+    constexpr int TILE = kTile * ld<DP>();
+    float *sq = reinterpret_cast<float *>(smem4), *sk2 = sq + TR * ld<DP>(), *sv2 = sk2 + 2 * TILE, *sp = sv2 + 2 * TILE;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
-    const int i0 = (gridDim.x - 1 - blockIdx.x) * kTile;  // the longest rows first
+    const int i0 = (gridDim.x - 1 - blockIdx.x) * TR;  // the longest rows first
     const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
     const int n = length_of(a, b);
-    const KeyTiles tiles(i0, i0 + kTile, n, a.window, a.sinks, kTile);
+    const KeyTiles tiles(i0, i0 + TR, n, a.window, a.sinks, kTile);
     const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
 
-    load_tile<T, DP>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec, a.scale_log2);
+    load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
     float o[4][NC] = {}, m[4], l[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) m[r] = kNone, l[r] = 0.f;
 
+    auto fetch = [&](int x) {
+        load_tile<T, DP, kTile, TR * 4>(sk2 + (x & 1) * TILE, kp, a.kt, tiles.at(x) * kTile, n, a.D, vec);
+        load_tile<T, DP, kTile, TR * 4>(sv2 + (x & 1) * TILE, vp, a.vt, tiles.at(x) * kTile, n, a.D, vec);
+        copies_issued();
+    };
+    if (tiles.count) fetch(0);
     for (int x = 0; x < tiles.count; ++x) {
         const int j0 = tiles.at(x) * kTile;
-        __syncthreads();
-        load_tile<T, DP>(sk, kp, a.kt, j0, n, a.D, vec, 1.f);
-        load_tile<T, DP>(sv, vp, a.vt, j0, n, a.D, vec, 1.f);
+        const float *sk = sk2 + (x & 1) * TILE, *sv = sv2 + (x & 1) * TILE;
+        if (x + 1 < tiles.count) fetch(x + 1), copies_done<1>();
+        else copies_done<0>();
         __syncthreads();
         float s[4][4] = {};
         dot_tile<DP>(sq, sk, s, ty, tx);
@@ -148,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) simt_forward(const AttnArgs a, bool 
             float top = kNone;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                if (!seen(i, j0 + tx + 16 * c, n, a.window, a.sinks)) s[r][c] = kNone;
+                s[r][c] = seen(i, j0 + tx + 16 * c, n, a.window, a.sinks) ? s[r][c] * a.scale_log2 : kNone;
                 top = fmaxf(top, s[r][c]);
             }
             top = fmaxf(m[r], half_max(top));
@@ -167,6 +196,7 @@ __global__ void __launch_bounds__(kThreads) simt_forward(const AttnArgs a, bool 
         }
         __syncwarp();  // a row of p is written and read by one warp
         out_tile<DP>(sp, sv, o, ty, tx);
+        __syncthreads();  // the tile's place is free
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -184,23 +214,25 @@ __global__ void __launch_bounds__(kThreads) simt_forward(const AttnArgs a, bool 
 }
 
 // dq and delta of 64 query rows
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) simt_dq(const AttnArgs a, bool vec) {
+template <typename T, int DP, int TR>
+__global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
     constexpr int NC = DP / 16;
+    constexpr int TILE = kTile * ld<DP>();
     extern __shared__ float4 smem4[];
-    float *sq = reinterpret_cast<float *>(smem4), *sg = sq + kTile * ld<DP>(), *sk = sg + kTile * ld<DP>(), *sv = sk + kTile * ld<DP>(),
-          *sp = sv + kTile * ld<DP>();
+    float *sq = reinterpret_cast<float *>(smem4), *sg = sq + TR * ld<DP>(), *sk2 = sg + TR * ld<DP>(), *sv2 = sk2 + 2 * TILE, *sp = sv2 + 2 * TILE;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
-    const int i0 = (gridDim.x - 1 - blockIdx.x) * kTile;
+    const int i0 = (gridDim.x - 1 - blockIdx.x) * TR;
     const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
     const int n = length_of(a, b);
-    const KeyTiles tiles(i0, i0 + kTile, n, a.window, a.sinks, kTile);
+    const KeyTiles tiles(i0, i0 + TR, n, a.window, a.sinks, kTile);
     const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
 
-    // o passes through the key tile's place
-    load_tile<T, DP>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec, a.scale_log2);
-    load_tile<T, DP>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec, 1.f);
-    load_tile<T, DP>(sk, a.o + b * a.ob + h * a.oh, a.ot, i0, n, a.D, vec, 1.f);
+    // o passes through the second key tile's place
+    load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(sk2 + TILE, a.o + b * a.ob + h * a.oh, a.ot, i0, n, a.D, vec);
+    copies_issued();
+    copies_done<0>();
     __syncthreads();
     float delta[4], lse[4], dq[4][NC] = {};
 #pragma unroll
@@ -208,17 +240,24 @@ __global__ void __launch_bounds__(kThreads) simt_dq(const AttnArgs a, bool vec) 
         const int row = ty * 4 + r, i = i0 + row;
         float s = 0.f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) s = fmaf(sg[row * ld<DP>() + tx + 16 * c], sk[row * ld<DP>() + tx + 16 * c], s);
+        for (int c = 0; c < NC; ++c) s = fmaf(sg[row * ld<DP>() + tx + 16 * c], sk2[TILE + row * ld<DP>() + tx + 16 * c], s);
         delta[r] = half_sum(s);
         const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + i;
         lse[r] = i < n ? a.lse[at] : 0.f;
         if (i < a.T && tx == 0) a.delta[at] = delta[r];
     }
+    auto fetch = [&](int x) {
+        load_tile<T, DP, kTile, TR * 4>(sk2 + (x & 1) * TILE, kp, a.kt, tiles.at(x) * kTile, n, a.D, vec);
+        load_tile<T, DP, kTile, TR * 4>(sv2 + (x & 1) * TILE, vp, a.vt, tiles.at(x) * kTile, n, a.D, vec);
+        copies_issued();
+    };
+    if (tiles.count) fetch(0);
+    __syncthreads();  // o's place is free
     for (int x = 0; x < tiles.count; ++x) {
         const int j0 = tiles.at(x) * kTile;
-        __syncthreads();
-        load_tile<T, DP>(sk, kp, a.kt, j0, n, a.D, vec, 1.f);
-        load_tile<T, DP>(sv, vp, a.vt, j0, n, a.D, vec, 1.f);
+        const float *sk = sk2 + (x & 1) * TILE, *sv = sv2 + (x & 1) * TILE;
+        if (x + 1 < tiles.count) fetch(x + 1), copies_done<1>();
+        else copies_done<0>();
         __syncthreads();
         float s[4][4] = {}, dp[4][4] = {};
         dot_tile<DP>(sq, sk, s, ty, tx);
@@ -229,10 +268,11 @@ __global__ void __launch_bounds__(kThreads) simt_dq(const AttnArgs a, bool vec) 
             for (int c = 0; c < 4; ++c) {
                 const int i = i0 + ty * 4 + r;
                 const bool on = seen(i, j0 + tx + 16 * c, n, a.window, a.sinks) && !one_key(i, a.window, a.sinks);
-                sp[(ty * 4 + r) * kLdP + tx + 16 * c] = on ? exp2_fast(s[r][c] - lse[r]) * (dp[r][c] - delta[r]) : 0.f;
+                sp[(ty * 4 + r) * kLdP + tx + 16 * c] = on ? exp2_fast(fmaf(s[r][c], a.scale_log2, -lse[r])) * (dp[r][c] - delta[r]) : 0.f;
             }
         __syncwarp();
         out_tile<DP>(sp, sk, dq, ty, tx);
+        __syncthreads();
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -248,50 +288,61 @@ __global__ void __launch_bounds__(kThreads) simt_dq(const AttnArgs a, bool vec) 
 }
 
 // dk and dv of 64 keys, over the group's heads and the query rows that see them
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) simt_dkv(const AttnArgs a, bool vec) {
+template <typename T, int DP, int TR>
+__global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
     constexpr int NC = DP / 16;
+    constexpr int TILE = kTile * ld<DP>();
     extern __shared__ float4 smem4[];
-    float *sk = reinterpret_cast<float *>(smem4), *sv = sk + kTile * ld<DP>(), *sq = sv + kTile * ld<DP>(), *sg = sq + kTile * ld<DP>(),
-          *sp = sg + kTile * ld<DP>(), *sd = sp + kTile * kLdP;
-    __shared__ float row_lse[kTile], row_delta[kTile];
+    float *sk = reinterpret_cast<float *>(smem4), *sv = sk + TR * ld<DP>(), *sq2 = sv + TR * ld<DP>(), *sg2 = sq2 + 2 * TILE,
+          *sp = sg2 + 2 * TILE, *sd = sp + TR * kLdP;
+    __shared__ float lse2[2][kTile], delta2[2][kTile];
     const int hk = blockIdx.y, b = blockIdx.z;
-    const int j0 = blockIdx.x * kTile;
+    const int j0 = blockIdx.x * TR;
     const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
     const int n = length_of(a, b);
     int begin, end;
-    query_range(j0, j0 + kTile, n, a.window, a.sinks, begin, end);
-    load_tile<T, DP>(sk, a.k + b * a.kb + hk * a.kh, a.kt, j0, n, a.D, vec, a.scale_log2);
-    load_tile<T, DP>(sv, a.v + b * a.vb + hk * a.vh, a.vt, j0, n, a.D, vec, 1.f);
+    query_range(j0, j0 + TR, n, a.window, a.sinks, begin, end);
+    load_tile<T, DP, TR, TR * 4>(sk, a.k + b * a.kb + hk * a.kh, a.kt, j0, n, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(sv, a.v + b * a.vb + hk * a.vh, a.vt, j0, n, a.D, vec);
     float dk[4][NC] = {}, dv[4][NC] = {};
-    for (int h = hk * a.group; h < (hk + 1) * a.group; ++h)
-        for (int i0 = begin / kTile * kTile; i0 < end; i0 += kTile) {
-            __syncthreads();
-            load_tile<T, DP>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec, 1.f);
-            load_tile<T, DP>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec, 1.f);
-            if (tid < kTile) {
-                const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + i0 + tid;
-                row_lse[tid] = i0 + tid < n ? a.lse[at] : 0.f;
-                row_delta[tid] = i0 + tid < n ? a.delta[at] : 0.f;
-            }
-            __syncthreads();
-            float s[4][4] = {}, dp[4][4] = {};
-            dot_tile<DP>(sk, sq, s, ty, tx);
-            dot_tile<DP>(sv, sg, dp, ty, tx);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int i = tx + 16 * c;
-                    const bool on = seen(i0 + i, j0 + ty * 4 + r, n, a.window, a.sinks);
-                    const float p = on ? exp2_fast(s[r][c] - row_lse[i]) : 0.f;
-                    sp[(ty * 4 + r) * kLdP + i] = p;
-                    sd[(ty * 4 + r) * kLdP + i] = on && !one_key(i0 + i, a.window, a.sinks) ? p * (dp[r][c] - row_delta[i]) : 0.f;
-                }
-            __syncwarp();
-            out_tile<DP>(sp, sg, dv, ty, tx);
-            out_tile<DP>(sd, sq, dk, ty, tx);
+    // the tiles that pass: the group's heads in turn, each over the rows that see these keys
+    const int t0 = begin / kTile, per = end > begin ? (end - 1) / kTile + 1 - t0 : 0, count = a.group * per;
+    auto fetch = [&](int x) {
+        const int h = hk * a.group + x / per, i0 = (t0 + x % per) * kTile, at = x & 1;
+        load_tile<T, DP, kTile, TR * 4>(sq2 + at * TILE, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
+        load_tile<T, DP, kTile, TR * 4>(sg2 + at * TILE, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec);
+        if (tid < kTile) {
+            const int64_t row = ((int64_t)b * a.H + h) * a.lse_row + i0 + tid;
+            lse2[at][tid] = i0 + tid < n ? a.lse[row] : 0.f;
+            delta2[at][tid] = i0 + tid < n ? a.delta[row] : 0.f;
         }
+        copies_issued();
+    };
+    if (count) fetch(0);
+    for (int x = 0; x < count; ++x) {
+        const int i0 = (t0 + x % per) * kTile;
+        const float *sq = sq2 + (x & 1) * TILE, *sg = sg2 + (x & 1) * TILE, *row_lse = lse2[x & 1], *row_delta = delta2[x & 1];
+        if (x + 1 < count) fetch(x + 1), copies_done<1>();
+        else copies_done<0>();
+        __syncthreads();
+        float s[4][4] = {}, dp[4][4] = {};
+        dot_tile<DP>(sk, sq, s, ty, tx);
+        dot_tile<DP>(sv, sg, dp, ty, tx);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int i = tx + 16 * c;
+                const bool on = seen(i0 + i, j0 + ty * 4 + r, n, a.window, a.sinks);
+                const float p = on ? exp2_fast(fmaf(s[r][c], a.scale_log2, -row_lse[i])) : 0.f;
+                sp[(ty * 4 + r) * kLdP + i] = p;
+                sd[(ty * 4 + r) * kLdP + i] = on && !one_key(i0 + i, a.window, a.sinks) ? p * (dp[r][c] - row_delta[i]) : 0.f;
+            }
+        __syncwarp();
+        out_tile<DP>(sp, sg, dv, ty, tx);
+        out_tile<DP>(sd, sq, dk, ty, tx);
+        __syncthreads();
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int j = j0 + ty * 4 + r;
@@ -311,27 +362,36 @@ template <typename K> int prepare(K kernel, size_t smem) {
     return e == cudaSuccess ? CAIL_OPS_OK : fail(CAIL_OPS_ECUDA, "window attention: %s", cudaGetErrorString(e));
 }
 
-template <typename T, int DP> int forward(const AttnArgs &a, bool vec, cudaStream_t st) {
-    const size_t smem = (3 * kTile * ld<DP>() + kTile * kLdP) * sizeof(float);
-    if (int rc = prepare(simt_forward<T, DP>, smem)) return rc;
-    simt_forward<T, DP><<<dim3((a.T + kTile - 1) / kTile, a.H, a.B), kThreads, smem, st>>>(a, vec);
+// Rows of a block: 64, or 32 while 64 would give an SM fewer than four blocks
+// (3 padded sequences of 333 tokens, 16 heads of 64, float32, window 100:
+// RESULT).
+template <typename T, int DP, int TR> int forward(const AttnArgs &a, bool vec, cudaStream_t st) {
+    const size_t smem = (TR * ld<DP>() + 4 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
+    if (int rc = prepare(simt_forward<T, DP, TR>, smem)) return rc;
+    simt_forward<T, DP, TR><<<dim3((a.T + TR - 1) / TR, a.H, a.B), TR * 4, smem, st>>>(a, vec);
     return launched("window attention");
 }
-template <typename T, int DP> int backward(const AttnArgs &a, bool vec, cudaStream_t st) {
-    const unsigned tiles = (a.T + kTile - 1) / kTile;
-    size_t smem = (4 * kTile * ld<DP>() + kTile * kLdP) * sizeof(float);
-    if (int rc = prepare(simt_dq<T, DP>, smem)) return rc;
-    simt_dq<T, DP><<<dim3(tiles, a.H, a.B), kThreads, smem, st>>>(a, vec);
+template <typename T, int DP, int TR> int backward(const AttnArgs &a, bool vec, cudaStream_t st) {
+    const unsigned tiles = (a.T + TR - 1) / TR;
+    size_t smem = (2 * TR * ld<DP>() + 4 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
+    if (int rc = prepare(simt_dq<T, DP, TR>, smem)) return rc;
+    simt_dq<T, DP, TR><<<dim3(tiles, a.H, a.B), TR * 4, smem, st>>>(a, vec);
     if (int rc = launched("window attention backward")) return rc;
-    smem += kTile * kLdP * sizeof(float);
-    if (int rc = prepare(simt_dkv<T, DP>, smem)) return rc;
-    simt_dkv<T, DP><<<dim3(tiles, a.Hkv, a.B), kThreads, smem, st>>>(a, vec);
+    smem += TR * kLdP * sizeof(float);
+    if (int rc = prepare(simt_dkv<T, DP, TR>, smem)) return rc;
+    simt_dkv<T, DP, TR><<<dim3(tiles, a.Hkv, a.B), TR * 4, smem, st>>>(a, vec);
     return launched("window attention backward");
 }
+template <typename T, int DP> int sized(const AttnArgs &a, bool vec, bool back, cudaStream_t st) {
+    const bool few = ((int64_t)a.T + 63) / 64 * (back ? a.Hkv : a.H) * a.B < 4 * (int64_t)sm_count();
+    if (few || DP == 128) return back ? backward<T, DP, 32>(a, vec, st) : forward<T, DP, 32>(a, vec, st);
+    if constexpr (DP < 128) return back ? backward<T, DP, 64>(a, vec, st) : forward<T, DP, 64>(a, vec, st);
+    return CAIL_OPS_EINVAL;
+}
 template <typename T> int run(const AttnArgs &a, bool vec, bool back, cudaStream_t st) {
-    if (a.D <= 32) return back ? backward<T, 32>(a, vec, st) : forward<T, 32>(a, vec, st);
-    if (a.D <= 64) return back ? backward<T, 64>(a, vec, st) : forward<T, 64>(a, vec, st);
-    return back ? backward<T, 128>(a, vec, st) : forward<T, 128>(a, vec, st);
+    if (a.D <= 32) return sized<T, 32>(a, vec, back, st);
+    if (a.D <= 64) return sized<T, 64>(a, vec, back, st);
+    return sized<T, 128>(a, vec, back, st);
 }
 
 }  // namespace

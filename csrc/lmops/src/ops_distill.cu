@@ -286,10 +286,10 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const Args a) {
     const T *z = static_cast<const T *>(a.z) + row * a.ldz;
     const float c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
 
-    // the first warp of the row's first block will need the teacher's entries and
-    // the student's logits there: the first of them are on their way from here
+    // the first warp of the row's first block will need the teacher's entries:
+    // the first of them are on their way from here
     Teacher teacher;
-    if (r == 0 && warp == 0) teacher.entries(a, row, lane), teacher.logits(a, z);
+    if (r == 0 && warp == 0) teacher.entries(a, row, lane);
     const float zy = a.hard != 0.f && r == 0 && tid == 0 ? to_f(z[y]) : 0.f;
 
     Running<MODE> run(c);
@@ -314,6 +314,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const Args a) {
         const uint4 x[1] = {zv[i]};
         run.template take<T, 1>(x);
     }
+    if (r == 0 && warp == 0) teacher.logits(a, z);
     for (int64_t e = lo + (int64_t)vecs * N + tid; e < hi; e += kThreads) run.take(to_f(z[e]));
     Sums<MODE> s = run.sums();
 

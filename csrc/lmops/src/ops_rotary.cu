@@ -7,6 +7,8 @@
 // kept.  Each (token, pair) is evaluated once per block into shared memory
 // and used by all heads of q and k.  Bound by memory: every element is read
 // and written once.
+#include <algorithm>
+
 #include "ops_common.cuh"
 
 namespace cailops {
@@ -26,7 +28,7 @@ struct RotaryArgs {
     const double *turns;
     int64_t tokens;
     int T, D, part, per_block;
-    int units, abreast, lanes;  // units of a head, how many of them side by side, heads in flight per block
+    int units, abreast, lanes, head_lanes;  // units of a head, how many of them side by side, times how many (token, head) pairs, of how many heads
     float amplitude;
     int inverse;
 };
@@ -57,55 +59,94 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     }
     __syncthreads();
 
-    // thread = (lane over (token, head), unit of the head); a unit is N pairs
-    // of the half layout, one vector of the interleaved one (one pair where
-    // vectors are single elements), or one vector of the part that passes
-    const int u0 = threadIdx.x % a.abreast, l = threadIdx.x / a.abreast;
+    // A unit of a head is N pairs of the half layout (two vectors), one vector
+    // of the interleaved one (one pair where vectors are single elements), or
+    // one vector of the part that passes.
+    const int l = threadIdx.x / a.abreast;
     if (l >= a.lanes) return;
     const int heads = a.s[0].heads + a.s[1].heads;
     const int rotated = INTER ? (N > 1 ? a.part / N : half) : half / N;
-    int tok = l / heads, h = l - tok * heads;
-    const int dt = a.lanes / heads, dh = a.lanes - dt * heads;
-    int64_t b = (first + tok) / a.T;
-    int t = (int)(first + tok - b * a.T);
-    while (tok < here) {
-        const Side &s = a.s[h >= a.s[0].heads];
-        const int hh = h >= a.s[0].heads ? h - a.s[0].heads : h;
-        const T *in = reinterpret_cast<const T *>(s.in + b * s.isb + t * s.ist + hh * s.ish);
-        T *out = reinterpret_cast<T *>(s.out + b * s.osb + t * s.ost + hh * s.osh);
-        const float2 *w = cs + tok * half;
-        for (int u = u0; u < a.units; u += a.abreast) {
-            if (u >= rotated) {
-                const int at = a.part + (u - rotated) * N;
-                *reinterpret_cast<V *>(out + at) = *reinterpret_cast<const V *>(in + at);
-            } else if constexpr (INTER && N > 1) {
-                V x = *reinterpret_cast<const V *>(in + u * N);
+    if constexpr (INTER && N > 1) {
+        // thread = (unit, token, head lane): it keeps its unit's angles of a
+        // token and goes over the heads, four on their way at a time (32767
+        // tokens of 40 heads of 128, float32: 314 us one at a time, 207 so)
+        constexpr int ANGLES = N / 2, U = 4;
+        for (int u = threadIdx.x % a.abreast; u < a.units; u += a.abreast) {
+            const bool pass = u >= rotated;
+            const int at = pass ? a.part + (u - rotated) * N : u * N;
+            for (int tok = l / a.head_lanes; tok < here; tok += a.lanes / a.head_lanes) {
+                const int64_t g = first + tok, b = g / a.T, t = g - b * a.T;
+                float2 w[ANGLES];
+                if (!pass)
 #pragma unroll
-                for (int i = 0; i < N; i += 2) {
-                    const float2 c = w[(u * N + i) / 2];
-                    const float p = to_f(x.v[i]), q = to_f(x.v[i + 1]);
-                    x.v[i] = from_f<T>(p * c.x - q * c.y);
-                    x.v[i + 1] = from_f<T>(q * c.x + p * c.y);
-                }
-                *reinterpret_cast<V *>(out + u * N) = x;
-            } else {
-                const int xo = INTER ? 2 * u : u * N, yo = INTER ? 2 * u + 1 : half + u * N;
-                V x = *reinterpret_cast<const V *>(in + xo);
-                V y = *reinterpret_cast<const V *>(in + yo);
+                    for (int i = 0; i < ANGLES; ++i) w[i] = cs[tok * half + u * ANGLES + i];
+                const char *in[2] = {a.s[0].in + b * a.s[0].isb + t * a.s[0].ist, a.s[1].in + b * a.s[1].isb + t * a.s[1].ist};
+                char *out[2] = {a.s[0].out + b * a.s[0].osb + t * a.s[0].ost, a.s[1].out + b * a.s[1].osb + t * a.s[1].ost};
+                for (int h0 = l % a.head_lanes; h0 < heads; h0 += U * a.head_lanes) {
+                    V x[U];
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float2 c = w[u * N + i];
-                    const float p = to_f(x.v[i]), q = to_f(y.v[i]);
-                    x.v[i] = from_f<T>(p * c.x - q * c.y);
-                    y.v[i] = from_f<T>(q * c.x + p * c.y);
+                    for (int i = 0; i < U; ++i) {
+                        const int h = h0 + i * a.head_lanes;
+                        if (h < heads) {
+                            const T *p = reinterpret_cast<const T *>(h < a.s[0].heads ? in[0] + h * a.s[0].ish : in[1] + (h - a.s[0].heads) * a.s[1].ish);
+                            x[i] = *reinterpret_cast<const V *>(p + at);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        const int h = h0 + i * a.head_lanes;
+                        if (h >= heads) break;
+                        T *p = reinterpret_cast<T *>(h < a.s[0].heads ? out[0] + h * a.s[0].osh : out[1] + (h - a.s[0].heads) * a.s[1].osh);
+                        if (!pass) {
+#pragma unroll
+                            for (int k = 0; k < ANGLES; ++k) {
+                                const float f0 = to_f(x[i].v[2 * k]), f1 = to_f(x[i].v[2 * k + 1]);
+                                x[i].v[2 * k] = from_f<T>(f0 * w[k].x - f1 * w[k].y);
+                                x[i].v[2 * k + 1] = from_f<T>(f1 * w[k].x + f0 * w[k].y);
+                            }
+                        }
+                        *reinterpret_cast<V *>(p + at) = x[i];
+                    }
                 }
-                *reinterpret_cast<V *>(out + xo) = x;
-                *reinterpret_cast<V *>(out + yo) = y;
             }
         }
-        tok += dt, t += dt, h += dh;
-        if (h >= heads) h -= heads, ++tok, ++t;
-        if (t >= a.T) b += t / a.T, t %= a.T;
+    } else {
+        // thread = (unit, lane over (token, head)); two vectors on their way
+        // are enough here, and more cost the occupancy that feeds the memory
+        // (the same in bf16, all 128 rotated: 115 us, 148 or more with two units)
+        int tok = l / heads, h = l - tok * heads;
+        const int dt = a.lanes / heads, dh = a.lanes - dt * heads;
+        int64_t b = (first + tok) / a.T;
+        int t = (int)(first + tok - b * a.T);
+        while (tok < here) {
+            const Side &s = a.s[h >= a.s[0].heads];
+            const int hh = h >= a.s[0].heads ? h - a.s[0].heads : h;
+            const T *in = reinterpret_cast<const T *>(s.in + b * s.isb + t * s.ist + hh * s.ish);
+            T *out = reinterpret_cast<T *>(s.out + b * s.osb + t * s.ost + hh * s.osh);
+            const float2 *w = cs + tok * half;
+            for (int u = threadIdx.x % a.abreast; u < a.units; u += a.abreast) {
+                if (u >= rotated) {
+                    const int at = a.part + (u - rotated) * N;
+                    *reinterpret_cast<V *>(out + at) = *reinterpret_cast<const V *>(in + at);
+                } else {
+                    const int xo = INTER ? 2 * u : u * N, yo = INTER ? 2 * u + 1 : half + u * N;
+                    V x = *reinterpret_cast<const V *>(in + xo);
+                    V y = *reinterpret_cast<const V *>(in + yo);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float2 c = w[u * N + i];
+                        const float p = to_f(x.v[i]), q = to_f(y.v[i]);
+                        x.v[i] = from_f<T>(p * c.x - q * c.y);
+                        y.v[i] = from_f<T>(q * c.x + p * c.y);
+                    }
+                    *reinterpret_cast<V *>(out + xo) = x;
+                    *reinterpret_cast<V *>(out + yo) = y;
+                }
+            }
+            tok += dt, t += dt, h += dh;
+            if (h >= heads) h -= heads, ++tok, ++t;
+            if (t >= a.T) b += t / a.T, t %= a.T;
+        }
     }
 }
 
@@ -169,15 +210,21 @@ extern "C" int cail_ops_rotary(const cail_ops_rotary_args *r, cail_ops_stream st
     a.units = (r->interleaved && n > 1 ? r->part / n : r->part / 2 / n) + (in_place ? 0 : (r->D - r->part) / n);
     a.abreast = a.units < kThreads ? a.units : kThreads;
     a.lanes = kThreads / a.abreast;
-    // tokens per block: four rounds of its threads, at most 16 KB of angles,
-    // fewer when that leaves SMs without a block
-    const int64_t per_round = (int64_t)a.units * (r->H + Hk);
-    int64_t per = (4 * kThreads + per_round - 1) / per_round;
-    const int64_t most = (16384 / 8) / (r->part / 2) > 0 ? (16384 / 8) / (r->part / 2) : 1;
-    if (per > most) per = most;
-    const int64_t spread = (tokens + 2 * (int64_t)sm_count() - 1) / (2 * (int64_t)sm_count() + 1);
-    if (per > spread) per = spread > 0 ? spread : 1;
+    // Tokens per block: four rounds of its threads (eight of the interleaved layout's), and an angle for every
+    // thread (one token of 40 heads of 128 a block left most threads waiting
+    // for the others' sines: 32767 such tokens 350 us); at most 16 KB of
+    // angles, fewer tokens when that leaves SMs without a block.
+    const int64_t heads = r->H + Hk, half = r->part / 2, sms = sm_count();
+    const int64_t per_round = (int64_t)a.units * heads;
+    int64_t per = std::max(((r->interleaved ? 8 : 4) * kThreads + per_round - 1) / per_round, (kThreads + half - 1) / half);
+    per = std::min(per, std::max<int64_t>(1, 2048 / half));
+    const int64_t spread = (tokens + 2 * sms - 1) / (2 * sms + 1);
+    per = std::min(per, std::max<int64_t>(1, spread));
     a.per_block = (int)per;
+    // interleaved vectors: as many lanes to a token as its block's tokens leave,
+    // and whole tokens only (a head that two lanes took would turn twice in place)
+    a.head_lanes = (int)std::min<int64_t>(std::min<int64_t>(a.lanes, heads), std::max<int64_t>(1, a.lanes / per));
+    if (r->interleaved && n > 1) a.lanes = a.lanes / a.head_lanes * a.head_lanes;
     const int64_t grid = (tokens + per - 1) / per;
     if (grid > 0x7fffffff) return fail(CAIL_OPS_EINVAL, "rotary: too many tokens");
     const size_t smem = (size_t)per * (r->part / 2) * sizeof(float2);
