@@ -66,25 +66,29 @@ __device__ __forceinline__ void load_tile(float *s, const char *base, int64_t st
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// acc[r][c] += sum_d x[ty*4+r][d] * y[tx+16c][d]
+// acc[r][c] = sum_d x[ty*4+r][d] * y[tx+16c][d], even and odd d apart until the end
 template <int DP> __device__ __forceinline__ void dot_tile(const float *x, const float *y, float acc[4][4], int ty, int tx) {
+    uint64_t acc2[4][4] = {};
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
-        float4 a[4], b[4];
+        ulonglong2 a[4], b[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4 *>(x + (ty * 4 + r) * ld<DP>() + d);
+        for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const ulonglong2 *>(x + (ty * 4 + r) * ld<DP>() + d);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const float4 *>(y + (tx + 16 * c) * ld<DP>() + d);
+        for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const ulonglong2 *>(y + (tx + 16 * c) * ld<DP>() + d);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                acc[r][c] = fmaf(a[r].x, b[c].x, acc[r][c]);
-                acc[r][c] = fmaf(a[r].y, b[c].y, acc[r][c]);
-                acc[r][c] = fmaf(a[r].z, b[c].z, acc[r][c]);
-                acc[r][c] = fmaf(a[r].w, b[c].w, acc[r][c]);
-            }
+            for (int c = 0; c < 4; ++c) acc2[r][c] = fma_two(a[r].y, b[c].y, fma_two(a[r].x, b[c].x, acc2[r][c]));
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float e, o;
+            apart(acc2[r][c], e, o);
+            acc[r][c] = e + o;
+        }
 }
 
 // column c of a thread's DP/16 output columns
@@ -93,22 +97,39 @@ template <int DP> __device__ __forceinline__ int column(int tx, int c) {
     if constexpr (NC <= 4) return tx * NC + c;
     return (c / 4) * 64 + tx * 4 + c % 4;
 }
-template <int DP> __device__ __forceinline__ void row_of(const float *y, float *w, int tx) {
-    constexpr int NC = DP / 16;
-    if constexpr (NC == 2) {
-        const float2 f = *reinterpret_cast<const float2 *>(y + tx * 2);
-        w[0] = f.x, w[1] = f.y;
+// a thread's columns in pairs: [r][NC / 2]
+template <int DP> struct Out {
+    static constexpr int NP = DP / 32;
+    uint64_t v[4][NP];
+    __device__ __forceinline__ Out() {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < NP; ++c) v[r][c] = 0;
+    }
+    __device__ __forceinline__ void scale(int r, float f) {
+#pragma unroll
+        for (int c = 0; c < NP; ++c) v[r][c] = mul_two(v[r][c], two(f, f));
+    }
+    __device__ __forceinline__ float at(int r, int c) const {
+        float lo, hi;
+        apart(v[r][c / 2], lo, hi);
+        return c % 2 ? hi : lo;
+    }
+};
+template <int DP> __device__ __forceinline__ void row_of(const float *y, uint64_t *w, int tx) {
+    if constexpr (DP == 32) {
+        w[0] = *reinterpret_cast<const uint64_t *>(y + tx * 2);
     } else {
 #pragma unroll
-        for (int g = 0; g < NC / 4; ++g) {
-            const float4 f = *reinterpret_cast<const float4 *>(y + g * 64 + tx * 4);
-            w[g * 4] = f.x, w[g * 4 + 1] = f.y, w[g * 4 + 2] = f.z, w[g * 4 + 3] = f.w;
+        for (int g = 0; g < DP / 64; ++g) {
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(y + g * 64 + tx * 4);
+            w[g * 2] = f.x, w[g * 2 + 1] = f.y;
         }
     }
 }
-// acc[r][:] += sum_j p[ty*4+r][j] * y[j][:]
-template <int DP> __device__ __forceinline__ void out_tile(const float *p, const float *y, float acc[4][DP / 16], int ty, int tx) {
-    constexpr int NC = DP / 16;
+// o[r][:] += sum_j p[ty*4+r][j] * y[j][:]
+template <int DP> __device__ __forceinline__ void out_tile(const float *p, const float *y, Out<DP> &o, int ty, int tx) {
 #pragma unroll 4
     for (int j = 0; j < kTile; j += 4) {
         float4 a[4];
@@ -116,13 +137,13 @@ template <int DP> __device__ __forceinline__ void out_tile(const float *p, const
         for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4 *>(p + (ty * 4 + r) * kLdP + j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float w[NC];
+            uint64_t w[Out<DP>::NP];
             row_of<DP>(y + (j + e) * ld<DP>(), w, tx);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float f = e == 0 ? a[r].x : e == 1 ? a[r].y : e == 2 ? a[r].z : a[r].w;
 #pragma unroll
-                for (int c = 0; c < NC; ++c) acc[r][c] = fmaf(f, w[c], acc[r][c]);
+                for (int c = 0; c < Out<DP>::NP; ++c) o.v[r][c] = fma_two(two(f, f), w[c], o.v[r][c]);
             }
         }
     }
@@ -153,7 +174,8 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
     const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
 
     load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
-    float o[4][NC] = {}, m[4], l[4];
+    Out<DP> o;
+    float m[4], l[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) m[r] = kNone, l[r] = 0.f;
 
@@ -169,7 +191,7 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
         if (x + 1 < tiles.count) fetch(x + 1), copies_done<1>();
         else copies_done<0>();
         __syncthreads();
-        float s[4][4] = {};
+        float s[4][4];
         dot_tile<DP>(sq, sk, s, ty, tx);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -191,8 +213,7 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
                 sp[(ty * 4 + r) * kLdP + tx + 16 * c] = p;
             }
             l[r] = l[r] * turn + half_sum(sum);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) o[r][c] *= turn;
+            o.scale(r, turn);
         }
         __syncwarp();  // a row of p is written and read by one warp
         out_tile<DP>(sp, sv, o, ty, tx);
@@ -207,7 +228,7 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = column<DP>(tx, c);
-            if (d < a.D) out[d] = from_f<T>(l[r] == 0.f ? 0.f : o[r][c] * inv);
+            if (d < a.D) out[d] = from_f<T>(l[r] == 0.f ? 0.f : o.at(r, c) * inv);
         }
         if (a.lse && tx == 0) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = l[r] == 0.f ? 0.f : m[r] + log2f(l[r]);
     }
@@ -234,7 +255,8 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
     copies_issued();
     copies_done<0>();
     __syncthreads();
-    float delta[4], lse[4], dq[4][NC] = {};
+    float delta[4], lse[4];
+    Out<DP> dq;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int row = ty * 4 + r, i = i0 + row;
@@ -259,7 +281,7 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
         if (x + 1 < tiles.count) fetch(x + 1), copies_done<1>();
         else copies_done<0>();
         __syncthreads();
-        float s[4][4] = {}, dp[4][4] = {};
+        float s[4][4], dp[4][4];
         dot_tile<DP>(sq, sk, s, ty, tx);
         dot_tile<DP>(sg, sv, dp, ty, tx);
 #pragma unroll
@@ -282,7 +304,7 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = column<DP>(tx, c);
-            if (d < a.D) out[d] = from_f<T>(dq[r][c] * a.scale);
+            if (d < a.D) out[d] = from_f<T>(dq.at(r, c) * a.scale);
         }
     }
 }
@@ -304,7 +326,7 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
     query_range(j0, j0 + TR, n, a.window, a.sinks, begin, end);
     load_tile<T, DP, TR, TR * 4>(sk, a.k + b * a.kb + hk * a.kh, a.kt, j0, n, a.D, vec);
     load_tile<T, DP, TR, TR * 4>(sv, a.v + b * a.vb + hk * a.vh, a.vt, j0, n, a.D, vec);
-    float dk[4][NC] = {}, dv[4][NC] = {};
+    Out<DP> dk, dv;
     // the tiles that pass: the group's heads in turn, each over the rows that see these keys
     const int t0 = begin / kTile, per = end > begin ? (end - 1) / kTile + 1 - t0 : 0, count = a.group * per;
     auto fetch = [&](int x) {
@@ -325,7 +347,7 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
         if (x + 1 < count) fetch(x + 1), copies_done<1>();
         else copies_done<0>();
         __syncthreads();
-        float s[4][4] = {}, dp[4][4] = {};
+        float s[4][4], dp[4][4];
         dot_tile<DP>(sk, sq, s, ty, tx);
         dot_tile<DP>(sv, sg, dp, ty, tx);
 #pragma unroll
@@ -352,7 +374,7 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = column<DP>(tx, c);
-            if (d < a.D) ok[d] = from_f<T>(dk[r][c] * a.scale), ov[d] = from_f<T>(dv[r][c]);
+            if (d < a.D) ok[d] = from_f<T>(dk.at(r, c) * a.scale), ov[d] = from_f<T>(dv.at(r, c));
         }
     }
 }
