@@ -11,10 +11,13 @@
 // touch O in no other way than the product.  p is rounded to the input type
 // for that product (its sum is not); everything else is 32-bit.
 //
-// 64 keys per tile and two blocks per SM (256 columns of tensor memory each):
-// the exponentials (16 a clock and SM) bound it at D = 64, 512 clocks per tile
-// against 320 for the products, so two blocks whose softmax and products
-// alternate beat one block with larger tiles.
+// 64 keys per tile.  The exponentials (16 a clock and SM: 512 clocks a tile)
+// bound it at D = 64, so what counts is that some warp always has some to do:
+// four blocks per SM with one buffer of S each (128 columns of tensor memory),
+// which read S twice to stay in 80 registers.  At D = 128 two blocks fit, with
+// two buffers of S each, so that a product runs under the softmax.
+#include <type_traits>
+
 #include "attn.cuh"
 #include "tc.cuh"
 
@@ -25,11 +28,15 @@ constexpr int kRows = 128, kKeys = 64, kThreads = 192;
 
 template <int DP> struct Shape {
     static constexpr int panels = DP / 64;
-    static constexpr int stages = DP == 64 ? 4 : 2;
+    static constexpr int stages = 2;
+    static constexpr int buffers = DP == 64 ? 1 : 2;  // of S
+    static constexpr int per_sm = DP == 64 ? 4 : 2;
+    static constexpr int columns = DP == 64 ? 128 : 256;
+    static constexpr bool twice = DP == 64;           // S is read twice, by the registers that four blocks leave
     static constexpr int q_bytes = kRows * DP * 2, kv_bytes = kKeys * DP * 2;
     static constexpr int barriers = 1 + 4 * stages + 2 + 2 + 2;
     static constexpr int smem = 1024 + q_bytes + 2 * stages * kv_bytes;
-    static constexpr int o_col = 2 * kKeys;  // S0, S1, O
+    static constexpr int o_col = buffers * kKeys;  // S, O
 };
 
 struct Maps {
@@ -37,8 +44,9 @@ struct Maps {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel(const AttnArgs a, const __grid_constant__ Maps maps) {
     using S = Shape<DP>;
+    constexpr int NB = S::buffers;
     constexpr bool bf = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ char raw[];
     __shared__ __align__(8) uint64_t bars[S::barriers];
@@ -90,7 +98,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
         for (int p = 0; p < S::panels; ++p) tma_load(sq + p * kRows * 128, &maps.q, q_full, p * 64, i0, h, b);
         for (int x = 0; x < S::stages && x < tiles.count; ++x) load_k(x), load_v(x);
     }
-    if (warp == 5) tmem_alloc<256>(smem_u32(&tmem_at));
+    if (warp == 5) tmem_alloc<S::columns>(smem_u32(&tmem_at));
     __syncwarp();
     tc_before();
     __syncthreads();
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             if (!warp_wait(k_full + 8 * s, (x / S::stages) & 1)) return false;
             tc_after();
             const uint64_t dks = moved(dk, s * S::kv_bytes);
-            const uint32_t d = tm + (x & 1) * kKeys;
+            const uint32_t d = tm + (x % NB) * kKeys;
             if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
@@ -137,27 +145,27 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
                         mma_ss(d, moved(dq, (kk / 4) * kRows * 128 + (kk % 4) * 32), moved(dks, (kk / 4) * kKeys * 128 + (kk % 4) * 32), kind_s,
                                kk > 0);
                 mma_commit(k_free + 8 * s);
-                mma_commit(s_full + 8 * (x & 1));
+                mma_commit(s_full + 8 * (x % NB));
             }
             __syncwarp();
             return true;
         };
-        ok = warp_wait(q_full, 0) && scores(0) && (tiles.count < 2 || scores(1));
+        ok = warp_wait(q_full, 0) && scores(0) && (NB == 1 || tiles.count < 2 || scores(1));
         for (int x = 0; x < tiles.count && ok; ++x) {
             const int s = x % S::stages;
-            ok = warp_wait(p_full + 8 * (x & 1), (x >> 1) & 1) && warp_wait(v_full + 8 * s, (x / S::stages) & 1);
+            ok = warp_wait(p_full + 8 * (x % NB), (x / NB) & 1) && warp_wait(v_full + 8 * s, (x / S::stages) & 1);
             if (!ok) break;
             tc_after();
             const uint64_t dvs = moved(dv, s * S::kv_bytes);
             if (leader) {
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
-                    mma_ts(tm + S::o_col, tm + (x & 1) * kKeys + kk * 8, moved(dvs, kk * 2048), kind_o, x > 0 || kk > 0);
+                    mma_ts(tm + S::o_col, tm + (x % NB) * kKeys + kk * 8, moved(dvs, kk * 2048), kind_o, x > 0 || kk > 0);
                 mma_commit(v_free + 8 * s);
                 mma_commit(o_done);
             }
             __syncwarp();
-            if (x + 2 < tiles.count) ok = scores(x + 2);
+            if (x + NB < tiles.count) ok = scores(x + NB);
         }
         if (leader) {
             mma_commit(o_last);
@@ -169,27 +177,42 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
         float m = -INFINITY, l = 0.f;  // m: the maximum in use, in scores
         for (int x = 0; x < tiles.count; ++x) {
             const int j0 = tiles.at(x) * kKeys;
-            ok = mbar_wait(s_full + 8 * (x & 1), (x >> 1) & 1);
+            ok = mbar_wait(s_full + 8 * (x % NB), (x / NB) & 1);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_after();
-            const uint32_t at = mine + (x & 1) * kKeys;
-            uint32_t u[kKeys];
-            float *f = reinterpret_cast<float *>(u);
-            tc_ld32(at, u);
-            tc_ld32(at + 32, u + 32);
-            tc_wait_ld(u);
-            tc_touch(u + 32);
+            const uint32_t at = mine + (x % NB) * kKeys;
             // every row of the tile sees every key, unless the tile crosses the diagonal or the window's edge
             const bool whole = j0 + kKeys - 1 <= i0 && (i0 + kRows - 1 - j0 < a.window || j0 + kKeys <= a.sinks);
-            if (!whole) {
-                const uint32_t on[2] = {keys_of_row(i, j0, a.window, a.sinks), keys_of_row(i, j0 + 32, a.window, a.sinks)};
+            uint32_t on[2] = {0xffffffffu, 0xffffffffu};
+            if (!whole) on[0] = keys_of_row(i, j0, a.window, a.sinks), on[1] = keys_of_row(i, j0 + 32, a.window, a.sinks);
+            auto mask = [&](uint32_t *u, int half) {
+                if (whole) return;
 #pragma unroll
-                for (int c = 0; c < kKeys; ++c)
-                    if (!(on[c / 32] & (1u << (c % 32)))) f[c] = -INFINITY;
+                for (int c = 0; c < 32; ++c)
+                    if (!(on[half] & (1u << c))) u[c] = 0xff800000u;  // minus infinity
+            };
+            uint32_t u[2][32];
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto highest = [&](const uint32_t *v) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) tops[c % 4] = fmaxf(tops[c % 4], __uint_as_float(v[c]));
+            };
+            if constexpr (S::twice) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    tc_ld32(at + half * 32, u[0]);
+                    tc_wait_ld(u[0]);
+                    mask(u[0], half);
+                    highest(u[0]);
+                }
+            } else {
+                tc_ld32(at, u[0]);
+                tc_ld32(at + 32, u[1]);
+                tc_wait_ld(u[0]);
+                tc_touch(u[1]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) mask(u[half], half), highest(u[half]);
             }
-            float tops[4] = {f[0], f[1], f[2], f[3]};
-#pragma unroll
-            for (int c = 4; c < kKeys; ++c) tops[c % 4] = fmaxf(tops[c % 4], f[c]);
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             float turn = 1.f;
             if (m == -INFINITY) {
@@ -200,8 +223,9 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
                 m = top;
             }
             if (__any_sync(0xffffffffu, turn != 1.f)) {
-                // until the previous product is in O (the scores of this tile were queued behind the one before it)
-                ok = mbar_wait(o_done, (x - 1) & 1);
+                // The previous product is in O: with one buffer of S, these scores were queued behind it; with two, behind
+                // the one before it.
+                if (NB > 1) ok = mbar_wait(o_done, (x - 1) & 1);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc_after();
 #pragma unroll
@@ -217,19 +241,28 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             const float off = m == -INFINITY ? 0.f : m * a.scale_log2;
             const uint64_t scale2 = two(a.scale_log2, a.scale_log2), off2 = two(-off, -off);
             uint64_t sum[4] = {};
-            uint32_t p[kKeys / 2];
 #pragma unroll
-            for (int c = 0; c < kKeys; c += 2) {
-                float p0, p1;
-                apart(fma_two(two(f[c], f[c + 1]), scale2, off2), p0, p1);
-                p0 = exp2_fast(p0), p1 = exp2_fast(p1);
-                sum[(c / 2) % 4] = add_two(sum[(c / 2) % 4], two(p0, p1));
-                p[c / 2] = pack2(p0, p1, T());
+            for (int half = 0; half < 2; ++half) {
+                uint32_t *v = u[S::twice ? 0 : half];
+                if constexpr (S::twice) {
+                    tc_ld32(at + half * 32, v);
+                    tc_wait_ld(v);
+                    mask(v, half);
+                }
+                uint32_t p[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    float p0, p1;
+                    apart(fma_two(two(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, off2), p0, p1);
+                    p0 = exp2_fast(p0), p1 = exp2_fast(p1);
+                    sum[(c / 2) % 4] = add_two(sum[(c / 2) % 4], two(p0, p1));
+                    p[c / 2] = pack2(p0, p1, T());
+                }
+                tc_st16(at + half * 16, p);  // over scores that have been read
             }
             float s0, s1;
             apart(add_two(add_two(sum[0], sum[1]), add_two(sum[2], sum[3])), s0, s1);
             l += s0 + s1;
-            tc_st32(at, p);
             // keys behind the sequence meet p = 0, but what they hold may be infinite: their values are zeroed
             if (n < a.T && j0 + kKeys > n) {
                 const int s = x % S::stages;
@@ -248,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
             tc_wait_st();
             tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 8 * (x & 1));
+            if (lane == 0) mbar_arrive(p_full + 8 * (x % NB));
         }
         if (ok) ok = mbar_wait(o_last, 0);
         if (__all_sync(0xffffffffu, ok)) {
@@ -294,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 2) tc_forward_kernel(const AttnArgs 
     }
     __syncwarp();
     __syncthreads();
-    if (warp == 5) tmem_free<256>(tm);
+    if (warp == 5) tmem_free<S::columns>(tm);
 }
 
 template <typename T, int DP> int launch(const cail_ops_attention_args *c, const AttnArgs &a, cudaStream_t st) {
