@@ -38,10 +38,14 @@ template <int DP, bool DKV> struct Shape {
     static constexpr int chunk = DKV && DP == 64 ? 16 : 32;  // columns at a time, by the registers that two blocks leave
     static constexpr int x_bytes = kRows * DP * 2, u_bytes = kStream * DP * 2;
     static constexpr int vec_bytes = DKV ? 2 * kStream * 4 : 0;  // lse and delta of a tile's queries
-    static constexpr int barriers = 1 + 2 * stages + 2 * buffers + 1;
+    static constexpr int barriers = 1 + 2 * stages + 2 * buffers + 3;
     static constexpr int o_bytes = DKV ? 0 : x_bytes;  // the output's rows, for delta
     static constexpr int smem = 1024 + 2 * x_bytes + stages * (2 * u_bytes + vec_bytes) + o_bytes;
     static constexpr int acc = buffers * 2 * kStream;  // column of acc0; acc1 follows
+    // One buffer: S of the next tile is computed as soon as this one's is read, for p and ds go elsewhere: into dP's
+    // columns (dk, dv), or ds into columns of its own, so that the next dP is early too (dq).
+    static constexpr bool early = buffers == 1, early_dp = early && !DKV;
+    static constexpr int ds = acc + DP;
     static constexpr int columns = DP == 64 ? 256 : 512;
 };
 
@@ -73,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
     const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + ST * S::u_bytes, svec = sw + ST * S::u_bytes, so = svec;
     const uint32_t bar0 = smem_u32(bars);
-    const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB;
+    const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB, s_read = last + 8, acc_done = s_read + 8;
 
     const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
     const BlockAt at_(DKV ? a.Hkv : a.H, a.B);
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         mbar_init(x_full, 1);
         for (int s = 0; s < ST; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
         for (int s = 0; s < NB; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(ds_full + 8 * s, kMath / 32);
-        mbar_init(last, 1);
+        mbar_init(last, 1), mbar_init(s_read, kMath / 32), mbar_init(acc_done, 1);
         fence_barrier_init();
         // what needs no free slot is on its way before the block has met
         mbar_expect(x_full, 2 * S::x_bytes + S::o_bytes);
@@ -207,18 +211,21 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         // U and W as operands along their rows (scores) and down them (sums)
         const uint64_t dx = operand(sx, 0), dy = operand(sy, 0), du = operand(su, 0), dw = operand(sw, 0), dut = operand(su, kStream * 128),
                        dwt = operand(sw, kStream * 128);
-        auto scores = [&](int x) {
+        // S and dP of a tile; the second of them announces both
+        auto scores = [&](int x, bool first, bool second) {
             const int s = x % ST;
-            if (!warp_wait(full + 8 * s, (x / ST) & 1)) return false;
+            if (first && !warp_wait(full + 8 * s, (x / ST) & 1)) return false;
             tc_after();
             const uint32_t d = tm + (x % NB) * 2 * kStream;
             const uint64_t dus = moved(du, s * S::u_bytes), dws = moved(dw, s * S::u_bytes);
-            if (leader) {
+            if (leader && first) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
                     if (kk < steps)
                         mma_ss(d, moved(dx, (kk / 4) * kRows * 128 + (kk % 4) * 32), moved(dus, (kk / 4) * kStream * 128 + (kk % 4) * 32), kind_s,
                                kk > 0);
+            }
+            if (leader && second) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
                     if (kk < steps)
@@ -230,29 +237,34 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             return true;
         };
         ok = warp_wait(x_full, 0);
-        for (int x = 0; x < NB && x < count && ok; ++x) ok = scores(x);
+        for (int x = 0; x < NB && x < count && ok; ++x) ok = scores(x, true, true);
         for (int x = 0; x < count && ok; ++x) {
             const int s = x % ST;
+            if (S::early && x + 1 < count) {
+                ok = warp_wait(s_read, x & 1) && scores(x + 1, true, S::early_dp);
+                if (!ok) break;
+            }
             ok = warp_wait(ds_full + 8 * (x % NB), (x / NB) & 1);
             if (!ok) break;
             tc_after();
             const uint32_t d = tm + (x % NB) * 2 * kStream;
             if (leader) {
-                // 32 columns of each half lie packed in the first 16 of their place
+                // p and ds of 16 rows each, 8 columns; in dP's place they alternate
                 if constexpr (DKV) {
 #pragma unroll
                     for (int kk = 0; kk < kStream / 16; ++kk)
-                        mma_ts(tm + S::acc + DP, d + (kk / 2) * 32 + (kk % 2) * 8, moved(dwt, s * S::u_bytes + kk * 2048), kind_acc,
-                               x > 0 || kk > 0);
+                        mma_ts(tm + S::acc + DP, d + kStream + kk * 16, moved(dwt, s * S::u_bytes + kk * 2048), kind_acc, x > 0 || kk > 0);
                 }
 #pragma unroll
                 for (int kk = 0; kk < kStream / 16; ++kk)
-                    mma_ts(tm + S::acc, d + kStream + (kk / 2) * 32 + (kk % 2) * 8, moved(dut, s * S::u_bytes + kk * 2048), kind_acc,
+                    mma_ts(tm + S::acc, S::early_dp ? tm + S::ds + kk * 8 : d + kStream + kk * 16 + 8, moved(dut, s * S::u_bytes + kk * 2048), kind_acc,
                            x > 0 || kk > 0);
                 mma_commit(free_ + 8 * s);
+                if (S::early_dp) mma_commit(acc_done);
             }
             __syncwarp();
-            if (x + NB < count) ok = scores(x + NB);
+            if (S::early && !S::early_dp && x + 1 < count) ok = scores(x + 1, false, true);
+            if (!S::early && x + NB < count) ok = scores(x + NB, true, true);
         }
         if (leader) {
             mma_commit(last);
@@ -319,12 +331,23 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                     on_ds = a.window == 1 && a.sinks == 0 ? 0u : on;
                     if (DKV ? c0 == 0 : r == 0) on_ds &= DKV ? ~1u : 0u;  // row 0 sees one key
                 }
+                uint32_t us[32];
+                tc_ld32(at, us);
 #pragma unroll
                 for (int c1 = 0; c1 < 32; c1 += CH) {
-                    uint32_t us[CH], ud[CH], pp[CH / 2], pd[CH / 2];
-                    tc_ld<CH>(at + c1, us);
+                    uint32_t ud[CH], pp[CH / 2], pd[CH / 2];
                     tc_ld<CH>(at + kStream + c1, ud);
-                    tc_wait_both<CH>(us, ud);
+                    if (c1 == 0) {
+                        tc_wait_ld(us);
+                        tc_touch_n<CH>(ud);
+                        if (S::early) {  // S is read: the next one may come
+                            tc_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(s_read);
+                        }
+                    } else {
+                        tc_wait_n<CH>(ud);
+                    }
 #pragma unroll
                     for (int c = 0; c < CH; c += 4) {
                         uint64_t l2[2] = {two(lse, lse), two(lse, lse)}, d2[2] = {two(delta_amp, delta_amp), two(delta_amp, delta_amp)};
@@ -342,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                         float p[4], d[4];
 #pragma unroll
                         for (int e = 0; e < 4; e += 2) {
-                            apart(fma_two(two(__uint_as_float(us[c + e]), __uint_as_float(us[c + e + 1])), scale2, l2[e / 2]), p[e], p[e + 1]);
+                            apart(fma_two(two(__uint_as_float(us[c1 + c + e]), __uint_as_float(us[c1 + c + e + 1])), scale2, l2[e / 2]), p[e], p[e + 1]);
                             p[e] = exp2_fast(-p[e]), p[e + 1] = exp2_fast(-p[e + 1]);
                             const uint64_t t = fma_two(two(__uint_as_float(ud[c + e]), __uint_as_float(ud[c + e + 1])), minus, d2[e / 2]);
                             apart(mul_two(t, two(p[e], p[e + 1])), d[e], d[e + 1]);
@@ -357,9 +380,18 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                         if constexpr (DKV) pp[c / 2] = pack2(p[0], p[1], T()), pp[c / 2 + 1] = pack2(p[2], p[3], T());
                         pd[c / 2] = pack2(d[0], d[1], T()), pd[c / 2 + 1] = pack2(d[2], d[3], T());
                     }
-                    // packed behind one another at the beginning of the 32 columns: over values that are in registers by now
-                    if constexpr (DKV) tc_st<CH / 2>(at + c1 / 2, pp);
-                    tc_st<CH / 2>(at + kStream + c1 / 2, pd);
+                    if (S::early_dp && c1 == 0 && x > 0) {  // ds of the tile before has been used
+                        if (ok) ok = mbar_wait(acc_done, (x - 1) & 1);
+                        __syncwarp();
+                        tc_after();
+                    }
+                    // over values that are in registers by now
+#pragma unroll
+                    for (int k = 0; k < CH / 16; ++k) {
+                        const uint32_t to = S::early_dp ? mine + S::ds + half * 16 + c1 / 2 + k * 8 : at + kStream + c1 + k * 16 + 8;
+                        if constexpr (DKV) tc_st8(at + kStream + c1 + k * 16, pp + k * 8);
+                        tc_st8(to, pd + k * 8);
+                    }
                 }
             };
             if (whole) math(std::false_type());

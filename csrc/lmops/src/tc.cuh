@@ -174,18 +174,15 @@ template <int N> __device__ __forceinline__ void tc_ld(uint32_t at, uint32_t *r)
     if constexpr (N == 16) tc_ld16(at, r);
     else tc_ld32(at, r);
 }
-template <int N> __device__ __forceinline__ void tc_st(uint32_t at, const uint32_t *r) {
-    if constexpr (N == 8) tc_st8(at, r);
-    else tc_st16(at, r);
-}
-// after loads into both
-template <int N> __device__ __forceinline__ void tc_wait_both(uint32_t *r, uint32_t *q) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// the first N registers of a load
+template <int N> __device__ __forceinline__ void tc_touch_n(uint32_t *r) {
 #pragma unroll
-    for (int i = 0; i < N; i += 8) {
+    for (int i = 0; i < N; i += 8)
         asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
-        asm volatile("" : "+r"(q[i]), "+r"(q[i + 1]), "+r"(q[i + 2]), "+r"(q[i + 3]), "+r"(q[i + 4]), "+r"(q[i + 5]), "+r"(q[i + 6]), "+r"(q[i + 7]));
-    }
+}
+template <int N> __device__ __forceinline__ void tc_wait_n(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tc_touch_n<N>(r);
 }
 
 // ---------------------------------------------------------------- operands
