@@ -25,6 +25,10 @@ struct AttnArgs {
 int attn_check(const cail_ops_attention_args *a, bool backward, const char *who);
 AttnArgs attn_args(const cail_ops_attention_args *a, bool backward);
 
+// The tensor-core kernels' grids: heads, sequences, then tiles of 128 rows, so
+// that blocks start in the tiles' order and find their place without a division.
+constexpr int kMostTiles = 65535;
+
 // the tensor-core path (attn_tc_*.cu): whether it takes the call, and the call
 bool tc_takes(const cail_ops_attention_args *a);
 bool tc_takes_backward(const cail_ops_attention_args *a);
@@ -83,19 +87,6 @@ __device__ __forceinline__ uint32_t keys_of_row(int i, int j0, int window, int s
 __device__ __forceinline__ uint32_t rows_of_key(int j, int i0, int n, int window, int sinks) {
     return bits(j - i0, (j < sinks || window > n - j ? n - 1 : j + window - 1) - i0) & bits(0, n - 1 - i0);
 }
-
-// A launch's blocks in one dimension: tiles in the outer place, heads of all
-// sequences in the inner one, so that blocks start in the tiles' order.
-struct BlockAt {
-    int tile, h, b;
-    __device__ __forceinline__ BlockAt(int heads, int B) {
-        const unsigned hb = (unsigned)heads * (unsigned)B;
-        tile = (int)(blockIdx.x / hb);
-        const unsigned r = blockIdx.x - (unsigned)tile * hb;
-        b = (int)(r / (unsigned)heads);
-        h = (int)(r - (unsigned)b * heads);
-    }
-};
 
 __device__ __forceinline__ int length_of(const AttnArgs &a, int b) {
     return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;

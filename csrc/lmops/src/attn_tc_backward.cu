@@ -80,15 +80,14 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB, s_read = last + 8, acc_done = s_read + 8;
 
     const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
-    const BlockAt at_(DKV ? a.Hkv : a.H, a.B);
-    const int b = at_.b, n = length_of(a, b);
+    const int b = blockIdx.y, n = length_of(a, b);
     // rows of this block, and the tiles that pass: x = 0 .. count - 1
     int r0, count, h, hk, split = 0, q_begin = 0, q_tiles = 0, first = 0;
     bool parted = false;
     KeyTiles keys(0, 0, 0, 1, 0, kStream);
     if constexpr (DKV) {
-        hk = at_.h, h = hk * a.group;
-        int tile = at_.tile;
+        hk = blockIdx.x, h = hk * a.group;
+        int tile = blockIdx.z;
         parted = ex.splits > 1 && tile < ex.sink_tiles * ex.splits;
         if (parted) split = tile % ex.splits, tile /= ex.splits;
         else if (ex.splits > 1) tile -= ex.sink_tiles * (ex.splits - 1);
@@ -104,8 +103,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             count = min(count, first + per) - first;
         }
     } else {
-        h = at_.h, hk = h / a.group;
-        r0 = ((a.T - 1) / kRows - at_.tile) * kRows;  // the longest rows first
+        h = blockIdx.x, hk = h / a.group;
+        r0 = (gridDim.z - 1 - blockIdx.z) * kRows;  // the longest rows first
         keys = KeyTiles(r0, r0 + kRows, n, a.window, a.sinks, kStream);
         count = keys.count;
     }
@@ -115,8 +114,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     };
     auto begin_walk = [&] {
         Walk w = {0, 0, h};
-        if constexpr (DKV) w.row = (q_begin + first % q_tiles) * kStream, w.head = h + first / q_tiles;
-        else w.row = keys.at(0) * kStream;
+        if constexpr (DKV) {
+            w.row = q_begin * kStream;
+            if (first > 0) w.row += first % q_tiles * kStream, w.head += first / q_tiles;
+        }
+        if constexpr (!DKV) w.row = keys.at(0) * kStream;
         return w;
     };
     auto step = [&](Walk &w) {
@@ -506,7 +508,8 @@ int splits_of(const cail_ops_attention_args *c, int sms) {
     if (sunk <= plain) return 1;
     const int64_t all = (int64_t)c->B * c->Hkv * ((tiles - sink_tiles) * plain + sink_tiles * sunk);
     const int64_t slots = (int64_t)sms * (c->D <= 64 ? 2 : 1), share = std::max(plain, all / slots);
-    return (int)std::min<int64_t>(32, (sunk + share - 1) / share);
+    // and no more tiles in all than a grid has
+    return (int)std::min<int64_t>(std::min<int64_t>(32, (sunk + share - 1) / share), 1 + (kMostTiles - tiles) / sink_tiles);
 }
 
 struct Layout {
@@ -555,11 +558,10 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     cudaError_t e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_q);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_k);
     if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
-    const int64_t blocks_q = (int64_t)tiles * a.H * a.B, blocks_k = ((int64_t)tiles + ex.sink_tiles * (ex.splits - 1)) * a.Hkv * a.B;
-    if (blocks_q > 0x7fffffff || blocks_k > 0x7fffffff) return fail(CAIL_OPS_EINVAL, "window attention backward: too many tokens");
-    tc_backward_kernel<T, DP, false><<<(unsigned)blocks_q, kThreads, sm_q, st>>>(a, ex, q);
+    tc_backward_kernel<T, DP, false><<<dim3(a.H, a.B, tiles), kThreads, sm_q, st>>>(a, ex, q);
     if (int rc = launched("window attention backward")) return rc;
-    tc_backward_kernel<T, DP, true><<<(unsigned)blocks_k, kThreads, sm_k, st>>>(a, ex, k);
+    const unsigned blocks = tiles + ex.sink_tiles * (ex.splits - 1);  // at most kMostTiles: splits_of()
+    tc_backward_kernel<T, DP, true><<<dim3(a.Hkv, a.B, blocks), kThreads, sm_k, st>>>(a, ex, k);
     if (int rc = launched("window attention backward")) return rc;
     if (ex.splits == 1) return CAIL_OPS_OK;
     const unsigned grid = ((unsigned)ex.sink_tiles * 2 * kRows * (DP / 8) + 255) / 256;

@@ -11,11 +11,14 @@
 // touch O in no other way than the product.  p is rounded to the input type
 // for that product (its sum is not); everything else is 32-bit.
 //
-// 64 keys per tile.  The exponentials (16 a clock and SM: 512 clocks a tile)
-// bound it at D = 64, so what counts is that some warp always has some to do:
-// four blocks per SM with one buffer of S each (128 columns of tensor memory),
-// which read S twice to stay in 80 registers.  At D = 128 two blocks fit, with
-// two buffers of S each, so that a product runs under the softmax.
+// 64 keys per tile, two blocks per SM with two buffers of S each, so a product
+// runs under the softmax.  At D = 64 the exponentials bound it (16 a clock and
+// SM: 512 clocks a tile, against 334 for the products, 50 for a 64-column
+// product from shared memory and 33 from tensor memory); at D = 128 the
+// products do (664 clocks).  Four blocks per SM with one buffer each, and a
+// quarter of the exponentials on the float pipes, both measured the same as
+// this (4 x 4096 tokens, 16 heads, causal: 206 us at D = 64, 274 at D = 128,
+// 670 and 1000 TFLOP/s); small calls took 8 us instead of 6.
 #include <type_traits>
 
 #include "attn.cuh"
@@ -28,11 +31,9 @@ constexpr int kRows = 128, kKeys = 64, kThreads = 192;
 
 template <int DP> struct Shape {
     static constexpr int panels = DP / 64;
-    static constexpr int stages = 2;
-    static constexpr int buffers = DP == 64 ? 1 : 2;  // of S
-    static constexpr int per_sm = DP == 64 ? 4 : 2;
-    static constexpr int columns = DP == 64 ? 128 : 256;
-    static constexpr bool twice = DP == 64;           // S is read twice, by the registers that four blocks leave
+    static constexpr int stages = DP == 64 ? 4 : 2;
+    static constexpr int buffers = 2;  // of S
+    static constexpr int per_sm = 2, columns = 256;
     static constexpr int q_bytes = kRows * DP * 2, kv_bytes = kKeys * DP * 2;
     static constexpr int barriers = 1 + 4 * stages + 2 + 2 + 2;
     static constexpr int smem = 1024 + q_bytes + 2 * stages * kv_bytes;
@@ -58,9 +59,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
     const uint32_t q_full = bar(0), k_full = bar(1), k_free = bar(1 + S::stages), v_full = bar(1 + 2 * S::stages),
                    v_free = bar(1 + 3 * S::stages), s_full = bar(1 + 4 * S::stages), p_full = s_full + 16, o_done = p_full + 16, o_last = o_done + 8;
 
-    const BlockAt at_(a.H, a.B);
-    const int h = at_.h, b = at_.b, hk = h / a.group;
-    const int i0 = ((a.T - 1) / kRows - at_.tile) * kRows;  // the longest rows first
+    const int h = blockIdx.x, b = blockIdx.y, hk = h / a.group;
+    const int i0 = (gridDim.z - 1 - blockIdx.z) * kRows;  // the longest rows first
     const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
     const int n = length_of(a, b);
     const KeyTiles tiles(i0, i0 + kRows, n, a.window, a.sinks, kKeys);
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
             __syncwarp();
             return true;
         };
-        ok = warp_wait(q_full, 0) && scores(0) && (NB == 1 || tiles.count < 2 || scores(1));
+        ok = warp_wait(q_full, 0) && scores(0) && (tiles.count < 2 || scores(1));
         for (int x = 0; x < tiles.count && ok; ++x) {
             const int s = x % S::stages;
             ok = warp_wait(p_full + 8 * (x % NB), (x / NB) & 1) && warp_wait(v_full + 8 * s, (x / S::stages) & 1);
@@ -197,22 +197,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
 #pragma unroll
                 for (int c = 0; c < 32; ++c) tops[c % 4] = fmaxf(tops[c % 4], __uint_as_float(v[c]));
             };
-            if constexpr (S::twice) {
+            tc_ld32(at, u[0]);
+            tc_ld32(at + 32, u[1]);
+            tc_wait_ld(u[0]);
+            tc_touch(u[1]);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    tc_ld32(at + half * 32, u[0]);
-                    tc_wait_ld(u[0]);
-                    mask(u[0], half);
-                    highest(u[0]);
-                }
-            } else {
-                tc_ld32(at, u[0]);
-                tc_ld32(at + 32, u[1]);
-                tc_wait_ld(u[0]);
-                tc_touch(u[1]);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) mask(u[half], half), highest(u[half]);
-            }
+            for (int half = 0; half < 2; ++half) mask(u[half], half), highest(u[half]);
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             float turn = 1.f;
             if (m == -INFINITY) {
@@ -223,9 +213,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
                 m = top;
             }
             if (__any_sync(0xffffffffu, turn != 1.f)) {
-                // The previous product is in O: with one buffer of S, these scores were queued behind it; with two, behind
-                // the one before it.
-                if (NB > 1) ok = mbar_wait(o_done, (x - 1) & 1);
+                // until the previous product is in O (these scores were queued behind the one before it)
+                ok = mbar_wait(o_done, (x - 1) & 1);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc_after();
 #pragma unroll
@@ -243,12 +232,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
             uint64_t sum[4] = {};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                uint32_t *v = u[S::twice ? 0 : half];
-                if constexpr (S::twice) {
-                    tc_ld32(at + half * 32, v);
-                    tc_wait_ld(v);
-                    mask(v, half);
-                }
+                const uint32_t *v = u[half];
                 uint32_t p[16];
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
@@ -338,18 +322,16 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, const
     if (int rc = tensor_map(&maps.v, c->v, c->type, a.B, a.T, a.Hkv, a.D, kKeys)) return rc;
     cudaError_t e = cudaFuncSetAttribute(tc_forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
     if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention: %s", cudaGetErrorString(e));
-    const int64_t grid = ((int64_t)a.T + kRows - 1) / kRows * a.H * a.B;
-    if (grid > 0x7fffffff) return fail(CAIL_OPS_EINVAL, "window attention: too many tokens");
-    tc_forward_kernel<T, DP><<<(unsigned)grid, kThreads, S::smem, st>>>(a, maps);
+    tc_forward_kernel<T, DP><<<dim3(a.H, a.B, (a.T + kRows - 1) / kRows), kThreads, S::smem, st>>>(a, maps);
     return launched("window attention");
 }
 
 }  // namespace
 
 // 16-bit elements in rows that TMA can load (16-byte multiples), a positive
-// scale (the row maximum is taken before scaling)
+// scale (the row maximum is taken before scaling), no more tiles than a grid has
 bool tc_takes(const cail_ops_attention_args *a) {
-    if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f)) return false;
+    if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f) || a->T > kMostTiles * kRows) return false;
     if (!tma_takes(a->q, a->B, a->T, a->H) || !tma_takes(a->k, a->B, a->T, a->Hkv) || !tma_takes(a->v, a->B, a->T, a->Hkv)) return false;
     return rows_aligned(a->o, a->B, a->T, a->H, 2, 16);
 }
