@@ -114,10 +114,11 @@ int cail_ops_distill_backward(const cail_ops_distill_args *a, cail_ops_stream st
 /* The text of this thread's last failure ("" if none). */
 const char *cail_ops_last_error(void);
 
-/* Nonzero when a kernel of this process gave up a bounded wait on the given
- * device since the last call (its results are then wrong): reads and clears
- * the flag; call it after the work has finished. */
-int cail_ops_device_error(int device);
+/* The host word that a kernel on the device sets when a bounded wait of its
+ * runs out (its results are then wrong); NULL before the first call that
+ * launches such a kernel there.  The next call of such a kernel on the device
+ * fails with CAIL_OPS_ECUDA, once, and clears the word. */
+int *cail_ops_device_error_word(int device);
 
 /* Kernels launched by this process so far (all entry points). */
 unsigned long long cail_ops_launches(void);

@@ -581,6 +581,7 @@ size_t tc_workspace(const cail_ops_attention_args *c) { return layout_of(c).tota
 
 int tc_backward(const cail_ops_attention_args *c, cudaStream_t st) {
     AttnArgs a = attn_args(c, true);
+    if (int rc = earlier_error("window attention backward")) return rc;
     a.error = device_error_flag();
     if (!a.error) return fail(CAIL_OPS_ECUDA, "window attention backward: no error word for this device");
     if (c->type == CAIL_OPS_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(c, a, st) : launch<__nv_bfloat16, 128>(c, a, st);

@@ -347,6 +347,7 @@ bool tc_takes_decode(const cail_ops_attention_args *a) {
 
 int tc_decode(const cail_ops_attention_args *c, cudaStream_t st) {
     AttnArgs a = attn_args(c, false);
+    if (int rc = earlier_error("window attention decode")) return rc;
     a.error = device_error_flag();
     if (!a.error) return fail(CAIL_OPS_ECUDA, "window attention decode: no error word for this device");
     if (c->type == CAIL_OPS_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(c, a, st) : launch<__nv_bfloat16, 128>(c, a, st);

@@ -835,6 +835,7 @@ template <typename T, int MODE> int launch(const Args &a, int blocks, cudaStream
     return launched("distill");
 }
 template <typename K> int ring(K kernel, int threads, const Args &a, const char *who, cudaStream_t st) {
+    if (int rc = earlier_error(who)) return rc;
     int *error = device_error_flag();
     if (!error) return fail(CAIL_OPS_ECUDA, "%s: no error word for this device", who);
     constexpr int smem = kStages * kPiece;

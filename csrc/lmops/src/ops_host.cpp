@@ -16,7 +16,7 @@ std::atomic<unsigned long long> g_launches{0};
 constexpr int kMaxDevices = 64;
 std::atomic<int> g_sms[kMaxDevices];
 std::mutex g_flag_mutex;
-int *g_flag_host[kMaxDevices] = {};
+std::atomic<int *> g_flag_host[kMaxDevices];
 std::atomic<int *> g_flag_dev[kMaxDevices];
 }  // namespace
 
@@ -46,6 +46,15 @@ int sm_count() {
     return n;
 }
 
+int earlier_error(const char *who) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CAIL_OPS_OK;
+    volatile int *h = g_flag_host[dev].load(std::memory_order_acquire);
+    if (!h || *h == 0) return CAIL_OPS_OK;
+    *h = 0;
+    return fail(CAIL_OPS_ECUDA, "%s: a kernel of an earlier call gave up waiting for its data; that call's results are wrong", who);
+}
+
 // One mapped host word per device: a kernel whose bounded wait ran out stores
 // there, and the host reads it without touching the device.  Made on first
 // use; the allocation is legal while another stream of this thread is being
@@ -70,7 +79,7 @@ int *device_error_flag() {
         return nullptr;
     }
     *static_cast<volatile int *>(h) = 0;
-    g_flag_host[dev] = static_cast<int *>(h);
+    g_flag_host[dev].store(static_cast<int *>(h), std::memory_order_release);
     g_flag_dev[dev].store(static_cast<int *>(d), std::memory_order_release);
     return static_cast<int *>(d);
 }
@@ -81,12 +90,7 @@ extern "C" const char *cail_ops_last_error(void) { return cailops::t_error; }
 
 extern "C" unsigned long long cail_ops_launches(void) { return cailops::g_launches.load(); }
 
-extern "C" int cail_ops_device_error(int device) {
-    if (device < 0 || device >= cailops::kMaxDevices) return 0;
-    std::lock_guard<std::mutex> lock(cailops::g_flag_mutex);
-    volatile int *h = cailops::g_flag_host[device];
-    if (!h) return 0;
-    int v = *h;
-    *h = 0;
-    return v;
+extern "C" int *cail_ops_device_error_word(int device) {
+    if (device < 0 || device >= cailops::kMaxDevices) return nullptr;
+    return cailops::g_flag_host[device].load();
 }

@@ -56,7 +56,6 @@ struct Lib {
     decltype(&cail_ops_distill) distill = nullptr;
     decltype(&cail_ops_distill_backward) distill_backward = nullptr;
     decltype(&cail_ops_last_error) last_error = nullptr;
-    decltype(&cail_ops_device_error) device_error = nullptr;
     decltype(&cail_ops_launches) launches = nullptr;
 } L;
 
@@ -75,7 +74,6 @@ void load(const std::string &path) {
     get(L.distill, "cail_ops_distill");
     get(L.distill_backward, "cail_ops_distill_backward");
     get(L.last_error, "cail_ops_last_error");
-    get(L.device_error, "cail_ops_device_error");
     get(L.launches, "cail_ops_launches");
 }
 
@@ -105,6 +103,20 @@ cail_ops_stream stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStr
 
 // rows whose elements lie side by side; a copy where they do not
 Tensor rows(const Tensor &t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// 16-bit rows that the tensor-core kernels' tile loads take: 16-byte
+// boundaries, no repeated rows
+bool tiled(const Tensor &t) {
+    auto ok = [&](int64_t i) { return t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0); };
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(3) == 1 || t.stride(3) == 1) && ok(0) && ok(1) && ok(2);
+}
+// the same values in rows that they take, where that pays: a copy costs one
+// pass over the tensor, the other kernels many times the products' time
+constexpr int64_t kCopyFrom = 128;  // tokens
+Tensor for_tiles(const Tensor &t) {
+    if (t.scalar_type() == at::kFloat || t.size(3) % 8 || t.size(1) <= kCopyFrom || t.numel() == 0 || tiled(t)) return t;
+    return t.clone(at::MemoryFormat::Contiguous);
+}
 
 cail_ops_bthd view(const Tensor &t) {
     if (t.dim() == 3) return {t.data_ptr(), t.stride(0), 0, t.stride(1)};
@@ -314,7 +326,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
         Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
         if (q.numel()) {
             c10::cuda::CUDAGuard guard(q.device());
-            const Tensor dout = rows(g[0]);
+            const Tensor dout = for_tiles(rows(g[0]));
             cail_ops_attention_args a = attention_args(q, k, v, o, {s[5], ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(),
                                                                    ctx->saved_data["scale"].toDouble()});
             a.dout = view(dout), a.dq = view(dq), a.dk = view(dk), a.dv = view(dv);
@@ -334,14 +346,25 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     }
 };
 
+Tensor window_attention_on(const Tensor &q_, const Tensor &k_, const Tensor &v_, const AttnHow &w) {
+    const Tensor q = for_tiles(q_), k = for_tiles(k_), v = for_tiles(v_);
+    if (wants_grad({&q, &k, &v})) return AttentionFn::apply(q, k, v, maybe(w.lengths), w.window, w.sinks, w.scale);
+    return attention_forward(rows(q), rows(k), rows(v), w, nullptr);
+}
+
 Tensor window_attention(const Tensor &q, const Tensor &k, const Tensor &v, int64_t window, int64_t sinks, const std::optional<Tensor> &lengths_,
                         const std::optional<double> &scale_) {
     AttnHow w{or_none(lengths_), window, sinks, 0.0};
     w.scale = scale_.has_value() ? *scale_ : q.dim() > 0 && q.size(-1) > 0 ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0;
     attention_check("window_attention", q, k, v, w, false);
     if (w.lengths.defined()) w.lengths = w.lengths.contiguous();
-    if (wants_grad({&q, &k, &v})) return AttentionFn::apply(q, k, v, maybe(w.lengths), window, sinks, w.scale);
-    return attention_forward(rows(q), rows(k), rows(v), w, nullptr);
+    const int64_t D = q.size(3);
+    if (D % 8 && q.scalar_type() != at::kFloat && q.size(1) > kCopyFrom && q.numel()) {
+        // heads of a size that the tile loads do not take, as the next size that they do: zeros add nothing to a product
+        auto padded = [&](const Tensor &t) { return at::constant_pad_nd(t, {0, 8 - D % 8}); };
+        return window_attention_on(padded(q), padded(k), padded(v), w).narrow(3, 0, D).contiguous();
+    }
+    return window_attention_on(q, k, v, w);
 }
 
 Tensor window_attention_decode(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &lengths, int64_t window, int64_t sinks,
@@ -466,7 +489,6 @@ Tensor distill_loss(const Tensor &z_, const Tensor &ids_, const Tensor &t_, cons
     return distill_forward(z, ids, t, y, tau, hard, mean, nullptr);
 }
 
-int64_t device_error(int64_t device) { return L.device_error((int)device); }
 int64_t launches() { return (int64_t)L.launches(); }
 
 }  // namespace
@@ -479,6 +501,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("window_attention", &window_attention);
     m.def("window_attention_decode", &window_attention_decode);
     m.def("distill_loss", &distill_loss);
-    m.def("device_error", &device_error);
     m.def("launches", &launches);
 }

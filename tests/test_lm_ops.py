@@ -272,6 +272,11 @@ ATTENTION = [
     (1, 700, 2, 1, 128, 1000, 0, [699]),
     (2, 640, 2, 2, 8, 250, 1000, [640, 3]),
     (1, 1100, 1, 1, 64, 300, 260, None),
+    (1, 1500, 4, 1, 128, 100, 3, [1400]),
+    (2, 1025, 2, 1, 64, 64, 129, [1025, 200]),
+    (1, 300, 2, 1, 100, 50, 2, [290]),
+    (2, 190, 2, 2, 1, 30, 2, None),
+    (1, 150, 3, 1, 127, 400, 0, None),
 ]
 
 
@@ -427,6 +432,51 @@ def test_window_attention_extreme_scores():
         out = o.window_attention(q, k, v, 90, 2)
         # scores of up to |s| = 64 * 8 * 8 * 4 / 8 = 1024 carry s * 2e in the exponent
         assert ref.rel(out, ref.attention(q, k, v, 90, 2)) <= 3 * ref.half_step(dtype) + 2048 * 2 * E
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("scale", [0.3, -0.2, 0.0])
+def test_window_attention_scale(dtype, scale):
+    o = ops()
+    case = (1, 200, 2, 1, 64, 90, 2, None)
+    q, k, v, do, _ = attention_inputs(case, dtype)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = o.window_attention(*leaves, 90, 2, scale=scale)
+    grads = torch.autograd.grad(out, leaves, do)
+    r = [x.detach().double().requires_grad_() for x in leaves]
+    want = ref.attention(*r, 90, 2, scale=scale)
+    dwant = torch.autograd.grad(want, r, do.double())
+    u = ref.half_step(dtype)
+    assert ref.rel(out, want) <= 3 * u + 64 * E
+    for got, w in zip(grads, dwant):
+        assert ref.rel(got, w) <= 5 * u + 256 * E
+    n = torch.tensor([150], dtype=torch.int32).cuda()
+    got = o.window_attention_decode(q[:, 149].detach(), k.detach(), v.detach(), n, 90, 2, scale=scale)
+    assert ref.rel(got, ref.decode(q[:, 149].detach(), k.detach(), v.detach(), n, 90, 2, scale)) <= 3 * u + 64 * E
+
+
+@pytest.mark.gpu
+def test_a_wait_that_ran_out_is_reported_by_the_next_call():
+    """The word that a kernel sets when a wait of its runs out is set here from
+    the host: the next call fails once, with its text, and the one after runs."""
+    import ctypes
+    import os
+
+    from conftest import LIB
+
+    o = ops()
+    q = torch.randn(1, 200, 2, 64, device="cuda").bfloat16()
+    want = o.window_attention(q, q, q, 50)
+    lib = ctypes.CDLL(os.path.join(LIB, "libcail_ops.so"))
+    lib.cail_ops_device_error_word.restype = ctypes.POINTER(ctypes.c_int)
+    word = lib.cail_ops_device_error_word(torch.cuda.current_device())
+    assert word and word[0] == 0
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        o.window_attention(q, q, q, 50)
+    assert word[0] == 0 and torch.equal(o.window_attention(q, q, q, 50), want)
+    assert not lib.cail_ops_device_error_word(-1)
 
 
 @pytest.mark.gpu
