@@ -69,6 +69,8 @@ typedef struct {
     cail_ops_bthd q, k, v, o;
     float *lse;             /* CAIL_OPS_LSE_FLOATS(B, H, T) values, 16-byte aligned, kept by forward for
                                backward (B * H rows, T rounded up to 4 apart); NULL: not kept */
+    cail_ops_bthd o_rest;   /* 16-bit types: what rounding took from o, in the same type, kept by forward and read by
+                               backward (for do.o, which the rounded o alone gives too coarsely); ptr NULL: not kept */
     /* backward only */
     cail_ops_bthd dout, dq, dk, dv;
     float *delta;           /* scratch of the same size and alignment */

@@ -11,9 +11,10 @@ struct AttnArgs {
     float scale, scale_log2;  // scale, scale * log2(e)
     const int32_t *lengths;
     const char *q, *k, *v, *dout;
-    char *o, *dq, *dk, *dv;
+    char *o, *rest, *dq, *dk, *dv;
     // strides in bytes
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
+    int64_t rb, rt, rh;  // rest
     int64_t gb, gt, gh;  // dout
     int64_t dqb, dqt, dqh, dkb, dkt, dkh, dvb, dvt, dvh;
     float *lse, *delta;  // [B, H] rows of `lse_row` values; lse in log2 units of the scaled scores
@@ -24,6 +25,19 @@ struct AttnArgs {
 // fills everything but D-dependent launch choices; 0 or an error code
 int attn_check(const cail_ops_attention_args *a, bool backward, const char *who);
 AttnArgs attn_args(const cail_ops_attention_args *a, bool backward);
+
+// The sinks' key tiles are seen by all queries; in backward their queries are
+// cut into parts where they would be the last blocks running, and the parts'
+// sums joined in order.
+struct SinkParts {
+    int splits, tiles;  // parts of a key tile, key tiles with sinks (1 and 0: none is cut)
+    float *sums;        // [B, Hkv, tiles, splits, 2, rows of a tile, DP]: partial dk and dv
+};
+// for blocks of `rows` keys that go over tiles of `stream` queries, `slots` of them at a time
+SinkParts sink_parts(const cail_ops_attention_args *a, int rows, int stream, int64_t slots);
+inline size_t sink_bytes(const cail_ops_attention_args *a, const SinkParts &p, int rows, int dp) {
+    return p.splits > 1 ? (size_t)a->B * a->Hkv * p.tiles * p.splits * 2 * rows * dp * sizeof(float) : 0;
+}
 
 // The tensor-core kernels' grids: heads, sequences, then tiles of 128 rows, so
 // that blocks start in the tiles' order and find their place without a division.
@@ -39,9 +53,37 @@ int tc_backward(const cail_ops_attention_args *a, cudaStream_t st);
 size_t tc_workspace(const cail_ops_attention_args *a);
 
 #ifdef __CUDACC__
+// dk and dv of the sinks' key tiles from their parts, in order
+template <typename T, int DP, int ROWS> __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, const SinkParts parts) {
+    const int hk = blockIdx.y, b = blockIdx.z;
+    const int64_t tile0 = ((int64_t)b * a.Hkv + hk) * parts.tiles;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < parts.tiles * 2 * ROWS * (DP / 4); i += gridDim.x * 256) {
+        const int d = (i % (DP / 4)) * 4, row = i / (DP / 4) % ROWS, which = i / (DP / 4) / ROWS % 2, tile = i / (DP / 4) / ROWS / 2;
+        const int j = tile * ROWS + row;
+        if (j >= a.T || d >= a.D) continue;
+        float s[4] = {};
+        for (int p = 0; p < parts.splits; ++p) {
+            const float4 x = *reinterpret_cast<const float4 *>(parts.sums + ((((tile0 + tile) * parts.splits + p) * 2 + which) * ROWS + row) * DP + d);
+            s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
+        }
+        T *out = reinterpret_cast<T *>(which ? a.dv + b * a.dvb + (int64_t)j * a.dvt + hk * a.dvh : a.dk + b * a.dkb + (int64_t)j * a.dkt + hk * a.dkh);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < a.D) out[d + e] = from_f<T>(s[e]);
+    }
+}
+template <typename T, int DP, int ROWS> int join(const AttnArgs &a, const SinkParts &parts, cudaStream_t st) {
+    const unsigned grid = ((unsigned)parts.tiles * 2 * ROWS * (DP / 4) + 255) / 256;
+    join_kernel<T, DP, ROWS><<<dim3(grid < 1024u ? grid : 1024u, a.Hkv, a.B), 256, 0, st>>>(a, parts);
+    return launched("window attention backward");
+}
+
 __device__ __forceinline__ bool seen(int i, int j, int n, int window, int sinks) {
     return i < n && j <= i && (i - j < window || j < sinks);
 }
+
+// what rounding to T takes from x
+template <typename T> __device__ __forceinline__ float rest_of(float x) { return x - to_f(from_f<T>(x)); }
 
 // A row that sees one key: its probability is 1 whatever the scores, so no
 // gradient reaches q and k through it.  (p (dp - delta) would leave the

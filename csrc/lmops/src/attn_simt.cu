@@ -228,7 +228,10 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = column<DP>(tx, c);
-            if (d < a.D) out[d] = from_f<T>(l[r] == 0.f ? 0.f : o.at(r, c) * inv);
+            const float f = l[r] == 0.f ? 0.f : o.at(r, c) * inv;
+            if (d >= a.D) continue;
+            out[d] = from_f<T>(f);
+            if (sizeof(T) == 2 && a.rest) reinterpret_cast<T *>(a.rest + b * a.rb + (int64_t)i * a.rt + h * a.rh)[d] = from_f<T>(rest_of<T>(f));
         }
         if (a.lse && tx == 0) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = l[r] == 0.f ? 0.f : m[r] + log2f(l[r]);
     }
@@ -248,10 +251,12 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
     const KeyTiles tiles(i0, i0 + TR, n, a.window, a.sinks, kTile);
     const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
 
-    // o passes through the second key tile's place
+    // o, and what rounding took from it, pass through the second key tile's place and the second value tile's
     load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
     load_tile<T, DP, TR, TR * 4>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec);
     load_tile<T, DP, TR, TR * 4>(sk2 + TILE, a.o + b * a.ob + h * a.oh, a.ot, i0, n, a.D, vec);
+    const bool rest = sizeof(T) == 2 && a.rest;
+    if (rest) load_tile<T, DP, TR, TR * 4>(sv2 + TILE, a.rest + b * a.rb + h * a.rh, a.rt, i0, n, a.D, vec);
     copies_issued();
     copies_done<0>();
     __syncthreads();
@@ -262,7 +267,10 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
         const int row = ty * 4 + r, i = i0 + row;
         float s = 0.f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) s = fmaf(sg[row * ld<DP>() + tx + 16 * c], sk2[TILE + row * ld<DP>() + tx + 16 * c], s);
+        for (int c = 0; c < NC; ++c) {
+            const int at = row * ld<DP>() + tx + 16 * c;
+            s = fmaf(sg[at], rest ? sk2[TILE + at] + sv2[TILE + at] : sk2[TILE + at], s);
+        }
         delta[r] = half_sum(s);
         const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + i;
         lse[r] = i < n ? a.lse[at] : 0.f;
@@ -311,7 +319,7 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
 
 // dk and dv of 64 keys, over the group's heads and the query rows that see them
 template <typename T, int DP, int TR>
-__global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
+__global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec, const SinkParts parts) {
     constexpr int NC = DP / 16;
     constexpr int TILE = kTile * ld<DP>();
     extern __shared__ float4 smem4[];
@@ -319,7 +327,11 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
           *sp = sg2 + 2 * TILE, *sd = sp + TR * kLdP;
     __shared__ float lse2[2][kTile], delta2[2][kTile];
     const int hk = blockIdx.y, b = blockIdx.z;
-    const int j0 = blockIdx.x * TR;
+    int tile = blockIdx.x, split = 0;
+    const bool parted = parts.splits > 1 && tile < parts.tiles * parts.splits;
+    if (parted) split = tile % parts.splits, tile /= parts.splits;
+    else if (parts.splits > 1) tile -= parts.tiles * (parts.splits - 1);
+    const int j0 = tile * TR;
     const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
     const int n = length_of(a, b);
     int begin, end;
@@ -328,7 +340,13 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
     load_tile<T, DP, TR, TR * 4>(sv, a.v + b * a.vb + hk * a.vh, a.vt, j0, n, a.D, vec);
     Out<DP> dk, dv;
     // the tiles that pass: the group's heads in turn, each over the rows that see these keys
-    const int t0 = begin / kTile, per = end > begin ? (end - 1) / kTile + 1 - t0 : 0, count = a.group * per;
+    const int t0 = begin / kTile, per = end > begin ? (end - 1) / kTile + 1 - t0 : 0;
+    int first = 0, count = a.group * per;
+    if (parted) {  // this part of them
+        const int share = (count + parts.splits - 1) / parts.splits;
+        first = min(count, split * share);
+        count = min(count, first + share);
+    }
     auto fetch = [&](int x) {
         const int h = hk * a.group + x / per, i0 = (t0 + x % per) * kTile, at = x & 1;
         load_tile<T, DP, kTile, TR * 4>(sq2 + at * TILE, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
@@ -340,8 +358,8 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
         }
         copies_issued();
     };
-    if (count) fetch(0);
-    for (int x = 0; x < count; ++x) {
+    if (first < count) fetch(first);
+    for (int x = first; x < count; ++x) {
         const int i0 = (t0 + x % per) * kTile;
         const float *sq = sq2 + (x & 1) * TILE, *sg = sg2 + (x & 1) * TILE, *row_lse = lse2[x & 1], *row_delta = delta2[x & 1];
         if (x + 1 < count) fetch(x + 1), copies_done<1>();
@@ -364,6 +382,17 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec) {
         out_tile<DP>(sp, sg, dv, ty, tx);
         out_tile<DP>(sd, sq, dk, ty, tx);
         __syncthreads();
+    }
+    if (parted) {
+        float *sums = parts.sums + ((((int64_t)b * a.Hkv + hk) * parts.tiles + tile) * parts.splits + split) * (2 * TR * DP);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int at = (ty * 4 + r) * DP + column<DP>(tx, c);
+                sums[at] = dk.at(r, c) * a.scale, sums[TR * DP + at] = dv.at(r, c);
+            }
+        return;
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -397,7 +426,7 @@ template <typename T, int DP, int TR> int forward(const AttnArgs &a, bool vec, c
     simt_forward<T, DP, TR><<<dim3((a.T + TR - 1) / TR, a.H, a.B), TR * 4, smem, st>>>(a, vec);
     return launched("window attention");
 }
-template <typename T, int DP, int TR> int backward(const AttnArgs &a, bool vec, cudaStream_t st) {
+template <typename T, int DP, int TR> int backward(const AttnArgs &a, const SinkParts &parts, bool vec, cudaStream_t st) {
     const unsigned tiles = (a.T + TR - 1) / TR;
     size_t smem = (2 * TR * ld<DP>() + 4 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
     if (int rc = prepare(simt_dq<T, DP, TR>, smem)) return rc;
@@ -405,22 +434,57 @@ template <typename T, int DP, int TR> int backward(const AttnArgs &a, bool vec, 
     if (int rc = launched("window attention backward")) return rc;
     smem += TR * kLdP * sizeof(float);
     if (int rc = prepare(simt_dkv<T, DP, TR>, smem)) return rc;
-    simt_dkv<T, DP, TR><<<dim3(tiles, a.Hkv, a.B), TR * 4, smem, st>>>(a, vec);
-    return launched("window attention backward");
+    simt_dkv<T, DP, TR><<<dim3(tiles + parts.tiles * (parts.splits - 1), a.Hkv, a.B), TR * 4, smem, st>>>(a, vec, parts);
+    if (int rc = launched("window attention backward")) return rc;
+    return parts.splits > 1 ? join<T, DP, TR>(a, parts, st) : CAIL_OPS_OK;
 }
-template <typename T, int DP> int sized(const AttnArgs &a, bool vec, bool back, cudaStream_t st) {
-    const bool few = ((int64_t)a.T + 63) / 64 * (back ? a.Hkv : a.H) * a.B < 4 * (int64_t)sm_count();
-    if (few || DP == 128) return back ? backward<T, DP, 32>(a, vec, st) : forward<T, DP, 32>(a, vec, st);
-    if constexpr (DP < 128) return back ? backward<T, DP, 64>(a, vec, st) : forward<T, DP, 64>(a, vec, st);
+// rows of a block, and the sinks' parts in backward
+bool few_blocks(const cail_ops_attention_args *a, bool back) {
+    return ((int64_t)a->T + 63) / 64 * (back ? a->Hkv : a->H) * a->B < 4 * (int64_t)sm_count();
+}
+int rows_of(const cail_ops_attention_args *a, bool back) { return few_blocks(a, back) || a->D > 64 ? 32 : 64; }
+SinkParts parts_of(const cail_ops_attention_args *a) { return sink_parts(a, rows_of(a, true), kTile, 2 * (int64_t)sm_count()); }
+int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+template <typename T, int DP> int sized(const AttnArgs &a, const SinkParts &parts, int rows, bool vec, bool back, cudaStream_t st) {
+    if (rows == 32) return back ? backward<T, DP, 32>(a, parts, vec, st) : forward<T, DP, 32>(a, vec, st);
+    if constexpr (DP < 128) return back ? backward<T, DP, 64>(a, parts, vec, st) : forward<T, DP, 64>(a, vec, st);
     return CAIL_OPS_EINVAL;
 }
-template <typename T> int run(const AttnArgs &a, bool vec, bool back, cudaStream_t st) {
-    if (a.D <= 32) return sized<T, 32>(a, vec, back, st);
-    if (a.D <= 64) return sized<T, 64>(a, vec, back, st);
-    return sized<T, 128>(a, vec, back, st);
+template <typename T> int run(const cail_ops_attention_args *c, bool vec, bool back, cudaStream_t st) {
+    const AttnArgs a = attn_args(c, back);
+    const int rows = rows_of(c, back);
+    SinkParts parts = {1, 0, nullptr};
+    if (back) {
+        parts = parts_of(c);
+        const size_t bytes = sink_bytes(c, parts, rows, padded(a.D));
+        if (c->workspace_bytes < bytes || (bytes && (!c->workspace || !aligned(c->workspace, 16))))
+            return fail(CAIL_OPS_EINVAL, "window attention backward: a workspace of %zu bytes is needed", bytes);
+        parts.sums = static_cast<float *>(c->workspace);
+    }
+    if (a.D <= 32) return sized<T, 32>(a, parts, rows, vec, back, st);
+    if (a.D <= 64) return sized<T, 64>(a, parts, rows, vec, back, st);
+    return sized<T, 128>(a, parts, rows, vec, back, st);
 }
 
 }  // namespace
+
+// so many parts that none is longer than a key tile without sinks or than a
+// block's share of all tiles, whichever is more; no more tiles in all than a grid has
+SinkParts sink_parts(const cail_ops_attention_args *c, int rows, int stream, int64_t slots) {
+    SinkParts none = {1, 0, nullptr};
+    if (c->sinks == 0 || c->window >= c->T) return none;
+    const int64_t group = c->H / c->Hkv, tiles = ((int64_t)c->T + rows - 1) / rows, q_tiles = ((int64_t)c->T + stream - 1) / stream;
+    const int64_t sink_tiles = ((int64_t)(c->sinks < c->T ? c->sinks : c->T) + rows - 1) / rows;
+    const int64_t plain = group * (((int64_t)c->window + rows) / stream + 1), sunk = group * q_tiles;
+    if (sunk <= plain) return none;
+    const int64_t all = (int64_t)c->B * c->Hkv * ((tiles - sink_tiles) * plain + sink_tiles * sunk);
+    const int64_t share = all / slots > plain ? all / slots : plain;
+    int64_t splits = (sunk + share - 1) / share;
+    if (splits > 32) splits = 32;
+    if (tiles < kMostTiles && splits > 1 + (kMostTiles - tiles) / sink_tiles) splits = 1 + (kMostTiles - tiles) / sink_tiles;
+    if (splits <= 1) return none;
+    return {(int)splits, (int)sink_tiles, nullptr};
+}
 
 int attn_check(const cail_ops_attention_args *a, bool backward, const char *who) {
     if (a->type < CAIL_OPS_F32 || a->type > CAIL_OPS_F16) return fail(CAIL_OPS_EINVAL, "%s: unknown element type %d", who, a->type);
@@ -444,6 +508,7 @@ AttnArgs attn_args(const cail_ops_attention_args *a, bool backward) {
     x.k = static_cast<const char *>(a->k.ptr), x.kb = a->k.sb * s, x.kt = a->k.st * s, x.kh = a->k.sh * s;
     x.v = static_cast<const char *>(a->v.ptr), x.vb = a->v.sb * s, x.vt = a->v.st * s, x.vh = a->v.sh * s;
     x.o = static_cast<char *>(a->o.ptr), x.ob = a->o.sb * s, x.ot = a->o.st * s, x.oh = a->o.sh * s;
+    if (a->type != CAIL_OPS_F32) x.rest = static_cast<char *>(a->o_rest.ptr), x.rb = a->o_rest.sb * s, x.rt = a->o_rest.st * s, x.rh = a->o_rest.sh * s;
     x.lse = a->lse, x.lse_row = (a->T + 3) / 4 * 4;
     if (backward) {
         x.dout = static_cast<const char *>(a->dout.ptr), x.gb = a->dout.sb * s, x.gt = a->dout.st * s, x.gh = a->dout.sh * s;
@@ -463,7 +528,7 @@ static bool attn_vectors(const cail_ops_attention_args *a, bool backward) {
     const size_t s = type_size(a->type);
     return a->D % (16 / s) == 0 && rows_aligned(a->q, a->B, a->T, a->H, s, 16) && rows_aligned(a->k, a->B, a->T, a->Hkv, s, 16) &&
            rows_aligned(a->v, a->B, a->T, a->Hkv, s, 16) &&
-           (!backward || (rows_aligned(a->o, a->B, a->T, a->H, s, 16) && rows_aligned(a->dout, a->B, a->T, a->H, s, 16)));
+           (!backward || ((!a->o_rest.ptr || rows_aligned(a->o_rest, a->B, a->T, a->H, s, 16)) && rows_aligned(a->o, a->B, a->T, a->H, s, 16) && rows_aligned(a->dout, a->B, a->T, a->H, s, 16)));
 }
 
 extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_ops_stream stream) {
@@ -471,16 +536,15 @@ extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_
     if (a->B == 0 || a->T == 0) return CAIL_OPS_OK;
     auto st = static_cast<cudaStream_t>(stream);
     if (tc_takes(a)) return tc_forward(a, st);
-    const AttnArgs x = attn_args(a, false);
     const bool vec = attn_vectors(a, false);
-    if (a->type == CAIL_OPS_F32) return run<float>(x, vec, false, st);
-    if (a->type == CAIL_OPS_BF16) return run<__nv_bfloat16>(x, vec, false, st);
-    return run<__half>(x, vec, false, st);
+    if (a->type == CAIL_OPS_F32) return run<float>(a, vec, false, st);
+    if (a->type == CAIL_OPS_BF16) return run<__nv_bfloat16>(a, vec, false, st);
+    return run<__half>(a, vec, false, st);
 }
 
 extern "C" size_t cail_ops_window_attention_workspace(const cail_ops_attention_args *a) {
     if (attn_check(a, true, "window attention backward") || a->B == 0 || a->T == 0) return 0;
-    return tc_takes_backward(a) ? tc_workspace(a) : 0;
+    return tc_takes_backward(a) ? tc_workspace(a) : sink_bytes(a, parts_of(a), rows_of(a, true), padded(a->D));
 }
 
 extern "C" int cail_ops_window_attention_backward(const cail_ops_attention_args *a, cail_ops_stream stream) {
@@ -488,9 +552,8 @@ extern "C" int cail_ops_window_attention_backward(const cail_ops_attention_args 
     if (a->B == 0 || a->T == 0) return CAIL_OPS_OK;
     auto st = static_cast<cudaStream_t>(stream);
     if (tc_takes_backward(a)) return tc_backward(a, st);
-    const AttnArgs x = attn_args(a, true);
     const bool vec = attn_vectors(a, true);
-    if (a->type == CAIL_OPS_F32) return run<float>(x, vec, true, st);
-    if (a->type == CAIL_OPS_BF16) return run<__nv_bfloat16>(x, vec, true, st);
-    return run<__half>(x, vec, true, st);
+    if (a->type == CAIL_OPS_F32) return run<float>(a, vec, true, st);
+    if (a->type == CAIL_OPS_BF16) return run<__nv_bfloat16>(a, vec, true, st);
+    return run<__half>(a, vec, true, st);
 }

@@ -38,7 +38,7 @@ template <int DP, bool DKV> struct Shape {
     static constexpr int chunk = DKV && DP == 64 ? 16 : 32;  // columns at a time, by the registers that two blocks leave
     static constexpr int x_bytes = kRows * DP * 2, u_bytes = kStream * DP * 2;
     static constexpr int vec_bytes = DKV ? 2 * kStream * 4 : 0;  // lse and delta of a tile's queries
-    static constexpr int barriers = 1 + 2 * stages + 2 * buffers + 3;
+    static constexpr int barriers = 1 + 2 * stages + 2 * buffers + 4;
     static constexpr int o_bytes = DKV ? 0 : x_bytes;  // the output's rows, for delta
     static constexpr int smem = 1024 + 2 * x_bytes + stages * (2 * u_bytes + vec_bytes) + o_bytes;
     static constexpr int acc = buffers * 2 * kStream;  // column of acc0; acc1 follows
@@ -50,13 +50,12 @@ template <int DP, bool DKV> struct Shape {
 };
 
 struct Maps {
-    CUtensorMap x, y, u, w, o;
+    CUtensorMap x, y, u, w, o, rest;
 };
 
 struct Extra {
     unsigned *amax;       // [B, Hkv] bits of max |do| (fp16)
-    float *parts;         // [B, Hkv, sink tiles, splits, 2, 128, DP] partial dk and dv
-    int splits, sink_tiles;
+    SinkParts parts;
 };
 
 // the power of two that brings a value whose largest is `bits` to [1/4, 1/2)
@@ -75,9 +74,13 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     __shared__ __align__(8) uint64_t bars[S::barriers];
     __shared__ uint32_t tmem_at;
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + ST * S::u_bytes, svec = sw + ST * S::u_bytes, so = svec;
+    const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + S::u_bytes;  // U and W of a stage side by side
+    constexpr uint32_t stage_bytes = 2 * S::u_bytes;
+    const uint32_t svec = su + ST * stage_bytes, so = svec;
+    const uint32_t srest = su + (ST - 1) * stage_bytes;  // dq: what rounding took from the output, in the last stage until its first tile
+    static_assert(DKV || stage_bytes == S::x_bytes);
     const uint32_t bar0 = smem_u32(bars);
-    const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB, s_read = last + 8, acc_done = s_read + 8;
+    const uint32_t x_full = bar0, full = bar0 + 8, free_ = full + 8 * ST, s_full = free_ + 8 * ST, ds_full = s_full + 8 * NB, last = ds_full + 8 * NB, s_read = last + 8, acc_done = s_read + 8, rest_read = acc_done + 8;
 
     const int tid = threadIdx.x, warp = warp_number(), lane = tid & 31;
     const int b = blockIdx.y, n = length_of(a, b);
@@ -88,9 +91,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     if constexpr (DKV) {
         hk = blockIdx.x, h = hk * a.group;
         int tile = blockIdx.z;
-        parted = ex.splits > 1 && tile < ex.sink_tiles * ex.splits;
-        if (parted) split = tile % ex.splits, tile /= ex.splits;
-        else if (ex.splits > 1) tile -= ex.sink_tiles * (ex.splits - 1);
+        parted = ex.parts.splits > 1 && tile < ex.parts.tiles * ex.parts.splits;
+        if (parted) split = tile % ex.parts.splits, tile /= ex.parts.splits;
+        else if (ex.parts.splits > 1) tile -= ex.parts.tiles * (ex.parts.splits - 1);
         r0 = tile * kRows;
         int begin, end;
         query_range(r0, r0 + kRows, n, a.window, a.sinks, begin, end);
@@ -98,7 +101,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         q_tiles = end > begin ? (end - 1) / kStream + 1 - q_begin : 0;
         count = a.group * q_tiles;
         if (parted) {  // this part of the tiles
-            const int per = (count + ex.splits - 1) / ex.splits;
+            const int per = (count + ex.parts.splits - 1) / ex.parts.splits;
             first = min(count, split * per);
             count = min(count, first + per) - first;
         }
@@ -134,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     if (count == 0) {  // nothing sees or is seen: zeros
         constexpr int C = DP / 8;
         if (DKV && parted) {
-            float4 *p = reinterpret_cast<float4 *>(ex.parts) +
-                        ((((int64_t)b * a.Hkv + hk) * ex.sink_tiles + r0 / kRows) * ex.splits + split) * (2 * kRows * DP / 4);
+            float4 *p = reinterpret_cast<float4 *>(ex.parts.sums) +
+                        ((((int64_t)b * a.Hkv + hk) * ex.parts.tiles + r0 / kRows) * ex.parts.splits + split) * (2 * kRows * DP / 4);
             for (int i = tid; i < 2 * kRows * DP / 4; i += kThreads) p[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             return;
         }
@@ -157,8 +160,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         const uint32_t bar = full + 8 * s;
         mbar_expect(bar, 2 * S::u_bytes + S::vec_bytes);
         for (int p = 0; p < S::panels; ++p) {
-            tma_load(su + s * S::u_bytes + p * kStream * 128, &maps.u, bar, p * 64, t0, th, b);
-            tma_load(sw + s * S::u_bytes + p * kStream * 128, &maps.w, bar, p * 64, t0, th, b);
+            tma_load(su + s * stage_bytes + p * kStream * 128, &maps.u, bar, p * 64, t0, th, b);
+            tma_load(sw + s * stage_bytes + p * kStream * 128, &maps.w, bar, p * 64, t0, th, b);
         }
         if constexpr (DKV) {
             // 64 values each, which may reach into the next row or the padding behind the last one: those are masked
@@ -172,17 +175,18 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         mbar_init(x_full, 1);
         for (int s = 0; s < ST; ++s) mbar_init(full + 8 * s, 1), mbar_init(free_ + 8 * s, 1);
         for (int s = 0; s < NB; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(ds_full + 8 * s, kMath / 32);
-        mbar_init(last, 1), mbar_init(s_read, kMath / 32), mbar_init(acc_done, 1);
+        mbar_init(last, 1), mbar_init(s_read, kMath / 32), mbar_init(acc_done, 1), mbar_init(rest_read, kMath / 32);
         fence_barrier_init();
         // what needs no free slot is on its way before the block has met
-        mbar_expect(x_full, 2 * S::x_bytes + S::o_bytes);
+        mbar_expect(x_full, 2 * S::x_bytes + S::o_bytes + (!DKV && a.rest ? S::x_bytes : 0));
         for (int p = 0; p < S::panels; ++p) tma_load(sx + p * kRows * 128, &maps.x, x_full, p * 64, r0, DKV ? hk : h, b);
         load(walk);
         for (int p = 0; p < S::panels; ++p) {
             tma_load(sy + p * kRows * 128, &maps.y, x_full, p * 64, r0, DKV ? hk : h, b);
             if (!DKV) tma_load(so + p * kRows * 128, &maps.o, x_full, p * 64, r0, h, b);
+            if (!DKV && a.rest) tma_load(srest + p * kRows * 128, &maps.rest, x_full, p * 64, r0, h, b);
         }
-        for (step(walk); walk.x < ST && walk.x < count; step(walk)) load(walk);
+        for (step(walk); walk.x < (DKV ? ST : ST - 1) && walk.x < count; step(walk)) load(walk);
     }
     if (warp == 9) tmem_alloc<S::columns>(smem_u32(&tmem_at));
     __syncwarp();
@@ -195,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     if (warp == 8) {
         if (lane == 0) {  // the loads that wait for a slot
             for (; walk.x < count; step(walk)) {
-                ok = mbar_wait(free_ + 8 * (walk.x % ST), ((walk.x / ST) & 1) ^ 1);
+                if (walk.x < ST) ok = mbar_wait(rest_read, 0);  // dq: the last stage's first tile
+                else ok = mbar_wait(free_ + 8 * (walk.x % ST), ((walk.x / ST) & 1) ^ 1);
                 if (!ok) break;
                 load(walk);
             }
@@ -219,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             if (first && !warp_wait(full + 8 * s, (x / ST) & 1)) return false;
             tc_after();
             const uint32_t d = tm + (x % NB) * 2 * kStream;
-            const uint64_t dus = moved(du, s * S::u_bytes), dws = moved(dw, s * S::u_bytes);
+            const uint64_t dus = moved(du, s * stage_bytes), dws = moved(dw, s * stage_bytes);
             if (leader && first) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
@@ -255,11 +260,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 if constexpr (DKV) {
 #pragma unroll
                     for (int kk = 0; kk < kStream / 16; ++kk)
-                        mma_ts(tm + S::acc + DP, d + kStream + kk * 16, moved(dwt, s * S::u_bytes + kk * 2048), kind_acc, x > 0 || kk > 0);
+                        mma_ts(tm + S::acc + DP, d + kStream + kk * 16, moved(dwt, s * stage_bytes + kk * 2048), kind_acc, x > 0 || kk > 0);
                 }
 #pragma unroll
                 for (int kk = 0; kk < kStream / 16; ++kk)
-                    mma_ts(tm + S::acc, S::early_dp ? tm + S::ds + kk * 8 : d + kStream + kk * 16 + 8, moved(dut, s * S::u_bytes + kk * 2048), kind_acc,
+                    mma_ts(tm + S::acc, S::early_dp ? tm + S::ds + kk * 8 : d + kStream + kk * 16 + 8, moved(dut, s * stage_bytes + kk * 2048), kind_acc,
                            x > 0 || kk > 0);
                 mma_commit(free_ + 8 * s);
                 if (S::early_dp) mma_commit(acc_done);
@@ -279,29 +284,36 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         if constexpr (!DKV) {
             const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + r;
             if (r < n) lse = a.lse[at];  // on its way while do and o arrive
-            ok = mbar_wait(x_full, 0);
+            ok = warp_wait(x_full, 0);
             if (ok) {
                 float top = 0.f;
                 if (r < n) {
 #pragma unroll
                     for (int c = 0; c < DP / 8; ++c) {
                         if (c * 8 >= a.D) break;
-                        Vec<T, 8> g, o;
+                        Vec<T, 8> g, o, rest;
                         const uint32_t at = (c / 8) * kRows * 128 + row * 128 + (((c % 8) ^ (row & 7)) * 16);
                         uint4 w;
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(sy + at));
                         *reinterpret_cast<uint4 *>(&g) = w;
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(so + at));
                         *reinterpret_cast<uint4 *>(&o) = w;
+                        if (a.rest)
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(srest + at));
+                        else
+                            w = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(&rest) = w;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const float f = to_f(g.v[e]);
-                            delta = fmaf(to_f(o.v[e]), f, delta);
+                            delta = fmaf(to_f(o.v[e]) + to_f(rest.v[e]), f, delta);
                             if (!bf) top = fmaxf(top, fabsf(f));
                         }
                     }
                     if (half == 0) a.delta[at] = delta;
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(rest_read);
                 if (!bf) {
                     amp = amp_of(__float_as_uint(top));
                     top = warp_max(top);
@@ -337,7 +349,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 tc_ld32(at, us);
 #pragma unroll
                 for (int c1 = 0; c1 < 32; c1 += CH) {
-                    uint32_t ud[CH], pp[CH / 2], pd[CH / 2];
+                    uint32_t ud[CH], pd[CH / 2];
+                    [[maybe_unused]] uint32_t pp[CH / 2];
                     tc_ld<CH>(at + kStream + c1, ud);
                     if (c1 == 0) {
                         tc_wait_ld(us);
@@ -404,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 const int lo = n - t0;
                 for (int e = tid; e < (kStream - lo) * C; e += kMath) {
                     const int rr = lo + e / C, c = e % C;
-                    const uint32_t off = s * S::u_bytes + (c / 8) * kStream * 128 + rr * 128 + (c % 8) * 16;
+                    const uint32_t off = s * stage_bytes + (c / 8) * kStream * 128 + rr * 128 + (c % 8) * 16;
                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(su + off), "r"(0) : "memory");
                     if (DKV) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sw + off), "r"(0) : "memory");
                 }
@@ -427,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             const bool live = r < n;
             float *part = nullptr;
             if (DKV && parted)
-                part = ex.parts + (((((int64_t)b * a.Hkv + hk) * ex.sink_tiles + r0 / kRows) * ex.splits + split) * 2 + half) * (kRows * DP) + row * DP;
+                part = ex.parts.sums + (((((int64_t)b * a.Hkv + hk) * ex.parts.tiles + r0 / kRows) * ex.parts.splits + split) * 2 + half) * (kRows * DP) + row * DP;
 #pragma unroll 1
             for (int c = c_lo; c < c_hi; c += 32) {
                 uint32_t w[32];
@@ -478,55 +491,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     if (warp == 9) tmem_free<S::columns>(tm);
 }
 
-// dk and dv of the sinks' key tiles from their parts, in order
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, const Extra ex) {
-    const int hk = blockIdx.y, b = blockIdx.z;
-    const int64_t tile0 = ((int64_t)b * a.Hkv + hk) * ex.sink_tiles;
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < ex.sink_tiles * 2 * kRows * (DP / 8); i += gridDim.x * 256) {
-        const int d = (i % (DP / 8)) * 8, row = i / (DP / 8) % kRows, which = i / (DP / 8) / kRows % 2, tile = i / (DP / 8) / kRows / 2;
-        const int j = tile * kRows + row;
-        if (j >= a.T || d >= a.D) continue;
-        float s[8] = {};
-        for (int p = 0; p < ex.splits; ++p) {
-            const float4 *f = reinterpret_cast<const float4 *>(ex.parts + ((((tile0 + tile) * ex.splits + p) * 2 + which) * kRows + row) * DP + d);
-            const float4 x = f[0], y = f[1];
-            s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w, s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
-        }
-        char *out = which ? a.dv + b * a.dvb + (int64_t)j * a.dvt + hk * a.dvh : a.dk + b * a.dkb + (int64_t)j * a.dkt + hk * a.dkh;
-        *reinterpret_cast<uint4 *>(out + d * 2) = make_uint4(pack2(s[0], s[1], T()), pack2(s[2], s[3], T()), pack2(s[4], s[5], T()), pack2(s[6], s[7], T()));
-    }
-}
-
-// how many parts the sinks' key tiles are cut into: so that a part is no longer than a key tile without sinks or than an SM's
-// share of all tiles, whichever is more
-int splits_of(const cail_ops_attention_args *c, int sms) {
-    if (c->sinks == 0 || c->window >= c->T) return 1;
-    const int64_t group = c->H / c->Hkv, tiles = (c->T + kRows - 1) / kRows, q_tiles = (c->T + kStream - 1) / kStream;
-    int64_t sink_tiles = (std::min(c->sinks, c->T) + kRows - 1) / kRows;
-    const int64_t plain = group * ((c->window + kRows) / kStream + 1), sunk = group * q_tiles;
-    if (sunk <= plain) return 1;
-    const int64_t all = (int64_t)c->B * c->Hkv * ((tiles - sink_tiles) * plain + sink_tiles * sunk);
-    const int64_t slots = (int64_t)sms * (c->D <= 64 ? 2 : 1), share = std::max(plain, all / slots);
-    // and no more tiles in all than a grid has
-    return (int)std::min<int64_t>(std::min<int64_t>(32, (sunk + share - 1) / share), 1 + (kMostTiles - tiles) / sink_tiles);
-}
-
 struct Layout {
-    size_t amax, parts, total;
-    int splits, sink_tiles;
+    size_t amax, sums, total;
+    SinkParts parts;
 };
 Layout layout_of(const cail_ops_attention_args *c) {
     Layout l = {};
-    l.splits = splits_of(c, sm_count());
-    l.sink_tiles = l.splits > 1 ? (std::min(c->sinks, c->T) + kRows - 1) / kRows : 0;
-    size_t at = 0;
-    l.amax = at;
-    if (c->type == CAIL_OPS_F16) at += ((size_t)c->B * c->Hkv * 4 + 255) / 256 * 256;
-    l.parts = at;
-    const size_t dp = c->D <= 64 ? 64 : 128;
-    if (l.splits > 1) at += (size_t)c->B * c->Hkv * l.sink_tiles * l.splits * 2 * kRows * dp * 4;
-    l.total = at;
+    l.parts = sink_parts(c, kRows, kStream, (int64_t)sm_count() * (c->D <= 64 ? 2 : 1));
+    l.sums = c->type == CAIL_OPS_F16 ? ((size_t)c->B * c->Hkv * 4 + 255) / 256 * 256 : 0;
+    l.total = l.sums + sink_bytes(c, l.parts, kRows, c->D <= 64 ? 64 : 128);
     return l;
 }
 
@@ -536,8 +509,8 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
         return fail(CAIL_OPS_EINVAL, "window attention backward: a workspace of %zu bytes is needed", l.total);
     Extra ex = {};
     ex.amax = reinterpret_cast<unsigned *>(static_cast<char *>(c->workspace) + l.amax);
-    ex.parts = reinterpret_cast<float *>(static_cast<char *>(c->workspace) + l.parts);
-    ex.splits = l.splits, ex.sink_tiles = l.sink_tiles;
+    ex.parts = l.parts;
+    ex.parts.sums = reinterpret_cast<float *>(static_cast<char *>(c->workspace) + l.sums);
     if (c->type == CAIL_OPS_F16) {
         cudaError_t e = cudaMemsetAsync(ex.amax, 0, (size_t)a.B * a.Hkv * 4, st);
         if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
@@ -545,6 +518,8 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     // the same arrays with boxes of 128 and of 64 rows
     Maps q = {}, k = {};
     if (int rc = tensor_map(&q.o, c->o, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
+    if (a.rest)
+        if (int rc = tensor_map(&q.rest, c->o_rest, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.x, c->q, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.y, c->dout, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.u, c->k, c->type, a.B, a.T, a.Hkv, a.D, kStream)) return rc;
@@ -560,19 +535,17 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
     tc_backward_kernel<T, DP, false><<<dim3(a.H, a.B, tiles), kThreads, sm_q, st>>>(a, ex, q);
     if (int rc = launched("window attention backward")) return rc;
-    const unsigned blocks = tiles + ex.sink_tiles * (ex.splits - 1);  // at most kMostTiles: splits_of()
+    const unsigned blocks = tiles + ex.parts.tiles * (ex.parts.splits - 1);  // at most kMostTiles: sink_parts()
     tc_backward_kernel<T, DP, true><<<dim3(a.Hkv, a.B, blocks), kThreads, sm_k, st>>>(a, ex, k);
     if (int rc = launched("window attention backward")) return rc;
-    if (ex.splits == 1) return CAIL_OPS_OK;
-    const unsigned grid = ((unsigned)ex.sink_tiles * 2 * kRows * (DP / 8) + 255) / 256;
-    join_kernel<T, DP><<<dim3(std::min(grid, 1024u), a.Hkv, a.B), 256, 0, st>>>(a, ex);
-    return launched("window attention backward");
+    if (ex.parts.splits == 1) return CAIL_OPS_OK;
+    return join<T, DP, kRows>(a, ex.parts, st);
 }
 
 }  // namespace
 
 bool tc_takes_backward(const cail_ops_attention_args *a) {
-    return tc_takes(a) && tma_takes(a->dout, a->B, a->T, a->H) && tma_takes(a->o, a->B, a->T, a->H) && rows_aligned(a->dq, a->B, a->T, a->H, 2, 16) &&
+    return tc_takes(a) && tma_takes(a->dout, a->B, a->T, a->H) && tma_takes(a->o, a->B, a->T, a->H) && (!a->o_rest.ptr || tma_takes(a->o_rest, a->B, a->T, a->H)) && rows_aligned(a->dq, a->B, a->T, a->H, 2, 16) &&
            rows_aligned(a->dk, a->B, a->T, a->Hkv, 2, 16) && rows_aligned(a->dv, a->B, a->T, a->Hkv, 2, 16) && aligned(a->lse, 16) &&
            aligned(a->delta, 16);
 }

@@ -69,7 +69,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
         constexpr int C = DP / 8;
         for (int i = tid; i < kRows * C; i += kThreads) {
             const int r = i0 + i / C, d = (i % C) * 8;
-            if (r < a.T && d < a.D) *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh + d * 2) = make_uint4(0, 0, 0, 0);
+            if (r >= a.T || d >= a.D) continue;
+            *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh + d * 2) = make_uint4(0, 0, 0, 0);
+            if (a.rest) *reinterpret_cast<uint4 *>(a.rest + b * a.rb + (int64_t)r * a.rt + h * a.rh + d * 2) = make_uint4(0, 0, 0, 0);
         }
         if (a.lse && tid < kRows && i0 + tid < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i0 + tid] = 0.f;
         return;
@@ -272,8 +274,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
             tc_after();
             const bool live = i < n;
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            // rows go through shared memory (the queries' place) so that stores are whole rows
-            const uint32_t row = sq + tid * 128;
+            // rows go through shared memory (the queries' place, and the keys' for what rounding takes) so that stores are
+            // whole rows
+            const uint32_t row = sq + tid * 128, rest = sk + tid * 128;
+            static_assert(S::stages * S::kv_bytes >= S::q_bytes);
 #pragma unroll
             for (int c = 0; c < DP; c += 32) {
                 uint32_t w[32];
@@ -281,27 +285,34 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
                 tc_wait_ld(w);
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
+                    float f[8];
                     uint32_t y[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        y[k] = live && l != 0.f
-                                   ? pack2(__uint_as_float(w[e + 2 * k]) * inv, __uint_as_float(w[e + 2 * k + 1]) * inv, T())
-                                   : 0u;
-                    const int chunk = (c % 64 + e) / 8;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (c / 64) * kRows * 128 + ((chunk ^ (tid & 7)) * 16)),
-                                 "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
-                                 : "memory");
+                    for (int k = 0; k < 8; ++k) f[k] = live && l != 0.f ? __uint_as_float(w[e + k]) * inv : 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] = pack2(f[2 * k], f[2 * k + 1], T());
+                    const uint32_t to = (c / 64) * kRows * 128 + ((((c % 64 + e) / 8) ^ (tid & 7)) * 16);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+                    if (a.rest) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) y[k] = pack2(rest_of<T>(f[2 * k]), rest_of<T>(f[2 * k + 1]), T());
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rest + to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+                    }
                 }
             }
             __syncwarp();
             constexpr int C = DP / 8;
             for (int e = lane; e < 32 * C; e += 32) {
                 const int r = warp * 32 + e / C, c = e % C;
-                uint4 y;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
-                             : "r"(sq + (c / 8) * kRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16)));
-                if (i0 + r < a.T && c * 8 < a.D) *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)(i0 + r) * a.ot + h * a.oh + c * 16) = y;
+                const uint32_t from = (c / 8) * kRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16);
+                if (i0 + r >= a.T || c * 8 >= a.D) continue;
+                auto copy = [&](uint32_t src, char *dst) {
+                    uint4 y;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w) : "r"(src));
+                    *reinterpret_cast<uint4 *>(dst + c * 16) = y;
+                };
+                copy(sq + from, a.o + b * a.ob + (int64_t)(i0 + r) * a.ot + h * a.oh);
+                if (a.rest) copy(sk + from, a.rest + b * a.rb + (int64_t)(i0 + r) * a.rt + h * a.rh);
             }
             if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = live && l > 0.f ? fmaf(m, a.scale_log2, log2f(l)) : 0.f;
         } else if (lane == 0) {
@@ -329,11 +340,15 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, const
 }  // namespace
 
 // 16-bit elements in rows that TMA can load (16-byte multiples), a positive
-// scale (the row maximum is taken before scaling), no more tiles than a grid has
+// scale (the row maximum is taken before scaling), no more tiles than a grid
+// has; and more than 64 tokens: below, the other kernels are as fast and round
+// neither p nor ds.  (The same holds for short windows, where rounding ds costs
+// most, but not their speed: 8 x 1024 tokens, 16 heads of 64, window 8, forward
+// and backward, 117 us here and 1130 there.)
 bool tc_takes(const cail_ops_attention_args *a) {
-    if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f) || a->T > kMostTiles * kRows) return false;
+    if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f) || a->T > kMostTiles * kRows || a->T <= 64) return false;
     if (!tma_takes(a->q, a->B, a->T, a->H) || !tma_takes(a->k, a->B, a->T, a->Hkv) || !tma_takes(a->v, a->B, a->T, a->Hkv)) return false;
-    return rows_aligned(a->o, a->B, a->T, a->H, 2, 16);
+    return rows_aligned(a->o, a->B, a->T, a->H, 2, 16) && (!a->o_rest.ptr || rows_aligned(a->o_rest, a->B, a->T, a->H, 2, 16));
 }
 
 int tc_forward(const cail_ops_attention_args *c, cudaStream_t st) {
