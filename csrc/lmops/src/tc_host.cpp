@@ -40,9 +40,16 @@ int tensor_map(CUtensorMap *m, const cail_ops_bthd &x, int type, int B, int T, i
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
     const cuuint64_t strides[3] = {T == 1 ? 16 : (cuuint64_t)x.st * 2, H == 1 ? 16 : (cuuint64_t)x.sh * 2, B == 1 ? 16 : (cuuint64_t)x.sb * 2};
     const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, steps[4] = {1, 1, 1, 1};
-    const CUresult r = e(m, type == CAIL_OPS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, x.ptr, dims, strides, box,
-                         steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return e(m, type == CAIL_OPS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, x.ptr, dims, strides, box, steps,
+                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // the first CUDA call of this thread (a thread of autograd's, a user's): setting the device makes its context current
+        int device = 0;
+        if (cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) r = encode();
+    }
     if (r != CUDA_SUCCESS) return fail(CAIL_OPS_ECUDA, "window attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
     return CAIL_OPS_OK;
 }

@@ -21,6 +21,7 @@ the type (bf16 2^-8 ... as torch.finfo(t).eps / 2), e = 2^-24 that of float32.
   Gradient: one rounding u, and 64 e from exponents of up to 32.
 """
 import random
+import threading
 
 import pytest
 import torch
@@ -316,6 +317,37 @@ def test_window_attention_matches_64_bit(dtype, case):
                 assert not x[b, m:].any()
     again = torch.autograd.grad(o.window_attention(*leaves, window, sinks, lengths=n), leaves, do)
     assert all(torch.equal(x, y) for x, y in zip(grads, again))
+
+
+@pytest.mark.gpu
+def test_the_first_cuda_call_of_a_thread():
+    """A thread in which no context is current yet: the tile loads' descriptors need one."""
+    o = ops()
+    q, k, v, do, _ = attention_inputs((1, 200, 2, 2, 64, 50, 0, None), torch.bfloat16)
+    lengths = torch.tensor([150], dtype=torch.int32).cuda()
+    cache = randn(gen(5), 1, 2000, 2, 64, dtype=torch.bfloat16)
+
+    def forward():
+        with torch.no_grad():
+            return o.window_attention(q, k, v, 50, 0)
+
+    def both():
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        return torch.autograd.grad(o.window_attention(*leaves, 50, 0), leaves, do)[0]
+
+    for call in (forward, both, lambda: o.window_attention_decode(q[:, 0], cache, cache, lengths, 2000)):
+        want, got, errors = call(), [], []
+
+        def run():
+            try:
+                got.append(call())
+            except Exception as e:
+                errors.append(e)
+
+        thread = threading.Thread(target=run)
+        thread.start()
+        thread.join()
+        assert not errors and torch.equal(got[0], want)
 
 
 @pytest.mark.gpu
