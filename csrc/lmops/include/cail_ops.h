@@ -71,12 +71,22 @@ typedef struct {
                                backward (B * H rows, T rounded up to 4 apart); NULL: not kept */
     cail_ops_bthd o_rest;   /* 16-bit types: what rounding took from o, in the same type, kept by forward and read by
                                backward (for do.o, which the rounded o alone gives too coarsely); ptr NULL: not kept */
+    int rest_rows;          /* o_rest is [B, rest_rows, H, D], of the first rest_rows tokens: cail_ops_rest_rows() */
     /* backward only */
     cail_ops_bthd dout, dq, dk, dv;
     float *delta;           /* scratch of the same size and alignment */
     void *workspace;        /* cail_ops_window_attention_workspace() bytes, 16-byte aligned */
     size_t workspace_bytes;
 } cail_ops_attention_args;
+/* How many of a sequence's first rows keep what rounding to 16 bits takes from
+ * o, and have p rounded to twice the bits.  delta = do.o, on which the
+ * gradients of q and k rest, is off where p and o are rounded: for a row of k
+ * keys and heads of D that adds about 2 (1/k + 1/D) to the two squared
+ * roundings that its gradient has anyway (ds and the result). */
+static inline int cail_ops_rest_rows(int T, int D, int window, int sinks) {
+    const long long keys = (long long)window + sinks;
+    return T <= 128 || keys <= 128 || D < 64 ? T : 128;
+}
 int cail_ops_window_attention(const cail_ops_attention_args *a, cail_ops_stream stream);
 size_t cail_ops_window_attention_workspace(const cail_ops_attention_args *a);
 int cail_ops_window_attention_backward(const cail_ops_attention_args *a, cail_ops_stream stream);

@@ -15,6 +15,8 @@ struct AttnArgs {
     // strides in bytes
     int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
     int64_t rb, rt, rh;  // rest
+    int rest_rows;       // the first rows of a sequence, whose rest is kept
+    int fine_rows;       // and whose p is rounded to twice the bits
     int64_t gb, gt, gh;  // dout
     int64_t dqb, dqt, dqh, dkb, dkt, dkh, dvb, dvt, dvh;
     float *lse, *delta;  // [B, H] rows of `lse_row` values; lse in log2 units of the scaled scores

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
             const float f = l[r] == 0.f ? 0.f : o.at(r, c) * inv;
             if (d >= a.D) continue;
             out[d] = from_f<T>(f);
-            if (sizeof(T) == 2 && a.rest) reinterpret_cast<T *>(a.rest + b * a.rb + (int64_t)i * a.rt + h * a.rh)[d] = from_f<T>(rest_of<T>(f));
+            if (sizeof(T) == 2 && i < a.rest_rows) reinterpret_cast<T *>(a.rest + b * a.rb + (int64_t)i * a.rt + h * a.rh)[d] = from_f<T>(rest_of<T>(f));
         }
         if (a.lse && tx == 0) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = l[r] == 0.f ? 0.f : m[r] + log2f(l[r]);
     }
@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
     load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
     load_tile<T, DP, TR, TR * 4>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec);
     load_tile<T, DP, TR, TR * 4>(sk2 + TILE, a.o + b * a.ob + h * a.oh, a.ot, i0, n, a.D, vec);
-    const bool rest = sizeof(T) == 2 && a.rest;
-    if (rest) load_tile<T, DP, TR, TR * 4>(sv2 + TILE, a.rest + b * a.rb + h * a.rh, a.rt, i0, n, a.D, vec);
+    const bool rest = sizeof(T) == 2 && i0 < a.rest_rows;
+    if (rest) load_tile<T, DP, TR, TR * 4>(sv2 + TILE, a.rest + b * a.rb + h * a.rh, a.rt, i0, min(n, a.rest_rows), a.D, vec);
     copies_issued();
     copies_done<0>();
     __syncthreads();
@@ -493,6 +493,8 @@ int attn_check(const cail_ops_attention_args *a, bool backward, const char *who)
     if (a->B > 65535 || a->H > 65535) return fail(CAIL_OPS_EINVAL, "%s: at most 65535 sequences and heads", who);
     if (a->T > (1 << 30)) return fail(CAIL_OPS_EINVAL, "%s: at most 2^30 tokens", who);
     if (a->window < 1 || a->sinks < 0) return fail(CAIL_OPS_EINVAL, "%s: window %d and sinks %d", who, a->window, a->sinks);
+    if (a->o_rest.ptr && (a->rest_rows < 0 || a->rest_rows > a->T))
+        return fail(CAIL_OPS_EINVAL, "%s: the rest of %d rows of %d", who, a->rest_rows, a->T);
     if (backward && (!a->lse || !a->delta)) return fail(CAIL_OPS_EINVAL, "%s: lse and delta are needed", who);
     return CAIL_OPS_OK;
 }
@@ -508,7 +510,11 @@ AttnArgs attn_args(const cail_ops_attention_args *a, bool backward) {
     x.k = static_cast<const char *>(a->k.ptr), x.kb = a->k.sb * s, x.kt = a->k.st * s, x.kh = a->k.sh * s;
     x.v = static_cast<const char *>(a->v.ptr), x.vb = a->v.sb * s, x.vt = a->v.st * s, x.vh = a->v.sh * s;
     x.o = static_cast<char *>(a->o.ptr), x.ob = a->o.sb * s, x.ot = a->o.st * s, x.oh = a->o.sh * s;
-    if (a->type != CAIL_OPS_F32) x.rest = static_cast<char *>(a->o_rest.ptr), x.rb = a->o_rest.sb * s, x.rt = a->o_rest.st * s, x.rh = a->o_rest.sh * s;
+    x.fine_rows = cail_ops_rest_rows(a->T, a->D, a->window, a->sinks);
+    if (a->type != CAIL_OPS_F32 && a->o_rest.ptr) {
+        x.rest = static_cast<char *>(a->o_rest.ptr), x.rb = a->o_rest.sb * s, x.rt = a->o_rest.st * s, x.rh = a->o_rest.sh * s;
+        x.rest_rows = a->rest_rows;
+    }
     x.lse = a->lse, x.lse_row = (a->T + 3) / 4 * 4;
     if (backward) {
         x.dout = static_cast<const char *>(a->dout.ptr), x.gb = a->dout.sb * s, x.gt = a->dout.st * s, x.gh = a->dout.sh * s;
@@ -528,7 +534,7 @@ static bool attn_vectors(const cail_ops_attention_args *a, bool backward) {
     const size_t s = type_size(a->type);
     return a->D % (16 / s) == 0 && rows_aligned(a->q, a->B, a->T, a->H, s, 16) && rows_aligned(a->k, a->B, a->T, a->Hkv, s, 16) &&
            rows_aligned(a->v, a->B, a->T, a->Hkv, s, 16) &&
-           (!backward || ((!a->o_rest.ptr || rows_aligned(a->o_rest, a->B, a->T, a->H, s, 16)) && rows_aligned(a->o, a->B, a->T, a->H, s, 16) && rows_aligned(a->dout, a->B, a->T, a->H, s, 16)));
+           (!backward || ((!a->o_rest.ptr || rows_aligned(a->o_rest, a->B, a->rest_rows, a->H, s, 16)) && rows_aligned(a->o, a->B, a->T, a->H, s, 16) && rows_aligned(a->dout, a->B, a->T, a->H, s, 16)));
 }
 
 extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_ops_stream stream) {

@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         keys = KeyTiles(r0, r0 + kRows, n, a.window, a.sinks, kStream);
         count = keys.count;
     }
+    const bool rested = !DKV && r0 < a.rest_rows;  // what rounding took from these rows' output is there
     // a walk over the tiles: the first row of the tile at hand, and its query head (dk, dv)
     struct Walk {
         int x, row, head;
@@ -178,13 +179,13 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         mbar_init(last, 1), mbar_init(s_read, kMath / 32), mbar_init(acc_done, 1), mbar_init(rest_read, kMath / 32);
         fence_barrier_init();
         // what needs no free slot is on its way before the block has met
-        mbar_expect(x_full, 2 * S::x_bytes + S::o_bytes + (!DKV && a.rest ? S::x_bytes : 0));
+        mbar_expect(x_full, 2 * S::x_bytes + S::o_bytes + (rested ? S::x_bytes : 0));
         for (int p = 0; p < S::panels; ++p) tma_load(sx + p * kRows * 128, &maps.x, x_full, p * 64, r0, DKV ? hk : h, b);
         load(walk);
         for (int p = 0; p < S::panels; ++p) {
             tma_load(sy + p * kRows * 128, &maps.y, x_full, p * 64, r0, DKV ? hk : h, b);
             if (!DKV) tma_load(so + p * kRows * 128, &maps.o, x_full, p * 64, r0, h, b);
-            if (!DKV && a.rest) tma_load(srest + p * kRows * 128, &maps.rest, x_full, p * 64, r0, h, b);
+            if (rested) tma_load(srest + p * kRows * 128, &maps.rest, x_full, p * 64, r0, h, b);
         }
         for (step(walk); walk.x < (DKV ? ST : ST - 1) && walk.x < count; step(walk)) load(walk);
     }
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                         *reinterpret_cast<uint4 *>(&g) = w;
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(so + at));
                         *reinterpret_cast<uint4 *>(&o) = w;
-                        if (a.rest)
+                        if (rested)
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(srest + at));
                         else
                             w = make_uint4(0, 0, 0, 0);
@@ -518,8 +519,8 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     // the same arrays with boxes of 128 and of 64 rows
     Maps q = {}, k = {};
     if (int rc = tensor_map(&q.o, c->o, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
-    if (a.rest)
-        if (int rc = tensor_map(&q.rest, c->o_rest, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
+    if (a.rest_rows)
+        if (int rc = tensor_map(&q.rest, c->o_rest, c->type, a.B, a.rest_rows, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.x, c->q, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.y, c->dout, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
     if (int rc = tensor_map(&q.u, c->k, c->type, a.B, a.T, a.Hkv, a.D, kStream)) return rc;
@@ -545,7 +546,7 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
 }  // namespace
 
 bool tc_takes_backward(const cail_ops_attention_args *a) {
-    return tc_takes(a) && tma_takes(a->dout, a->B, a->T, a->H) && tma_takes(a->o, a->B, a->T, a->H) && (!a->o_rest.ptr || tma_takes(a->o_rest, a->B, a->T, a->H)) && rows_aligned(a->dq, a->B, a->T, a->H, 2, 16) &&
+    return tc_takes(a) && tma_takes(a->dout, a->B, a->T, a->H) && tma_takes(a->o, a->B, a->T, a->H) && (!a->o_rest.ptr || tma_takes(a->o_rest, a->B, a->rest_rows, a->H)) && rows_aligned(a->dq, a->B, a->T, a->H, 2, 16) &&
            rows_aligned(a->dk, a->B, a->T, a->Hkv, 2, 16) && rows_aligned(a->dv, a->B, a->T, a->Hkv, 2, 16) && aligned(a->lse, 16) &&
            aligned(a->delta, 16);
 }

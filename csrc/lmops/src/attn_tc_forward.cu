@@ -65,13 +65,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
     const int n = length_of(a, b);
     const KeyTiles tiles(i0, i0 + kRows, n, a.window, a.sinks, kKeys);
 
+    const bool fine = i0 < a.fine_rows;  // p in two parts
+
     if (tiles.count == 0) {  // rows behind the sequence: zeros
         constexpr int C = DP / 8;
         for (int i = tid; i < kRows * C; i += kThreads) {
             const int r = i0 + i / C, d = (i % C) * 8;
             if (r >= a.T || d >= a.D) continue;
             *reinterpret_cast<uint4 *>(a.o + b * a.ob + (int64_t)r * a.ot + h * a.oh + d * 2) = make_uint4(0, 0, 0, 0);
-            if (a.rest) *reinterpret_cast<uint4 *>(a.rest + b * a.rb + (int64_t)r * a.rt + h * a.rh + d * 2) = make_uint4(0, 0, 0, 0);
+            if (r < a.rest_rows) *reinterpret_cast<uint4 *>(a.rest + b * a.rb + (int64_t)r * a.rt + h * a.rh + d * 2) = make_uint4(0, 0, 0, 0);
         }
         if (a.lse && tid < kRows && i0 + tid < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i0 + tid] = 0.f;
         return;
@@ -163,6 +165,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
                     mma_ts(tm + S::o_col, tm + (x % NB) * kKeys + kk * 8, moved(dvs, kk * 2048), kind_o, x > 0 || kk > 0);
+                if (fine) {
+#pragma unroll
+                    for (int kk = 0; kk < kKeys / 16; ++kk)
+                        mma_ts(tm + S::o_col, tm + (x % NB) * kKeys + kKeys / 2 + kk * 8, moved(dvs, kk * 2048), kind_o, true);
+                }
                 mma_commit(v_free + 8 * s);
                 mma_commit(o_done);
             }
@@ -234,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
             uint64_t sum[4] = {};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const uint32_t *v = u[half];
+                uint32_t *v = u[half];
                 uint32_t p[16];
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
@@ -243,8 +250,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
                     p0 = exp2_fast(p0), p1 = exp2_fast(p1);
                     sum[(c / 2) % 4] = add_two(sum[(c / 2) % 4], two(p0, p1));
                     p[c / 2] = pack2(p0, p1, T());
+                    v[c] = __float_as_uint(p0), v[c + 1] = __float_as_uint(p1);
                 }
                 tc_st16(at + half * 16, p);  // over scores that have been read
+                if (fine) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2)
+                        p[c / 2] = pack2(rest_of<T>(__uint_as_float(v[c])), rest_of<T>(__uint_as_float(v[c + 1])), T());
+                    tc_st16(at + kKeys / 2 + half * 16, p);
+                }
             }
             float s0, s1;
             apart(add_two(add_two(sum[0], sum[1]), add_two(sum[2], sum[3])), s0, s1);
@@ -293,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
                     for (int k = 0; k < 4; ++k) y[k] = pack2(f[2 * k], f[2 * k + 1], T());
                     const uint32_t to = (c / 64) * kRows * 128 + ((((c % 64 + e) / 8) ^ (tid & 7)) * 16);
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
-                    if (a.rest) {
+                    if (i0 < a.rest_rows) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) y[k] = pack2(rest_of<T>(f[2 * k]), rest_of<T>(f[2 * k + 1]), T());
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rest + to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
@@ -312,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
                     *reinterpret_cast<uint4 *>(dst + c * 16) = y;
                 };
                 copy(sq + from, a.o + b * a.ob + (int64_t)(i0 + r) * a.ot + h * a.oh);
-                if (a.rest) copy(sk + from, a.rest + b * a.rb + (int64_t)(i0 + r) * a.rt + h * a.rh);
+                if (i0 + r < a.rest_rows) copy(sk + from, a.rest + b * a.rb + (int64_t)(i0 + r) * a.rt + h * a.rh);
             }
             if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = live && l > 0.f ? fmaf(m, a.scale_log2, log2f(l)) : 0.f;
         } else if (lane == 0) {
@@ -348,7 +362,7 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, const
 bool tc_takes(const cail_ops_attention_args *a) {
     if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f) || a->T > kMostTiles * kRows || a->T <= 64) return false;
     if (!tma_takes(a->q, a->B, a->T, a->H) || !tma_takes(a->k, a->B, a->T, a->Hkv) || !tma_takes(a->v, a->B, a->T, a->Hkv)) return false;
-    return rows_aligned(a->o, a->B, a->T, a->H, 2, 16) && (!a->o_rest.ptr || rows_aligned(a->o_rest, a->B, a->T, a->H, 2, 16));
+    return rows_aligned(a->o, a->B, a->T, a->H, 2, 16) && (!a->o_rest.ptr || rows_aligned(a->o_rest, a->B, a->rest_rows, a->H, 2, 16));
 }
 
 int tc_forward(const cail_ops_attention_args *c, cudaStream_t st) {

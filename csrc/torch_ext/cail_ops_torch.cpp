@@ -302,7 +302,7 @@ Tensor attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, cons
     c10::cuda::CUDAGuard guard(q.device());
     cail_ops_attention_args a = attention_args(q, k, v, o, w);
     a.lse = lse;
-    if (rest.defined()) a.o_rest = view(rest);
+    if (rest.defined()) a.o_rest = view(rest), a.rest_rows = (int)rest.size(1);
     done(L.attention(&a, stream_of(q)));
     return o;
 }
@@ -313,13 +313,8 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
         const Tensor lengths = or_none(lengths_);
         const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
         Tensor lse = at::empty({(int64_t)CAIL_OPS_LSE_FLOATS(q.size(0), q.size(2), q.size(1))}, q.options().dtype(at::kFloat));
-        // delta = do.o, on which the gradients of q and k rest, is off when o is rounded to 16 bits, the more the fewer keys
-        // rows see and the smaller a head is.  Keeping what rounding took mends that and costs a write and a read of o's
-        // size.  Relative errors of dq in bf16 without and with it, where rounding dq alone gives 0.0017: 4 keys 0.0029 and
-        // 0.0025; heads of 16, 1129 tokens, causal, 0.0026 and 0.0024; 1024 tokens, heads of 64, window 256, 0.0025 and
-        // 0.0024, there for 140 us instead of 133.
-        const bool coarse = std::min(std::min(window, kIntMax) + std::min(sinks, kIntMax), q.size(1)) <= 128 || q.size(1) < 1024 || q.size(3) < 64;
-        Tensor rest = q.scalar_type() == at::kFloat || !coarse ? Tensor() : at::empty(q.sizes(), q.options());
+        const int64_t kept = cail_ops_rest_rows((int)q.size(1), (int)q.size(3), clamped(window), clamped(sinks));
+        Tensor rest = q.scalar_type() == at::kFloat ? Tensor() : at::empty({q.size(0), kept, q.size(2), q.size(3)}, q.options());
         Tensor o = attention_forward(q, k, v, {lengths, window, sinks, scale}, lse.data_ptr<float>(), rest);
         ctx->save_for_backward({q, k, v, o, lse, lengths, rest});
         ctx->saved_data["window"] = window;
@@ -339,7 +334,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
                                                                    ctx->saved_data["scale"].toDouble()});
             a.dout = view(dout), a.dq = view(dq), a.dk = view(dk), a.dv = view(dv);
             a.lse = lse.data_ptr<float>();
-            if (s[6].defined()) a.o_rest = view(s[6]);
+            if (s[6].defined()) a.o_rest = view(s[6]), a.rest_rows = (int)s[6].size(1);
             Tensor delta = at::empty_like(lse);
             a.delta = delta.data_ptr<float>();
             a.workspace_bytes = L.workspace(&a);

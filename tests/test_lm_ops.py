@@ -320,6 +320,39 @@ def test_window_attention_matches_64_bit(dtype, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=ids_of)
+@pytest.mark.parametrize("window, sinks, D", [(2, 0, 64), (3, 1, 128), (5, 4, 72), (200, 0, 16)])
+def test_rows_of_few_keys_lose_one_rounding(dtype, window, sinks, D):
+    """Element by element: o is off by its own rounding, dq and dk by their own and that of ds.  With u half a step, p and o
+    reach delta = do.o to 2 u^2 and u^2 relative to their terms, so ds_ij to p_ij (A_ij + sum_j p_ij A_ij) 4 u^2 with
+    A_ij = sum_d |do_id v_jd| (4 covers both ends of ds' own rounding); 256 E stands for the 32-bit sums of at most 128 terms
+    and the exponentials; 16 E max|do| for ds that are tiny beside max|do|.  One more rounding of p or o in delta would be off
+    by u times the same terms, 2^6 and more over this."""
+    o = ops()
+    T, H = 300, 2
+    q, k, v, do, _ = attention_inputs((1, T, H, H, D, window, sinks, None), dtype)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    out = o.window_attention(*leaves, window, sinks)
+    got = torch.autograd.grad(out, leaves, do)
+    u, scale = ref.half_step(dtype), D ** -0.5
+    on = ref.seen_mask(T, T, window, sinks, q.device)
+    rows = 128 if window > 128 else T  # of few keys
+    for h in range(H):
+        qh, kh, vh, gh = (x[0, :, h].double() for x in (q, k, v, do))
+        p = torch.softmax(torch.where(on, scale * qh @ kh.T, -1e300), -1) * on
+        dp, A = gh @ vh.T, gh.abs() @ vh.abs().T
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+        off = p * (A + (p * A).sum(-1, keepdim=True)) * (4 * u * u + 256 * E) + on * 16 * E * float(gh.abs().max()) + u * ds.abs()
+        want = p @ vh
+        assert ((out[0, :, h].double() - want).abs() <= u * want.abs() + (2 * u * u + 256 * E) * (p @ vh.abs()))[:rows].all()
+        want = scale * ds @ kh
+        assert ((got[0][0, :, h].double() - want).abs() <= u * want.abs() + 1.01 * scale * off @ kh.abs())[:rows].all()
+        want = scale * ds.T @ qh
+        if rows == T:
+            assert ((got[1][0, :, h].double() - want).abs() <= u * want.abs() + 1.01 * scale * off.T @ qh.abs()).all()
+
+
+@pytest.mark.gpu
 def test_the_first_cuda_call_of_a_thread():
     """A thread in which no context is current yet: the tile loads' descriptors need one."""
     o = ops()
