@@ -105,9 +105,9 @@ class Block(nn.Module):
         if plan is not None:
             q, k = (z[:, 0] for z in ops.rotary(q[:, None], k[:, None], plan, at[:, None]))
         row = torch.arange(b, device=x.device)
-        k_cache[row, at] = k
-        v_cache[row, at] = v
-        a = ops.window_attention_decode(q, k_cache, v_cache, lengths, self.window or k_cache.size(1), self.sinks)
+        k_cache[row, at] = k.to(k_cache.dtype)
+        v_cache[row, at] = v.to(v_cache.dtype)
+        a = ops.window_attention_decode(q.to(k_cache.dtype), k_cache, v_cache, lengths, self.window or k_cache.size(1), self.sinks)
         return self._rest(x, a.reshape(b, d))
 
 
@@ -201,12 +201,14 @@ class GPT2(nn.Module):
     @torch.no_grad()
     def decode(self, idx: torch.Tensor, cache: KVCache) -> torch.Tensor:
         """Appends one token per sequence, idx [B], and gives the logits that
-        follow, [B, vocab]."""
+        follow, [B, vocab].  Captured into a CUDA graph, each replay appends a
+        token; the caller counts them: past the cache's length they overwrite
+        its last place."""
         if idx.shape != cache.lengths.shape:
             raise ValueError(f"one token for each of {cache.lengths.numel()} sequences, got {tuple(idx.shape)}")
         if cache.filled >= cache.length:
             raise ValueError(f"the cache is full ({cache.length} tokens)")
-        at = cache.lengths.long()
+        at = cache.lengths.clamp(max=cache.length - 1).long()
         x = self.wte(idx)
         if self.c.rotary == 0:
             x = x + self.wpe(at)

@@ -152,6 +152,48 @@ def test_prefill_and_decode_follow_forward(kw):
 
 
 @pytest.mark.gpu
+def test_decode_under_autocast():
+    """bf16 keys and values into a float32 cache: forward's logits, to bf16's roundings (10 of 2^-8 deep)."""
+    torch.manual_seed(8)
+    m = GPT2(config(rotary=16, window=50, sinks=2)).cuda()
+    idx = torch.randint(0, 512, (2, 40)).cuda()
+    cache = m.new_cache(2)
+    with torch.autocast("cuda", torch.bfloat16):
+        out = m.prefill(idx[:, :35], cache)
+        for t in range(35, 40):
+            out = m.decode(idx[:, t], cache)
+    with torch.no_grad():
+        assert ref.rel(out, m(idx)[:, 39]) <= 10 * 2.0 ** -8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [0, 16])
+def test_captured_decode(rotary):
+    """Replays append tokens as eager calls do; past the cache's length they stay inside it."""
+    torch.manual_seed(9)
+    m = GPT2(config(rotary=rotary, window=20, sinks=2)).cuda()
+    idx = torch.randint(0, 512, (2, 30)).cuda()
+    eager, cache = m.new_cache(2, 30), m.new_cache(2, 30)
+    m.prefill(idx[:, :10], eager)
+    m.prefill(idx[:, :10], cache)
+    static = idx[:, 10].clone()
+    m.decode(static, m.new_cache(2, 30))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.decode(static, cache)
+    for t in range(10, 30):
+        static.copy_(idx[:, t])
+        graph.replay()
+        want = m.decode(idx[:, t], eager)
+        assert torch.equal(out, want)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a[:, :29], b[:, :29]) for a, b in zip(cache.k, eager.k))
+
+
+@pytest.mark.gpu
 def test_bf16_model_runs_on_the_tensor_cores():
     """A bf16 model of heads of 64: step and decoding run, gradients are finite
     and near the float32 model's (10 roundings of 2^-8 deep)."""
