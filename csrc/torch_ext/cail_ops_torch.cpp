@@ -77,6 +77,8 @@ void load(const std::string &path) {
     get(L.launches, "cail_ops_launches");
 }
 
+constexpr int64_t kIntMax = std::numeric_limits<int>::max();
+
 void done(int rc) {
     if (rc == CAIL_OPS_OK) return;
     VALUE_CHECK(rc != CAIL_OPS_EINVAL, L.last_error());
@@ -97,6 +99,17 @@ void same_device(const char *who, const Tensor &first, std::initializer_list<con
     VALUE_CHECK(first.is_cuda(), who, ": needs CUDA tensors, not ", first.device());
     for (const Tensor *t : others)
         VALUE_CHECK(!t->defined() || t->device() == first.device(), who, ": tensors on ", first.device(), " and ", t->device());
+}
+
+// what a kernel that is handed a pointer would get wrong without a word: a
+// layout without strides, a negation still to be done, a forward-mode tangent
+void plain(const char *who, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts) {
+        if (!t->defined()) continue;
+        VALUE_CHECK(t->layout() == at::kStrided, who, ": needs strided tensors");
+        VALUE_CHECK(!t->is_neg(), who, ": a tensor whose negation is still to be done; call resolve_neg()");
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), cat(who, ": has no forward-mode derivative"));
+    }
 }
 
 cail_ops_stream stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -144,7 +157,10 @@ struct RotaryHow {
 };
 
 void rotary_check(const char *who, const Tensor &q, const Tensor &k, const RotaryHow &w) {
+    plain(who, {&q, &k, &w.positions});
     VALUE_CHECK(q.dim() == 4, who, ": q must be [B, T, H, D], got ", q.sizes());
+    for (int64_t i = 0; i < 3; ++i)
+        VALUE_CHECK(q.size(i) <= kIntMax && (!k.defined() || k.dim() != 4 || k.size(i) <= kIntMax), who, ": at most 2^31 - 1 sequences, tokens and heads");
     type_of(q, who, "q");
     VALUE_CHECK(w.part <= q.size(3), who, ": the plan rotates ", w.part, " elements of heads of ", q.size(3));
     VALUE_CHECK(q.size(3) <= 1024, who, ": heads of at most 1024 elements");
@@ -232,6 +248,7 @@ void rotary_inplace(const Tensor &q, const std::optional<Tensor> &k_, const Tens
         VALUE_CHECK(t.size(-1) == 1 || t.stride(-1) == 1, "rotary_: the elements of a head must lie side by side");
         VALUE_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, "rotary_: heads of one tensor share memory");
     };
+    plain("rotary_", {&q, &k});
     VALUE_CHECK(q.dim() == 4, "rotary_: q must be [B, T, H, D], got ", q.sizes());
     check(q);
     if (k.defined()) {
@@ -241,9 +258,10 @@ void rotary_inplace(const Tensor &q, const std::optional<Tensor> &k_, const Tens
         VALUE_CHECK(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial, "rotary_: q and k share memory");
     }
     rotary_check("rotary_", q, k, w);
-    if (q.numel() || (k.defined() && k.numel())) rotary_launch(q, k, q, k, w);
+    // first, as it refuses inference tensors outside inference mode
     q.unsafeGetTensorImpl()->bump_version();
     if (k.defined()) k.unsafeGetTensorImpl()->bump_version();
+    if (q.numel() || (k.defined() && k.numel())) rotary_launch(q, k, q, k, w);
 }
 
 // --------------------------------------------------------- window attention
@@ -254,11 +272,10 @@ struct AttnHow {
     double scale;
 };
 
-constexpr int64_t kIntMax = std::numeric_limits<int>::max();
-
 int32_t clamped(int64_t x) { return (int32_t)std::min(x, (int64_t)1 << 30); }
 
 void attention_check(const char *who, const Tensor &q, const Tensor &k, const Tensor &v, const AttnHow &w, bool decode) {
+    plain(who, {&q, &k, &v, &w.lengths});
     if (decode) {
         VALUE_CHECK(q.dim() == 3, who, ": q must be [B, H, D], got ", q.sizes());
     } else {
@@ -273,7 +290,7 @@ void attention_check(const char *who, const Tensor &q, const Tensor &k, const Te
     VALUE_CHECK(D >= 1 && D <= 128, who, ": heads of 1 to 128 elements, got ", D);
     VALUE_CHECK(w.window >= 1, who, ": window must be at least 1, got ", w.window);
     VALUE_CHECK(w.sinks >= 0, who, ": sinks must not be negative, got ", w.sinks);
-    VALUE_CHECK(std::isfinite(w.scale), who, ": scale must be finite");
+    VALUE_CHECK(std::isfinite((float)w.scale), who, ": scale must be finite");
     VALUE_CHECK(q.size(0) <= 65535 && H <= 65535, who, ": at most 65535 sequences and heads");
     VALUE_CHECK(k.size(1) <= (int64_t)1 << 30, who, ": at most 2^30 tokens");
     type_of(q, who, "q");
@@ -468,6 +485,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
 Tensor distill_loss(const Tensor &z_, const Tensor &ids_, const Tensor &t_, const std::optional<Tensor> &y_, double tau, double hard, int64_t mean) {
     const char *who = "distill_loss";
     Tensor y = or_none(y_);
+    plain(who, {&z_, &ids_, &t_, &y});
     VALUE_CHECK(z_.dim() == 2 && z_.size(1) > 0, who, ": logits must be [N, V], got ", z_.sizes());
     VALUE_CHECK(z_.size(1) <= kIntMax, who, ": at most 2^31 - 1 logits in a row");
     VALUE_CHECK(ids_.dim() == 2 && ids_.size(0) == z_.size(0) && t_.sizes() == ids_.sizes(), who,

@@ -143,6 +143,40 @@ def test_distill_loss_refuses():
         o.distill_loss(z, ids, t)
 
 
+def test_tensors_that_a_pointer_does_not_show_are_refused():
+    """A negation still to be done, a forward-mode tangent, a sparse layout, sizes past 32 bits."""
+    import torch.autograd.forward_ad as fwd
+    o = ops()
+    plan = o.Rotary(8, device="cpu")
+    q, z = torch.zeros(2, 5, 2, 8), torch.zeros(3, 11)
+    n = torch.zeros(2, dtype=torch.int32)
+    ids, t = torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2)
+
+    def calls(q, z):
+        return [lambda: o.rotary(q, None, plan), lambda: o.rotary_(q, None, plan), lambda: o.window_attention(q, q, q, 4),
+                lambda: o.window_attention_decode(q[:, 0], q, q, n, 4), lambda: o.distill_loss(z, ids, t)]
+
+    negated = [torch.zeros(x.shape, dtype=torch.complex64).conj().imag for x in (q, z)]
+    assert negated[0].is_neg()
+    for call in calls(*negated):
+        with pytest.raises(ValueError, match="negation"):
+            call()
+    for call in calls(q.to_sparse(), z.to_sparse()):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+    with fwd.dual_level():
+        for call in calls(*(fwd.make_dual(x, torch.ones_like(x)) for x in (q, z))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    for shape in ((1, 2 ** 32 + 5, 1, 8), (2 ** 32 + 1, 1, 1, 8), (1, 1, 2 ** 32 + 1, 8)):
+        with pytest.raises(ValueError, match="at most"):
+            o.rotary(torch.zeros(1).expand(shape), None, plan)
+        with pytest.raises(ValueError, match="at most"):
+            o.window_attention(*[torch.zeros(1).expand(shape)] * 3, 4)
+    with pytest.raises(ValueError, match="scale"):
+        o.window_attention(q, q, q, 4, scale=1e300)
+
+
 def test_c_entries_refuse_without_touching_a_device():
     """Bad sizes come back as CAIL_OPS_EINVAL with a text, before any CUDA call."""
     import ctypes
