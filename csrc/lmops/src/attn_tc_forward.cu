@@ -9,7 +9,10 @@
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown
 // by more than 2^8 since the scale in use, so p stays below 256 and most tiles
 // touch O in no other way than the product.  p is rounded to the input type
-// for that product (its sum is not); everything else is 32-bit.
+// for that product (its sum is not); everything else is 32-bit.  Rows of few
+// keys (cail_ops_rest_rows) take p in two parts, the second what rounding took
+// from the first, and so twice the second product, in loops of their own (one
+// loop with the choice inside took 3 % more): 0.4 us of 34 below.
 //
 // 64 keys per tile, two blocks per SM with two buffers of S each, so a product
 // runs under the softmax.  At D = 64 the exponentials bound it (16 a clock and
@@ -17,8 +20,12 @@
 // product from shared memory and 33 from tensor memory); at D = 128 the
 // products do (664 clocks).  Four blocks per SM with one buffer each, and a
 // quarter of the exponentials on the float pipes, both measured the same as
-// this (4 x 4096 tokens, 16 heads, causal: 206 us at D = 64, 274 at D = 128,
-// 670 and 1000 TFLOP/s); small calls took 8 us instead of 6.
+// this (4 x 4096 tokens, 16 heads, causal: 214 us at D = 64, 273 at D = 128,
+// 640 and 1000 TFLOP/s); small calls took 8 us instead of 6.
+//
+// Short windows are bound by neither: 8 x 1024 tokens, 16 heads of 64, window
+// 256 and 4 sinks, take 34 us (products 15 % of the tensor pipe, exponentials
+// 35 %), as a block has five tiles between its prologue and its epilogue.
 #include <type_traits>
 
 #include "attn.cuh"
@@ -155,27 +162,31 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
             return true;
         };
         ok = warp_wait(q_full, 0) && scores(0) && (tiles.count < 2 || scores(1));
-        for (int x = 0; x < tiles.count && ok; ++x) {
-            const int s = x % S::stages;
-            ok = warp_wait(p_full + 8 * (x % NB), (x / NB) & 1) && warp_wait(v_full + 8 * s, (x / S::stages) & 1);
-            if (!ok) break;
-            tc_after();
-            const uint64_t dvs = moved(dv, s * S::kv_bytes);
-            if (leader) {
-#pragma unroll
-                for (int kk = 0; kk < kKeys / 16; ++kk)
-                    mma_ts(tm + S::o_col, tm + (x % NB) * kKeys + kk * 8, moved(dvs, kk * 2048), kind_o, x > 0 || kk > 0);
-                if (fine) {
+        auto products = [&](auto two_parts) {
+            for (int x = 0; x < tiles.count && ok; ++x) {
+                const int s = x % S::stages;
+                ok = warp_wait(p_full + 8 * (x % NB), (x / NB) & 1) && warp_wait(v_full + 8 * s, (x / S::stages) & 1);
+                if (!ok) break;
+                tc_after();
+                const uint64_t dvs = moved(dv, s * S::kv_bytes);
+                if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        mma_ts(tm + S::o_col, tm + (x % NB) * kKeys + kKeys / 2 + kk * 8, moved(dvs, kk * 2048), kind_o, true);
+                        mma_ts(tm + S::o_col, tm + (x % NB) * kKeys + kk * 8, moved(dvs, kk * 2048), kind_o, x > 0 || kk > 0);
+                    if (two_parts.value) {
+#pragma unroll
+                        for (int kk = 0; kk < kKeys / 16; ++kk)
+                            mma_ts(tm + S::o_col, tm + (x % NB) * kKeys + kKeys / 2 + kk * 8, moved(dvs, kk * 2048), kind_o, true);
+                    }
+                    mma_commit(v_free + 8 * s);
+                    mma_commit(o_done);
                 }
-                mma_commit(v_free + 8 * s);
-                mma_commit(o_done);
+                __syncwarp();
+                if (x + NB < tiles.count) ok = scores(x + NB);
             }
-            __syncwarp();
-            if (x + NB < tiles.count) ok = scores(x + NB);
-        }
+        };
+        if (fine) products(std::true_type());
+        else products(std::false_type());
         if (leader) {
             mma_commit(o_last);
             if (!ok) report(a.error);
@@ -184,105 +195,112 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
         const int i = i0 + tid;
         const uint32_t mine = tm + ((uint32_t)(warp * 32) << 16);
         float m = -INFINITY, l = 0.f;  // m: the maximum in use, in scores
-        for (int x = 0; x < tiles.count; ++x) {
-            const int j0 = tiles.at(x) * kKeys;
-            ok = mbar_wait(s_full + 8 * (x % NB), (x / NB) & 1);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            tc_after();
-            const uint32_t at = mine + (x % NB) * kKeys;
-            // every row of the tile sees every key, unless the tile crosses the diagonal or the window's edge
-            const bool whole = j0 + kKeys - 1 <= i0 && (i0 + kRows - 1 - j0 < a.window || j0 + kKeys <= a.sinks);
-            uint32_t on[2] = {0xffffffffu, 0xffffffffu};
-            if (!whole) on[0] = keys_of_row(i, j0, a.window, a.sinks), on[1] = keys_of_row(i, j0 + 32, a.window, a.sinks);
-            auto mask = [&](uint32_t *u, int half) {
-                if (whole) return;
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                    if (!(on[half] & (1u << c))) u[c] = 0xff800000u;  // minus infinity
-            };
-            uint32_t u[2][32];
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            auto highest = [&](const uint32_t *v) {
-#pragma unroll
-                for (int c = 0; c < 32; ++c) tops[c % 4] = fmaxf(tops[c % 4], __uint_as_float(v[c]));
-            };
-            tc_ld32(at, u[0]);
-            tc_ld32(at + 32, u[1]);
-            tc_wait_ld(u[0]);
-            tc_touch(u[1]);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) mask(u[half], half), highest(u[half]);
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            float turn = 1.f;
-            if (m == -INFINITY) {
-                m = top;  // nothing of this row is in O yet
-            } else if ((top - m) * a.scale_log2 > 8.f) {
-                turn = exp2_fast((m - top) * a.scale_log2);
-                l *= turn;
-                m = top;
-            }
-            if (__any_sync(0xffffffffu, turn != 1.f)) {
-                // until the previous product is in O (these scores were queued behind the one before it)
-                ok = mbar_wait(o_done, (x - 1) & 1);
+        auto softmax = [&](auto two_parts) {
+            for (int x = 0; x < tiles.count; ++x) {
+                const int j0 = tiles.at(x) * kKeys;
+                ok = mbar_wait(s_full + 8 * (x % NB), (x / NB) & 1);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc_after();
+                const uint32_t at = mine + (x % NB) * kKeys;
+                // every row of the tile sees every key, unless the tile crosses the diagonal or the window's edge
+                const bool whole = j0 + kKeys - 1 <= i0 && (i0 + kRows - 1 - j0 < a.window || j0 + kKeys <= a.sinks);
+                uint32_t on[2] = {0xffffffffu, 0xffffffffu};
+                if (!whole) on[0] = keys_of_row(i, j0, a.window, a.sinks), on[1] = keys_of_row(i, j0 + 32, a.window, a.sinks);
+                auto mask = [&](uint32_t *u, int half) {
+                    if (whole) return;
 #pragma unroll
-                for (int c = 0; c < DP; c += 32) {
-                    uint32_t w[32];
-                    tc_ld32(mine + S::o_col + c, w);
-                    tc_wait_ld(w);
+                    for (int c = 0; c < 32; ++c)
+                        if (!(on[half] & (1u << c))) u[c] = 0xff800000u;  // minus infinity
+                };
+                uint32_t u[2][32];
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto highest = [&](const uint32_t *v) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * turn);
-                    tc_st32(mine + S::o_col + c, w);
+                    for (int c = 0; c < 32; ++c) tops[c % 4] = fmaxf(tops[c % 4], __uint_as_float(v[c]));
+                };
+                tc_ld32(at, u[0]);
+                tc_ld32(at + 32, u[1]);
+                tc_wait_ld(u[0]);
+                tc_touch(u[1]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) mask(u[half], half), highest(u[half]);
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                float turn = 1.f;
+                if (m == -INFINITY) {
+                    m = top;  // nothing of this row is in O yet
+                } else if ((top - m) * a.scale_log2 > 8.f) {
+                    turn = exp2_fast((m - top) * a.scale_log2);
+                    l *= turn;
+                    m = top;
                 }
-            }
-            const float off = m == -INFINITY ? 0.f : m * a.scale_log2;
-            const uint64_t scale2 = two(a.scale_log2, a.scale_log2), off2 = two(-off, -off);
-            uint64_t sum[4] = {};
+                if (__any_sync(0xffffffffu, turn != 1.f)) {
+                    // until the previous product is in O (these scores were queued behind the one before it)
+                    ok = mbar_wait(o_done, (x - 1) & 1);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    tc_after();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t *v = u[half];
-                uint32_t p[16];
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t w[32];
+                        tc_ld32(mine + S::o_col + c, w);
+                        tc_wait_ld(w);
 #pragma unroll
-                for (int c = 0; c < 32; c += 2) {
-                    float p0, p1;
-                    apart(fma_two(two(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, off2), p0, p1);
-                    p0 = exp2_fast(p0), p1 = exp2_fast(p1);
-                    sum[(c / 2) % 4] = add_two(sum[(c / 2) % 4], two(p0, p1));
-                    p[c / 2] = pack2(p0, p1, T());
-                    v[c] = __float_as_uint(p0), v[c + 1] = __float_as_uint(p1);
+                        for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * turn);
+                        tc_st32(mine + S::o_col + c, w);
+                    }
                 }
-                tc_st16(at + half * 16, p);  // over scores that have been read
-                if (fine) {
+                const float off = m == -INFINITY ? 0.f : m * a.scale_log2;
+                const uint64_t scale2 = two(a.scale_log2, a.scale_log2), off2 = two(-off, -off);
+                uint64_t sum[4] = {};
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2)
-                        p[c / 2] = pack2(rest_of<T>(__uint_as_float(v[c])), rest_of<T>(__uint_as_float(v[c + 1])), T());
-                    tc_st16(at + kKeys / 2 + half * 16, p);
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t *v = u[half];
+                    uint32_t p[16];
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        float p0, p1;
+                        apart(fma_two(two(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, off2), p0, p1);
+                        p0 = exp2_fast(p0), p1 = exp2_fast(p1);
+                        sum[(c / 2) % 4] = add_two(sum[(c / 2) % 4], two(p0, p1));
+                        p[c / 2] = pack2(p0, p1, T());
+                        if (two_parts.value) v[c] = __float_as_uint(p0), v[c + 1] = __float_as_uint(p1);
+                    }
+                    tc_st16(at + half * 16, p);  // over scores that have been read
+                    if (two_parts.value) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float h0, h1;
+                            unpack2(p[c / 2], h0, h1, T());
+                            p[c / 2] = pack2(__uint_as_float(v[c]) - h0, __uint_as_float(v[c + 1]) - h1, T());
+                        }
+                        tc_st16(at + kKeys / 2 + half * 16, p);
+                    }
                 }
-            }
-            float s0, s1;
-            apart(add_two(add_two(sum[0], sum[1]), add_two(sum[2], sum[3])), s0, s1);
-            l += s0 + s1;
-            // keys behind the sequence meet p = 0, but what they hold may be infinite: their values are zeroed
-            if (n < a.T && j0 + kKeys > n) {
-                const int s = x % S::stages;
-                ok = mbar_wait(v_full + 8 * s, (x / S::stages) & 1);
-                if (!__all_sync(0xffffffffu, ok)) break;
-                constexpr int C = DP / 8;
-                const int first = n - j0;
-                for (int e = tid; e < (kKeys - first) * C; e += kRows) {
-                    const int r = first + e / C, c = e % C;
-                    const uint32_t dst = sv + s * S::kv_bytes + (c / 8) * kKeys * 128 + r * 128 + (c % 8) * 16;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+                float s0, s1;
+                apart(add_two(add_two(sum[0], sum[1]), add_two(sum[2], sum[3])), s0, s1);
+                l += s0 + s1;
+                // keys behind the sequence meet p = 0, but what they hold may be infinite: their values are zeroed
+                if (n < a.T && j0 + kKeys > n) {
+                    const int s = x % S::stages;
+                    ok = mbar_wait(v_full + 8 * s, (x / S::stages) & 1);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    constexpr int C = DP / 8;
+                    const int first = n - j0;
+                    for (int e = tid; e < (kKeys - first) * C; e += kRows) {
+                        const int r = first + e / C, c = e % C;
+                        const uint32_t dst = sv + s * S::kv_bytes + (c / 8) * kKeys * 128 + r * 128 + (c % 8) * 16;
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+                    }
+                    fence_async();
+                    __syncwarp();
                 }
-                fence_async();
+                tc_wait_st();
+                tc_before();
                 __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * (x % NB));
             }
-            tc_wait_st();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 8 * (x % NB));
-        }
+        };
+        if (fine) softmax(std::true_type());
+        else softmax(std::false_type());
         if (ok) ok = mbar_wait(o_last, 0);
         if (__all_sync(0xffffffffu, ok)) {
             tc_after();

@@ -55,6 +55,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+__device__ __forceinline__ void unpack2(uint32_t u, float &lo, float &hi, __nv_bfloat16) {
+    lo = __uint_as_float(u << 16), hi = __uint_as_float(u & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t u, float &lo, float &hi, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u));
+    lo = f.x, hi = f.y;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
