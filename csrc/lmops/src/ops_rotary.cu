@@ -6,7 +6,9 @@
 // a few hundred thousand costs no accuracy and no table of positions is
 // kept.  Each (token, pair) is evaluated once per block into shared memory
 // and used by all heads of q and k.  Bound by memory: every element is read
-// and written once.
+// and written once (32767 tokens of 40 heads of 128, float32, interleaved:
+// 1.34 GB in 207 us, 6.5 TB/s; 8 x 1024 tokens of 32 heads of 64, bf16: 67 MB
+// in 13.6 us).
 #include <algorithm>
 
 #include "ops_common.cuh"
