@@ -13,6 +13,8 @@
 // shared memory (41 to 46 % of its wavefronts): 3 x 333 tokens, 16 heads of 64,
 // window 100 and 3 sinks, 24 us forward and 100 with the gradients; 4 x 4 rows
 // and columns a thread, as 4 x 8 measured the same.
+#include <algorithm>
+
 #include "attn.cuh"
 
 namespace cailops {
@@ -25,20 +27,20 @@ constexpr float kNone = -INFINITY;
 template <int DP> constexpr int ld() { return DP + 4; }
 constexpr int kLdP = kTile + 4;
 
-// ROWS rows of x from row r0 (rows >= n as zeros, columns >= D as zeros), as
-// floats.  32-bit rows in whole vectors go by asynchronous copies (the caller
-// commits and waits); the others through registers, all loads before the
-// first store.
-template <typename T, int DP, int ROWS, int THREADS>
-__device__ __forceinline__ void load_tile(float *s, const char *base, int64_t st, int r0, int n, int D, bool vec) {
+// ROWS rows of x, row r of the tile from row `row_of(r)` of x (rows below zero
+// as zeros, columns >= D as zeros), as floats.  32-bit rows in whole vectors go
+// by asynchronous copies (the caller commits and waits); the others through
+// registers, all loads before the first store.
+template <typename T, int DP, int ROWS, int THREADS, typename F>
+__device__ __forceinline__ void load_tile(float *s, const char *base, int64_t st, F row_of, int D, bool vec) {
     constexpr int N = 16 / (int)sizeof(T), C = DP / N, ITER = ROWS * C / THREADS;
     static_assert(ROWS * C % THREADS == 0);
     if (vec && sizeof(T) == 4) {
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
-            const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N;
-            const bool in = r0 + r < n && c < D;
-            const char *src = in ? base + (int64_t)(r0 + r) * st + c * sizeof(T) : base;
+            const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N, from = row_of(r);
+            const bool in = from >= 0 && c < D;
+            const char *src = in ? base + (int64_t)from * st + c * sizeof(T) : base;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(s + r * ld<DP>() + c)), "l"(src),
                          "r"(in ? 16 : 0)
                          : "memory");
@@ -47,25 +49,45 @@ __device__ __forceinline__ void load_tile(float *s, const char *base, int64_t st
         Vec<T, N> x[ITER];
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
-            const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N;
-            if (r0 + r < n && c < D) x[k] = *reinterpret_cast<const Vec<T, N> *>(base + (int64_t)(r0 + r) * st + c * sizeof(T));
+            const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N, from = row_of(r);
+            if (from >= 0 && c < D) x[k] = *reinterpret_cast<const Vec<T, N> *>(base + (int64_t)from * st + c * sizeof(T));
         }
 #pragma unroll
         for (int k = 0; k < ITER; ++k) {
             const int i = threadIdx.x + k * THREADS, r = i / C, c = (i % C) * N;
-            const bool in = r0 + r < n && c < D;
+            const bool in = row_of(r) >= 0 && c < D;
 #pragma unroll
             for (int e = 0; e < N; ++e) s[r * ld<DP>() + c + e] = in ? to_f(x[k].v[e]) : 0.f;
         }
     } else {
 #pragma unroll 4
         for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
-            const int r = i / DP, c = i % DP;
-            const bool in = r0 + r < n && c < D;
-            s[r * ld<DP>() + c] = in ? to_f(*reinterpret_cast<const T *>(base + (int64_t)(r0 + r) * st + c * sizeof(T))) : 0.f;
+            const int r = i / DP, c = i % DP, from = row_of(r);
+            const bool in = from >= 0 && c < D;
+            s[r * ld<DP>() + c] = in ? to_f(*reinterpret_cast<const T *>(base + (int64_t)from * st + c * sizeof(T))) : 0.f;
         }
     }
 }
+// rows r0 .. of a sequence that ends at n
+struct From {
+    int r0, n;
+    __device__ __forceinline__ int operator()(int r) const { return r0 + r < n ? r0 + r : -1; }
+};
+// The keys that the query rows [i0, i1) of a sequence of n tokens need: the
+// sinks before the window, then the window, side by side in tiles, so that a
+// few sinks take a few rows of a tile and no tile starts before the window.
+struct Keys {
+    int sinks, first, total, count;
+    __device__ __forceinline__ Keys(int i0, int i1, int n, int window, int all_sinks) {
+        i1 = min(i1, n);
+        first = window > i0 ? 0 : i0 - window + 1;
+        sinks = min(all_sinks, first);
+        total = i0 < i1 ? sinks + i1 - first : 0;
+        count = (total + kTile - 1) / kTile;
+    }
+    // the key in place x (a key behind the last row where x is behind the last place)
+    __device__ __forceinline__ int key(int x) const { return x < sinks ? x : x - sinks + first; }
+};
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -168,32 +190,29 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
     constexpr int NC = DP / 16;
     extern __shared__ float4 smem4[];
     constexpr int TILE = kTile * ld<DP>();
-    float *sq = reinterpret_cast<float *>(smem4), *sk2 = sq + TR * ld<DP>(), *sv2 = sk2 + 2 * TILE, *sp = sv2 + 2 * TILE;
+    float *sq = reinterpret_cast<float *>(smem4), *sk = sq + TR * ld<DP>(), *sv = sk + TILE, *sp = sv + TILE;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
     const int i0 = (gridDim.x - 1 - blockIdx.x) * TR;  // the longest rows first
     const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
     const int n = length_of(a, b);
-    const KeyTiles tiles(i0, i0 + TR, n, a.window, a.sinks, kTile);
+    const Keys keys(i0, i0 + TR, n, a.window, a.sinks);
     const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
 
-    load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, From{i0, n}, a.D, vec);
     Out<DP> o;
     float m[4], l[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) m[r] = kNone, l[r] = 0.f;
 
-    auto fetch = [&](int x) {
-        load_tile<T, DP, kTile, TR * 4>(sk2 + (x & 1) * TILE, kp, a.kt, tiles.at(x) * kTile, n, a.D, vec);
-        load_tile<T, DP, kTile, TR * 4>(sv2 + (x & 1) * TILE, vp, a.vt, tiles.at(x) * kTile, n, a.D, vec);
+    auto fetch = [&](float *s, const char *from, int64_t st, int x) {
+        load_tile<T, DP, kTile, TR * 4>(s, from, st, [&](int r) { return x * kTile + r < keys.total ? keys.key(x * kTile + r) : -1; }, a.D, vec);
         copies_issued();
     };
-    if (tiles.count) fetch(0);
-    for (int x = 0; x < tiles.count; ++x) {
-        const int j0 = tiles.at(x) * kTile;
-        const float *sk = sk2 + (x & 1) * TILE, *sv = sv2 + (x & 1) * TILE;
-        if (x + 1 < tiles.count) fetch(x + 1), copies_done<1>();
-        else copies_done<0>();
-        __syncthreads();
+    fetch(sk, kp, a.kt, 0);
+    for (int x = 0; x < keys.count; ++x) {
+        copies_done<0>();
+        __syncthreads();  // the keys are there, the values' place is free
+        fetch(sv, vp, a.vt, x);
         float s[4][4];
         dot_tile<DP>(sq, sk, s, ty, tx);
 #pragma unroll
@@ -202,7 +221,7 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
             float top = kNone;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                s[r][c] = seen(i, j0 + tx + 16 * c, n, a.window, a.sinks) ? s[r][c] * a.scale_log2 : kNone;
+                s[r][c] = seen(i, keys.key(x * kTile + tx + 16 * c), n, a.window, a.sinks) ? s[r][c] * a.scale_log2 : kNone;
                 top = fmaxf(top, s[r][c]);
             }
             top = fmaxf(m[r], half_max(top));
@@ -218,9 +237,10 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
             l[r] = l[r] * turn + half_sum(sum);
             o.scale(r, turn);
         }
-        __syncwarp();  // a row of p is written and read by one warp
+        copies_done<0>();
+        __syncthreads();  // the values are there, the keys' place is free
+        if (x + 1 < keys.count) fetch(sk, kp, a.kt, x + 1);
         out_tile<DP>(sp, sv, o, ty, tx);
-        __syncthreads();  // the tile's place is free
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -246,22 +266,30 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
     constexpr int NC = DP / 16;
     constexpr int TILE = kTile * ld<DP>();
     extern __shared__ float4 smem4[];
-    float *sq = reinterpret_cast<float *>(smem4), *sg = sq + TR * ld<DP>(), *sk2 = sg + TR * ld<DP>(), *sv2 = sk2 + 2 * TILE, *sp = sv2 + 2 * TILE;
+    float *sq = reinterpret_cast<float *>(smem4), *sg = sq + TR * ld<DP>(), *sk = sg + TR * ld<DP>(), *sv = sk + TILE, *sp = sv + TILE;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / a.group;
     const int i0 = (gridDim.x - 1 - blockIdx.x) * TR;
     const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
     const int n = length_of(a, b);
-    const KeyTiles tiles(i0, i0 + TR, n, a.window, a.sinks, kTile);
+    const Keys keys(i0, i0 + TR, n, a.window, a.sinks);
     const char *kp = a.k + b * a.kb + hk * a.kh, *vp = a.v + b * a.vb + hk * a.vh;
 
-    // o, and what rounding took from it, pass through the second key tile's place and the second value tile's
-    load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
-    load_tile<T, DP, TR, TR * 4>(sg, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec);
-    load_tile<T, DP, TR, TR * 4>(sk2 + TILE, a.o + b * a.ob + h * a.oh, a.ot, i0, n, a.D, vec);
+    auto fetch = [&](float *s, const char *from, int64_t st, int x) {
+        load_tile<T, DP, kTile, TR * 4>(s, from, st, [&](int r) { return x * kTile + r < keys.total ? keys.key(x * kTile + r) : -1; }, a.D, vec);
+        copies_issued();
+    };
+    // o, and what rounding took from it, pass through the keys' place (or the probabilities')
+    float *so = sk, *srest = TR == 32 ? sk + TR * ld<DP>() : sp;
+    static_assert(TR == 32 || ld<DP>() <= kLdP);
+    const From rows = {i0, n};
+    load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, rows, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(sg, a.dout + b * a.gb + h * a.gh, a.gt, rows, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(so, a.o + b * a.ob + h * a.oh, a.ot, rows, a.D, vec);
     const bool rest = sizeof(T) == 2 && i0 < a.rest_rows;
-    if (rest) load_tile<T, DP, TR, TR * 4>(sv2 + TILE, a.rest + b * a.rb + h * a.rh, a.rt, i0, min(n, a.rest_rows), a.D, vec);
+    if (rest) load_tile<T, DP, TR, TR * 4>(srest, a.rest + b * a.rb + h * a.rh, a.rt, From{i0, min(n, a.rest_rows)}, a.D, vec);
     copies_issued();
-    copies_done<0>();
+    fetch(sv, vp, a.vt, 0);
+    copies_done<1>();
     __syncthreads();
     float delta[4], lse[4];
     Out<DP> dq;
@@ -272,40 +300,33 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int at = row * ld<DP>() + tx + 16 * c;
-            s = fmaf(sg[at], rest ? sk2[TILE + at] + sv2[TILE + at] : sk2[TILE + at], s);
+            s = fmaf(sg[at], rest ? so[at] + srest[at] : so[at], s);
         }
         delta[r] = half_sum(s);
         const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + i;
         lse[r] = i < n ? a.lse[at] : 0.f;
         if (i < a.T && tx == 0) a.delta[at] = delta[r];
     }
-    auto fetch = [&](int x) {
-        load_tile<T, DP, kTile, TR * 4>(sk2 + (x & 1) * TILE, kp, a.kt, tiles.at(x) * kTile, n, a.D, vec);
-        load_tile<T, DP, kTile, TR * 4>(sv2 + (x & 1) * TILE, vp, a.vt, tiles.at(x) * kTile, n, a.D, vec);
-        copies_issued();
-    };
-    if (tiles.count) fetch(0);
-    __syncthreads();  // o's place is free
-    for (int x = 0; x < tiles.count; ++x) {
-        const int j0 = tiles.at(x) * kTile;
-        const float *sk = sk2 + (x & 1) * TILE, *sv = sv2 + (x & 1) * TILE;
-        if (x + 1 < tiles.count) fetch(x + 1), copies_done<1>();
-        else copies_done<0>();
-        __syncthreads();
+    for (int x = 0; x < keys.count; ++x) {
+        copies_done<0>();
+        __syncthreads();  // the values are there, the keys' place is free
+        fetch(sk, kp, a.kt, x);
         float s[4][4], dp[4][4];
-        dot_tile<DP>(sq, sk, s, ty, tx);
         dot_tile<DP>(sg, sv, dp, ty, tx);
+        copies_done<0>();
+        __syncthreads();  // the keys are there, the values' place is free
+        if (x + 1 < keys.count) fetch(sv, vp, a.vt, x + 1);
+        dot_tile<DP>(sq, sk, s, ty, tx);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int i = i0 + ty * 4 + r;
-                const bool on = seen(i, j0 + tx + 16 * c, n, a.window, a.sinks) && !one_key(i, a.window, a.sinks);
+                const bool on = seen(i, keys.key(x * kTile + tx + 16 * c), n, a.window, a.sinks) && !one_key(i, a.window, a.sinks);
                 sp[(ty * 4 + r) * kLdP + tx + 16 * c] = on ? exp2_fast(fmaf(s[r][c], a.scale_log2, -lse[r])) * (dp[r][c] - delta[r]) : 0.f;
             }
         __syncwarp();
         out_tile<DP>(sp, sk, dq, ty, tx);
-        __syncthreads();
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -326,9 +347,9 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec, c
     constexpr int NC = DP / 16;
     constexpr int TILE = kTile * ld<DP>();
     extern __shared__ float4 smem4[];
-    float *sk = reinterpret_cast<float *>(smem4), *sv = sk + TR * ld<DP>(), *sq2 = sv + TR * ld<DP>(), *sg2 = sq2 + 2 * TILE,
-          *sp = sg2 + 2 * TILE, *sd = sp + TR * kLdP;
-    __shared__ float lse2[2][kTile], delta2[2][kTile];
+    float *sk = reinterpret_cast<float *>(smem4), *sv = sk + TR * ld<DP>(), *sq = sv + TR * ld<DP>(), *sg = sq + TILE, *sp = sg + TILE,
+          *sd = sp + TR * kLdP;
+    __shared__ float row_lse[kTile], row_delta[kTile];
     const int hk = blockIdx.y, b = blockIdx.z;
     int tile = blockIdx.x, split = 0;
     const bool parted = parts.splits > 1 && tile < parts.tiles * parts.splits;
@@ -339,38 +360,43 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec, c
     const int n = length_of(a, b);
     int begin, end;
     query_range(j0, j0 + TR, n, a.window, a.sinks, begin, end);
-    load_tile<T, DP, TR, TR * 4>(sk, a.k + b * a.kb + hk * a.kh, a.kt, j0, n, a.D, vec);
-    load_tile<T, DP, TR, TR * 4>(sv, a.v + b * a.vb + hk * a.vh, a.vt, j0, n, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(sk, a.k + b * a.kb + hk * a.kh, a.kt, From{j0, n}, a.D, vec);
+    load_tile<T, DP, TR, TR * 4>(sv, a.v + b * a.vb + hk * a.vh, a.vt, From{j0, n}, a.D, vec);
     Out<DP> dk, dv;
     // the tiles that pass: the group's heads in turn, each over the rows that see these keys
-    const int t0 = begin / kTile, per = end > begin ? (end - 1) / kTile + 1 - t0 : 0;
+    const int per = end > begin ? (end - begin + kTile - 1) / kTile : 0;
     int first = 0, count = a.group * per;
     if (parted) {  // this part of them
         const int share = (count + parts.splits - 1) / parts.splits;
         first = min(count, split * share);
         count = min(count, first + share);
     }
-    auto fetch = [&](int x) {
-        const int h = hk * a.group + x / per, i0 = (t0 + x % per) * kTile, at = x & 1;
-        load_tile<T, DP, kTile, TR * 4>(sq2 + at * TILE, a.q + b * a.qb + h * a.qh, a.qt, i0, n, a.D, vec);
-        load_tile<T, DP, kTile, TR * 4>(sg2 + at * TILE, a.dout + b * a.gb + h * a.gh, a.gt, i0, n, a.D, vec);
+    auto rows = [&](int x) { return begin + x % per * kTile; };
+    auto fetch_g = [&](int x) {
+        load_tile<T, DP, kTile, TR * 4>(sg, a.dout + b * a.gb + (hk * a.group + x / per) * a.gh, a.gt, From{rows(x), n}, a.D, vec);
+        copies_issued();
+    };
+    auto fetch_q = [&](int x) {
+        const int h = hk * a.group + x / per, i0 = rows(x);
+        load_tile<T, DP, kTile, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, From{i0, n}, a.D, vec);
         if (tid < kTile) {
             const int64_t row = ((int64_t)b * a.H + h) * a.lse_row + i0 + tid;
-            lse2[at][tid] = i0 + tid < n ? a.lse[row] : 0.f;
-            delta2[at][tid] = i0 + tid < n ? a.delta[row] : 0.f;
+            row_lse[tid] = i0 + tid < n ? a.lse[row] : 0.f;
+            row_delta[tid] = i0 + tid < n ? a.delta[row] : 0.f;
         }
         copies_issued();
     };
-    if (first < count) fetch(first);
+    if (first < count) fetch_g(first);
     for (int x = first; x < count; ++x) {
-        const int i0 = (t0 + x % per) * kTile;
-        const float *sq = sq2 + (x & 1) * TILE, *sg = sg2 + (x & 1) * TILE, *row_lse = lse2[x & 1], *row_delta = delta2[x & 1];
-        if (x + 1 < count) fetch(x + 1), copies_done<1>();
-        else copies_done<0>();
-        __syncthreads();
+        const int i0 = rows(x);
+        copies_done<0>();
+        __syncthreads();  // do is there, q's place is free
+        fetch_q(x);
         float s[4][4], dp[4][4];
-        dot_tile<DP>(sk, sq, s, ty, tx);
         dot_tile<DP>(sv, sg, dp, ty, tx);
+        copies_done<0>();
+        __syncthreads();  // q is there
+        dot_tile<DP>(sk, sq, s, ty, tx);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -383,8 +409,9 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec, c
             }
         __syncwarp();
         out_tile<DP>(sp, sg, dv, ty, tx);
+        __syncthreads();  // do's place is free
+        if (x + 1 < count) fetch_g(x + 1);
         out_tile<DP>(sd, sq, dk, ty, tx);
-        __syncthreads();
     }
     if (parted) {
         float *sums = parts.sums + ((((int64_t)b * a.Hkv + hk) * parts.tiles + tile) * parts.splits + split) * (2 * TR * DP);
@@ -424,14 +451,14 @@ template <typename K> int prepare(K kernel, size_t smem) {
 // rate); 4 x 8 values a thread read less and measured no better, for want of
 // warps.
 template <typename T, int DP, int TR> int forward(const AttnArgs &a, bool vec, cudaStream_t st) {
-    const size_t smem = (TR * ld<DP>() + 4 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
+    const size_t smem = (TR * ld<DP>() + 2 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
     if (int rc = prepare(simt_forward<T, DP, TR>, smem)) return rc;
     simt_forward<T, DP, TR><<<dim3((a.T + TR - 1) / TR, a.H, a.B), TR * 4, smem, st>>>(a, vec);
     return launched("window attention");
 }
 template <typename T, int DP, int TR> int backward(const AttnArgs &a, const SinkParts &parts, bool vec, cudaStream_t st) {
     const unsigned tiles = (a.T + TR - 1) / TR;
-    size_t smem = (2 * TR * ld<DP>() + 4 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
+    size_t smem = (2 * TR * ld<DP>() + 2 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
     if (int rc = prepare(simt_dq<T, DP, TR>, smem)) return rc;
     simt_dq<T, DP, TR><<<dim3(tiles, a.H, a.B), TR * 4, smem, st>>>(a, vec);
     if (int rc = launched("window attention backward")) return rc;
@@ -445,7 +472,11 @@ template <typename T, int DP, int TR> int backward(const AttnArgs &a, const Sink
 bool few_blocks(const cail_ops_attention_args *a, bool back) {
     return ((int64_t)a->T + 63) / 64 * (back ? a->Hkv : a->H) * a->B < 4 * (int64_t)sm_count();
 }
-int rows_of(const cail_ops_attention_args *a, bool back) { return few_blocks(a, back) || a->D > 64 ? 32 : 64; }
+// tiles that a block of so many rows goes over, where no sequence ends
+int64_t tiles_of(const cail_ops_attention_args *a, int rows) { return ((int64_t)std::min(a->window, a->T) + std::min(a->sinks, a->T) + rows - 1 + kTile - 1) / kTile; }
+int rows_of(const cail_ops_attention_args *a, bool back) {
+    return few_blocks(a, back) || a->D > 64 || 10 * tiles_of(a, 32) < 9 * tiles_of(a, 64) ? 32 : 64;
+}
 SinkParts parts_of(const cail_ops_attention_args *a) { return sink_parts(a, rows_of(a, true), kTile, 2 * (int64_t)sm_count()); }
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 template <typename T, int DP> int sized(const AttnArgs &a, const SinkParts &parts, int rows, bool vec, bool back, cudaStream_t st) {
