@@ -1,26 +1,26 @@
 // attn_simt.cu — window attention on the FP32 pipes: 32-bit inputs, and head
 // sizes or strides that the tensor-core kernels do not take.
 //
-// Forward: a block owns 64 query rows (32 where there are few) of one head and goes once over the key
-// tiles that some of them see, with the running maximum and sum of each row
-// (16 threads share a row; each thread holds 4 rows x 4 columns of the scores
-// and 4 rows x D/16 of the output).  Backward: p is recomputed from the kept
-// log-sum; one kernel owns query tiles and writes dq (and delta = do.o), the
-// other owns key tiles, goes over the group's heads and the query tiles that
-// see them, and writes dk and dv.  No atomics: results do not change from run
-// to run.  Rows and keys at or beyond a sequence's length are never read, so
-// what lies there may be anything.  Bound by the FP32 pipe and by reads of
-// shared memory (41 to 46 % of its wavefronts): 3 x 333 tokens, 16 heads of 64,
-// window 100 and 3 sinks, 24 us forward and 100 with the gradients; 4 x 4 rows
-// and columns a thread, as 4 x 8 measured the same.
-#include <algorithm>
-
+// Forward: a block owns 32 query rows of one head and goes once over the keys
+// that some of them see (the sinks, then the window, side by side in tiles of
+// 64), with the running maximum and sum of each row (16 threads share a row;
+// each thread holds 4 rows x 4 columns of the scores and 4 rows x D/16 of the
+// output).  Backward: p is recomputed from the kept log-sum; one kernel owns
+// query rows and writes dq (and delta = do.o), the other owns keys, goes over
+// the group's heads and the query rows that see them, and writes dk and dv.
+// No atomics: results do not change from run to run.  Rows and keys at or
+// beyond a sequence's length are never read, so what lies there may be
+// anything.  Bound by the FP32 pipe and by reads of shared memory: 3 padded
+// sequences of 333 tokens, 16 heads of 64, window 100 and 3 sinks, 21 us
+// forward and 82 with the gradients; 2 x 2048, 16 heads, window 512, 251 us
+// forward, 30 TFLOP/s.  4 x 4 rows and columns a thread: 4 x 8 measured the same.
 #include "attn.cuh"
 
 namespace cailops {
 namespace {
 
-constexpr int kTile = 64;  // rows of the tiles that pass; a block owns TR rows, 4 threads' worth each
+constexpr int TR = 32;     // rows of a block, 4 threads' worth each
+constexpr int kTile = 64;  // rows of the tiles that pass
 constexpr float kNone = -INFINITY;
 
 // rows of shared tiles are DP + 4 floats apart: 16-byte reads of 8 rows in a phase hit different banks
@@ -91,29 +91,40 @@ struct Keys {
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// acc[r][c] = sum_d x[ty*4+r][d] * y[tx+16c][d], even and odd d apart until the end
-template <int DP> __device__ __forceinline__ void dot_tile(const float *x, const float *y, float acc[4][4], int ty, int tx) {
-    uint64_t acc2[4][4] = {};
+// acc[r][c] = sum_d x[ty*4+r][d] * y[tx+16c][d] for c < C, even and odd d apart until the end
+template <int DP, int C> __device__ __forceinline__ void dot_columns(const float *x, const float *y, float acc[4][4], int ty, int tx) {
+    uint64_t acc2[4][C] = {};
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
-        ulonglong2 a[4], b[4];
+        ulonglong2 a[4], b[C];
 #pragma unroll
         for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const ulonglong2 *>(x + (ty * 4 + r) * ld<DP>() + d);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const ulonglong2 *>(y + (tx + 16 * c) * ld<DP>() + d);
+        for (int c = 0; c < C; ++c) b[c] = *reinterpret_cast<const ulonglong2 *>(y + (tx + 16 * c) * ld<DP>() + d);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc2[r][c] = fma_two(a[r].y, b[c].y, fma_two(a[r].x, b[c].x, acc2[r][c]));
+            for (int c = 0; c < C; ++c) acc2[r][c] = fma_two(a[r].y, b[c].y, fma_two(a[r].x, b[c].x, acc2[r][c]));
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < C; ++c) {
             float e, o;
             apart(acc2[r][c], e, o);
             acc[r][c] = e + o;
         }
+}
+
+// the same for the first `valid` rows of y, in halves (what lies behind is left zero)
+template <int DP> __device__ __forceinline__ void dot_tile(const float *x, const float *y, float acc[4][4], int ty, int tx, int valid) {
+    if (valid > kTile / 2) {
+        dot_columns<DP, 4>(x, y, acc, ty, tx);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r][2] = acc[r][3] = 0.f;
+        dot_columns<DP, 2>(x, y, acc, ty, tx);
+    }
 }
 
 // column c of a thread's DP/16 output columns
@@ -153,24 +164,31 @@ template <int DP> __device__ __forceinline__ void row_of(const float *y, uint64_
         }
     }
 }
-// o[r][:] += sum_j p[ty*4+r][j] * y[j][:]
-template <int DP> __device__ __forceinline__ void out_tile(const float *p, const float *y, Out<DP> &o, int ty, int tx) {
-#pragma unroll 4
-    for (int j = 0; j < kTile; j += 4) {
-        float4 a[4];
+// o[r][:] += sum_j p[ty*4+r][j] * y[j][:], over four j
+template <int DP> __device__ __forceinline__ void out_four(const float *p, const float *y, Out<DP> &o, int ty, int tx, int j) {
+    float4 a[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4 *>(p + (ty * 4 + r) * kLdP + j);
+    for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4 *>(p + (ty * 4 + r) * kLdP + j);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            uint64_t w[Out<DP>::NP];
-            row_of<DP>(y + (j + e) * ld<DP>(), w, tx);
+    for (int e = 0; e < 4; ++e) {
+        uint64_t w[Out<DP>::NP];
+        row_of<DP>(y + (j + e) * ld<DP>(), w, tx);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float f = e == 0 ? a[r].x : e == 1 ? a[r].y : e == 2 ? a[r].z : a[r].w;
+        for (int r = 0; r < 4; ++r) {
+            const float f = e == 0 ? a[r].x : e == 1 ? a[r].y : e == 2 ? a[r].z : a[r].w;
 #pragma unroll
-                for (int c = 0; c < Out<DP>::NP; ++c) o.v[r][c] = fma_two(two(f, f), w[c], o.v[r][c]);
-            }
+            for (int c = 0; c < Out<DP>::NP; ++c) o.v[r][c] = fma_two(two(f, f), w[c], o.v[r][c]);
         }
+    }
+}
+// over the first `valid` j, in fours; all of them, unrolled, where few are left out (p is zero behind them)
+template <int DP> __device__ __forceinline__ void out_tile(const float *p, const float *y, Out<DP> &o, int ty, int tx, int valid) {
+    if (valid > kTile * 3 / 4) {
+#pragma unroll 4
+        for (int j = 0; j < kTile; j += 4) out_four<DP>(p, y, o, ty, tx, j);
+    } else {
+#pragma unroll 1
+        for (int j = 0; j < valid; j += 4) out_four<DP>(p, y, o, ty, tx, j);
     }
 }
 
@@ -185,7 +203,7 @@ __device__ __forceinline__ float half_sum(float x) {
     return x;
 }
 
-template <typename T, int DP, int TR>
+template <typename T, int DP>
 __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool vec) {
     constexpr int NC = DP / 16;
     extern __shared__ float4 smem4[];
@@ -210,11 +228,12 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
     };
     fetch(sk, kp, a.kt, 0);
     for (int x = 0; x < keys.count; ++x) {
+        const int valid = keys.total - x * kTile;
         copies_done<0>();
         __syncthreads();  // the keys are there, the values' place is free
         fetch(sv, vp, a.vt, x);
         float s[4][4];
-        dot_tile<DP>(sq, sk, s, ty, tx);
+        dot_tile<DP>(sq, sk, s, ty, tx, valid);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = i0 + ty * 4 + r;
@@ -240,7 +259,7 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
         copies_done<0>();
         __syncthreads();  // the values are there, the keys' place is free
         if (x + 1 < keys.count) fetch(sk, kp, a.kt, x + 1);
-        out_tile<DP>(sp, sv, o, ty, tx);
+        out_tile<DP>(sp, sv, o, ty, tx, valid);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -260,8 +279,8 @@ __global__ void __launch_bounds__(TR * 4) simt_forward(const AttnArgs a, bool ve
     }
 }
 
-// dq and delta of 64 query rows
-template <typename T, int DP, int TR>
+// dq and delta of a block's query rows
+template <typename T, int DP>
 __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
     constexpr int NC = DP / 16;
     constexpr int TILE = kTile * ld<DP>();
@@ -278,9 +297,9 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
         load_tile<T, DP, kTile, TR * 4>(s, from, st, [&](int r) { return x * kTile + r < keys.total ? keys.key(x * kTile + r) : -1; }, a.D, vec);
         copies_issued();
     };
-    // o, and what rounding took from it, pass through the keys' place (or the probabilities')
-    float *so = sk, *srest = TR == 32 ? sk + TR * ld<DP>() : sp;
-    static_assert(TR == 32 || ld<DP>() <= kLdP);
+    // o, and what rounding took from it, pass through the keys' place
+    float *so = sk, *srest = sk + TR * ld<DP>();
+    static_assert(2 * TR <= kTile);
     const From rows = {i0, n};
     load_tile<T, DP, TR, TR * 4>(sq, a.q + b * a.qb + h * a.qh, a.qt, rows, a.D, vec);
     load_tile<T, DP, TR, TR * 4>(sg, a.dout + b * a.gb + h * a.gh, a.gt, rows, a.D, vec);
@@ -308,15 +327,16 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
         if (i < a.T && tx == 0) a.delta[at] = delta[r];
     }
     for (int x = 0; x < keys.count; ++x) {
+        const int valid = keys.total - x * kTile;
         copies_done<0>();
         __syncthreads();  // the values are there, the keys' place is free
         fetch(sk, kp, a.kt, x);
         float s[4][4], dp[4][4];
-        dot_tile<DP>(sg, sv, dp, ty, tx);
+        dot_tile<DP>(sg, sv, dp, ty, tx, valid);
         copies_done<0>();
         __syncthreads();  // the keys are there, the values' place is free
         if (x + 1 < keys.count) fetch(sv, vp, a.vt, x + 1);
-        dot_tile<DP>(sq, sk, s, ty, tx);
+        dot_tile<DP>(sq, sk, s, ty, tx, valid);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -326,7 +346,7 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
                 sp[(ty * 4 + r) * kLdP + tx + 16 * c] = on ? exp2_fast(fmaf(s[r][c], a.scale_log2, -lse[r])) * (dp[r][c] - delta[r]) : 0.f;
             }
         __syncwarp();
-        out_tile<DP>(sp, sk, dq, ty, tx);
+        out_tile<DP>(sp, sk, dq, ty, tx, valid);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -341,8 +361,8 @@ __global__ void __launch_bounds__(TR * 4) simt_dq(const AttnArgs a, bool vec) {
     }
 }
 
-// dk and dv of 64 keys, over the group's heads and the query rows that see them
-template <typename T, int DP, int TR>
+// dk and dv of a block's keys, over the group's heads and the query rows that see them
+template <typename T, int DP>
 __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec, const SinkParts parts) {
     constexpr int NC = DP / 16;
     constexpr int TILE = kTile * ld<DP>();
@@ -388,15 +408,15 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec, c
     };
     if (first < count) fetch_g(first);
     for (int x = first; x < count; ++x) {
-        const int i0 = rows(x);
+        const int i0 = rows(x), valid = end - i0;
         copies_done<0>();
         __syncthreads();  // do is there, q's place is free
         fetch_q(x);
         float s[4][4], dp[4][4];
-        dot_tile<DP>(sv, sg, dp, ty, tx);
+        dot_tile<DP>(sv, sg, dp, ty, tx, valid);
         copies_done<0>();
         __syncthreads();  // q is there
-        dot_tile<DP>(sk, sq, s, ty, tx);
+        dot_tile<DP>(sk, sq, s, ty, tx, valid);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -408,10 +428,10 @@ __global__ void __launch_bounds__(TR * 4) simt_dkv(const AttnArgs a, bool vec, c
                 sd[(ty * 4 + r) * kLdP + i] = on && !one_key(i0 + i, a.window, a.sinks) ? p * (dp[r][c] - row_delta[i]) : 0.f;
             }
         __syncwarp();
-        out_tile<DP>(sp, sg, dv, ty, tx);
+        out_tile<DP>(sp, sg, dv, ty, tx, valid);
         __syncthreads();  // do's place is free
         if (x + 1 < count) fetch_g(x + 1);
-        out_tile<DP>(sd, sq, dk, ty, tx);
+        out_tile<DP>(sd, sq, dk, ty, tx, valid);
     }
     if (parted) {
         float *sums = parts.sums + ((((int64_t)b * a.Hkv + hk) * parts.tiles + tile) * parts.splits + split) * (2 * TR * DP);
@@ -443,61 +463,48 @@ template <typename K> int prepare(K kernel, size_t smem) {
     return e == cudaSuccess ? CAIL_OPS_OK : fail(CAIL_OPS_ECUDA, "window attention: %s", cudaGetErrorString(e));
 }
 
-// Rows of a block: 64, or 32 while 64 would give an SM fewer than four blocks
-// (3 padded sequences of 333 tokens, 16 heads of 64, float32, window 100,
-// forward and backward: 149 us with 64, 145 with 32; 106 with the tiles on
-// their way while the one before is worked on).  2 x 2048 tokens, 16 heads,
-// window 512: 28 TFLOP/s forward, bound by shared-memory reads (70 % of their
-// rate); 4 x 8 values a thread read less and measured no better, for want of
-// warps.
-template <typename T, int DP, int TR> int forward(const AttnArgs &a, bool vec, cudaStream_t st) {
+// 32 rows a block and one place each for the keys and the values, whose loads
+// pass under the other's products: four blocks of four warps per SM forward,
+// three backward.  (64 rows and two places of each, two blocks of eight warps:
+// 2 x 2048 tokens, 16 heads of 64, window 512, forward and backward 1214 us
+// instead of 1071; 2 x 4096, 8 heads, window 250, 718 instead of 632, window 8,
+// 310 instead of 148.)
+template <typename T, int DP> int forward(const AttnArgs &a, bool vec, cudaStream_t st) {
     const size_t smem = (TR * ld<DP>() + 2 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
-    if (int rc = prepare(simt_forward<T, DP, TR>, smem)) return rc;
-    simt_forward<T, DP, TR><<<dim3((a.T + TR - 1) / TR, a.H, a.B), TR * 4, smem, st>>>(a, vec);
+    if (int rc = prepare(simt_forward<T, DP>, smem)) return rc;
+    simt_forward<T, DP><<<dim3((a.T + TR - 1) / TR, a.H, a.B), TR * 4, smem, st>>>(a, vec);
     return launched("window attention");
 }
-template <typename T, int DP, int TR> int backward(const AttnArgs &a, const SinkParts &parts, bool vec, cudaStream_t st) {
+template <typename T, int DP> int backward(const AttnArgs &a, const SinkParts &parts, bool vec, cudaStream_t st) {
     const unsigned tiles = (a.T + TR - 1) / TR;
     size_t smem = (2 * TR * ld<DP>() + 2 * kTile * ld<DP>() + TR * kLdP) * sizeof(float);
-    if (int rc = prepare(simt_dq<T, DP, TR>, smem)) return rc;
-    simt_dq<T, DP, TR><<<dim3(tiles, a.H, a.B), TR * 4, smem, st>>>(a, vec);
+    if (int rc = prepare(simt_dq<T, DP>, smem)) return rc;
+    simt_dq<T, DP><<<dim3(tiles, a.H, a.B), TR * 4, smem, st>>>(a, vec);
     if (int rc = launched("window attention backward")) return rc;
     smem += TR * kLdP * sizeof(float);
-    if (int rc = prepare(simt_dkv<T, DP, TR>, smem)) return rc;
-    simt_dkv<T, DP, TR><<<dim3(tiles + parts.tiles * (parts.splits - 1), a.Hkv, a.B), TR * 4, smem, st>>>(a, vec, parts);
+    if (int rc = prepare(simt_dkv<T, DP>, smem)) return rc;
+    simt_dkv<T, DP><<<dim3(tiles + parts.tiles * (parts.splits - 1), a.Hkv, a.B), TR * 4, smem, st>>>(a, vec, parts);
     if (int rc = launched("window attention backward")) return rc;
     return parts.splits > 1 ? join<T, DP, TR>(a, parts, st) : CAIL_OPS_OK;
 }
-// rows of a block, and the sinks' parts in backward
-bool few_blocks(const cail_ops_attention_args *a, bool back) {
-    return ((int64_t)a->T + 63) / 64 * (back ? a->Hkv : a->H) * a->B < 4 * (int64_t)sm_count();
-}
-// tiles that a block of so many rows goes over, where no sequence ends
-int64_t tiles_of(const cail_ops_attention_args *a, int rows) { return ((int64_t)std::min(a->window, a->T) + std::min(a->sinks, a->T) + rows - 1 + kTile - 1) / kTile; }
-int rows_of(const cail_ops_attention_args *a, bool back) {
-    return few_blocks(a, back) || a->D > 64 || 10 * tiles_of(a, 32) < 9 * tiles_of(a, 64) ? 32 : 64;
-}
-SinkParts parts_of(const cail_ops_attention_args *a) { return sink_parts(a, rows_of(a, true), kTile, 2 * (int64_t)sm_count()); }
+SinkParts parts_of(const cail_ops_attention_args *a) { return sink_parts(a, TR, kTile, 3 * (int64_t)sm_count()); }
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
-template <typename T, int DP> int sized(const AttnArgs &a, const SinkParts &parts, int rows, bool vec, bool back, cudaStream_t st) {
-    if (rows == 32) return back ? backward<T, DP, 32>(a, parts, vec, st) : forward<T, DP, 32>(a, vec, st);
-    if constexpr (DP < 128) return back ? backward<T, DP, 64>(a, parts, vec, st) : forward<T, DP, 64>(a, vec, st);
-    return CAIL_OPS_EINVAL;
+template <typename T, int DP> int sized(const AttnArgs &a, const SinkParts &parts, bool vec, bool back, cudaStream_t st) {
+    return back ? backward<T, DP>(a, parts, vec, st) : forward<T, DP>(a, vec, st);
 }
 template <typename T> int run(const cail_ops_attention_args *c, bool vec, bool back, cudaStream_t st) {
     const AttnArgs a = attn_args(c, back);
-    const int rows = rows_of(c, back);
     SinkParts parts = {1, 0, nullptr};
     if (back) {
         parts = parts_of(c);
-        const size_t bytes = sink_bytes(c, parts, rows, padded(a.D));
+        const size_t bytes = sink_bytes(c, parts, TR, padded(a.D));
         if (c->workspace_bytes < bytes || (bytes && (!c->workspace || !aligned(c->workspace, 16))))
             return fail(CAIL_OPS_EINVAL, "window attention backward: a workspace of %zu bytes is needed", bytes);
         parts.sums = static_cast<float *>(c->workspace);
     }
-    if (a.D <= 32) return sized<T, 32>(a, parts, rows, vec, back, st);
-    if (a.D <= 64) return sized<T, 64>(a, parts, rows, vec, back, st);
-    return sized<T, 128>(a, parts, rows, vec, back, st);
+    if (a.D <= 32) return sized<T, 32>(a, parts, vec, back, st);
+    if (a.D <= 64) return sized<T, 64>(a, parts, vec, back, st);
+    return sized<T, 128>(a, parts, vec, back, st);
 }
 
 }  // namespace
@@ -584,7 +591,7 @@ extern "C" int cail_ops_window_attention(const cail_ops_attention_args *a, cail_
 
 extern "C" size_t cail_ops_window_attention_workspace(const cail_ops_attention_args *a) {
     if (attn_check(a, true, "window attention backward") || a->B == 0 || a->T == 0) return 0;
-    return tc_takes_backward(a) ? tc_workspace(a) : sink_bytes(a, parts_of(a), rows_of(a, true), padded(a->D));
+    return tc_takes_backward(a) ? tc_workspace(a) : sink_bytes(a, parts_of(a), TR, padded(a->D));
 }
 
 extern "C" int cail_ops_window_attention_backward(const cail_ops_attention_args *a, cail_ops_stream stream) {
