@@ -19,13 +19,16 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     tokens, itself among them, and the first ``sinks``.  A window of T or more
     is full causal attention.  ``lengths`` (int32 [B], on the device, clamped to
     [0, T]) are the sequences' lengths; rows at or behind them give zeros and
-    get zero gradients, and what they hold is not used.  ``scale`` is
-    D ** -0.5 unless given.
+    get zero gradients, and what they hold is not used.  Inside a sequence a
+    value that is not finite may reach rows that do not see it, as in a matrix
+    product with zeros.  ``scale`` is D ** -0.5 unless given.
 
     float32, bfloat16 or float16, D from 1 to 128, any strides (elements of a
     head that do not lie side by side are copied first).  Scores, softmax
     statistics and sums are 32-bit.  Gradients flow to q, k and v, each summed
-    in a fixed order: the same inputs give the same bits.
+    in a fixed order: the same inputs give the same bits.  A kernel that waits in
+    vain for its data (two seconds) gives up, and the next call on the device
+    raises RuntimeError.
     """
     return ext.get_ops().window_attention(q, k, v, window, sinks, lengths, scale)
 
