@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                         for (int e = 0; e < 8; ++e) {
                             const float f = to_f(g.v[e]);
                             delta = fmaf(to_f(o.v[e]) + to_f(rest.v[e]), f, delta);
-                            if (!bf) top = fmaxf(top, fabsf(f));
+                            if (!bf) top = fmaxf(top, fabsf(f) < INFINITY ? fabsf(f) : 0.f);  // an infinite gradient scales no other
                         }
                     }
                     if (half == 0) a.delta[at] = delta;

@@ -387,6 +387,27 @@ def test_rows_of_few_keys_lose_one_rounding(dtype, window, sinks, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_a_gradient_that_is_not_finite_stays_with_its_rows(dtype, what):
+    """An overflowed gradient of one row changes no gradient beyond the tiles it is in."""
+    o = ops()
+    q, k, v, do, _ = attention_inputs((1, 500, 2, 1, 64, 20, 0, None), dtype)
+    got = []
+    for d in (do, do.clone()):
+        if got:
+            d[0, 5, 1, 7] = what
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        got.append(torch.autograd.grad(o.window_attention(*leaves, 20, 0), leaves, d))
+    u = ref.half_step(dtype)
+    for a, b in zip(*got):
+        # rows from 256 on share no tile with row 5; fp16 may have scaled ds by another power of two
+        assert torch.isfinite(b[:, 256:]).all()
+        assert ref.rel(b[:, 256:], a[:, 256:].double()) <= 2 * u
+    assert not torch.isfinite(got[1][0][0, 5, 1]).all()
+
+
+@pytest.mark.gpu
 def test_the_first_cuda_call_of_a_thread():
     """A thread in which no context is current yet: the tile loads' descriptors need one."""
     o = ops()
