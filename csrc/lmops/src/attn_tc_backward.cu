@@ -17,7 +17,7 @@
 //
 // p and ds are rounded to the input type for their products, all else is
 // 32-bit.  fp16 has no range for small gradients: ds is scaled by a power of
-// two taken from max |do| (of the row for dq; of the key head for dk), taken
+// two taken from max |do| (of the row for dq; of the rows gone over for dk), taken
 // back out of the sums.
 //
 // D = 64: two blocks per SM, S of the next tile computed under this one's
@@ -61,7 +61,8 @@ struct Maps {
 };
 
 struct Extra {
-    unsigned *amax;       // [B, Hkv] bits of max |do| (fp16)
+    unsigned *amax;       // [B, Hkv, tiles of 128 rows] bits of max |do| (fp16)
+    int tiles;
     SinkParts parts;
 };
 
@@ -325,11 +326,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 if (!bf) {
                     amp = amp_of(__float_as_uint(top));
                     top = warp_max(top);
-                    if (half == 0 && lane == 0 && top > 0.f) atomicMax(ex.amax + b * a.Hkv + hk, __float_as_uint(top));
+                    if (half == 0 && lane == 0 && top > 0.f) atomicMax(ex.amax + ((int64_t)b * a.Hkv + hk) * ex.tiles + r0 / kRows, __float_as_uint(top));
                 }
             }
         } else if (!bf) {
-            amp = amp_of(ex.amax[b * a.Hkv + hk]);
+            // the largest gradient of the rows that this block goes over
+            unsigned top = 0;
+            for (int t = q_begin * kStream / kRows + lane; t <= ((q_begin + q_tiles) * kStream - 1) / kRows; t += 32)
+                top = max(top, ex.amax[((int64_t)b * a.Hkv + hk) * ex.tiles + t]);
+            amp = amp_of(__reduce_max_sync(0xffffffffu, top));
         }
         const float delta_amp = delta * amp;
         for (; walk.x < count; step(walk)) {
@@ -506,7 +511,7 @@ struct Layout {
 Layout layout_of(const cail_ops_attention_args *c) {
     Layout l = {};
     l.parts = sink_parts(c, kRows, kStream, (int64_t)sm_count() * (c->D <= 64 ? 2 : 1));
-    l.sums = c->type == CAIL_OPS_F16 ? ((size_t)c->B * c->Hkv * 4 + 255) / 256 * 256 : 0;
+    l.sums = c->type == CAIL_OPS_F16 ? ((size_t)c->B * c->Hkv * ((c->T + kRows - 1) / kRows) * 4 + 255) / 256 * 256 : 0;
     l.total = l.sums + sink_bytes(c, l.parts, kRows, c->D <= 64 ? 64 : 128);
     return l;
 }
@@ -516,11 +521,12 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     if (c->workspace_bytes < l.total || (l.total && (!c->workspace || !aligned(c->workspace, 16))))
         return fail(CAIL_OPS_EINVAL, "window attention backward: a workspace of %zu bytes is needed", l.total);
     Extra ex = {};
+    ex.tiles = (a.T + kRows - 1) / kRows;
     ex.amax = reinterpret_cast<unsigned *>(static_cast<char *>(c->workspace) + l.amax);
     ex.parts = l.parts;
     ex.parts.sums = reinterpret_cast<float *>(static_cast<char *>(c->workspace) + l.sums);
     if (c->type == CAIL_OPS_F16) {
-        cudaError_t e = cudaMemsetAsync(ex.amax, 0, (size_t)a.B * a.Hkv * 4, st);
+        cudaError_t e = cudaMemsetAsync(ex.amax, 0, (size_t)a.B * a.Hkv * ex.tiles * 4, st);
         if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
     }
     // the same arrays with boxes of 128 and of 64 rows

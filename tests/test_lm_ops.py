@@ -408,6 +408,23 @@ def test_a_gradient_that_is_not_finite_stays_with_its_rows(dtype, what):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+def test_a_large_gradient_costs_others_no_bits(dtype):
+    """Gradients of 1e-3 beside one row of 3e4: dq, dk and dv of rows that share no tile with it, to the bounds of a call without it."""
+    o = ops()
+    q, k, v, do, _ = attention_inputs((1, 500, 2, 1, 64, 20, 0, None), dtype)
+    do = do * 1e-3
+    got = []
+    for d in (do, do.clone()):
+        if got:
+            d[0, 5] = 3e4
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        got.append(torch.autograd.grad(o.window_attention(*leaves, 20, 0), leaves, d))
+    for a, b in zip(*got):
+        assert ref.rel(b[:, 256:], a[:, 256:].double()) <= 2 * ref.half_step(dtype)
+
+
+@pytest.mark.gpu
 def test_the_first_cuda_call_of_a_thread():
     """A thread in which no context is current yet: the tile loads' descriptors need one."""
     o = ops()
