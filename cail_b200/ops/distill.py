@@ -31,6 +31,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     above 0 needs targets.  ``reduction`` is "mean" over the rows that count (0
     if none does), "sum", or "none" ([N]).
 
+    A row whose teacher entries hold NaN or plus infinity, or minus infinity
+    alone, has a loss and a gradient of NaN.
+
     The gradient flows to ``logits``.  Softmax statistics and sums are 32-bit,
     the sum over rows 64-bit, in a fixed order: the same inputs give the same
     bits.

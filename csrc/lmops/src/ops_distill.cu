@@ -224,14 +224,16 @@ struct Teacher {
     __device__ __forceinline__ void finish(const Args &a, int64_t row, const T *z, int lane, float m, float s1, float st, float zy) {
         const int64_t base = row * a.K;
         float tmax = -INFINITY, tsum = 0.f, kl = 0.f;
+        bool any = false;  // an entry that counts; what is not finite among them makes the row NaN
         if (a.hard != 1.f) {
 #pragma unroll
             for (int k = 0; k < E; ++k)
-                if (valid(a, ids[k])) tmax = fmaxf(tmax, t[k]);
+                if (valid(a, ids[k])) any = true, tmax = fmaxf(tmax, t[k]);
             for (int k = lane + 32 * E; k < a.K; k += 32)
-                if (valid(a, id_at(a, base + k))) tmax = fmaxf(tmax, teacher_at(a, base + k) * a.inv_tau);
+                if (valid(a, id_at(a, base + k))) any = true, tmax = fmaxf(tmax, teacher_at(a, base + k) * a.inv_tau);
             tmax = warp_max(tmax);
-            if (tmax != -INFINITY) {
+            any = __any_sync(0xffffffffu, any);
+            if (any) {
 #pragma unroll
                 for (int k = 0; k < E; ++k)
                     if (valid(a, ids[k])) tsum += expf(t[k] - tmax);
@@ -242,7 +244,7 @@ struct Teacher {
                 auto entry = [&](float te, float xe) {
                     const float lt = te - tmax, p = expf(lt) * inv;
                     // p = 0 adds nothing, whatever the student says
-                    if (p > 0.f) kl += p * ((lt - log_tsum) - ((xe - m) * a.inv_tau - log_st));
+                    if (p != 0.f) kl += p * ((lt - log_tsum) - ((xe - m) * a.inv_tau - log_st));
                 };
 #pragma unroll
                 for (int k = 0; k < E; ++k)
@@ -265,7 +267,7 @@ struct Teacher {
         q[1] = MODE == kOne ? st : s1;
         q[2] = st;
         q[3] = tmax;
-        q[4] = tmax == -INFINITY ? 0.f : 1.f / tsum;
+        q[4] = any ? 1.f / tsum : 0.f;
         q[5] = 1.f;
     }
 };
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Args a
     f.c = (MODE == kOne && a.hard == 1.f ? 1.f : a.inv_tau) * kLog2e;
     f.b = -(m * f.c), f.b1 = -(m * kLog2e);
     // the factors of exp((z - m) / tau) and of exp(z - m)
-    f.at = q[4] != 0.f ? soft / q[2] : 0.f, f.a1 = a.hard * scale / q[1];
+    f.at = q[4] != 0.f ? fmaf(0.f, q[4], soft / q[2]) : 0.f, f.a1 = a.hard * scale / q[1];
     if (MODE == kOne) f.at += f.a1;
 
     auto one = [&](int64_t i) { g[i] = from_f<T>(f.one(to_f(z[i]))); };
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(kRingThreads, 3) distill_backward_ring_kernel(
         const float scale = a.per_row_grad ? a.grad_loss[row] : factor;
         const float m = base_of(q[0]), soft = (1.f - a.hard) * a.tau * scale;
         f.b = -(m * f.c), f.b1 = -(m * kLog2e);
-        f.at = q[4] != 0.f ? soft / q[2] : 0.f, f.a1 = a.hard * scale / q[1];
+        f.at = q[4] != 0.f ? fmaf(0.f, q[4], soft / q[2]) : 0.f, f.a1 = a.hard * scale / q[1];
         if (MODE == kOne) f.at += f.a1;
 
         // the terms of single entries: the same id twice adds up, at its first place

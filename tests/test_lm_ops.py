@@ -425,6 +425,32 @@ def test_a_large_gradient_costs_others_no_bits(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_what_is_not_finite_is_not_hidden(dtype, what):
+    """A query, or a key that rows see, that is not finite: NaN in those rows, on every path, and no others of the head's tiles."""
+    o = ops()
+    for T, D in ((20, 64), (300, 64), (300, 128), (150, 33)):
+        q, k, v, _, _ = attention_inputs((2, T, 2, 1, D, 8, 0, None), dtype)
+        q[0, 10, 1] = what
+        out = o.window_attention(q, k, v, 8)
+        assert torch.isnan(out[0, 10, 1]).all()
+        assert torch.isfinite(out[1]).all() and torch.isfinite(out[0, :, 0]).all() and torch.isfinite(out[0, :10, 1]).all()
+        assert torch.isfinite(out[0, 11:, 1]).all()
+    for T, H, Hkv, D, window in ((40, 2, 2, 64, 40), (3000, 4, 1, 64, 3000), (3000, 16, 2, 128, 2500), (3000, 2, 2, 33, 3000)):
+        g = gen(T + D)
+        q, k, v = randn(g, 2, H, D, dtype=dtype), randn(g, 2, T, Hkv, D, dtype=dtype), randn(g, 2, T, Hkv, D, dtype=dtype)
+        n = torch.tensor([T, T], dtype=torch.int32).cuda()
+        q[0, 0] = what
+        out = o.window_attention_decode(q, k, v, n, window)
+        assert torch.isnan(out[0, 0]).all() and torch.isfinite(out[1]).all() and torch.isfinite(out[0, 1:]).all()
+        q[0, 0] = 1.0
+        v[0, T - 3] = what
+        out = o.window_attention_decode(q, k, v, n, window)
+        assert not torch.isfinite(out[0]).any() and torch.isfinite(out[1]).all()
+
+
+@pytest.mark.gpu
 def test_the_first_cuda_call_of_a_thread():
     """A thread in which no context is current yet: the tile loads' descriptors need one."""
     o = ops()
@@ -837,6 +863,38 @@ def test_distill_many_rows(dtype, case):
         (again,) = torch.autograd.grad(o.distill_loss(x, ids, t, y, temperature=tau, hard_weight=hard), x, torch.tensor(512.0).cuda())
         assert torch.equal(again, dz)
     assert torch.equal(wide[:, :5], torch.zeros_like(wide[:, :5])) and not wide[:, V + 5:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("N, V", [(5, 301), (6, 30011), (200, 20003)])
+@pytest.mark.parametrize("tau", [1.0, 2.0, 3.0])
+def test_distill_hides_nothing_that_is_not_finite(dtype, N, V, tau):
+    """NaN or plus infinity in a row of logits or among the teacher's, a row of minus infinity: no finite loss or gradient for
+    that row, and the others' bits unchanged."""
+    o = ops()
+    g = gen(N + V)
+    z, t = randn(g, N, V, dtype=dtype), randn(g, N, 5)
+    ids, y = torch.randint(0, V, (N, 5), generator=g).cuda(), torch.randint(0, V, (N,), generator=g).cuda()
+
+    def run(z, t):
+        z = z.clone().requires_grad_()
+        loss = o.distill_loss(z, ids, t, y, temperature=tau, hard_weight=0.5, reduction="none")
+        return loss.detach(), torch.autograd.grad(loss.sum(), z)[0]
+
+    loss, grad = run(z, t)
+    assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+    others = torch.arange(N).cuda() != 3
+    nan, inf = float("nan"), float("inf")
+    cases = [(z, (3, 0), nan), (z, (3, V - 1), nan), (z, (3, V // 2), inf), (z, 3, -inf), (t, (3, 2), nan), (t, (3, 2), inf), (t, 3, nan),
+             (t, 3, -inf)]
+    for of, at, what in cases:
+        zz, tt = z.clone(), t.clone()
+        (tt if of is t else zz)[at] = what
+        l, d = run(zz, tt)
+        assert not torch.isfinite(l[3])
+        assert not torch.isfinite(d[3]).all()
+        assert torch.equal(l[others], loss[others]) and torch.equal(d[others], grad[others])
 
 
 @pytest.mark.gpu
