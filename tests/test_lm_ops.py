@@ -964,6 +964,69 @@ def test_distill_empty_and_nothing_counts():
         torch.autograd.grad(o.distill_loss(z, torch.zeros(3, 2, dtype=torch.int64).cuda(), torch.zeros(3, 2).cuda()), z, create_graph=True)
 
 
+
+
+def distill_rows(z, ids, t, y, tau, hard):
+    """The rows' losses in 64 bits, many rows at once; y within the vocabulary, a valid teacher entry in every row."""
+    ok = (ids >= 0) & (ids < z.size(1))
+    p = torch.where(ok, torch.softmax(torch.where(ok, t.double() / tau, -1e300), 1), 0.0)
+    lq = torch.log_softmax(z / tau, 1).gather(1, ids.clamp(min=0))
+    soft = (torch.special.xlogy(p, p) - torch.where(ok, p * lq, 0.0)).sum(1)
+    return (1 - hard) * tau * tau * soft - hard * torch.log_softmax(z, 1).gather(1, y[:, None])[:, 0]
+
+
+def check_distill_rows(z, ids, t, y, tau, hard=0.3):
+    o = ops()
+    z = z.detach().requires_grad_()
+    loss = o.distill_loss(z, ids, t, y, temperature=tau, hard_weight=hard, reduction="none")
+    (dz,) = torch.autograd.grad(loss, z, torch.full_like(loss, 64.0))
+    r = z.detach().double().requires_grad_()
+    want = distill_rows(r, ids, t, y, tau, hard)
+    (dwant,) = torch.autograd.grad(want, r, torch.full_like(want, 64.0))
+    assert float((loss.double() - want).abs().max()) <= 2e-6 * (1 + float(want.abs().max()))
+    floor = 2.0 ** -25 * dz.numel() ** 0.5 / float(dwant.norm()) if z.dtype == torch.float16 else 0.0
+    assert ref.rel(dz, dwant) <= ref.half_step(z.dtype) + 64 * E + floor
+
+
+# V of less than a block's threads, of a row for several blocks, and rows that stream
+DISTILL_RANGES = [(3, 301), (6, 30011), (200, 20003)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("N, V", DISTILL_RANGES)
+@pytest.mark.parametrize("tau", [1.0, 2.0, 3.0, 0.5])
+def test_distill_does_not_depend_on_what_rows_have_in_common(dtype, N, V, tau):
+    """Logits and teachers' logits around -100, -1e4, 1e4: both are differences from the row's reference before anything is
+    rounded (exact where they lie within a factor of two), so the bounds are those of logits around 0."""
+    g = gen(N + V)
+    z, t = randn(g, N, V, by=2.0), randn(g, N, 7, by=1.5)
+    ids, y = torch.randint(0, V, (N, 7), generator=g).cuda(), torch.randint(0, V, (N,), generator=g).cuda()
+    for shift in (-50.0, -100.0, -200.0, -1e4, 300.0, 1e4):
+        check_distill_rows((z + shift).to(dtype), ids, t + shift, y, tau)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("N, V", DISTILL_RANGES)
+@pytest.mark.parametrize("tau", [1.0, 2.0, 3.0, 0.5])
+def test_distill_over_a_masked_vocabulary(dtype, N, V, tau):
+    """A third of the vocabulary at -1e4 or at the type's lowest value, at the row's start, middle or end, and a row of nothing
+    else (equal logits: log V)."""
+    g = gen(N + V + 1)
+    z, t = randn(g, N, V, dtype=dtype, by=2.0), randn(g, N, 7, by=1.5)
+    for fill in (-1e4, torch.finfo(dtype).min):
+        for lo, hi in ((0, V // 3), (V // 3, 2 * V // 3), (2 * V // 3, V)):
+            x = z.clone()
+            x[:, lo:hi] = fill
+            ids, y = (torch.randint(0, V - hi + lo, s, generator=g).cuda() for s in ((N, 7), (N,)))
+            ids, y = (torch.where(i < lo, i, i + hi - lo) for i in (ids, y))  # outside the masked third
+            check_distill_rows(x, ids, t, y, tau)
+            if lo:
+                x[1] = fill
+                check_distill_rows(x, ids, t, y, tau)
+
+
 # ------------------------------------------------- streams, graphs, together
 
 
