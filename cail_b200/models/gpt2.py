@@ -124,6 +124,12 @@ class GPT2(nn.Module):
         for blk in self.blocks:
             for lin in (blk.proj, blk.out):
                 nn.init.normal_(lin.weight, std=0.02 / math.sqrt(2 * c.n_layer))
+        self._plan(self.wte.weight.device)
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        self._plan(self.wte.weight.device)  # here, as a first call may be under capture, where nothing is copied from the host
+        return self
 
     @staticmethod
     def _init(m: nn.Module) -> None:
@@ -134,7 +140,7 @@ class GPT2(nn.Module):
             nn.init.normal_(m.weight, std=0.02)
 
     def _plan(self, device: torch.device) -> Optional[ops.Rotary]:
-        """The rotary frequencies on ``device`` (made once per device)."""
+        """The rotary frequencies on ``device``, made once per device: when the model is built or moved."""
         c = self.c
         if c.rotary == 0:
             return None

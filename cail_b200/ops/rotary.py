@@ -59,13 +59,15 @@ class Rotary:
         self.dim = dim
         self.interleaved = bool(interleaved)
         self.amplitude = 1.0 if amplitude is None else float(amplitude)
-        self.turns = torch.tensor([x / (2 * math.pi) for x in f], dtype=torch.float64, device=device)
+        with torch.inference_mode(False):  # a plan outlives the call that made it, and training keeps it for the backward pass
+            self.turns = torch.tensor([x / (2 * math.pi) for x in f], dtype=torch.float64, device=device)
 
     def to(self, device: Union[str, torch.device]) -> "Rotary":
         """The same plan on another device."""
         other = object.__new__(Rotary)
         other.__dict__.update(self.__dict__)
-        other.turns = self.turns.to(device)
+        with torch.inference_mode(False):
+            other.turns = self.turns.to(device)
         return other
 
 

@@ -53,6 +53,20 @@ def test_refusals_on_cpu():
     assert GPT2(config(rotary=8)).new_cache(1, 500).length == 500
 
 
+def test_rotary_plans_belong_to_no_mode():
+    """A plan made under inference_mode serves training; a model's plan is there once it is built or moved."""
+    from cail_b200 import ops
+
+    m = GPT2(config(rotary=8))
+    assert set(m._plans) == {torch.device("cpu")}
+    m.to("meta")
+    assert set(m._plans) == {torch.device("cpu"), torch.device("meta")}
+    with torch.inference_mode():
+        plans = [ops.Rotary(8, device="cpu"), ops.Rotary(8, device="cpu").to("meta"), GPT2(config(rotary=8))._plan(torch.device("cpu"))]
+    assert not any(p.turns.is_inference() for p in plans)
+    assert "_plans" not in GPT2(config()).__dict__
+
+
 def plain_logits(m, idx, lengths=None):
     """The model in 64 bits, from its parameters, by the operators' plain forms."""
     c, p = m.c, {n: q.detach().double().requires_grad_() for n, q in m.named_parameters()}
@@ -191,6 +205,36 @@ def test_captured_decode(rotary):
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a[:, :29], b[:, :29]) for a, b in zip(cache.k, eager.k))
+
+
+@pytest.mark.gpu
+def test_training_after_inference_mode():
+    """The same gradients whether or not the model's first call was under inference_mode, and a first call under capture."""
+    torch.manual_seed(10)
+    m = GPT2(config(rotary=16, window=9)).cuda()
+    idx = torch.randint(0, 512, (2, 50)).cuda()
+    m(idx, idx).backward()
+    want = [p.grad.clone() for p in m.parameters()]
+    again = GPT2(m.c).cuda()
+    again.load_state_dict(m.state_dict())
+    with torch.inference_mode():
+        again(idx)
+        cache = again.new_cache(2)
+        again.decode(again.prefill(idx, cache).argmax(-1), cache)
+    again(idx, idx).backward()
+    for p, w in zip(again.parameters(), want):
+        assert ref.rel(p.grad, w) <= 64 * E  # torch's own sums may come in another order
+    from cail_b200 import ops
+
+    fresh = GPT2(m.c).cuda()
+    q = torch.randn(1, 7, 2, 16, device="cuda")
+    ops.rotary(q, None, m._plan(q.device))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.rotary(q, None, fresh._plan(q.device))
+    graph.replay()
+    assert torch.equal(out, ops.rotary(q, None, m._plan(q.device)))
 
 
 @pytest.mark.gpu
