@@ -167,12 +167,17 @@ class GPT2(nn.Module):
         ``teacher`` (ids and logits, [B, T, K]) the distillation loss, in which the
         cross entropy against ``targets`` has the weight ``hard_weight``
         (cail_b200.ops.distill_loss).  ``lengths`` (int32 [B]) are the sequences'
-        lengths in a padded batch: pad ``targets`` with -100."""
+        lengths in a padded batch: pad ``targets`` with -100.  With a teacher and
+        no targets, the positions behind a length are left out of the loss."""
         logits = F.linear(self.ln_f(self._trunk(idx, lengths, None)), self.wte.weight)
         if teacher is not None:
             ids, top = (z.reshape(-1, z.size(-1)) for z in teacher)
-            return ops.distill_loss(logits.view(-1, logits.size(-1)), ids, top, None if targets is None else targets.view(-1),
-                                    temperature=temperature, hard_weight=0.0 if targets is None else hard_weight)
+            if targets is None:
+                hard_weight = 0.0  # targets then only say which positions count
+                if lengths is not None:
+                    targets = torch.where(torch.arange(idx.size(1), device=idx.device) < lengths[:, None], 0, -100)
+            return ops.distill_loss(logits.view(-1, logits.size(-1)), ids, top, None if targets is None else targets.reshape(-1),
+                                    temperature=temperature, hard_weight=hard_weight)
         if targets is None:
             return logits
         return F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))

@@ -141,6 +141,33 @@ def test_padded_batch_and_distillation_match_64_bit():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[50, 31, 1], [0, 7, 50], None], ids=str)
+def test_distillation_without_targets_leaves_padding_out(lengths):
+    """The teacher alone over a padded batch: the mean is over the sequences' tokens, whatever lies behind them."""
+    torch.manual_seed(3)
+    m = GPT2(config(window=11, sinks=3, rotary=16)).cuda()
+    g = torch.Generator().manual_seed(5)
+    idx = torch.randint(0, 512, (3, 50), generator=g).cuda()
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32).cuda()
+    ids = torch.randint(0, 512, (3, 50, 6), generator=g).cuda()
+    top = torch.randn(3, 50, 6, generator=g).cuda()
+    got = m(idx, teacher=(ids, top), temperature=2.0, hard_weight=0.7, lengths=n)
+    got.backward()
+    want, p = plain_logits(m, idx, n)
+    rows = torch.cat([torch.arange(50) + 50 * b for b in range(3)] if n is None else [torch.arange(k) + 50 * b for b, k in enumerate(lengths)]).cuda()
+    wloss = ref.distill(want.flatten(0, 1)[rows], ids.flatten(0, 1)[rows], top.flatten(0, 1)[rows], None, 2.0, 0.0)
+    wloss.backward()
+    assert abs(float(got.detach()) - float(wloss.detach())) <= 512 * E * float(wloss.detach())
+    for name, q in m.named_parameters():
+        if not name.endswith("qkv.bias"):
+            assert ref.rel(q.grad, p[name].grad) <= 4096 * E, name
+    if n is not None:  # what the padding holds is nothing to the loss
+        for b, k in enumerate(lengths):
+            idx[b, k:], ids[b, k:], top[b, k:] = 3, 5, float("nan")
+        assert torch.equal(m(idx, teacher=(ids, top), temperature=2.0, lengths=n), got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kw", [dict()] + OPTIONS, ids=str)
 def test_prefill_and_decode_follow_forward(kw):
     """Prompts of unequal length, then tokens one by one: the logits of the
