@@ -16,7 +16,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // ------------------------------------------------------------------- host
 int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 int launched(const char *what);  // after a launch: counts it, reports a launch error
-int sm_count();                  // of the current device (0: no device)
+int sm_count();                  // of the current device; a B200's where none answers (sizes may be asked for without one)
 int earlier_error(const char *who);  // fails, once, when a kernel of an earlier call on the current device gave up a wait
 int *device_error_flag();        // device address of the current device's error word (nullptr: none could be made)
 

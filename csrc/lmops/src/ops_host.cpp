@@ -14,6 +14,7 @@ namespace {
 thread_local char t_error[512] = "";
 std::atomic<unsigned long long> g_launches{0};
 constexpr int kMaxDevices = 64;
+constexpr int kSms = 148;  // of a B200
 std::atomic<int> g_sms[kMaxDevices];
 std::mutex g_flag_mutex;
 std::atomic<int *> g_flag_host[kMaxDevices];
@@ -36,13 +37,19 @@ int launched(const char *what) {
 }
 
 int sm_count() {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-    int n = g_sms[dev].load(std::memory_order_relaxed);
-    if (n == 0) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        g_sms[dev].store(n, std::memory_order_relaxed);
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return kSms;
     }
+    const bool kept = dev >= 0 && dev < kMaxDevices;
+    if (kept) n = g_sms[dev].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        return kSms;
+    }
+    if (kept) g_sms[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 

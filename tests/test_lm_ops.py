@@ -193,6 +193,43 @@ def test_c_entries_refuse_without_touching_a_device():
         assert lib.cail_ops_last_error() != b""
 
 
+def attention_args(T, window, sinks, dtype, B=1, H=1, Hkv=1, D=64):
+    """cail_ops_attention_args of contiguous arrays at made-up addresses, for questions that touch no device."""
+    import ctypes as c
+
+    class Bthd(c.Structure):
+        _fields_ = [("ptr", c.c_void_p), ("sb", c.c_int64), ("st", c.c_int64), ("sh", c.c_int64)]
+
+    class Args(c.Structure):
+        _fields_ = ([(n, c.c_int) for n in ("type", "B", "T", "H", "Hkv", "D", "window", "sinks")] + [("scale", c.c_float), ("lengths", c.c_void_p)] +
+                    [(n, Bthd) for n in "qkvo"] + [("lse", c.c_void_p), ("o_rest", Bthd), ("rest_rows", c.c_int)] +
+                    [(n, Bthd) for n in ("dout", "dq", "dk", "dv")] + [("delta", c.c_void_p), ("workspace", c.c_void_p), ("workspace_bytes", c.c_size_t)])
+
+    a = Args(TYPES.index(dtype), B, T, H, Hkv, D, window, sinks, 0.125, None)
+    at = lambda h, n=T: Bthd(1 << 20, n * h * D, h * D, D)  # noqa: E731
+    a.q = a.o = a.dout = a.dq = at(H)
+    a.k = a.v = a.dk = a.dv = at(Hkv)
+    a.lse = a.delta = 1 << 20
+    a.rest_rows = min(T, 128)
+    a.o_rest = at(H, a.rest_rows)
+    return a
+
+
+def test_a_workspace_can_be_asked_for_without_a_device():
+    """In a process of its own: a division by the number of a missing device's SMs would end it."""
+    import os
+    import subprocess
+    import sys
+
+    code = ("import ctypes, sys; sys.path[:0] = ['tests', '.']; import torch, test_lm_ops as t; from conftest import LIB\n"
+            "lib = ctypes.CDLL(LIB + '/libcail_ops.so'); f = lib.cail_ops_window_attention_workspace; f.restype = ctypes.c_size_t\n"
+            "print([f(ctypes.byref(t.attention_args(T, 20, 4, d))) for d in t.TYPES for T in (500, 100000)])")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       env={**os.environ, "CUDA_VISIBLE_DEVICES": ""})
+    assert r.returncode == 0, r.stderr[-500:]
+    assert all(n > 0 for n in eval(r.stdout.splitlines()[-1])[1::2])
+
+
 # -------------------------------------------------------------------- rotary
 
 SCALINGS = [dict(), dict(scaling="linear", factor=8.0), dict(scaling="ntk", factor=4.0), dict(scaling="parts", factor=16.0, original=2048)]
