@@ -522,7 +522,7 @@ SinkParts sink_parts(const cail_ops_attention_args *c, int rows, int stream, int
     const int64_t share = all / slots > plain ? all / slots : plain;
     int64_t splits = (sunk + share - 1) / share;
     if (splits > 32) splits = 32;
-    if (tiles < kMostTiles && splits > 1 + (kMostTiles - tiles) / sink_tiles) splits = 1 + (kMostTiles - tiles) / sink_tiles;
+    if (tiles <= kMostTiles && splits > 1 + (kMostTiles - tiles) / sink_tiles) splits = 1 + (kMostTiles - tiles) / sink_tiles;
     if (splits <= 1) return none;
     return {(int)splits, (int)sink_tiles, nullptr};
 }

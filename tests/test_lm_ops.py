@@ -215,6 +215,26 @@ def attention_args(T, window, sinks, dtype, B=1, H=1, Hkv=1, D=64):
     return a
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=ids_of)
+@pytest.mark.parametrize("T", [65533 * 128, 65534 * 128, 65534 * 128 + 1, 65535 * 128])
+@pytest.mark.parametrize("sinks", [4, 128, 129, 1000])
+def test_parts_of_the_sinks_stay_inside_a_grid(dtype, T, sinks):
+    """The tensor-core kernels' grid has one block in z for every tile of 128 keys, and more where the sinks' tiles are cut into
+    parts (as many as the workspace has room for): at most 65535 in all."""
+    import ctypes
+    import os
+
+    from conftest import LIB
+
+    lib = ctypes.CDLL(os.path.join(LIB, "libcail_ops.so"))
+    lib.cail_ops_window_attention_workspace.restype = ctypes.c_size_t
+    room = [lib.cail_ops_window_attention_workspace(ctypes.byref(attention_args(T, 20, n, dtype))) for n in (sinks, 0)]
+    tiles, sunk, part = (T + 127) // 128, (sinks + 127) // 128, 2 * 128 * 64 * 4
+    assert (room[0] - room[1]) % (sunk * part) == 0
+    parts = (room[0] - room[1]) // (sunk * part)
+    assert tiles + sunk * max(parts - 1, 0) <= 65535
+
+
 def test_a_workspace_can_be_asked_for_without_a_device():
     """In a process of its own: a division by the number of a missing device's SMs would end it."""
     import os
