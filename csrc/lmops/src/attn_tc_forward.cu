@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::per_sm) tc_forward_kernel
                 copy(sq + from, a.o + b * a.ob + (int64_t)(i0 + r) * a.ot + h * a.oh);
                 if (i0 + r < a.rest_rows) copy(sk + from, a.rest + b * a.rb + (int64_t)(i0 + r) * a.rt + h * a.rh);
             }
-            if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = live && l > 0.f ? fmaf(m, a.scale_log2, log2f(l)) : 0.f;
+            if (a.lse && i < a.T) a.lse[((int64_t)b * a.H + h) * a.lse_row + i] = live && l != 0.f ? fmaf(m, a.scale_log2, log2f(l)) : 0.f;  // NaN stays
         } else if (lane == 0) {
             report(a.error);
         }

@@ -508,6 +508,30 @@ def test_what_is_not_finite_is_not_hidden(dtype, what):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+@pytest.mark.parametrize("T, D", [(40, 64), (200, 64), (200, 128), (300, 72)])
+def test_gradients_of_rows_that_are_not_finite(dtype, what, T, D):
+    """A key or a query that is not finite makes NaN of the rows that meet it, and of the values' gradients of all keys that
+    those rows see (p is NaN there): of those and of no others."""
+    o = ops()
+    window = 8
+    for bad in "kq":
+        q, k, v, do, _ = attention_inputs((1, T, 1, 1, D, window, 0, None), dtype)
+        {"q": q, "k": k}[bad][0, 10] = what
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        out = o.window_attention(*leaves, window)
+        dq, dk, dv = torch.autograd.grad(out, leaves, do)
+        rows = range(10, 11) if bad == "q" else range(10, 10 + window)
+        assert torch.isnan(out[0, rows]).all() and int(torch.isfinite(out[0, :, 0, 0]).sum()) == T - len(rows)
+        assert torch.isnan(dq[0, rows]).all()
+        keys = sorted({j for i in rows for j in range(i - window + 1, i + 1)})
+        assert not torch.isfinite(dv[0, keys]).any() and not torch.isfinite(dk[0, keys]).any()
+        others = [j for j in range(T) if j not in keys]
+        assert torch.isfinite(dv[0, others]).all()
+
+
+@pytest.mark.gpu
 def test_the_first_cuda_call_of_a_thread():
     """A thread in which no context is current yet: the tile loads' descriptors need one."""
     o = ops()
