@@ -11,10 +11,12 @@
 #include <dlfcn.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "../lmops/include/cail_ops.h"
 
@@ -239,6 +241,30 @@ std::vector<Tensor> rotary(const Tensor &q, const std::optional<Tensor> &k_, con
     return wants_grad({&q, &k}) ? RotaryFn::apply(q, k_, w.turns, positions_, part, interleaved, false, amplitude) : rotary_out(q, k, w);
 }
 
+// Whether an element of t lies `off` elements behind its first, the dimension `skip` aside: the largest strides first, which
+// is exact for slices of one tensor (no inner part longer than an outer stride); what it finds is there in any case.
+bool reaches(const Tensor &t, int64_t off, int64_t skip = -1) {
+    std::vector<int64_t> dims;
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (i != skip && t.size(i) > 1 && t.stride(i) > 0) dims.push_back(i);
+    std::sort(dims.begin(), dims.end(), [&](int64_t a, int64_t b) { return t.stride(a) > t.stride(b); });
+    for (int64_t i : dims) off -= std::min(off / t.stride(i), t.size(i) - 1) * t.stride(i);
+    return off == 0;
+}
+bool overlaps_itself(const Tensor &t) {
+    if (at::has_internal_overlap(t) == at::MemOverlap::Yes) return true;
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1 && reaches(t, t.stride(i), i)) return true;
+    return false;
+}
+bool overlap(const Tensor &a, const Tensor &b) {
+    const auto s = at::get_overlap_status(a, b);
+    if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial) return true;
+    if (s == at::MemOverlapStatus::No || !a.is_alias_of(b)) return false;
+    const int64_t off = b.storage_offset() - a.storage_offset();
+    return off < 0 ? reaches(b, -off) : reaches(a, off);
+}
+
 void rotary_inplace(const Tensor &q, const std::optional<Tensor> &k_, const Tensor &turns, const std::optional<Tensor> &positions_,
                     int64_t part, bool interleaved, double amplitude) {
     const Tensor k = or_none(k_);
@@ -246,7 +272,7 @@ void rotary_inplace(const Tensor &q, const std::optional<Tensor> &k_, const Tens
     VALUE_CHECK(!wants_grad({&q, &k}), "rotary_: in place on a tensor that requires a gradient; use rotary()");
     auto check = [](const Tensor &t) {
         VALUE_CHECK(t.size(-1) == 1 || t.stride(-1) == 1, "rotary_: the elements of a head must lie side by side");
-        VALUE_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, "rotary_: heads of one tensor share memory");
+        VALUE_CHECK(!overlaps_itself(t), "rotary_: heads of one tensor share memory");
     };
     plain("rotary_", {&q, &k});
     VALUE_CHECK(q.dim() == 4, "rotary_: q must be [B, T, H, D], got ", q.sizes());
@@ -254,8 +280,7 @@ void rotary_inplace(const Tensor &q, const std::optional<Tensor> &k_, const Tens
     if (k.defined()) {
         VALUE_CHECK(k.dim() == 4, "rotary_: k must be [B, T, Hk, D], got ", k.sizes());
         check(k);
-        const auto s = at::get_overlap_status(q, k);
-        VALUE_CHECK(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial, "rotary_: q and k share memory");
+        VALUE_CHECK(!overlap(q, k), "rotary_: q and k share memory");
     }
     rotary_check("rotary_", q, k, w);
     // first, as it refuses inference tensors outside inference mode

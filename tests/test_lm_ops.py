@@ -96,6 +96,28 @@ def test_rotary_refuses():
         o.rotary_(torch.zeros(2, 3, 8, 4).transpose(2, 3), None, plan)
 
 
+def test_rotary_in_place_refuses_slices_that_overlap():
+    """Slices of one projection: what overlaps is refused, what does not goes on (to the next check: the device)."""
+    o = ops()
+    plan = o.Rotary(8, device="cpu")
+    x = torch.zeros(2, 3, 6, 8)
+    wide = torch.zeros(2, 3, 2, 20)
+    for q, k in ((x[:, :, :4], x[:, :, :4]), (x[:, :, :4], x[:, :, 2:6]), (x[:, :, 2:6], x[:, :, 1:3]), (x[:, :, ::2], x[:, :, :3]),
+                 (wide[..., :8], wide[..., 7:15]), (wide[..., 4:12], wide[..., :8]), (x[:, :, 5:], x[:, :, 3:])):
+        with pytest.raises(ValueError, match="share memory"):
+            o.rotary_(q, k, plan)
+    for t in (torch.zeros(100).as_strided((1, 6, 1, 8), (1, 4, 1, 1)), torch.zeros(400).as_strided((2, 3, 2, 8), (8, 16, 8, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            o.rotary_(t, None, plan)
+    flat = torch.zeros(2, 3, 6 * 8)
+    views = [z.view(2, 3, 2, 8) for z in flat.split(16, dim=2)]
+    for q, k in ((x[:, :, :4], x[:, :, 4:]), (x[:, :, ::2], x[:, :, 1::2]), (wide[..., :8], wide[..., 8:16]), (views[0], views[1]),
+                 (views[2], views[0]), (x[:1], x[1:]), (x[:, :1], x[:, 1:2]), (x[:, :, :0], x), (x.transpose(0, 1), None),
+                 (torch.zeros(2, 3, 1, 8)[:, :, :1], None), (torch.zeros(1, 1, 1, 8), None)):
+        with pytest.raises(ValueError, match="CUDA"):
+            o.rotary_(q, k, plan)
+
+
 def test_window_attention_refuses():
     o = ops()
     q, k = torch.zeros(2, 5, 4, 8), torch.zeros(2, 5, 2, 8)
