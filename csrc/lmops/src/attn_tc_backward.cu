@@ -17,8 +17,8 @@
 //
 // p and ds are rounded to the input type for their products, all else is
 // 32-bit.  fp16 has no range for small gradients: ds is scaled by a power of
-// two taken from max |do| (of the row for dq; of the rows gone over for dk), taken
-// back out of the sums.
+// two taken from max |do| (of the row for dq; of the rows that see the key for
+// dk), taken back out of the sums.
 //
 // D = 64: two blocks per SM, S of the next tile computed under this one's
 // softmax (dq: dP too); 8 x 1024 tokens, 16 heads, window 256 and 4 sinks: dq
@@ -61,8 +61,7 @@ struct Maps {
 };
 
 struct Extra {
-    unsigned *amax;       // [B, Hkv, tiles of 128 rows] bits of max |do| (fp16)
-    int tiles;
+    unsigned *amax;       // [B, Hkv, T] bits of max |do| of a row, over the group's heads (fp16)
     SinkParts parts;
 };
 
@@ -70,6 +69,40 @@ struct Extra {
 __device__ __forceinline__ float amp_of(unsigned bits) {
     const int e = min(max((int)(bits >> 23) - 127, -30), 30);
     return bits == 0 ? 1.f : __uint_as_float((unsigned)(125 - e) << 23);
+}
+
+// The largest of a value per query row (bits of floats of no sign, a sequence's
+// n of them) over the rows that see key j0 + k, k < 128: for k = tid & 127 of
+// kMath threads.  With w the window, those are the rows from the key's own to
+// w - 1 behind it: 256 values side by side, the tile's own rows and the 128
+// that begin max(w, 128) behind its first, over which a maximum of min(w, 128)
+// slides (by doubling), and between the two what all of these keys meet.  A sink is seen by
+// every row behind it.
+__device__ __forceinline__ unsigned largest_met(const unsigned *values, int j0, int n, int window, int sinks, unsigned (*buf)[kMath], unsigned *shared) {
+    const int tid = threadIdx.x, k = tid & 127, w = min(window, n), width = min(w, 128), far = max(w, 128);
+    const int at = j0 + k + (tid < 128 ? 0 : far);
+    unsigned x = at < n ? values[at] : 0u, common = 0u, behind = 0u;
+    buf[0][tid] = x;
+    for (int i = j0 + 128 + tid; i < min(j0 + w, n); i += kMath) common = max(common, values[i]);
+    if (j0 < sinks)
+        for (int i = j0 + 128 + tid; i < n; i += kMath) behind = max(behind, values[i]);
+    common = __reduce_max_sync(0xffffffffu, common), behind = __reduce_max_sync(0xffffffffu, behind);
+    if ((tid & 31) == 0) shared[tid >> 5] = common, shared[kMath / 32 + (tid >> 5)] = behind;
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kMath) : "memory"); };
+    meet();
+    int now = 0, wide = 1;
+    for (; wide * 2 <= width; wide *= 2) {
+        x = max(x, tid + wide < kMath ? buf[now][tid + wide] : 0u);
+        now ^= 1;
+        buf[now][tid] = x;
+        meet();
+    }
+    unsigned top = max(buf[now][k], buf[now][k + width - wide]);
+    const bool sink = j0 + k < sinks;
+    for (int i = 0; i < kMath / 32; ++i) top = max(top, max(shared[i], sink ? shared[kMath / 32 + i] : 0u));
+    if (sink)
+        for (int i = j0 + k; i < min(j0 + 128, n); ++i) top = max(top, values[i]);
+    return top;
 }
 
 template <typename T, int DP, bool DKV>
@@ -81,6 +114,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     extern __shared__ char raw[];
     __shared__ __align__(8) uint64_t bars[S::barriers];
     __shared__ uint32_t tmem_at;
+    [[maybe_unused]] __shared__ unsigned met[bf || !DKV ? 1 : 2][bf || !DKV ? 1 : kMath], met_all[bf || !DKV ? 1 : 2 * kMath / 32];
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
     const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + S::u_bytes;  // U and W of a stage side by side
     constexpr uint32_t stage_bytes = 2 * S::u_bytes;
@@ -325,16 +359,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 if (lane == 0) mbar_arrive(rest_read);
                 if (!bf) {
                     amp = amp_of(__float_as_uint(top));
-                    top = warp_max(top);
-                    if (half == 0 && lane == 0 && top > 0.f) atomicMax(ex.amax + ((int64_t)b * a.Hkv + hk) * ex.tiles + r0 / kRows, __float_as_uint(top));
+                    if (half == 0 && top > 0.f) atomicMax(ex.amax + ((int64_t)b * a.Hkv + hk) * a.T + r, __float_as_uint(top));
                 }
             }
-        } else if (!bf) {
-            // the largest gradient of the rows that this block goes over
-            unsigned top = 0;
-            for (int t = q_begin * kStream / kRows + lane; t <= ((q_begin + q_tiles) * kStream - 1) / kRows; t += 32)
-                top = max(top, ex.amax[((int64_t)b * a.Hkv + hk) * ex.tiles + t]);
-            amp = amp_of(__reduce_max_sync(0xffffffffu, top));
+        } else if constexpr (!bf) {
+            // a scale for every key, from the rows that see it and from no others
+            amp = amp_of(largest_met(ex.amax + ((int64_t)b * a.Hkv + hk) * a.T, r0, n, a.window, a.sinks, met, met_all));
         }
         const float delta_amp = delta * amp;
         for (; walk.x < count; step(walk)) {
@@ -511,7 +541,7 @@ struct Layout {
 Layout layout_of(const cail_ops_attention_args *c) {
     Layout l = {};
     l.parts = sink_parts(c, kRows, kStream, (int64_t)sm_count() * (c->D <= 64 ? 2 : 1));
-    l.sums = c->type == CAIL_OPS_F16 ? ((size_t)c->B * c->Hkv * ((c->T + kRows - 1) / kRows) * 4 + 255) / 256 * 256 : 0;
+    l.sums = c->type == CAIL_OPS_F16 ? ((size_t)c->B * c->Hkv * c->T * 4 + 255) / 256 * 256 : 0;
     l.total = l.sums + sink_bytes(c, l.parts, kRows, c->D <= 64 ? 64 : 128);
     return l;
 }
@@ -521,12 +551,11 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     if (c->workspace_bytes < l.total || (l.total && (!c->workspace || !aligned(c->workspace, 16))))
         return fail(CAIL_OPS_EINVAL, "window attention backward: a workspace of %zu bytes is needed", l.total);
     Extra ex = {};
-    ex.tiles = (a.T + kRows - 1) / kRows;
     ex.amax = reinterpret_cast<unsigned *>(static_cast<char *>(c->workspace) + l.amax);
     ex.parts = l.parts;
     ex.parts.sums = reinterpret_cast<float *>(static_cast<char *>(c->workspace) + l.sums);
     if (c->type == CAIL_OPS_F16) {
-        cudaError_t e = cudaMemsetAsync(ex.amax, 0, (size_t)a.B * a.Hkv * ex.tiles * 4, st);
+        cudaError_t e = cudaMemsetAsync(ex.amax, 0, (size_t)a.B * a.Hkv * a.T * 4, st);
         if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
     }
     // the same arrays with boxes of 128 and of 64 rows

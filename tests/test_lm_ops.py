@@ -505,6 +505,31 @@ def test_a_large_gradient_costs_others_no_bits(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("window, sinks, row", [(20, 4, 400), (20, 0, 200), (20, 0, 130), (20, 0, 128), (128, 130, 300), (129, 1, 300), (200, 0, 383),
+                                                (200, 7, 699), (300, 3, 450), (1, 2, 257), (600, 0, 650)])
+@pytest.mark.parametrize("D, group", [(64, 1), (128, 2), (72, 2)])
+def test_a_large_gradient_costs_keys_that_it_does_not_meet_no_bits(dtype, window, sinks, row, D, group):
+    """Gradients of 1e-3 beside one row of 3e4: dk and dv of every key that the row does not see, and dq of every other row, to
+    the bounds of a call without it.  float16 results are held to 2^-24 absolute: 2^-25 / rms more, as below."""
+    o = ops()
+    T = 700
+    q, k, v, do, _ = attention_inputs((1, T, group, 1, D, window, sinks, None), dtype)
+    do = do * 1e-3
+    do[0, row, 0] = 3e4
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(o.window_attention(*leaves, window, sinks), leaves, do)
+    r = [x.detach().double().requires_grad_() for x in leaves]
+    dwant = torch.autograd.grad(ref.attention(*r, window, sinks), r, do.double())
+    meets = ref.seen_mask(T, T, window, sinks)[row]
+    rest = torch.arange(T) != row
+    for name, at, got, want in zip("qkv", (rest, ~meets, ~meets), grads, dwant):
+        got, want = got[0, at.cuda()].double(), want[0, at.cuda()]
+        floor = 2.0 ** -25 / float(want.square().mean().sqrt()) if dtype == torch.float16 and want.any() else 0.0
+        assert ref.rel(got, want) <= 5 * ref.half_step(dtype) + 256 * E + floor, "d" + name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 @pytest.mark.parametrize("what", [float("inf"), float("nan")])
 def test_what_is_not_finite_is_not_hidden(dtype, what):
     """A query, or a key that rows see, that is not finite: NaN in those rows, on every path, and no others of the head's tiles."""
@@ -1065,8 +1090,6 @@ def test_distill_empty_and_nothing_counts():
     assert float(loss) == 0.0 and not torch.autograd.grad(loss, z)[0].any()
     with pytest.raises(NotImplementedError):
         torch.autograd.grad(o.distill_loss(z, torch.zeros(3, 2, dtype=torch.int64).cuda(), torch.zeros(3, 2).cuda()), z, create_graph=True)
-
-
 
 
 def distill_rows(z, ids, t, y, tau, hard):
