@@ -16,9 +16,14 @@
 // parts joined in order by a third kernel.
 //
 // p and ds are rounded to the input type for their products, all else is
-// 32-bit.  fp16 has no range for small gradients: ds is scaled by a power of
-// two taken from max |do| (of the row for dq; of the rows that see the key for
-// dk), taken back out of the sums.
+// 32-bit.  fp16 has no range for small gradients, nor for large ones: ds is
+// scaled by a power of two, taken back out of the sums.  It comes from a bound
+// of |ds| for each row, 2 sum |do| max |v| over the keys that the row sees
+// (|ds| <= |do.v| + |do.o|), brought to [2^14, 2^15): the row's own for dq, the
+// largest of the rows that see the key for dk.  So nothing overflows, and no
+// row or key loses bits to one that it does not meet.  A small kernel goes over
+// v for it first (8 x 1024 tokens, 16 heads of 64, window 256, forward and
+// backward: 152 us, and 145 with scales from max |do| alone).
 //
 // D = 64: two blocks per SM, S of the next tile computed under this one's
 // softmax (dq: dP too); 8 x 1024 tokens, 16 heads, window 256 and 4 sinks: dq
@@ -61,31 +66,39 @@ struct Maps {
 };
 
 struct Extra {
-    unsigned *amax;       // [B, Hkv, T] bits of max |do| of a row, over the group's heads (fp16)
+    // fp16: what ds can reach.  Bits of max |v| of a key, and of the largest |ds| that a row can have, over the group's
+    // heads: [B, Hkv, T] each.
+    unsigned *v_top, *reach;
     SinkParts parts;
 };
 
-// the power of two that brings a value whose largest is `bits` to [1/4, 1/2)
+// the power of two that brings a value whose largest is `bits` to [2^14, 2^15)
 __device__ __forceinline__ float amp_of(unsigned bits) {
-    const int e = min(max((int)(bits >> 23) - 127, -30), 30);
-    return bits == 0 ? 1.f : __uint_as_float((unsigned)(125 - e) << 23);
+    const int e = min(max((int)(bits >> 23) - 127, -100), 100);
+    return bits == 0 ? 1.f : __uint_as_float((unsigned)(127 + 14 - e) << 23);
 }
 
 // The largest of a value per query row (bits of floats of no sign, a sequence's
-// n of them) over the rows that see key j0 + k, k < 128: for k = tid & 127 of
-// kMath threads.  With w the window, those are the rows from the key's own to
-// w - 1 behind it: 256 values side by side, the tile's own rows and the 128
-// that begin max(w, 128) behind its first, over which a maximum of min(w, 128)
-// slides (by doubling), and between the two what all of these keys meet.  A sink is seen by
+// n of them) over the rows that see key r0 + k, k < 128, or (KEYS) of a value
+// per key over the keys that row r0 + k sees: for k = tid & 127 of kMath
+// threads.  With w the window, the rows that see a key are its own to w - 1
+// behind it: 256 values side by side, the tile's own rows and the 128 that
+// begin max(w, 128) behind its first, over which a maximum of min(w, 128)
+// slides (by doubling), and between the two what all 128 meet.  The keys that
+// a row sees are the same in mirror image, and the sinks; a sink is seen by
 // every row behind it.
-__device__ __forceinline__ unsigned largest_met(const unsigned *values, int j0, int n, int window, int sinks, unsigned (*buf)[kMath], unsigned *shared) {
+template <bool KEYS>
+__device__ __forceinline__ unsigned largest_met(const unsigned *values, int r0, int n, int window, int sinks, unsigned (*buf)[kMath], unsigned *shared) {
     const int tid = threadIdx.x, k = tid & 127, w = min(window, n), width = min(w, 128), far = max(w, 128);
-    const int at = j0 + k + (tid < 128 ? 0 : far);
-    unsigned x = at < n ? values[at] : 0u, common = 0u, behind = 0u;
+    const int at = r0 + k + (KEYS ? (tid < 128 ? -far : 0) : (tid < 128 ? 0 : far));
+    unsigned x = at >= 0 && at < n ? values[at] : 0u, common = 0u, behind = 0u;
     buf[0][tid] = x;
-    for (int i = j0 + 128 + tid; i < min(j0 + w, n); i += kMath) common = max(common, values[i]);
-    if (j0 < sinks)
-        for (int i = j0 + 128 + tid; i < n; i += kMath) behind = max(behind, values[i]);
+    const int from = KEYS ? max(r0 - w + 128, 0) : r0 + 128, to = KEYS ? r0 : min(r0 + w, n);
+    for (int i = from + tid; i < to; i += kMath) common = max(common, values[i]);
+    if (KEYS)
+        for (int i = tid; i < min(sinks, r0); i += kMath) common = max(common, values[i]);
+    if (!KEYS && r0 < sinks)
+        for (int i = r0 + 128 + tid; i < n; i += kMath) behind = max(behind, values[i]);
     common = __reduce_max_sync(0xffffffffu, common), behind = __reduce_max_sync(0xffffffffu, behind);
     if ((tid & 31) == 0) shared[tid >> 5] = common, shared[kMath / 32 + (tid >> 5)] = behind;
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kMath) : "memory"); };
@@ -97,12 +110,36 @@ __device__ __forceinline__ unsigned largest_met(const unsigned *values, int j0, 
         buf[now][tid] = x;
         meet();
     }
-    unsigned top = max(buf[now][k], buf[now][k + width - wide]);
-    const bool sink = j0 + k < sinks;
+    const int place = KEYS ? 129 + k - width : k;
+    unsigned top = max(buf[now][place], buf[now][place + width - wide]);
+    const bool sink = !KEYS && r0 + k < sinks;
     for (int i = 0; i < kMath / 32; ++i) top = max(top, max(shared[i], sink ? shared[kMath / 32 + i] : 0u));
     if (sink)
-        for (int i = j0 + k; i < min(j0 + 128, n); ++i) top = max(top, values[i]);
+        for (int i = r0 + k; i < min(r0 + 128, n); ++i) top = max(top, values[i]);
+    if (KEYS)
+        for (int i = r0; i < min(min(sinks, n), r0 + k + 1); ++i) top = max(top, values[i]);
     return top;
+}
+
+// fp16: max |v| of every key (what is not finite aside: the rows that see it are not finite either), and zeros for the rows' reach
+template <int DP> __global__ void __launch_bounds__(256) v_top_kernel(const AttnArgs a, const Extra ex) {
+    constexpr int LANES = DP / 8, ROWS = 256 / LANES;
+    const int hk = blockIdx.y, b = blockIdx.z, r = blockIdx.x * ROWS + threadIdx.x / LANES, c = threadIdx.x % LANES * 8;
+    float top = 0.f;
+    if (r < length_of(a, b) && c < a.D) {
+        const Vec<__half, 8> v = *reinterpret_cast<const Vec<__half, 8> *>(a.v + b * a.vb + (int64_t)r * a.vt + hk * a.vh + c * 2);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = fabsf(to_f(v.v[e]));
+            if (f < INFINITY) top = fmaxf(top, f);
+        }
+    }
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (c == 0 && r < a.T) {
+        const int64_t at = ((int64_t)b * a.Hkv + hk) * a.T + r;
+        ex.v_top[at] = __float_as_uint(top), ex.reach[at] = 0u;
+    }
 }
 
 template <typename T, int DP, bool DKV>
@@ -114,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
     extern __shared__ char raw[];
     __shared__ __align__(8) uint64_t bars[S::barriers];
     __shared__ uint32_t tmem_at;
-    [[maybe_unused]] __shared__ unsigned met[bf || !DKV ? 1 : 2][bf || !DKV ? 1 : kMath], met_all[bf || !DKV ? 1 : 2 * kMath / 32];
+    [[maybe_unused]] __shared__ unsigned met[bf ? 1 : 2][bf ? 1 : kMath], met_all[bf ? 1 : 2 * kMath / 32];
     const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
     const uint32_t sx = base, sy = sx + S::x_bytes, su = sy + S::x_bytes, sw = su + S::u_bytes;  // U and W of a stage side by side
     constexpr uint32_t stage_bytes = 2 * S::u_bytes;
@@ -327,9 +364,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
         if constexpr (!DKV) {
             const int64_t at = ((int64_t)b * a.H + h) * a.lse_row + r;
             if (r < n) lse = a.lse[at];  // on its way while do and o arrive
+            [[maybe_unused]] float v_met = 0.f;
+            if constexpr (!bf)
+                v_met = __uint_as_float(largest_met<true>(ex.v_top + ((int64_t)b * a.Hkv + hk) * a.T, r0, n, a.window, a.sinks, met, met_all));
             ok = warp_wait(x_full, 0);
             if (ok) {
-                float top = 0.f;
+                float size = 0.f;  // sum |do|
                 if (r < n) {
 #pragma unroll
                     for (int c = 0; c < DP / 8; ++c) {
@@ -350,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                         for (int e = 0; e < 8; ++e) {
                             const float f = to_f(g.v[e]);
                             delta = fmaf(to_f(o.v[e]) + to_f(rest.v[e]), f, delta);
-                            if (!bf) top = fmaxf(top, fabsf(f) < INFINITY ? fabsf(f) : 0.f);  // an infinite gradient scales no other
+                            if (!bf) size += fabsf(f) < INFINITY ? fabsf(f) : 0.f;  // an infinite gradient scales no other
                         }
                     }
                     if (half == 0) a.delta[at] = delta;
@@ -358,13 +398,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(rest_read);
                 if (!bf) {
-                    amp = amp_of(__float_as_uint(top));
-                    if (half == 0 && top > 0.f) atomicMax(ex.amax + ((int64_t)b * a.Hkv + hk) * a.T + r, __float_as_uint(top));
+                    // |do.v| and |do.o| are at most this times |v|, and p at most 1
+                    const unsigned most = __float_as_uint(2.f * size * v_met);
+                    amp = amp_of(most);
+                    if (half == 0 && most) atomicMax(ex.reach + ((int64_t)b * a.Hkv + hk) * a.T + r, most);
                 }
             }
         } else if constexpr (!bf) {
             // a scale for every key, from the rows that see it and from no others
-            amp = amp_of(largest_met(ex.amax + ((int64_t)b * a.Hkv + hk) * a.T, r0, n, a.window, a.sinks, met, met_all));
+            amp = amp_of(largest_met<false>(ex.reach + ((int64_t)b * a.Hkv + hk) * a.T, r0, n, a.window, a.sinks, met, met_all));
         }
         const float delta_amp = delta * amp;
         for (; walk.x < count; step(walk)) {
@@ -535,13 +577,14 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
 }
 
 struct Layout {
-    size_t amax, sums, total;
+    size_t v_top, reach, sums, total;
     SinkParts parts;
 };
 Layout layout_of(const cail_ops_attention_args *c) {
     Layout l = {};
     l.parts = sink_parts(c, kRows, kStream, (int64_t)sm_count() * (c->D <= 64 ? 2 : 1));
-    l.sums = c->type == CAIL_OPS_F16 ? ((size_t)c->B * c->Hkv * c->T * 4 + 255) / 256 * 256 : 0;
+    const size_t values = c->type == CAIL_OPS_F16 ? ((size_t)c->B * c->Hkv * c->T * 4 + 255) / 256 * 256 : 0;
+    l.reach = values, l.sums = 2 * values;
     l.total = l.sums + sink_bytes(c, l.parts, kRows, c->D <= 64 ? 64 : 128);
     return l;
 }
@@ -551,13 +594,10 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     if (c->workspace_bytes < l.total || (l.total && (!c->workspace || !aligned(c->workspace, 16))))
         return fail(CAIL_OPS_EINVAL, "window attention backward: a workspace of %zu bytes is needed", l.total);
     Extra ex = {};
-    ex.amax = reinterpret_cast<unsigned *>(static_cast<char *>(c->workspace) + l.amax);
+    ex.v_top = reinterpret_cast<unsigned *>(static_cast<char *>(c->workspace) + l.v_top);
+    ex.reach = reinterpret_cast<unsigned *>(static_cast<char *>(c->workspace) + l.reach);
     ex.parts = l.parts;
     ex.parts.sums = reinterpret_cast<float *>(static_cast<char *>(c->workspace) + l.sums);
-    if (c->type == CAIL_OPS_F16) {
-        cudaError_t e = cudaMemsetAsync(ex.amax, 0, (size_t)a.B * a.Hkv * a.T * 4, st);
-        if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
-    }
     // the same arrays with boxes of 128 and of 64 rows
     Maps q = {}, k = {};
     if (int rc = tensor_map(&q.o, c->o, c->type, a.B, a.T, a.H, a.D, kRows)) return rc;
@@ -576,6 +616,11 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, AttnA
     cudaError_t e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_q);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(tc_backward_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_k);
     if (e != cudaSuccess) return fail(CAIL_OPS_ECUDA, "window attention backward: %s", cudaGetErrorString(e));
+    if (c->type == CAIL_OPS_F16) {
+        constexpr int rows = 256 / (DP / 8);
+        v_top_kernel<DP><<<dim3((a.T + rows - 1) / rows, a.Hkv, a.B), 256, 0, st>>>(a, ex);
+        if (int rc = launched("window attention backward")) return rc;
+    }
     tc_backward_kernel<T, DP, false><<<dim3(a.H, a.B, tiles), kThreads, sm_q, st>>>(a, ex, q);
     if (int rc = launched("window attention backward")) return rc;
     const unsigned blocks = tiles + ex.parts.tiles * (ex.parts.splits - 1);  // at most kMostTiles: sink_parts()

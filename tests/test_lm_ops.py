@@ -528,6 +528,53 @@ def test_a_large_gradient_costs_keys_that_it_does_not_meet_no_bits(dtype, window
         assert ref.rel(got, want) <= 5 * ref.half_step(dtype) + 256 * E + floor, "d" + name
 
 
+def fp16_floor(dtype, want):
+    """float16 results are held to 2^-24 absolute where they are small: 2^-25 on values of this root mean square."""
+    return 2.0 ** -25 / float(want.square().mean().sqrt()) if dtype == torch.float16 and bool(want.any()) else 0.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("T, D, group", [(60, 128, 1), (300, 128, 1), (300, 64, 2), (700, 72, 1)])
+@pytest.mark.parametrize("by", [1e-3, 1.0, 2000.0, 60000.0])
+def test_gradients_over_values_of_any_size(dtype, T, D, group, by):
+    """Rows of v of one sign along a gradient of ones, so that do.v is D |v| (2^23 here, and ds half of it) while the gradients
+    themselves are in range: two keys a row and a small scale."""
+    o = ops()
+    q, k, v, do, _ = attention_inputs((1, T, group, 1, D, 2, 0, None), dtype)
+    v = (torch.where(v[..., :1] < 0, -by, by) * torch.ones_like(v)).to(dtype)
+    do = torch.ones_like(do)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(o.window_attention(*leaves, 2, scale=2e-4), leaves, do)
+    r = [x.double().requires_grad_() for x in (q, k, v)]
+    dwant = torch.autograd.grad(ref.attention(*r, 2, 0, scale=2e-4), r, do.double())
+    for name, got, want in zip("qkv", grads, dwant):
+        assert ref.rel(got, want) <= 5 * ref.half_step(dtype) + 256 * E + fp16_floor(dtype, want), "d" + name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("window, sinks, key", [(20, 0, 150), (20, 4, 2), (20, 4, 127), (128, 0, 128), (129, 3, 300), (200, 0, 256), (300, 200, 350)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_large_value_costs_rows_that_do_not_see_it_no_bits(dtype, window, sinks, key, D):
+    """Values of 1e-3 beside one of 3e4: dq of the rows that do not see it, dk of the keys that none of its rows sees, all of dv."""
+    o = ops()
+    T = 700
+    q, k, v, do, _ = attention_inputs((1, T, 2, 1, D, window, sinks, None), dtype)
+    v = v * 1e-3
+    v[0, key] = 3e4
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(o.window_attention(*leaves, window, sinks), leaves, do)
+    r = [x.detach().double().requires_grad_() for x in leaves]
+    dwant = torch.autograd.grad(ref.attention(*r, window, sinks), r, do.double())
+    on = ref.seen_mask(T, T, window, sinks)
+    rows = ~on[:, key]
+    keys = ~on[on[:, key]].any(0)
+    for name, at, got, want in zip("qkv", (rows, keys, torch.ones(T, dtype=torch.bool)), grads, dwant):
+        got, want = got[0, at.cuda()].double(), want[0, at.cuda()]
+        assert ref.rel(got, want) <= 5 * ref.half_step(dtype) + 256 * E + fp16_floor(dtype, want), "d" + name
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 @pytest.mark.parametrize("what", [float("inf"), float("nan")])
