@@ -408,7 +408,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             // a scale for every key, from the rows that see it and from no others
             amp = amp_of(largest_met<false>(ex.reach + ((int64_t)b * a.Hkv + hk) * a.T, r0, n, a.window, a.sinks, met, met_all));
         }
-        const float delta_amp = delta * amp;
+        // fp16, dv: p goes into its product 2^15 times as large, as it has no bits left for rows of many keys otherwise
+        // (2^-18 is four bits)
+        constexpr int lift = DKV && !bf ? 15 : 0;
+        const float ds_amp = amp * (1.f / (1 << lift)), delta_amp = delta * ds_amp;
         for (; walk.x < count; step(walk)) {
             const int x = walk.x, t0 = walk.row, s = x % ST;
             if (ok) ok = mbar_wait(s_full + 8 * (x % NB), (x / NB) & 1);
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             if (DKV) whole = r0 + kRows - 1 <= t0 && t0 + kStream <= n && (t0 + kStream - 1 - r0 < a.window || r0 + kRows <= a.sinks);
             else whole = t0 + kStream - 1 <= r0 && (r0 + kRows - 1 - t0 < a.window || t0 + kStream <= a.sinks);
             // signs turned where that costs nothing: exp2(-(lse - s)), and -ds = p (delta - dp), put right in the sums' scale
-            const uint64_t scale2 = two(-a.scale_log2, -a.scale_log2), minus = two(-amp, -amp);
+            const uint64_t scale2 = two(-a.scale_log2, -a.scale_log2), minus = two(-ds_amp, -ds_amp);
             constexpr int CH = S::chunk;
             auto math = [&](auto masked) {
                 uint32_t on = 0, on_ds = 0;  // which of the 32 are seen; which of them carry ds
@@ -460,7 +463,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
                                          : "r"(v + kStream * 4));
                             l2[0] = two(l4[0], l4[1]), l2[1] = two(l4[2], l4[3]);
                             d2[0] = two(d4[0], d4[1]), d2[1] = two(d4[2], d4[3]);
-                            if (!bf) d2[0] = mul_two(d2[0], two(amp, amp)), d2[1] = mul_two(d2[1], two(amp, amp));
+                            if (!bf) {
+                                l2[0] = add_two(l2[0], two(-lift, -lift)), l2[1] = add_two(l2[1], two(-lift, -lift));
+                                d2[0] = mul_two(d2[0], two(ds_amp, ds_amp)), d2[1] = mul_two(d2[1], two(ds_amp, ds_amp));
+                            }
                         }
                         float p[4], d[4];
 #pragma unroll
@@ -521,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, DKV>::per_sm)
             const uint32_t stage = DKV && half ? sy : sx;
             const uint32_t from = mine + S::acc + (DKV && half ? DP : 0);
             const int c_lo = DKV ? 0 : half * (DP / 2), c_hi = DKV ? DP : c_lo + DP / 2;
-            const float by = DKV && half ? 1.f : -a.scale / amp;
+            const float by = DKV && half ? 1.f / (1 << lift) : -a.scale / amp;
             const bool live = r < n;
             float *part = nullptr;
             if (DKV && parted)

@@ -576,6 +576,25 @@ def test_a_large_value_costs_rows_that_do_not_see_it_no_bits(dtype, window, sink
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=ids_of)
+def test_value_gradients_of_rows_of_many_keys(dtype):
+    """Equal scores: p = 1 / (i + 1), down to 2^-18.6, and dv_j = sum of do_i / (i + 1) over i >= j.  p is off by u of its own
+    size whatever that is, the sums of 4e5 terms in 32 bits by far less."""
+    o = ops()
+    T = 400000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(1, T, 1, 64, generator=g, device="cuda").to(dtype) for _ in range(2))
+    do = (torch.randn(1, T, 1, 64, generator=g, device="cuda") * 64).to(dtype)
+    q = torch.zeros_like(k)
+    v.requires_grad_()
+    (dv,) = torch.autograd.grad(o.window_attention(q, k, v, T), v, do)
+    terms = do[0, :, 0].double() / torch.arange(1, T + 1, device="cuda").double()[:, None]
+    want = terms.flip(0).cumsum(0).flip(0)
+    for lo, hi in ((0, T // 4), (T // 4, T // 2), (T // 2, 3 * T // 4)):
+        assert ref.rel(dv[0, lo:hi, 0], want[lo:hi]) <= 3 * ref.half_step(dtype) + 256 * E
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 @pytest.mark.parametrize("what", [float("inf"), float("nan")])
 def test_what_is_not_finite_is_not_hidden(dtype, what):
