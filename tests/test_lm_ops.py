@@ -898,6 +898,24 @@ def test_decode_matches_64_bit(dtype, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=ids_of)
+@pytest.mark.parametrize("H, Hkv, D", [(2, 2, 64), (32, 8, 128), (8, 1, 64), (7, 1, 128), (9, 1, 64), (16, 1, 128), (20, 1, 80), (32, 2, 64)])
+@pytest.mark.parametrize("T, window, sinks", [(4000, 3000, 4), (1300, 1300, 0), (300, 40, 20)])
+def test_decode_loses_one_rounding(dtype, H, Hkv, D, T, window, sinks):
+    """Element by element: o is off by its own rounding; p reaches its sum to 2 u^2 and 256 E (exponentials and sums of up to 3000
+    terms in 32 bits) relative to the terms p |v|, and float16 holds small results to 2^-25."""
+    o = ops()
+    g = gen(T + H)
+    q, k, v = randn(g, 2, H, D, dtype=dtype, by=2.0), randn(g, 2, T, Hkv, D, dtype=dtype), randn(g, 2, T, Hkv, D, dtype=dtype)
+    n = torch.tensor([T, T - 77], dtype=torch.int32).cuda()
+    got = o.window_attention_decode(q, k, v, n, window, sinks).double()
+    want, size = ref.decode(q, k, v, n, window, sinks), ref.decode(q, k, v.abs(), n, window, sinks)
+    u = ref.half_step(dtype)
+    small = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    assert ((got - want).abs() <= u * want.abs() * (1 + u) + (2 * u * u + 256 * E) * size * (1 + u) + small).all()
+
+
+@pytest.mark.gpu
 def test_decode_past_32_bit_offsets():
     """A cache of more than 2^32 bytes and 2^31 elements: the last token of the
     last sequence."""
