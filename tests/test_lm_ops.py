@@ -331,6 +331,27 @@ def test_rotary_matches_64_bit(dtype, inter, B, T, H, Hk, D, part):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("inter", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("first", [0, 100000, 2 ** 30])
+def test_rotary_angles_lose_nothing(inter, first):
+    """The pair (1, 0) turns into cosine and sine themselves: sincospif is good to one unit in the last place, E below 1, and what
+    is left of the angle is put in with one more rounding, E / 2: 1.5 E in all (1.6 for the second order).  An angle rounded to
+    32 bits would be off by up to pi / 2 E by itself."""
+    o = ops()
+    plan = o.Rotary(64, interleaved=inter)
+    ia = torch.arange(0, 64, 2) if inter else torch.arange(32)
+    ib = ia + (1 if inter else 32)
+    q = torch.zeros(1, 5000, 1, 64, device="cuda")
+    q[..., ia] = 1.0
+    pos = (torch.arange(5000) + first).cuda()
+    got = o.rotary(q, None, plan, pos)[0, :, 0].double()
+    turns = pos.double()[:, None] * plan.turns
+    angle = (turns - turns.round()) * 2 * torch.pi
+    assert float((got[:, ia] - angle.cos()).abs().max()) <= 1.6 * E
+    assert float((got[:, ib] - angle.sin()).abs().max()) <= 1.6 * E
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inter", [False, True], ids=["half", "interleaved"])
 def test_rotary_strides(inter):
     """q and k as parts of one projection, heads before tokens, elements apart,
     rows on odd addresses, expanded gradients."""
