@@ -182,15 +182,10 @@ template <typename T, int LANES, int G, bool VEC> int launch(const AttnArgs &a, 
     int blocks = 1;
     while (blocks < 8 && work * blocks < 8 * (int64_t)sm_count() && keys >= blocks * 2 * 64) blocks *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks, a.Hkv * chunks, a.B);
+    cfg.gridDim = dim3(1, a.Hkv * chunks, a.B);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)blocks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, decode_kernel<T, LANES, G, VEC>, a);
+    launch_clusters(cfg, 1, blocks, decode_kernel<T, LANES, G, VEC>, a);
     return launched("window attention decode");
 }
 template <typename T, int LANES, bool VEC> int by_group(const AttnArgs &a, cudaStream_t st) {

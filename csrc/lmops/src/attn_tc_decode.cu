@@ -336,16 +336,11 @@ template <typename T, int DP, int HEADS> int launch(const cail_ops_attention_arg
     int blocks = 1;
     while (blocks < 16 && work * blocks * 2 <= (blocks < 8 ? 2 * sms : sms) && keys >= blocks * 2 * 2 * kKeys) blocks *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks, a.Hkv * chunks, a.B);
+    cfg.gridDim = dim3(1, a.Hkv * chunks, a.B);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = S::smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)blocks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, tc_decode_kernel<T, DP, HEADS>, a, maps);
+    launch_clusters(cfg, 1, blocks, tc_decode_kernel<T, DP, HEADS>, a, maps);
     return launched("window attention decode");
 }
 

@@ -31,6 +31,23 @@ inline bool rows_aligned(const cail_ops_bthd &x, int B, int T, int H, size_t siz
 }
 
 #ifdef __CUDACC__
+// Launches `groups` clusters of `blocks` blocks side by side in x (cfg gives the
+// rest), of fewer where so many do not fit: a process, or a stream's context,
+// may have been given a part of the SMs.  Kernels ask for the size they got.
+template <typename... P, typename... A>
+void launch_clusters(cudaLaunchConfig_t cfg, unsigned groups, int blocks, void (*kernel)(P...), const A &...args) {
+    for (;; blocks /= 2) {
+        cfg.gridDim.x = groups * (unsigned)blocks;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)blocks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaErrorInvalidClusterSize || blocks == 1) return;
+        cudaGetLastError();
+    }
+}
+
 // ----------------------------------------------------------------- device
 template <typename T> __device__ __forceinline__ float to_f(T x);
 template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }

@@ -836,15 +836,10 @@ bool streams(const Args &a, size_t size) { return a.N >= sm_count() && a.V * (in
 
 template <typename T, int MODE> int launch(const Args &a, int blocks, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.N * blocks));
+    cfg.gridDim = dim3(1);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)blocks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, distill_kernel<T, MODE>, a);
+    launch_clusters(cfg, (unsigned)a.N, blocks, distill_kernel<T, MODE>, a);
     return launched("distill");
 }
 template <typename K> int ring(K kernel, int threads, const Args &a, const char *who, cudaStream_t st) {

@@ -1367,6 +1367,46 @@ def test_decode_captured_follows_the_lengths():
         assert ref.rel(out, ref.decode(q, k, v, lengths, 100, 4)) <= 3 * ref.half_step(torch.bfloat16) + 64 * E
 
 
+def part_of_the_sms(count):
+    """A stream whose kernels run on `count` SMs (a green context of this process; nothing outlasts it)."""
+    d = pytest.importorskip("cuda.bindings.driver")
+
+    def get(r):
+        if r[0] != d.CUresult.CUDA_SUCCESS:
+            pytest.skip(f"no part of the SMs to be had: {r[0]}")
+        return r[1] if len(r) == 2 else r[1:]
+
+    dev = get(d.cuDeviceGet(torch.cuda.current_device()))
+    sms = get(d.cuDeviceGetDevResource(dev, d.CUdevResourceType.CU_DEV_RESOURCE_TYPE_SM))
+    flags = int(d.CUdevSmResourceSplit_flags.CU_DEV_SM_RESOURCE_SPLIT_IGNORE_SM_COSCHEDULING) if count < 8 else 0
+    groups = get(d.cuDevSmResourceSplitByCount(1, sms, flags, count))[0]
+    ctx = get(d.cuGreenCtxCreate(get(d.cuDevResourceGenerateDesc([groups[0]], 1)), dev, d.CUgreenCtxCreate_flags.CU_GREEN_CTX_DEFAULT_STREAM))
+    return torch.cuda.ExternalStream(int(get(d.cuGreenCtxStreamCreate(ctx, d.CUstream_flags.CU_STREAM_NON_BLOCKING, 0))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sms", [2, 8, 16])
+def test_clusters_on_a_part_of_the_sms(sms):
+    """Where a cluster of the size that the whole GPU would have does not fit, smaller ones run: the same results but for the
+    sums' order, by the bounds against 64 bits."""
+    o = ops()
+    g = gen(sms)
+    q, k, v = randn(g, 1, 2, 64), randn(g, 1, 16384, 2, 64), randn(g, 1, 16384, 2, 64)
+    n = torch.tensor([16000], dtype=torch.int32).cuda()
+    z, ids, t, y = distill_inputs((2, 50257, 33, 2.0, 0.3, True, 0.1), torch.float32)
+    o.window_attention_decode(q, k, v, n, 16384)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(part_of_the_sms(sms)):
+        for dtype in TYPES:
+            x = [c.to(dtype) for c in (q, k, v)]
+            got = o.window_attention_decode(*x, n, 16384)
+            assert ref.rel(got, ref.decode(*x, n, 16384, 0)) <= 3 * ref.half_step(dtype) + 64 * E
+        loss = o.distill_loss(z, ids, t, y, temperature=2.0, hard_weight=0.3)
+        want = float(ref.distill(z, ids, t, y, 2.0, 0.3))
+        assert abs(float(loss) - want) <= 2e-6 * (1 + want)
+        torch.cuda.current_stream().synchronize()
+
+
 @pytest.mark.gpu
 def test_operators_from_two_threads():
     """Two threads on streams of their own, the same bits as one after the other."""
