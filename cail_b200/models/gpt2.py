@@ -57,9 +57,10 @@ class KVCache:
 
     def __init__(self, c: GPT2Config, batch: int, length: int, device, dtype):
         shape = (batch, length, c.n_head, c.d_model // c.n_head)
-        self.k = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(c.n_layer)]
-        self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(c.n_layer)]
-        self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
+        with torch.inference_mode(False):  # so that what fills it may run in inference mode or outside
+            self.k = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(c.n_layer)]
+            self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(c.n_layer)]
+            self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
         self.length = length
         self.filled = 0
 

@@ -264,6 +264,32 @@ def test_training_after_inference_mode():
     assert torch.equal(out, ops.rotary(q, None, m._plan(q.device)))
 
 
+def test_caches_belong_to_no_mode_on_cpu():
+    with torch.inference_mode():
+        cache = GPT2(config(window=8)).new_cache(2, 4)
+    assert not any(t.is_inference() for t in (*cache.k, *cache.v, cache.lengths))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("made, filled, read", [(True, True, False), (True, False, True), (False, True, False)])
+def test_caches_belong_to_no_mode(made, filled, read):
+    """A cache made, filled and read inside inference_mode or outside, in any mixture: the same logits."""
+    torch.manual_seed(11)
+    m = GPT2(config(rotary=16, window=9)).cuda()
+    idx = torch.randint(0, 512, (2, 20)).cuda()
+
+    def run(made, filled, read):
+        with torch.inference_mode(made):
+            cache = m.new_cache(2)
+        with torch.inference_mode(filled):
+            m.prefill(idx[:, :18], cache)
+            m.decode(idx[:, 18], cache)
+        with torch.inference_mode(read):
+            return m.decode(idx[:, 19], cache)
+
+    assert torch.equal(run(made, filled, read), run(False, False, False))
+
+
 @pytest.mark.gpu
 def test_bf16_model_runs_on_the_tensor_cores():
     """A bf16 model of heads of 64: step and decoding run, gradients are finite
