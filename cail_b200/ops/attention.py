@@ -25,10 +25,18 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
     float32, bfloat16 or float16, D from 1 to 128, any strides (elements of a
     head that do not lie side by side are copied first).  Scores, softmax
-    statistics and sums are 32-bit.  Gradients flow to q, k and v, each summed
-    in a fixed order: the same inputs give the same bits.  A kernel that waits in
-    vain for its data (two seconds) gives up, and the next call on the device
-    raises RuntimeError.
+    statistics and sums are 32-bit.  With 16-bit inputs of more than 64 tokens
+    the probabilities, and in the backward pass their gradients, are rounded to
+    the input type where they enter a matrix product; rows of few keys (the
+    first 128, or all where window + sinks <= 128 or D < 64) keep twice the bits
+    of the probabilities.  float16 scales those gradients by a bound of their
+    own size, row by row and key by key, so nothing overflows before the result
+    does; what lies 2^29 below that bound loses bits.  A row whose scores are all
+    minus infinity gives zeros.
+
+    Gradients flow to q, k and v, each summed in a fixed order: the same inputs
+    give the same bits.  A kernel that waits in vain for its data (two seconds)
+    gives up, and the next call on the device raises RuntimeError.
     """
     return ext.get_ops().window_attention(q, k, v, window, sinks, lengths, scale)
 
@@ -41,6 +49,8 @@ def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     own key and value: the query is token ``lengths[b] - 1`` of its sequence and
     sees what that row of ``window_attention`` sees.  ``lengths`` (int32 [B], on
     the device) are clamped to [0, T]; a length of 0 gives zeros.  Only the keys
-    and values that are seen are read.  No backward pass.
+    and values that are seen are used.  Everything is 32-bit but the result's
+    own rounding (16-bit caches: p is kept to twice the type's bits).  No
+    backward pass.
     """
     return ext.get_ops().window_attention_decode(q, k_cache, v_cache, lengths, window, sinks, scale)

@@ -35,8 +35,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     alone, has a loss and a gradient of NaN.
 
     The gradient flows to ``logits``.  Softmax statistics and sums are 32-bit,
-    the sum over rows 64-bit, in a fixed order: the same inputs give the same
-    bits.
+    of differences from the row's largest values, so logits may lie around any
+    level and be masked by any value; the sum over rows is 64-bit, in a fixed
+    order: the same inputs give the same bits.
     """
     try:
         mean = _REDUCTIONS[reduction]

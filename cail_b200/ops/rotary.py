@@ -78,7 +78,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], plan: Rotary,
     or int64 (0 .. T-1 if not given).  Elements from ``plan.dim`` on pass
     unchanged.  Gradients flow to q and k (the inverse turn).  One launch; any
     strides; float32, bfloat16 or float16, computed in 32 bits with the angle
-    in 64."""
+    in 64 (sine and cosine of it to 1.5 units of 2^-24)."""
     out = ext.get_ops().rotary(q, k, plan.turns, positions, plan.dim, plan.interleaved, plan.amplitude)
     return out[0] if k is None else (out[0], out[1])
 
@@ -86,6 +86,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], plan: Rotary,
 def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], plan: Rotary,
             positions: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``rotary()`` in place (only the rotated part is touched); not on tensors
-    that require a gradient, share memory with each other, or repeat elements."""
+    that require a gradient, share memory with each other, or repeat elements
+    (ValueError)."""
     ext.get_ops().rotary_inplace(q, k, plan.turns, positions, plan.dim, plan.interleaved, plan.amplitude)
     return q if k is None else (q, k)

@@ -1,11 +1,14 @@
 /* cail_ops.h — language-model operators of libcail_ops.so (sm_100a kernels).
  *
  * Every entry point queues its work on `stream` of the current device and
- * returns without waiting: no allocation, no synchronisation, nothing kept
- * from one call to the next, so calls may run from several host threads and
- * may be captured into CUDA graphs.  Pointers are device pointers; strides
- * are in elements.  Scratch memory is the caller's and belongs to one call
- * until that call's work has finished.
+ * returns without waiting, so calls may run from several host threads and may
+ * be captured into CUDA graphs.  Pointers are device pointers; strides are in
+ * elements.  Scratch memory is the caller's and belongs to one call until that
+ * call's work has finished.  Nothing is allocated or kept from one call to the
+ * next but one word of mapped host memory per device: the first call of a
+ * kernel that waits for its data (16-bit attention and decoding, the loss of
+ * many rows) allocates it, which may synchronise, and where such a kernel gave
+ * up, the next such call on the device fails (cail_ops_device_error_word).
  *
  * Return value: CAIL_OPS_OK, CAIL_OPS_EINVAL (refused before any launch) or
  * CAIL_OPS_ECUDA (a CUDA call failed); cail_ops_last_error() gives the text

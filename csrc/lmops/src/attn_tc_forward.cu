@@ -9,19 +9,23 @@
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown
 // by more than 2^8 since the scale in use, so p stays below 256 and most tiles
 // touch O in no other way than the product.  p is rounded to the input type
-// for that product (its sum is not); everything else is 32-bit.  Rows of few
+// for that product (its sum is not), as a second part of it would double the
+// product, 40 % more for the tensor pipe; everything else is 32-bit.  Rows of few
 // keys (cail_ops_rest_rows) take p in two parts, the second what rounding took
 // from the first, and so twice the second product, in loops of their own (one
 // loop with the choice inside took 3 % more): 0.4 us of 34 below.
 //
 // 64 keys per tile, two blocks per SM with two buffers of S each, so a product
-// runs under the softmax.  At D = 64 the exponentials bound it (16 a clock and
-// SM: 512 clocks a tile, against 334 for the products, 50 for a 64-column
-// product from shared memory and 33 from tensor memory); at D = 128 the
-// products do (664 clocks).  Four blocks per SM with one buffer each, and a
-// quarter of the exponentials on the float pipes, both measured the same as
-// this (4 x 4096 tokens, 16 heads, causal: 214 us at D = 64, 273 at D = 128,
-// 640 and 1000 TFLOP/s); small calls took 8 us instead of 6.
+// runs under the softmax.  4 x 4096 tokens, 16 heads, causal: 217 us at D = 64,
+// 280 at D = 128, 635 and 980 TFLOP/s, about 900 and 1160 clocks a tile and SM.
+// A tile's exponentials take 512 of them (16 a clock and SM), its products 334
+// at D = 64 and 664 at D = 128 (50 for a 64-column product from shared memory,
+// whose operations alone are 32, and 33 from tensor memory).  So at D = 64
+// neither bounds it by itself, as a quarter of the exponentials on the float
+// pipes, which measured the same, says too: the softmax warps wait on their own
+// row's chain (scores out, maximum, exponentials, p back).
+// Four blocks per SM with one buffer each measured the same; small calls took
+// 8 us instead of 6.
 //
 // Short windows are bound by neither: 8 x 1024 tokens, 16 heads of 64, window
 // 256 and 4 sinks, take 34 us (products 15 % of the tensor pipe, exponentials
@@ -373,10 +377,12 @@ template <typename T, int DP> int launch(const cail_ops_attention_args *c, const
 
 // 16-bit elements in rows that TMA can load (16-byte multiples), a positive
 // scale (the row maximum is taken before scaling), no more tiles than a grid
-// has; and more than 64 tokens: below, the other kernels are as fast and round
-// neither p nor ds.  (The same holds for short windows, where rounding ds costs
-// most, but not their speed: 8 x 1024 tokens, 16 heads of 64, window 8, forward
-// and backward, 117 us here and 1130 there.)
+// has; and more than 64 tokens: below, rows have few keys, where rounding ds
+// costs most, and the other kernels round neither p nor ds.  That is a choice
+// for accuracy and costs time, the more the larger the batch: 8 heads of 64,
+// forward and backward, 8 x 32 tokens 25 us (19 here), 64 x 64 114 (37), 4096
+// x 64 6660 (1730).  Short windows over more tokens are not left to the other
+// kernels: 8 x 1024 tokens, 16 heads of 64, window 8, 117 us here, 1130 there.
 bool tc_takes(const cail_ops_attention_args *a) {
     if (a->type == CAIL_OPS_F32 || a->D % 8 || !(a->scale > 0.f) || a->T > kMostTiles * kRows || a->T <= 64) return false;
     if (!tma_takes(a->q, a->B, a->T, a->H) || !tma_takes(a->k, a->B, a->T, a->Hkv) || !tma_takes(a->v, a->B, a->T, a->Hkv)) return false;
